@@ -546,6 +546,63 @@ int nl_dist_merge_counters_strided(const int* gathered, int stride_ints, int wor
 int nl_dist_rows_union_prefix(const int* gathered, int stride_ints, int offset_ints, int world, unsigned* union_bitmap, int n_words, int* prefix,
                               int* total, int* workspace, void* stream);
 
+/* ---- layer operators: what a decoder of any size trains with -----------------------------------------------------
+ * The reference builds these from torch.nn.Linear, ReLU and F.embedding (src/variations/lidar.py:105-123, src/variations/render_helpers.py:85-89).
+ * Element types of tensors (x, weight, bias, residual, output and their gradients share one), activations, and what is kept for the backward pass. */
+#define NL_DT_F32 0
+#define NL_DT_BF16 1
+#define NL_DT_F16 2
+#define NL_ACT_NONE 0
+#define NL_ACT_RELU 1
+#define NL_ACT_GELU 2           /* z (1 + erf(z / sqrt 2)) / 2 */
+#define NL_ACT_SILU 3           /* z / (1 + exp(-z)) */
+#define NL_MX8_BLOCK 32         /* 8-bit checkpoints: e4m3 codes; 32 neighbouring features of a row share a power of two, stored as one byte e + 127 */
+
+/* One linear layer: z = x w^T + b, y = act(z) + r;  x [M,K], w [N,K], b [N], r [M,N], y [M,N], rows `ld*` elements apart, elements of a row adjacent.
+ * nl_linear_forward reads x w b(or NULL) r(or NULL), writes y and, where the pointer is set, what the backward pass needs of z:
+ *   z     gelu / silu: z [M,N] in dtype, rows N apart                     z8, z8e   instead of z: codes [M][up(N,32)] and exponents [M][ceil(N/32)]
+ *   bits  relu: one bit per element, z > 0: words [M][ceil(N/32)], column n in bit n % 32 of word n / 32
+ * nl_linear_backward reads gy, w (for gx), x or x8 / x8e (for gw), what the forward pass kept of z, and writes gx [M,K], gw [N,K], gb [N], each where its
+ * pointer is set, in dtype.  dz = gy act'(z) is rounded to dtype once for the two products (fp32: not at all); gb sums the unrounded values.
+ * fp32 products run as six bf16 products of the exact three-term splits of both operands (dropped terms below 2^-26 of |x||w|); an infinity among the
+ * operands gives NaN there.  Sums are fp32 and their order depends on the sizes only.  M = 0 is a legal call (gw, gb = 0).
+ * x8 / x8e: [M][up(K,32)] and [M][ceil(K/32)] as nl_mx8_encode writes them; a decoded value beyond dtype's largest number counts as that.
+ * ws: nl_linear_workspace(desc, backward) bytes, 256-byte aligned; contents are free between calls. */
+typedef struct NlLinear {
+    int struct_size, dtype, act, K, N, reserved;
+    long long M;
+    const void* x; long long ldx;
+    const void* w; long long ldw;
+    const void* b;
+    const void* r; long long ldr;
+    void* y; long long ldy;
+    void* z; unsigned* bits; unsigned char* z8; unsigned char* z8e;
+    const unsigned char* x8; const unsigned char* x8e;
+    const void* gy; long long ldgy;
+    void* gx; void* gw; void* gb;
+    void* ws; long long ws_bytes;
+} NlLinear;
+int nl_linear_forward(const NlLinear* desc, void* stream);
+int nl_linear_backward(const NlLinear* desc, void* stream);
+long long nl_linear_workspace(const NlLinear* desc, int backward);      /* bytes; -1: the descriptor is invalid */
+
+/* 8-bit checkpoints: x [M,K] of dtype, rows ldx apart -> codes [M][up(K,32)] (padding: zeros), exponents [M][ceil(K/32)]; and back.
+ * e = the smallest exponent >= -126 with max |x| <= 448 2^e over the block; codes to nearest, ties to even; infinities and NaN become NaN;
+ * a decoded value beyond dtype's largest number (the largest ones round up) is that number. */
+int nl_mx8_encode(const void* x, long long ldx, long long M, int K, int dtype, unsigned char* codes, unsigned char* exps, void* stream);
+int nl_mx8_decode(const unsigned char* codes, const unsigned char* exps, long long M, int K, int dtype, void* out, void* stream);
+
+/* Embedding lookup: out[i] = scale sum_k weights[i,k] table[ids[i,k]], k < bag (weights NULL: all 1), sums in fp32, one rounding.  ids int32 (id64 = 0) or
+ * int64; an id outside [0, V) selects no row.  table [V,D], out [M,D] of dtype.
+ * nl_embedding_backward: g_table [V,D] of dtype (every row written: zero where no id selects it), g_weights [M,bag] fp32; each where its pointer is set.
+ * The (id, position) pairs are sorted and every row's sum runs over its positions in ascending order, in pieces joined in order: no float atomics, the same
+ * bits every run.  ws: nl_embedding_workspace bytes (0 without g_table). */
+int nl_embedding_forward(const void* table, long long V, int D, int dtype, const void* ids, int id64, const float* weights, long long M, int bag, float scale,
+                         void* out, void* stream);
+int nl_embedding_backward(const void* table, long long V, int D, int dtype, const void* ids, int id64, const float* weights, long long M, int bag, float scale,
+                          const void* g_out, void* g_table, float* g_weights, void* ws, long long ws_bytes, void* stream);
+long long nl_embedding_workspace(long long V, int D, long long M, int bag);
+
 /* ---- (b2) host octree behind torch.classes.svo.Octree (third_party/sparse_octree/src/bindings.cpp:4-31) */
 void* nl_octree_create(long long grid_dim);                              /* Octree::init   octree.cpp:36-50   */
 void nl_octree_destroy(void* h);

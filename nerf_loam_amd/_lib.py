@@ -84,6 +84,21 @@ class NlTouchedRows(ctypes.Structure):
     _fields_ = [("struct_size", ctypes.c_int), ("list", ctypes.c_void_p), ("count", ctypes.c_void_p), ("flags", ctypes.c_void_p), ("copies", ctypes.c_int), ("copy_stride", ctypes.c_longlong)]
 
 
+NL_DTYPES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}
+NL_ACTS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+NL_MX8_BLOCK = 32
+
+
+class NlLinear(ctypes.Structure):
+    """ctypes mirror of NlLinear (include/nerfloam_hip.h): field order and types must match (tests/test_layers_host.py)"""
+    _fields_ = ([(n, ctypes.c_int) for n in ("struct_size", "dtype", "act", "K", "N", "reserved")] + [("M", ctypes.c_longlong)]
+                + [("x", ctypes.c_void_p), ("ldx", ctypes.c_longlong), ("w", ctypes.c_void_p), ("ldw", ctypes.c_longlong), ("b", ctypes.c_void_p),
+                   ("r", ctypes.c_void_p), ("ldr", ctypes.c_longlong), ("y", ctypes.c_void_p), ("ldy", ctypes.c_longlong)]
+                + [(n, ctypes.c_void_p) for n in ("z", "bits", "z8", "z8e", "x8", "x8e")]
+                + [("gy", ctypes.c_void_p), ("ldgy", ctypes.c_longlong)] + [(n, ctypes.c_void_p) for n in ("gx", "gw", "gb")]
+                + [("ws", ctypes.c_void_p), ("ws_bytes", ctypes.c_longlong)])
+
+
 # communicator of the ray-sharded iteration (NlComm, include/nerfloam_hip.h)
 NL_COMM_F32, NL_COMM_F64, NL_COMM_I32 = 0, 1, 2
 NL_COMM_ALL_GATHER = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p)
@@ -192,6 +207,14 @@ _SIGS = {
     "nl_dist_mark_rows": ([_I, _P, _P, _P, _P, _P], _I),
     "nl_dist_rows_prefix": ([_P, _I, _P, _P, _P, _P], _I),
     "nl_dist_rows_move": ([_I, _P, _P, _I, _P, _P, _I, _P, _P], _I),
+    "nl_linear_forward": ([_P, _P], _I),
+    "nl_linear_backward": ([_P, _P], _I),
+    "nl_linear_workspace": ([_P, _I], _LL),
+    "nl_mx8_encode": ([_P, _LL, _LL, _I, _I, _P, _P, _P], _I),
+    "nl_mx8_decode": ([_P, _P, _LL, _I, _I, _P, _P], _I),
+    "nl_embedding_forward": ([_P, _LL, _I, _I, _P, _I, _P, _LL, _I, _F, _P, _P], _I),
+    "nl_embedding_backward": ([_P, _LL, _I, _I, _P, _I, _P, _LL, _I, _F, _P, _P, _P, _P, _LL, _P], _I),
+    "nl_embedding_workspace": ([_LL, _I, _LL, _I], _LL),
     "nl_octree_create": ([_LL], _P),
     "nl_octree_destroy": ([_P], None),
     "nl_octree_insert": ([_P, _P, _LL], _I),

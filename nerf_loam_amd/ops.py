@@ -268,3 +268,173 @@ def select_rays_batch(Ms, ns, seeds, rays_d, points, cos_in, masks, out_off, out
 def scan_hit_rays(hit_count, hit_rank, ray_of_rank, N, total_out, total_out2, workspace):
     check(L.lib().nl_scan_hit_rays(ptr(hit_count), ptr(hit_rank), ptr(ray_of_rank), int(N), ptr(total_out), ptr(total_out2), ptr(workspace),
                                    stream_ptr()), "nl_scan_hit_rays")
+
+
+# ---- layer operators (include/nerfloam_hip.h NlLinear, nl_mx8_*, nl_embedding_*) --------------------------------------------------------
+# nerf_loam_amd.layers puts autograd on top of these; called directly they allocate nothing but a workspace and can be captured into a graph,
+# the backward pass included.
+
+def _layer_dtype(t, name):
+    code = L.NL_DTYPES.get(str(t.dtype))
+    if code is None:
+        raise L.NerfLoamHipError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+def _rows(t, cols, like, name):
+    """a [M, cols] tensor on the device and of the type of `like`, elements of a row adjacent -> (pointer, row stride)"""
+    if t is None:
+        return None, 0
+    if t.device != like.device or t.dtype != like.dtype:
+        raise L.NerfLoamHipError(f"{name} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
+    if t.dim() != 2 or t.shape[1] != cols or (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols):
+        raise L.NerfLoamHipError(f"{name} must be [rows, {cols}] with adjacent elements in a row, got shape {tuple(t.shape)}, strides {t.stride()}")
+    return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else cols)
+
+
+def _flat(t, shape, dtype, like, name):
+    """a contiguous tensor of exactly this shape and type on the device of `like` -> pointer"""
+    if t is None:
+        return None
+    if t.device != like.device or t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise L.NerfLoamHipError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {like.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _on_device(t):
+    """(stream pointer, context) of the tensor's device: kernels run there on its current stream, whatever device is current"""
+    if not t.is_cuda:
+        raise L.NerfLoamHipError("the layer operators run on the GPU only - no CPU path")
+    return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream), torch.cuda.device(t.device)
+
+
+def _workspace(need, ws, like, name):
+    if need < 0:
+        raise L.NerfLoamHipError(f"{name} failed: {L._ERR[1]}")
+    if need == 0:
+        return None, 0
+    if ws is None:
+        ws = torch.empty(need, dtype=torch.uint8, device=like.device)
+    if ws.device != like.device or ws.dtype != torch.uint8 or not ws.is_contiguous() or ws.numel() < need:
+        raise L.NerfLoamHipError(f"{name}: workspace must be a contiguous uint8 tensor of at least {need} bytes on {like.device}")
+    return ws, need
+
+
+def linear_forward(x, weight, bias=None, act="none", residual=None, out=None, z=None, bits=None, z8=None, z8e=None, workspace=None):
+    """y = act(x weight^T + bias) + residual; x [M,K], weight [N,K], bias [N], residual / out [M,N], rows may be strided.  z, bits, z8 / z8e: what
+    linear_backward needs of z, written where given (layers.linear_act allocates them)"""
+    stream, guard = _on_device(x)
+    if x.dim() != 2 or weight.dim() != 2:
+        raise L.NerfLoamHipError(f"linear_forward: x {tuple(x.shape)} must be [M, K] and weight {tuple(weight.shape)} [N, K]")
+    M, K = x.shape
+    N = weight.shape[0]
+    if out is None:
+        out = torch.empty(M, N, dtype=x.dtype, device=x.device)
+    for t, n in ((residual, "residual"), (out, "out")):
+        if t is not None and t.shape[0] != M:
+            raise L.NerfLoamHipError(f"linear_forward: {n} {tuple(t.shape)} must be [{M}, {N}]")
+    d = L.NlLinear(struct_size=ctypes.sizeof(L.NlLinear), dtype=_layer_dtype(x, "x"), act=L.NL_ACTS[act], K=K, N=N, M=M)
+    d.x, d.ldx = _rows(x, K, x, "x")
+    d.w, d.ldw = _rows(weight, K, x, "weight")
+    d.b = _flat(bias, (N,), x.dtype, x, "bias")
+    d.r, d.ldr = _rows(residual, N, x, "residual")
+    d.y, d.ldy = _rows(out, N, x, "out")
+    NB = (N + 31) // 32
+    d.z = _flat(z, (M, N), x.dtype, x, "z")
+    d.bits = _flat(bits, (M, NB), I32, x, "bits")
+    d.z8 = _flat(z8, (M, 32 * NB), torch.uint8, x, "z8")
+    d.z8e = _flat(z8e, (M, NB), torch.uint8, x, "z8e")
+    with guard:
+        ws, d.ws_bytes = _workspace(L.lib().nl_linear_workspace(ctypes.byref(d), 0), workspace, x, "nl_linear_forward")
+        d.ws = ws.data_ptr() if ws is not None else None
+        check(L.lib().nl_linear_forward(ctypes.byref(d), stream), "nl_linear_forward")
+    return out
+
+
+def linear_backward(gy, x, weight, act="none", z=None, bits=None, z8=None, z8e=None, x8=None, x8e=None, gx=None, gw=None, gb=None, workspace=None):
+    """gradients of linear_forward: gx [M,K] = dz weight, gw [N,K] = dz^T x (x8 / x8e instead of x: codes of mx8_encode), gb [N] = column sums of dz,
+    dz = gy act'(z); each is written where a tensor is given"""
+    stream, guard = _on_device(gy)
+    if gy.dim() != 2 or weight.dim() != 2:
+        raise L.NerfLoamHipError(f"linear_backward: gy {tuple(gy.shape)} must be [M, N] and weight {tuple(weight.shape)} [N, K]")
+    M, N = gy.shape
+    K = weight.shape[1]
+    d = L.NlLinear(struct_size=ctypes.sizeof(L.NlLinear), dtype=_layer_dtype(gy, "gy"), act=L.NL_ACTS[act], K=K, N=N, M=M)
+    d.gy, d.ldgy = _rows(gy, N, gy, "gy")
+    d.w, d.ldw = _rows(weight, K, gy, "weight")
+    if weight.shape[0] != N or (x is not None and x.shape[0] != M):
+        raise L.NerfLoamHipError(f"linear_backward: gy {tuple(gy.shape)} does not fit weight {tuple(weight.shape)} and x")
+    d.x, d.ldx = _rows(x, K, gy, "x")
+    NB, KB = (N + 31) // 32, (K + 31) // 32
+    d.z = _flat(z, (M, N), gy.dtype, gy, "z")
+    d.bits = _flat(bits, (M, NB), I32, gy, "bits")
+    d.z8 = _flat(z8, (M, 32 * NB), torch.uint8, gy, "z8")
+    d.z8e = _flat(z8e, (M, NB), torch.uint8, gy, "z8e")
+    d.x8 = _flat(x8, (M, 32 * KB), torch.uint8, gy, "x8")
+    d.x8e = _flat(x8e, (M, KB), torch.uint8, gy, "x8e")
+    d.gx = _flat(gx, (M, K), gy.dtype, gy, "gx")
+    d.gw = _flat(gw, (N, K), gy.dtype, gy, "gw")
+    d.gb = _flat(gb, (N,), gy.dtype, gy, "gb")
+    with guard:
+        ws, d.ws_bytes = _workspace(L.lib().nl_linear_workspace(ctypes.byref(d), 1), workspace, gy, "nl_linear_backward")
+        d.ws = ws.data_ptr() if ws is not None else None
+        check(L.lib().nl_linear_backward(ctypes.byref(d), stream), "nl_linear_backward")
+
+
+def mx8_encode(x, codes=None, exps=None):
+    """x [M,K], rows may be strided -> codes uint8 [M, up(K, 32)], exps uint8 [M, ceil(K / 32)] (include/nerfloam_hip.h nl_mx8_encode)"""
+    stream, guard = _on_device(x)
+    if x.dim() != 2:
+        raise L.NerfLoamHipError(f"mx8_encode: x {tuple(x.shape)} must be [M, K]")
+    M, K = x.shape
+    KB = (K + 31) // 32
+    codes = torch.empty(M, 32 * KB, dtype=torch.uint8, device=x.device) if codes is None else codes
+    exps = torch.empty(M, KB, dtype=torch.uint8, device=x.device) if exps is None else exps
+    p, ld = _rows(x, K, x, "x")
+    with guard:
+        check(L.lib().nl_mx8_encode(p, ld, M, K, _layer_dtype(x, "x"), _flat(codes, (M, 32 * KB), torch.uint8, x, "codes"),
+                                    _flat(exps, (M, KB), torch.uint8, x, "exps"), stream), "nl_mx8_encode")
+    return codes, exps
+
+
+def mx8_decode(codes, exps, K, dtype, out=None):
+    """the values the codes stand for, [M,K] of dtype"""
+    stream, guard = _on_device(codes)
+    M, KB = codes.shape[0], (int(K) + 31) // 32
+    out = torch.empty(M, K, dtype=dtype, device=codes.device) if out is None else out
+    with guard:
+        check(L.lib().nl_mx8_decode(_flat(codes, (M, 32 * KB), torch.uint8, codes, "codes"), _flat(exps, (M, KB), torch.uint8, codes, "exps"), M, int(K),
+                                    _layer_dtype(out, "out"), _flat(out, (M, K), dtype, codes, "out"), stream), "nl_mx8_decode")
+    return out
+
+
+def _embedding_args(table, ids, weights):
+    if table.dim() != 2 or ids.dim() != 2 or ids.dtype not in (torch.int32, torch.int64):
+        raise L.NerfLoamHipError(f"embedding: table {tuple(table.shape)} must be [V, D] and ids {tuple(ids.shape)} [M, bag] of int32 or int64, got {ids.dtype}")
+    M, bag = ids.shape
+    return (_flat(table, table.shape, table.dtype, table, "table"), table.shape[0], table.shape[1], _layer_dtype(table, "table"),
+            _flat(ids, ids.shape, ids.dtype, table, "ids"), int(ids.dtype == torch.int64), _flat(weights, (M, bag), F32, table, "weights"), M, bag)
+
+
+def embedding_forward(table, ids, weights=None, scale=1.0, out=None):
+    """out[i] = scale sum_k weights[i,k] table[ids[i,k]]; table [V,D], ids [M,bag] (outside [0, V): no row), weights [M,bag] float32 -> out [M,D]"""
+    stream, guard = _on_device(table)
+    a = _embedding_args(table, ids, weights)
+    out = torch.empty(ids.shape[0], table.shape[1], dtype=table.dtype, device=table.device) if out is None else out
+    with guard:
+        check(L.lib().nl_embedding_forward(*a, float(scale), _flat(out, (ids.shape[0], table.shape[1]), table.dtype, table, "out"), stream),
+              "nl_embedding_forward")
+    return out
+
+
+def embedding_backward(table, ids, g_out, weights=None, scale=1.0, g_table=None, g_weights=None, workspace=None):
+    """gradients of embedding_forward: g_table [V,D] (every row written), g_weights [M,bag] float32, each where a tensor is given; the same bits every run"""
+    stream, guard = _on_device(table)
+    a = _embedding_args(table, ids, weights)
+    M, bag = ids.shape
+    with guard:
+        need = L.lib().nl_embedding_workspace(table.shape[0], table.shape[1], M, bag) if g_table is not None else 0
+        ws, need = _workspace(need, workspace, table, "nl_embedding_backward")
+        check(L.lib().nl_embedding_backward(*a, float(scale), _flat(g_out, (M, table.shape[1]), table.dtype, table, "g_out"),
+                                            _flat(g_table, table.shape, table.dtype, table, "g_table"), _flat(g_weights, (M, bag), F32, table, "g_weights"),
+                                            ws.data_ptr() if ws is not None else None, need, stream), "nl_embedding_backward")
