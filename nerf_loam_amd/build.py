@@ -13,7 +13,8 @@ CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libnerfloam_hip.so")
 SOURCES = ["nl_geometry.hip", "nl_decoder.hip", "nl_field.hip", "nl_optim.hip", "nl_select.hip", "nl_dist.hip", "nl_criterion.hip", "nl_mesh.hip", "nl_linear.hip", "nl_checkpoint.hip", "nl_embedding.hip", "nl_octree.cpp", "nl_iteration.cpp", "nl_exchange.cpp"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-munsafe-fp-atomics",
-         "-Wno-unused-result"]
+         "-Wno-unused-result",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def needs_build():
