@@ -19,10 +19,7 @@ static inline bool nl_dtype_ok(int dt) { return dt == NL_DT_F32 || dt == NL_DT_B
 static inline int nl_dtype_size(int dt) { return dt == NL_DT_F32 ? 4 : 2; }
 static inline long long nl_up(long long a, long long b) { return (a + b - 1) / b * b; }
 
-// operand of a product as it lies in memory: element (i, k) - i the row or column of the result, k the contraction index - at p + i si + k sk.
-// NL_DT_MX8: 8-bit codes, whose power of two is e[k se + i / 32] (the blocks run along i).
-#define NL_DT_MX8 3
-struct NlOperand { const void* p; const unsigned char* e; long long si, sk, se; int type; };
+#define NL_DT_MX8 3                     // 8-bit codes with their powers of two, as an operand of a product
 
 // what happens to an element of the product: y = act(v + b) + r, and what the backward pass keeps of z = v + b
 struct NlEpilogue {
@@ -65,6 +62,25 @@ __device__ __forceinline__ void nl_store4(void* p, long long i, int dt, nl_f32x4
     if (dt == NL_DT_BF16) u = make_ushort4(nl_f2bf(v[0]), nl_f2bf(v[1]), nl_f2bf(v[2]), nl_f2bf(v[3]));
     else u = make_ushort4(nl_f2h(v[0]), nl_f2h(v[1]), nl_f2h(v[2]), nl_f2h(v[3]));
     *reinterpret_cast<ushort4*>((unsigned short*)p + i) = u;
+}
+
+// eight consecutive elements, `left` of them inside the row; aligned: the address is a multiple of 16 bytes wherever n is one of eight elements
+__device__ __forceinline__ void nl_store8(void* p, long long i, int dt, const float* v, int left, bool aligned)
+{
+    if (!aligned || left < 8) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) if (j < left) nl_store_elem(p, i + j, dt, v[j]);
+        return;
+    }
+    if (dt == NL_DT_F32) {
+        *reinterpret_cast<nl_f32x4*>((float*)p + i) = nl_f32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<nl_f32x4*>((float*)p + i + 4) = nl_f32x4{v[4], v[5], v[6], v[7]};
+        return;
+    }
+    nl_s16x8 u;
+#pragma unroll
+    for (int j = 0; j < 8; j++) u[j] = (short)(dt == NL_DT_BF16 ? nl_f2bf(v[j]) : nl_f2h(v[j]));
+    *reinterpret_cast<nl_s16x8*>((unsigned short*)p + i) = u;
 }
 
 // activations and their slopes.  erff, not the tanh form: the exact definition is what a checkpoint or another framework's model was trained with.
@@ -119,95 +135,75 @@ __device__ __forceinline__ nl_f32x4 nl_mx_decode4(unsigned w, float scale, float
 }
 
 // ---- epilogue ----
-// One call: a wave's 16 rows x 32 columns of the result.  Lane l holds, of row m = m0 + (l & 15), the columns n0 + 4 (l >> 4) + 0..3 in a and the same + 16
-// in b (the matrix instruction gets the column operand as its first one: four neighbouring columns of a row per lane, one 8- or 16-byte store each).
-__device__ __forceinline__ void nl_epilogue_pair(const NlEpilogue& ep, nl_f32x4 va, nl_f32x4 vb, long long m0, int n0, long long M, int N, long long split_off)
+// A lane holds eight neighbouring columns n .. n + 7 (n a multiple of 8) of row m of the product; four neighbouring lanes hold 32 columns from a multiple of 32 on.
+// Every lane of a wave calls (rows and columns beyond the result do not store).
+__device__ __forceinline__ void nl_act8(float* v, int act)
 {
-    const int lane = threadIdx.x & 63, g = lane >> 4;
-    const long long m = m0 + (lane & 15);
-    const bool row = m < M;
-    if (n0 >= N) return;                                          // (uniform over the wave)
+    if (act == NL_ACT_NONE) return;
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = nl_act(v[j], act);
+}
+__device__ __forceinline__ void nl_epilogue8(const NlEpilogue& ep, float* v, long long m, int n, long long M, int N, long long split_off)
+{
+    const bool row = m < M, live = row && n < N, whole = n + 7 < N;
+    const int lane = threadIdx.x & 63;
     if (ep.part) {
-        if (!row) return;
+        if (!live) return;
+        float* o = ep.part + split_off + m * N + n;
+        if (whole && (N & 3) == 0) {
+            *reinterpret_cast<nl_f32x4*>(o) = nl_f32x4{v[0], v[1], v[2], v[3]};
+            *reinterpret_cast<nl_f32x4*>(o + 4) = nl_f32x4{v[4], v[5], v[6], v[7]};
+        } else {
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int n = n0 + 16 * h + 4 * g;
-            const nl_f32x4 v = h ? vb : va;
-            float* o = ep.part + split_off + m * N + n;
-            if ((N & 3) == 0 && n < N) *reinterpret_cast<nl_f32x4*>(o) = v;
-            else {
-#pragma unroll
-                for (int j = 0; j < 4; j++) if (n + j < N) o[j] = v[j];
-            }
+            for (int j = 0; j < 8; j++) if (n + j < N) o[j] = v[j];
         }
         return;
     }
-    float z[8];
+    if (ep.b && live) {
+        if (whole && ((uintptr_t)ep.b & (ep.dt == NL_DT_F32 ? 15 : 7)) == 0) {
+            const nl_f32x4 a = nl_load4(ep.b, n, ep.dt), c = nl_load4(ep.b, n + 4, ep.dt);
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        const int n = n0 + 16 * h + 4 * g;
-        const nl_f32x4 v = h ? vb : va;
+            for (int j = 0; j < 4; j++) { v[j] += a[j]; v[4 + j] += c[j]; }
+        } else {
 #pragma unroll
-        for (int j = 0; j < 4; j++) z[4 * h + j] = v[j] + ((ep.b && n + j < N) ? nl_load_elem(ep.b, n + j, ep.dt) : 0.0f);
+            for (int j = 0; j < 8; j++) if (n + j < N) v[j] += nl_load_elem(ep.b, n + j, ep.dt);
+        }
     }
     if (ep.bits) {                                                // one bit per element: z > 0
         unsigned w = 0;
 #pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) w |= (unsigned)(z[4 * h + j] > 0.0f && n0 + 16 * h + 4 * g + j < N) << (16 * h + 4 * g + j);
-        w |= __shfl_xor(w, 16);
-        w |= __shfl_xor(w, 32);
-        if (row && g == 0) ep.bits[m * ep.ldbits + (n0 >> 5)] = w;
+        for (int j = 0; j < 8; j++) w |= (unsigned)(v[j] > 0.0f && n + j < N) << j;
+        w <<= 8 * (lane & 3);
+        w |= __shfl_xor(w, 1);
+        w |= __shfl_xor(w, 2);
+        if (live && (lane & 3) == 0) ep.bits[m * ep.ldbits + (n >> 5)] = w;
     }
-    if (ep.z8) {                                                  // z in 8 bits, from the fp32 values
+    if (ep.z8) {                                                  // z in 8 bits, from the fp32 values; rows of codes are padded to whole blocks with zeros
         float amax = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; j++) amax = fmaxf(amax, n0 + 16 * (j >> 2) + 4 * g + (j & 3) < N ? nl_finite_abs(z[j]) : 0.0f);
-        amax = fmaxf(amax, __shfl_xor(amax, 16));
-        amax = fmaxf(amax, __shfl_xor(amax, 32));
+        for (int j = 0; j < 8; j++) { if (n + j >= N) v[j] = 0.0f; amax = fmaxf(amax, nl_finite_abs(v[j])); }
+        amax = fmaxf(amax, __shfl_xor(amax, 1));
+        amax = fmaxf(amax, __shfl_xor(amax, 2));
         const int e = nl_mx_exponent(amax);
         const float s = nl_pow2(-e);
-        if (row) {
-#pragma unroll
-            for (int h = 0; h < 2; h++) {                         // (rows of codes are padded to whole blocks: always a whole word; columns behind N hold zeros)
-                const int n = n0 + 16 * h + 4 * g;
-                *reinterpret_cast<unsigned*>(ep.z8 + m * ep.ldz8 + n) =
-                    nl_mx_encode4(n < N ? z[4 * h] : 0.0f, n + 1 < N ? z[4 * h + 1] : 0.0f, n + 2 < N ? z[4 * h + 2] : 0.0f, n + 3 < N ? z[4 * h + 3] : 0.0f, s);
-            }
-            if (g == 0) ep.z8e[m * ep.ldz8e + (n0 >> 5)] = (unsigned char)(e + 127);
+        if (row && n < ep.ldz8) {
+            *reinterpret_cast<nl_i32x2*>(ep.z8 + m * ep.ldz8 + n) = nl_i32x2{(int)nl_mx_encode4(v[0], v[1], v[2], v[3], s), (int)nl_mx_encode4(v[4], v[5], v[6], v[7], s)};
+            if ((lane & 3) == 0) ep.z8e[m * ep.ldz8e + (n >> 5)] = (unsigned char)(e + 127);
         }
     }
-    if (!row) return;
-    const int es = ep.dt == NL_DT_F32 ? 16 : 8;                   // bytes of four elements
+    if (!live) return;
+    if (ep.z) nl_store8(ep.z, m * ep.ldz + n, ep.dt, v, N - n, (ep.ldz & 7) == 0);
+    nl_act8(v, ep.act);
+    if (ep.r) {
+        if (whole && (ep.ldr & 3) == 0 && ((uintptr_t)ep.r & (ep.dt == NL_DT_F32 ? 15 : 7)) == 0) {
+            const nl_f32x4 a = nl_load4(ep.r, m * ep.ldr + n, ep.dt), c = nl_load4(ep.r, m * ep.ldr + n + 4, ep.dt);
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        const int n = n0 + 16 * h + 4 * g;
-        if (n >= N) continue;
-        const bool whole = n + 3 < N;
-        if (ep.z) {
-            const nl_f32x4 v = {z[4 * h], z[4 * h + 1], z[4 * h + 2], z[4 * h + 3]};
-            if (whole && (ep.ldz & 3) == 0) nl_store4(ep.z, m * ep.ldz + n, ep.dt, v);
-            else {
+            for (int j = 0; j < 4; j++) { v[j] += a[j]; v[4 + j] += c[j]; }
+        } else {
 #pragma unroll
-                for (int j = 0; j < 4; j++) if (n + j < N) nl_store_elem(ep.z, m * ep.ldz + n + j, ep.dt, v[j]);
-            }
-        }
-        nl_f32x4 o;
-#pragma unroll
-        for (int j = 0; j < 4; j++) o[j] = nl_act(z[4 * h + j], ep.act);
-        if (ep.r) {
-            if (whole && (ep.ldr & 3) == 0 && ((uintptr_t)ep.r & (es - 1)) == 0) o += nl_load4(ep.r, m * ep.ldr + n, ep.dt);
-            else {
-#pragma unroll
-                for (int j = 0; j < 4; j++) if (n + j < N) o[j] += nl_load_elem(ep.r, m * ep.ldr + n + j, ep.dt);
-            }
-        }
-        if (whole && (ep.ldy & 3) == 0 && ((uintptr_t)ep.y & (es - 1)) == 0) nl_store4(ep.y, m * ep.ldy + n, ep.dt, o);
-        else {
-#pragma unroll
-            for (int j = 0; j < 4; j++) if (n + j < N) nl_store_elem(ep.y, m * ep.ldy + n + j, ep.dt, o[j]);
+            for (int j = 0; j < 8; j++) if (n + j < N) v[j] += nl_load_elem(ep.r, m * ep.ldr + n + j, ep.dt);
         }
     }
+    nl_store8(ep.y, m * ep.ldy + n, ep.dt, v, N - n, (ep.ldy & 7) == 0 && ((uintptr_t)ep.y & 15) == 0);
 }
 #endif
