@@ -47,6 +47,28 @@ def build_torch_ext(force=False):
     return SVO_TORCH_OUT
 
 
+LAYERS_TORCH_SRC = os.path.join(HERE, "torch_ext", "layers_torch.cpp")
+LAYERS_TORCH_OUT = os.path.join(HERE, "_layers_torch.so")
+
+
+def build_layers_ext(force=False):
+    """_layers_torch.so: the autograd nodes of nerf_loam_amd.layers (host code only: g++ with the torch headers; the kernels are bound by address at load)"""
+    deps = [LAYERS_TORCH_SRC, os.path.join(HERE, "..", "include", "nerfloam_hip.h")]
+    if not force and os.path.exists(LAYERS_TORCH_OUT) and all(os.path.getmtime(d) <= os.path.getmtime(LAYERS_TORCH_OUT) for d in deps):
+        return LAYERS_TORCH_OUT
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension as ce
+    inc = [f"-I{p}" for p in ce.include_paths()] + ["-I/opt/rocm/include", "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(HERE, "..", "include")]
+    libdir = ce.library_paths()[0]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-w", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_layers_torch",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *inc, LAYERS_TORCH_SRC, "-L" + libdir, "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_hip",
+           "-Wl,-rpath," + libdir, "-o", LAYERS_TORCH_OUT]
+    subprocess.check_call(cmd)
+    return LAYERS_TORCH_OUT
+
+
 def build(force=False, verbose=False):
     if not force and not needs_build():
         return OUT
@@ -74,3 +96,4 @@ def build(force=False, verbose=False):
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose=True))
     print(build_torch_ext(force="--force" in sys.argv))
+    print(build_layers_ext(force="--force" in sys.argv))

@@ -160,20 +160,27 @@ __global__ __launch_bounds__(256) void k_linear_dz(NlDz a)
     a.part[(long long)blockIdx.y * a.N + col] = s;
 }
 
-// gb[n] = sum over the chunks: 32 columns x 8 runs of chunks per workgroup, joined in order
+// gb[n] = sum over the chunks: 16 columns (four to a thread) x 64 runs of neighbouring chunks per workgroup, the runs joined pairwise
 __global__ __launch_bounds__(256) void k_linear_gb(const float* __restrict__ part, int chunks, int N, void* gb, int dt)
 {
-    __shared__ float s_sum[256];
-    const int n = blockIdx.x * 32 + (threadIdx.x & 31), run = threadIdx.x >> 5;
-    const int per = (chunks + 7) / 8, c1 = (run + 1) * per < chunks ? (run + 1) * per : chunks;
-    float s = 0.0f;
-    if (n < N)
-        for (int c = run * per; c < c1; c++) s += part[(long long)c * N + n];
+    __shared__ nl_f32x4 s_sum[256];
+    const int n = blockIdx.x * 16 + 4 * (threadIdx.x & 3), run = threadIdx.x >> 2;
+    const int per = (chunks + 63) / 64, c1 = (run + 1) * per < chunks ? (run + 1) * per : chunks;
+    nl_f32x4 s = {};
+    if (n + 3 < N && (N & 3) == 0)
+        for (int c = run * per; c < c1; c++) s += *reinterpret_cast<const nl_f32x4*>(part + (long long)c * N + n);
+    else
+        for (int c = run * per; c < c1; c++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) if (n + j < N) s[j] += part[(long long)c * N + n + j];
     s_sum[threadIdx.x] = s;
-    __syncthreads();
-    if (run != 0 || n >= N) return;
-    for (int r = 1; r < 8; r++) s += s_sum[threadIdx.x + 32 * r];
-    nl_store_elem(gb, n, dt, s);
+    for (int off = 128; off >= 4; off >>= 1) {
+        __syncthreads();
+        if (threadIdx.x < off) s_sum[threadIdx.x] += s_sum[threadIdx.x + off];
+    }
+    if (run != 0) return;
+#pragma unroll
+    for (int j = 0; j < 4; j++) if (n + j < N) nl_store_elem(gb, n + j, dt, s_sum[threadIdx.x][j]);
 }
 
 __global__ __launch_bounds__(256) void k_linear_zero(unsigned char* p, long long bytes)
@@ -292,7 +299,7 @@ static void nl_backward_run(const NlLinear* d, NlWork& w)
         }
         if (!w.dry) {
             hipLaunchKernelGGL(k_linear_dz, dim3(colblocks, (unsigned)chunks), dim3(256), 0, w.st, a);
-            if (d->gb) hipLaunchKernelGGL(k_linear_gb, dim3((d->N + 31) / 32), dim3(256), 0, w.st, a.part, (int)chunks, d->N, d->gb, d->dtype);
+            if (d->gb) hipLaunchKernelGGL(k_linear_gb, dim3((d->N + 15) / 16), dim3(256), 0, w.st, a.part, (int)chunks, d->N, d->gb, d->dtype);
         }
     }
     NlEpilogue ep = {};

@@ -458,3 +458,9 @@ def test_mixed_types_and_shapes_are_refused():
                 lambda: ops.linear_forward(x, w, b, "relu", bits=torch.empty(8, 2, dtype=torch.int32, device="cuda"))):
         with pytest.raises(RuntimeError):
             bad()
+    for bad, word in ((lambda: layers.linear_act(x, w[:, :7]), "weight"), (lambda: layers.linear_act(x, w, b[:4]), "bias"), (lambda: layers.linear_act(x, w, residual=r[:, :1]), "residual"),
+                      (lambda: layers.linear_act(x[:, :0], w[:, :0]), "elements"), (lambda: layers.checkpoint_encode(x[:, :0]), "checkpoint_encode"),
+                      (lambda: layers.embedding_lookup(x[0], torch.zeros(2, dtype=torch.int64, device="cuda")), "table"),
+                      (lambda: layers.embedding_lookup(x, torch.zeros(2, 3, dtype=torch.int64, device="cuda"), weights=torch.zeros(2, 2, device="cuda")), "weights")):
+        with pytest.raises(ValueError, match=word):
+            bad()
