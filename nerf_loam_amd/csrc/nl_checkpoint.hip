@@ -2,10 +2,11 @@
 #include "nl_layers.h"
 
 // A thread: eight neighbouring elements; four threads share a block of 32 and find its maximum among themselves.
-__global__ __launch_bounds__(256) void k_mx8_encode(const void* x, long long ldx, long long M, int K, int dt, unsigned char* codes, unsigned char* exps, long long pitch)
+template <int DT>
+__global__ __launch_bounds__(256) void k_mx8_encode(const void* __restrict__ x, long long ldx, long long M, int K, unsigned char* codes, unsigned char* exps, long long pitch)
 {
     const long long per_row = pitch / 8, total = M * per_row;
-    const bool row_aligned = (ldx & 3) == 0 && ((uintptr_t)x & (dt == NL_DT_F32 ? 15 : 7)) == 0;
+    const bool row_aligned = nl_rows_aligned<DT>(x, ldx);
     // whole blocks of threads run every round: the four threads of a 32-block stay together
     for (long long t0 = (long long)blockIdx.x * 256; t0 < total; t0 += (long long)gridDim.x * 256) {
         const long long t = t0 + threadIdx.x;
@@ -14,15 +15,7 @@ __global__ __launch_bounds__(256) void k_mx8_encode(const void* x, long long ldx
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) v[j] = 0.0f;
-        if (t < total) {
-            if (row_aligned && k + 7 < K) {
-                const nl_f32x4 a = nl_load4(x, m * ldx + k, dt), b = nl_load4(x, m * ldx + k + 4, dt);
-#pragma unroll
-                for (int j = 0; j < 4; j++) { v[j] = a[j]; v[4 + j] = b[j]; }
-            } else
-#pragma unroll
-                for (int j = 0; j < 8; j++) if (k + j < K) v[j] = nl_load_elem(x, m * ldx + k + j, dt);
-        }
+        if (t < total) nl_load8<DT>(v, x, m * ldx + k, K - k, row_aligned);
         float amax = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; j++) amax = fmaxf(amax, nl_finite_abs(v[j]));
@@ -37,7 +30,8 @@ __global__ __launch_bounds__(256) void k_mx8_encode(const void* x, long long ldx
     }
 }
 
-__global__ __launch_bounds__(256) void k_mx8_decode(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ exps, long long M, int K, int dt, void* out, long long pitch)
+template <int DT>
+__global__ __launch_bounds__(256) void k_mx8_decode(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ exps, long long M, int K, void* __restrict__ out, long long pitch)
 {
     const long long per_row = (K + 7) / 8, total = M * per_row;
     for (long long t = (long long)blockIdx.x * 256 + threadIdx.x; t < total; t += (long long)gridDim.x * 256) {
@@ -45,13 +39,9 @@ __global__ __launch_bounds__(256) void k_mx8_decode(const unsigned char* __restr
         const int k = (int)(t - m * per_row) * 8;
         const nl_i32x2 c = *reinterpret_cast<const nl_i32x2*>(codes + m * pitch + k);
         const float s = nl_mx_scale(exps[m * (pitch / 32) + (k >> 5)]);
-        const nl_f32x4 a = nl_mx_decode4((unsigned)c[0], s, nl_dtype_max(dt)), b = nl_mx_decode4((unsigned)c[1], s, nl_dtype_max(dt));
-        if ((K & 3) == 0) {
-            nl_store4(out, m * K + k, dt, a);
-            if (k + 7 < K) nl_store4(out, m * K + k + 4, dt, b);
-        } else
-#pragma unroll
-            for (int j = 0; j < 8; j++) if (k + j < K) nl_store_elem(out, m * K + k + j, dt, j < 4 ? a[j & 3] : b[j & 3]);
+        const nl_f32x4 a = nl_mx_decode4((unsigned)c[0], s, nl_dtype_max(DT)), b = nl_mx_decode4((unsigned)c[1], s, nl_dtype_max(DT));
+        const float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        nl_store8<DT>(out, m * K + k, v, K - k, nl_rows_aligned<DT>(out, K));
     }
 }
 
@@ -65,7 +55,7 @@ int nl_mx8_encode(const void* x, long long ldx, long long M, int K, int dtype, u
     if (M == 0) return NL_OK;
     if (!x || !codes || !exps || ((uintptr_t)codes & 7) || ((uintptr_t)x & (nl_dtype_size(dtype) - 1))) return NL_ERR_INVALID_ARG;
     const long long pitch = nl_up(K, NL_MX_BLOCK);
-    hipLaunchKernelGGL(k_mx8_encode, dim3(mx_grid(M * (pitch / 8))), dim3(256), 0, (hipStream_t)stream, x, ldx, M, K, dtype, codes, exps, pitch);
+    NL_WITH_DTYPE(dtype, hipLaunchKernelGGL(k_mx8_encode<DT>, dim3(mx_grid(M * (pitch / 8))), dim3(256), 0, (hipStream_t)stream, x, ldx, M, K, codes, exps, pitch));
     NL_LAUNCH_CHECK();
     return NL_OK;
 }
@@ -75,7 +65,7 @@ int nl_mx8_decode(const unsigned char* codes, const unsigned char* exps, long lo
     if (!nl_dtype_ok(dtype) || M < 0 || K < 1) return NL_ERR_INVALID_ARG;
     if (M == 0) return NL_OK;
     if (!codes || !exps || !out || ((uintptr_t)codes & 7) || ((uintptr_t)out & 15)) return NL_ERR_INVALID_ARG;
-    hipLaunchKernelGGL(k_mx8_decode, dim3(mx_grid(M * ((K + 7) / 8))), dim3(256), 0, (hipStream_t)stream, codes, exps, M, K, dtype, out, nl_up(K, NL_MX_BLOCK));
+    NL_WITH_DTYPE(dtype, hipLaunchKernelGGL(k_mx8_decode<DT>, dim3(mx_grid(M * ((K + 7) / 8))), dim3(256), 0, (hipStream_t)stream, codes, exps, M, K, out, nl_up(K, NL_MX_BLOCK)));
     NL_LAUNCH_CHECK();
     return NL_OK;
 }

@@ -2,65 +2,105 @@
 //
 // Reference behaviour: F.embedding of the voxels' corner rows and the weighted sum over the eight corners (/root/reference/src/variations/render_helpers.py:40-89);
 // torch's embedding backward adds with atomics.  Here the lookups are sorted by id (a stable radix sort, eight bits a pass) and a row's gradient is a sum over
-// neighbouring entries in ascending position: pieces of at most EMB_CHUNK entries, the pieces of a row that spans several joined in order, level by level.
+// neighbouring entries in ascending position: pieces of a fixed number of entries, the pieces of a row that spans several joined in order, level by level.
 #include "nl_layers.h"
 
-#define EMB_CHUNK 64            // sorted entries per run-summing group
-#define RS_TILE 2048            // keys per workgroup of a sorting pass: 4 waves x 8 rounds x 64 lanes
+// Entries per run-summing group: at the first level 16 while there are at most EMB_FEW lookups, so that there are enough groups (32768 lookups x 1024 bf16: 31 us,
+// 91 us with 64 entries and one row in flight), else 64; at the later levels, which mostly hold entries without a piece, 128: one level less.
+#define EMB_CHUNK_FIRST 16
+#define EMB_CHUNK_MANY 64
+#define EMB_CHUNK_LATER 128
+#define EMB_FEW 65536
+#define EMB_BATCH 8             // entries whose rows are in flight together, first level
+#define EMB_BATCH_LATER 16      // later levels
+#define RS_TILE 1024            // keys per workgroup of a sorting pass: 4 waves x 4 rounds x 64 lanes
 #define RS_ROUNDS (RS_TILE / 256)
+#define RS_SMALL 4096           // up to here one workgroup sorts everything in LDS: one launch instead of three per pass
 
 __device__ __forceinline__ long long emb_id(const void* ids, int id64, long long i) { return id64 ? ((const long long*)ids)[i] : (long long)((const int*)ids)[i]; }
 
 // VEC neighbouring columns of a row as fp32 (VEC 1, 4, 8; 4 and 8 need D divisible by it)
 template <int VEC> struct EmbVec { float v[VEC]; };
-template <int VEC>
-__device__ __forceinline__ EmbVec<VEC> emb_load(const void* p, long long i, int dt)
+template <int VEC, int DT>
+__device__ __forceinline__ EmbVec<VEC> emb_load(const void* p, long long i)
 {
     EmbVec<VEC> o;
-    if (VEC == 1) { o.v[0] = nl_load_elem(p, i, dt); return o; }
+    if constexpr (VEC == 1) o.v[0] = nl_load_elem<DT>(p, i);
+    else if constexpr (VEC == 8) nl_load8_aligned<DT>(o.v, p, i);
+    else {
+        const nl_f32x4 a = nl_load4<DT>(p, i);
 #pragma unroll
-    for (int h = 0; h < VEC / 4; h++) {
-        const nl_f32x4 a = nl_load4(p, i + 4 * h, dt);
-#pragma unroll
-        for (int j = 0; j < 4; j++) o.v[(4 * h + j) % VEC] = a[j];
+        for (int j = 0; j < 4; j++) o.v[j] = a[j];
     }
     return o;
 }
-template <int VEC>
-__device__ __forceinline__ void emb_store(void* p, long long i, int dt, const EmbVec<VEC>& a)
+template <int VEC, int DT>
+__device__ __forceinline__ void emb_store(void* p, long long i, const EmbVec<VEC>& a)
 {
-    if (VEC == 1) { nl_store_elem(p, i, dt, a.v[0]); return; }
-#pragma unroll
-    for (int h = 0; h < VEC / 4; h++) nl_store4(p, i + 4 * h, dt, nl_f32x4{a.v[4 * h % VEC], a.v[(4 * h + 1) % VEC], a.v[(4 * h + 2) % VEC], a.v[(4 * h + 3) % VEC]});
+    if constexpr (VEC == 1) nl_store_elem<DT>(p, i, a.v[0]);
+    else if constexpr (VEC == 8) nl_store8<DT>(p, i, a.v, 8, true);
+    else nl_store4<DT>(p, i, nl_f32x4{a.v[0], a.v[1], a.v[2], a.v[3]});
 }
 
-// One group of `lanes` threads (a power of two, at most 256) per output row
-template <int VEC>
-__global__ __launch_bounds__(256) void k_emb_forward(const void* __restrict__ table, long long V, int D, int dt, const void* __restrict__ ids, int id64,
+// One group of `lanes` threads (a power of two, at most 256) per output row.  The ids of a bag are read BAG at a time and their rows fetched together: what bounds
+// a small row is the way id -> row, once per batch instead of once per lookup.
+template <int DT, int VEC, int BAG>
+__global__ __launch_bounds__(256) void k_emb_forward(const void* __restrict__ table, long long V, int D, const void* __restrict__ ids, int id64,
                                                      const float* __restrict__ weights, long long M, int bag, float scale, void* __restrict__ out, int lanes)
 {
     const int per = 256 / lanes, grp = threadIdx.x / lanes;
     const long long m = (long long)blockIdx.x * per + grp;
     if (m >= M) return;
+    const bool ids32 = !id64 && ((uintptr_t)ids & 15) == 0 && ((uintptr_t)weights & 15) == 0;
     for (int d = (threadIdx.x & (lanes - 1)) * VEC; d < D; d += lanes * VEC) {
         EmbVec<VEC> acc = {};
-        for (int k = 0; k < bag; k++) {
-            const long long id = emb_id(ids, id64, m * bag + k);
-            if (id < 0 || id >= V) continue;
-            const float w = weights ? weights[m * bag + k] : 1.0f;
-            const EmbVec<VEC> r = emb_load<VEC>(table, id * D + d, dt);
+        for (int k0 = 0; k0 < bag; k0 += BAG) {
+            long long id[BAG];
+            float w[BAG];
+            EmbVec<VEC> r[BAG];
+            if (BAG == 8 && bag == 8 && ids32) {                      // a row of eight 32-bit ids and weights: two 16-byte loads each
+                const nl_i32x4 a = reinterpret_cast<const nl_i32x4*>(ids)[2 * m], b = reinterpret_cast<const nl_i32x4*>(ids)[2 * m + 1];
+                const nl_f32x4 p = weights ? reinterpret_cast<const nl_f32x4*>(weights)[2 * m] : nl_f32x4{1, 1, 1, 1};
+                const nl_f32x4 q = weights ? reinterpret_cast<const nl_f32x4*>(weights)[2 * m + 1] : nl_f32x4{1, 1, 1, 1};
 #pragma unroll
-            for (int j = 0; j < VEC; j++) acc.v[j] += w * r.v[j];
+                for (int k = 0; k < BAG; k++) { id[k] = k < 4 ? a[k & 3] : b[k & 3]; w[k] = k < 4 ? p[k & 3] : q[k & 3]; }
+            } else
+#pragma unroll
+            for (int k = 0; k < BAG; k++) {
+                const bool in = k0 + k < bag;
+                id[k] = in ? emb_id(ids, id64, m * bag + k0 + k) : -1;
+                w[k] = in && weights ? weights[m * bag + k0 + k] : 1.0f;
+            }
+#pragma unroll
+            for (int k = 0; k < BAG; k++) {
+                const bool in = id[k] >= 0 && id[k] < V;
+                r[k] = emb_load<VEC, DT>(table, (in ? id[k] : 0) * D + d);
+                if (!in) {                                            // no row: its place in memory may hold anything
+#pragma unroll
+                    for (int j = 0; j < VEC; j++) r[k].v[j] = 0.0f;
+                    w[k] = 0.0f;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < BAG; k++)
+#pragma unroll
+                for (int j = 0; j < VEC; j++) acc.v[j] += w[k] * r[k].v[j];
         }
 #pragma unroll
         for (int j = 0; j < VEC; j++) acc.v[j] *= scale;
-        emb_store<VEC>(out, m * D + d, dt, acc);
+        emb_store<VEC, DT>(out, m * D + d, acc);
     }
+}
+template <int VEC> static void emb_forward(dim3 grid, hipStream_t st, const void* table, long long V, int D, int dt, const void* ids, int id64, const float* weights, long long M, int bag,
+                                           float scale, void* out, int lanes)
+{
+    NL_WITH_DTYPE(dt, if (bag == 1) hipLaunchKernelGGL((k_emb_forward<DT, VEC, 1>), grid, dim3(256), 0, st, table, V, D, ids, id64, weights, M, bag, scale, out, lanes);
+                      else hipLaunchKernelGGL((k_emb_forward<DT, VEC, 8>), grid, dim3(256), 0, st, table, V, D, ids, id64, weights, M, bag, scale, out, lanes));
 }
 
 // g_weights[i,k] = scale <g[i], table[ids[i,k]]>: one group of at most 64 lanes per lookup
-template <int VEC>
-__global__ __launch_bounds__(256) void k_emb_gweights(const void* __restrict__ table, long long V, int D, int dt, const void* __restrict__ ids, int id64, long long L,
+template <int DT, int VEC>
+__global__ __launch_bounds__(256) void k_emb_gweights(const void* __restrict__ table, long long V, int D, const void* __restrict__ ids, int id64, long long L,
                                                       int bag, float scale, const void* __restrict__ g, float* __restrict__ gw, int lanes)
 {
     const int per = 256 / lanes, grp = threadIdx.x / lanes;
@@ -70,7 +110,7 @@ __global__ __launch_bounds__(256) void k_emb_gweights(const void* __restrict__ t
     float s = 0.0f;
     if (id >= 0 && id < V)
         for (int d = (threadIdx.x & (lanes - 1)) * VEC; d < D; d += lanes * VEC) {
-            const EmbVec<VEC> a = emb_load<VEC>(g, (i / bag) * D + d, dt), b = emb_load<VEC>(table, id * D + d, dt);
+            const EmbVec<VEC> a = emb_load<VEC, DT>(g, (i / bag) * D + d), b = emb_load<VEC, DT>(table, id * D + d);
 #pragma unroll
             for (int j = 0; j < VEC; j++) s += a.v[j] * b.v[j];
         }
@@ -87,7 +127,15 @@ struct RsArgs {
     int* hist;                                         // [256][nblk], then its exclusive sums along a row
     int* totals;                                       // [256]
     int L, nblk, shift;
+    unsigned* zero; long long zero_words;              // first pass: the launch's workgroups behind the sorting ones clear these (the gradient's rows)
 };
+__device__ __forceinline__ bool rs_zero(const RsArgs& a, int sorting)
+{
+    if ((int)blockIdx.x < sorting) return false;
+    const long long step = (long long)(gridDim.x - sorting) * blockDim.x;
+    for (long long i = (long long)(blockIdx.x - sorting) * blockDim.x + threadIdx.x; i < a.zero_words; i += step) a.zero[i] = 0;
+    return true;
+}
 __device__ __forceinline__ unsigned rs_key(const RsArgs& a, int i)
 {
     if (!a.ids) return a.keys[i];
@@ -97,6 +145,7 @@ __device__ __forceinline__ unsigned rs_key(const RsArgs& a, int i)
 __global__ __launch_bounds__(256) void k_rs_hist(RsArgs a)
 {
     __shared__ int s_h[256];
+    if (rs_zero(a, a.nblk)) return;
     s_h[threadIdx.x] = 0;
     __syncthreads();
     const int base = blockIdx.x * RS_TILE;
@@ -112,6 +161,7 @@ __global__ __launch_bounds__(256) void k_rs_hist(RsArgs a)
 __global__ __launch_bounds__(256) void k_rs_scan(RsArgs a)
 {
     __shared__ int s_w[4];
+    if (rs_zero(a, 256)) return;
     int* row = a.hist + (long long)blockIdx.x * a.nblk;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int run = 0;
@@ -134,6 +184,7 @@ __global__ __launch_bounds__(256) void k_rs_scan(RsArgs a)
 __global__ __launch_bounds__(256) void k_rs_scatter(RsArgs a)
 {
     __shared__ int s_cnt[4][256], s_base[256], s_w[4];
+    if (rs_zero(a, a.nblk)) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d0 = threadIdx.x;
     // where the digit begins: sums of the totals in front of it
     {
@@ -183,69 +234,156 @@ __global__ __launch_bounds__(256) void k_rs_scatter(RsArgs a)
     }
 }
 
+// All passes of at most RS_SMALL keys by one workgroup of 16 waves, keys and positions in LDS
+__global__ __launch_bounds__(1024) void k_rs_small(RsArgs a, int passes)
+{
+    constexpr int R = RS_SMALL / 1024;
+    __shared__ unsigned s_key[RS_SMALL], s_pos[RS_SMALL];
+    __shared__ int s_cnt[16][256], s_w[4];
+    if (rs_zero(a, 1)) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, first = wave * (64 * R);
+    unsigned key[R], pos[R], rank[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const int i = first + r * 64 + lane;
+        key[r] = i < a.L ? rs_key(a, i) : 0; pos[r] = i;
+    }
+    for (int p = 0; p < passes; p++) {
+        const int shift = 8 * p;
+        for (int i = threadIdx.x; i < 16 * 256; i += 1024) s_cnt[0][i] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const bool in = first + r * 64 + lane < a.L;
+            const unsigned d = key[r] >> shift & 255;
+            unsigned long long same = __ballot(in);
+#pragma unroll
+            for (int b = 0; b < 8; b++) { const unsigned long long m = __ballot(d >> b & 1); same &= (d >> b & 1) ? m : ~m; }
+            const unsigned long long below = same & ((1ull << lane) - 1);
+            const int seen = s_cnt[wave][d];
+            rank[r] = seen + __popcll(below);
+            __builtin_amdgcn_wave_barrier();
+            if (in && below == 0) s_cnt[wave][d] = seen + __popcll(same);
+            __builtin_amdgcn_wave_barrier();
+        }
+        __syncthreads();
+        int total = 0, incl = 0;
+        if (threadIdx.x < 256) {
+            for (int w = 0; w < 16; w++) total += s_cnt[w][threadIdx.x];
+            incl = total;
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) { const int t = __shfl_up(incl, off); if (lane >= off) incl += t; }
+            if (lane == 63) s_w[wave] = incl;
+        }
+        __syncthreads();
+        if (threadIdx.x < 256) {
+            int before = incl - total;
+            for (int w = 0; w < wave; w++) before += s_w[w];
+            for (int w = 0; w < 16; w++) { const int c = s_cnt[w][threadIdx.x]; s_cnt[w][threadIdx.x] = before; before += c; }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < R; r++)
+            if (first + r * 64 + lane < a.L) {
+                const unsigned to = s_cnt[wave][key[r] >> shift & 255] + rank[r];
+                s_key[to] = key[r]; s_pos[to] = pos[r];
+            }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const int i = first + r * 64 + lane;
+            if (i < a.L) { key[r] = s_key[i]; pos[r] = s_pos[i]; }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const int i = first + r * 64 + lane;
+        if (i < a.L) { a.out_keys[i] = key[r]; a.out_pos[i] = pos[r]; }
+    }
+}
+
 // ---- sums of neighbouring entries with one key ----
 // A group of `lanes` threads walks one chunk of the sorted list.  A run of equal keys that begins and ends inside the chunk is a finished row of the gradient;
 // a run that touches a chunk border which the row crosses becomes a piece.  Every chunk leaves two entries for the next level, its first and its last run's key
 // (a chunk of one run: the same key twice), each with a flag that says whether a piece stands behind it: the keys of the next level are sorted again.
+// What bounds it is the way position -> row: EMB_BATCH entries' keys and positions are read together, then their rows.
 struct EmbSum {
     const unsigned* keys; const unsigned char* any;    // any: null at level 0 (every entry counts)
     const unsigned* pos; const void* g; const float* weights;      // level 0: rows of the output gradient
     const float* piece;                                // later levels
     unsigned* out_keys; unsigned char* out_any; float* out_piece;  // null: this level is the last one
     void* g_table; long long V;
-    int L, D, dt, bag; float scale;
+    int L, D, bag, chunk; float scale;
 };
-template <int VEC, bool LEVEL0>
+template <int DT, int VEC, bool LEVEL0>
 __global__ __launch_bounds__(256) void k_emb_sum(EmbSum a, int lanes)
 {
     const int per = 256 / lanes, chunk = (int)(blockIdx.x * per + threadIdx.x / lanes);
-    const int s = chunk * EMB_CHUNK;
-    if (s >= a.L) return;
-    const int e = s + EMB_CHUNK < a.L ? s + EMB_CHUNK : a.L;
+    const long long s0 = (long long)chunk * a.chunk;
+    if (s0 >= a.L) return;
+    const int s = (int)s0, e = s + a.chunk < a.L ? s + a.chunk : a.L;
     const int d = (int)(blockIdx.y * lanes + (threadIdx.x & (lanes - 1))) * VEC;
     const bool lead = d == 0, col = d < a.D;
     const unsigned k_first = a.keys[s], k_last = a.keys[e - 1];
     const bool open_l = s > 0 && a.keys[s - 1] == k_first, open_r = e < a.L && a.keys[e] == k_last;
     EmbVec<VEC> acc = {};
-    bool some = false, any0 = false, any1 = false;
+    bool some = false, any0 = false, any1 = false, in_first = true;
     unsigned cur = k_first;
-    bool in_first = true;
-    for (int j = s; j <= e; j++) {
-        const unsigned k = j < e ? a.keys[j] : ~0u;
-        if (k != cur) {
-            // the run of `cur` ends at j
-            const bool cut = (in_first && open_l) || (j == e && open_r);
-            if (some && cur < a.V) {
-                if (!cut) { if (col) emb_store<VEC>(a.g_table, (long long)cur * a.D + d, a.dt, acc); }
-                else {
-                    const int slot = in_first ? 0 : 1;
-                    if (in_first) any0 = true; else any1 = true;
-                    if (col) {
-                        float* o = a.out_piece + (2LL * chunk + slot) * a.D + d;
+    // the run of `cur` ends, at the chunk's end or before it
+    auto flush = [&](bool at_end) {
+        if (!some || cur >= a.V) return;
+        if (!((in_first && open_l) || (at_end && open_r))) { if (col) emb_store<VEC, DT>(a.g_table, (long long)cur * a.D + d, acc); return; }
+        const int slot = in_first ? 0 : 1;
+        if (in_first) any0 = true; else any1 = true;
+        if (!col) return;
+        float* o = a.out_piece + (2LL * chunk + slot) * a.D + d;
 #pragma unroll
-                        for (int q = 0; q < VEC; q++) o[q] = acc.v[q];
-                    }
-                }
-            }
-            if (j == e) break;
-            acc = EmbVec<VEC>{};
-            some = false; in_first = false; cur = k;
+        for (int q = 0; q < VEC; q++) o[q] = acc.v[q];
+    };
+    constexpr int B = LEVEL0 ? EMB_BATCH : EMB_BATCH_LATER;
+    unsigned nkey[B], np[B];
+    bool nlive[B];
+    auto look = [&](int j0) {                                         // keys and positions of the next batch
+#pragma unroll
+        for (int b = 0; b < B; b++) {
+            const int j = j0 + b < e ? j0 + b : e - 1;
+            nkey[b] = a.keys[j];
+            np[b] = LEVEL0 ? a.pos[j] : (unsigned)j;
+            nlive[b] = j0 + b < e && (LEVEL0 || a.any[j]);
         }
-        if (!LEVEL0 && !a.any[j]) continue;
-        some = true;
-        if (!col || cur >= a.V) continue;
-        if (LEVEL0) {
-            const unsigned p = a.pos[j];
-            const EmbVec<VEC> r = emb_load<VEC>(a.g, (long long)(p / (unsigned)a.bag) * a.D + d, a.dt);
-            const float w = a.weights ? a.scale * a.weights[p] : a.scale;
+    };
+    look(s);
+    for (int j0 = s; j0 < e; j0 += B) {
+        unsigned key[B], p[B];
+        bool live[B];
+        float w[B];
+        EmbVec<VEC> r[B];
 #pragma unroll
-            for (int q = 0; q < VEC; q++) acc.v[q] += w * r.v[q];
-        } else {
-            const float* r = a.piece + (long long)j * a.D + d;
+        for (int b = 0; b < B; b++) { key[b] = nkey[b]; p[b] = np[b]; live[b] = nlive[b]; }
 #pragma unroll
-            for (int q = 0; q < VEC; q++) acc.v[q] += r[q];
+        for (int b = 0; b < B; b++) {
+            w[b] = LEVEL0 && a.weights ? a.scale * a.weights[p[b]] : a.scale;
+            // always loaded, used where the entry counts (a load under a condition is waited for where the branch ends: one row in flight)
+            if (LEVEL0) r[b] = emb_load<VEC, DT>(a.g, (long long)(p[b] / (unsigned)a.bag) * a.D + (col ? d : 0));
+            else r[b] = emb_load<VEC, NL_DT_F32>(a.piece, (long long)p[b] * a.D + (col ? d : 0));
+        }
+        if (j0 + B < e) look(j0 + B);
+#pragma unroll
+        for (int b = 0; b < B; b++) {
+            if (j0 + b >= e) break;
+            if (key[b] != cur) {
+                flush(false);
+                acc = EmbVec<VEC>{};
+                some = false; in_first = false; cur = key[b];
+            }
+            if (!live[b]) continue;
+            some = true;
+            if (col && cur < a.V)
+#pragma unroll
+                for (int q = 0; q < VEC; q++) acc.v[q] += LEVEL0 ? w[b] * r[b].v[q] : r[b].v[q];
         }
     }
+    flush(true);
     if (lead && a.out_keys) {
         a.out_keys[2 * chunk] = k_first; a.out_keys[2 * chunk + 1] = k_last;
         a.out_any[2 * chunk] = any0; a.out_any[2 * chunk + 1] = any1;
@@ -260,7 +398,7 @@ __global__ void k_emb_zero_tail(unsigned short* p) { *p = 0; }
 
 // ---- host ----
 #define EMB_MAX_LOOKUPS 0x7FFF0000LL
-struct EmbPlan { int L, nblk, passes, levels; long long keys, hist, key_l[2], any_l[2], piece_l[2], total; };
+struct EmbPlan { int L, nblk, passes, levels, first; long long keys, hist, key_l[2], any_l[2], piece_l[2], total; };
 static EmbPlan emb_plan(long long V, int D, long long L)
 {
     EmbPlan p = {};
@@ -271,8 +409,9 @@ static EmbPlan emb_plan(long long V, int D, long long L)
     p.keys = nl_up(4 * L, 256);
     p.hist = nl_up(4LL * 256 * p.nblk + 1024, 256);
     p.total = 4 * p.keys + p.hist;
-    for (long long n = L; n > EMB_CHUNK;) {                                    // two entries per chunk for the next level; levels take two buffers in turn
-        n = 2 * ((n + EMB_CHUNK - 1) / EMB_CHUNK);
+    p.first = L <= EMB_FEW ? EMB_CHUNK_FIRST : EMB_CHUNK_MANY;
+    for (long long n = L, c = p.first; n > c; c = EMB_CHUNK_LATER) {                 // two entries per chunk for the next level; levels take two buffers in turn
+        n = 2 * ((n + c - 1) / c);
         if (p.levels < 2) {
             const int i = p.levels;
             p.key_l[i] = nl_up(4 * n, 256); p.any_l[i] = nl_up(n, 256); p.piece_l[i] = nl_up(4 * n * D, 256);
@@ -291,7 +430,7 @@ static int emb_lanes(int D, int vec, int most)
 static int emb_vec(int D, int dt, const void* a, const void* b)
 {
     const uintptr_t m = (uintptr_t)a | (uintptr_t)b;
-    if (dt != NL_DT_F32 && (D & 7) == 0 && (m & 7) == 0) return 8;
+    if (dt != NL_DT_F32 && (D & 7) == 0 && (m & 15) == 0) return 8;
     if ((D & 3) == 0 && (m & (dt == NL_DT_F32 ? 15 : 7)) == 0) return 4;
     return 1;
 }
@@ -302,12 +441,17 @@ static int emb_check(const void* table, long long V, int D, int dtype, const voi
     if ((uintptr_t)table & (nl_dtype_size(dtype) - 1)) return NL_ERR_INVALID_ARG;
     return NL_OK;
 }
-template <int VEC> static void emb_level(const EmbSum& a, bool level0, hipStream_t st)
+static unsigned emb_zero_blocks(long long words, int threads)
 {
-    const int lanes = emb_lanes(a.D, VEC, 256), per = 256 / lanes, chunks = (a.L + EMB_CHUNK - 1) / EMB_CHUNK;
+    const long long b = (words + 8LL * threads - 1) / (8LL * threads);
+    return (unsigned)(b < 2048 ? b : 2048);
+}
+template <int VEC> static void emb_level(const EmbSum& a, int dt, bool level0, hipStream_t st)
+{
+    const int lanes = emb_lanes(a.D, VEC, 256), per = 256 / lanes, chunks = (a.L + a.chunk - 1) / a.chunk;
     const dim3 grid((chunks + per - 1) / per, (a.D + lanes * VEC - 1) / (lanes * VEC));
-    if (level0) hipLaunchKernelGGL((k_emb_sum<VEC, true>), grid, dim3(256), 0, st, a, lanes);
-    else hipLaunchKernelGGL((k_emb_sum<VEC, false>), grid, dim3(256), 0, st, a, lanes);
+    NL_WITH_DTYPE(dt, if (level0) hipLaunchKernelGGL((k_emb_sum<DT, VEC, true>), grid, dim3(256), 0, st, a, lanes);
+                      else hipLaunchKernelGGL((k_emb_sum<DT, VEC, false>), grid, dim3(256), 0, st, a, lanes));
 }
 
 extern "C" {
@@ -327,9 +471,9 @@ int nl_embedding_forward(const void* table, long long V, int D, int dtype, const
     hipStream_t st = (hipStream_t)stream;
     const int vec = emb_vec(D, dtype, table, out), lanes = emb_lanes(D, vec, 256), per = 256 / lanes;
     const dim3 grid((unsigned)((M + per - 1) / per));
-    if (vec == 8) hipLaunchKernelGGL(k_emb_forward<8>, grid, dim3(256), 0, st, table, V, D, dtype, ids, id64, weights, M, bag, scale, out, lanes);
-    else if (vec == 4) hipLaunchKernelGGL(k_emb_forward<4>, grid, dim3(256), 0, st, table, V, D, dtype, ids, id64, weights, M, bag, scale, out, lanes);
-    else hipLaunchKernelGGL(k_emb_forward<1>, grid, dim3(256), 0, st, table, V, D, dtype, ids, id64, weights, M, bag, scale, out, lanes);
+    if (vec == 8) emb_forward<8>(grid, st, table, V, D, dtype, ids, id64, weights, M, bag, scale, out, lanes);
+    else if (vec == 4) emb_forward<4>(grid, st, table, V, D, dtype, ids, id64, weights, M, bag, scale, out, lanes);
+    else emb_forward<1>(grid, st, table, V, D, dtype, ids, id64, weights, M, bag, scale, out, lanes);
     NL_LAUNCH_CHECK();
     return NL_OK;
 }
@@ -346,15 +490,18 @@ int nl_embedding_backward(const void* table, long long V, int D, int dtype, cons
     if (g_weights && M > 0) {
         const int vec = emb_vec(D, dtype, table, g_out), lanes = emb_lanes(D, vec, 64), per = 256 / lanes;
         const dim3 grid((unsigned)((L + per - 1) / per));
-        if (vec == 8) hipLaunchKernelGGL(k_emb_gweights<8>, grid, dim3(256), 0, st, table, V, D, dtype, ids, id64, L, bag, scale, g_out, g_weights, lanes);
-        else if (vec == 4) hipLaunchKernelGGL(k_emb_gweights<4>, grid, dim3(256), 0, st, table, V, D, dtype, ids, id64, L, bag, scale, g_out, g_weights, lanes);
-        else hipLaunchKernelGGL(k_emb_gweights<1>, grid, dim3(256), 0, st, table, V, D, dtype, ids, id64, L, bag, scale, g_out, g_weights, lanes);
+        if (vec == 8) NL_WITH_DTYPE(dtype, hipLaunchKernelGGL((k_emb_gweights<DT, 8>), grid, dim3(256), 0, st, table, V, D, ids, id64, L, bag, scale, g_out, g_weights, lanes));
+        else if (vec == 4) NL_WITH_DTYPE(dtype, hipLaunchKernelGGL((k_emb_gweights<DT, 4>), grid, dim3(256), 0, st, table, V, D, ids, id64, L, bag, scale, g_out, g_weights, lanes));
+        else NL_WITH_DTYPE(dtype, hipLaunchKernelGGL((k_emb_gweights<DT, 1>), grid, dim3(256), 0, st, table, V, D, ids, id64, L, bag, scale, g_out, g_weights, lanes));
     }
     if (!g_table) { NL_LAUNCH_CHECK(); return NL_OK; }
     const long long bytes = V * D * nl_dtype_size(dtype);
-    hipLaunchKernelGGL(k_emb_zero, dim3((unsigned)(bytes / 4 < 256 * 2048 ? bytes / 1024 + 1 : 2048)), dim3(256), 0, st, (unsigned*)g_table, bytes / 4);
     if (bytes & 3) hipLaunchKernelGGL(k_emb_zero_tail, dim3(1), dim3(1), 0, st, (unsigned short*)((char*)g_table + bytes - 2));
-    if (M == 0) { NL_LAUNCH_CHECK(); return NL_OK; }
+    if (M == 0) {
+        hipLaunchKernelGGL(k_emb_zero, dim3((unsigned)(bytes / 4 < 256 * 2048 ? bytes / 1024 + 1 : 2048)), dim3(256), 0, st, (unsigned*)g_table, bytes / 4);
+        NL_LAUNCH_CHECK();
+        return NL_OK;
+    }
     const EmbPlan p = emb_plan(V, D, L);
     if (!ws || ws_bytes < p.total || ((uintptr_t)ws & 255)) return NL_ERR_INVALID_ARG;
     char* w = (char*)ws;
@@ -364,13 +511,25 @@ int nl_embedding_backward(const void* table, long long V, int D, int dtype, cons
     RsArgs r = {};
     r.totals = (int*)w; r.hist = (int*)(w + 1024); r.L = p.L; r.nblk = p.nblk; r.V = V;
     w += p.hist;
-    for (int i = 0; i < p.passes; i++) {
-        r.ids = i == 0 ? ids : nullptr; r.id64 = id64; r.shift = 8 * i;
-        r.keys = keys[(i + 1) & 1]; r.pos = pos[(i + 1) & 1]; r.out_keys = keys[i & 1]; r.out_pos = pos[i & 1];
-        hipLaunchKernelGGL(k_rs_hist, dim3(p.nblk), dim3(256), 0, st, r);
-        hipLaunchKernelGGL(k_rs_scan, dim3(256), dim3(256), 0, st, r);
-        hipLaunchKernelGGL(k_rs_scatter, dim3(p.nblk), dim3(256), 0, st, r);
-    }
+    // the gradient's rows are cleared beside the first sorting pass, a third of them by each of its launches
+    const long long words = bytes / 4, third = p.L <= RS_SMALL ? words : (words / 3 + 63) / 64 * 64;
+    if (p.L <= RS_SMALL) {
+        r.ids = ids; r.id64 = id64; r.out_keys = keys[(p.passes - 1) & 1]; r.out_pos = pos[(p.passes - 1) & 1];
+        r.zero = (unsigned*)g_table; r.zero_words = words;
+        hipLaunchKernelGGL(k_rs_small, dim3(1 + emb_zero_blocks(words, 1024)), dim3(1024), 0, st, r, p.passes);
+    } else
+        for (int i = 0; i < p.passes; i++) {
+            r.ids = i == 0 ? ids : nullptr; r.id64 = id64; r.shift = 8 * i;
+            r.keys = keys[(i + 1) & 1]; r.pos = pos[(i + 1) & 1]; r.out_keys = keys[i & 1]; r.out_pos = pos[i & 1];
+            for (int k = 0; k < 3; k++) {
+                const long long z0 = k * third < words ? k * third : words, z1 = k == 2 ? words : (k + 1) * third < words ? (k + 1) * third : words;
+                r.zero = (unsigned*)g_table + z0; r.zero_words = i == 0 ? z1 - z0 : 0;
+                const dim3 grid((k == 1 ? 256 : p.nblk) + emb_zero_blocks(r.zero_words, 256));
+                if (k == 0) hipLaunchKernelGGL(k_rs_hist, grid, dim3(256), 0, st, r);
+                else if (k == 1) hipLaunchKernelGGL(k_rs_scan, grid, dim3(256), 0, st, r);
+                else hipLaunchKernelGGL(k_rs_scatter, grid, dim3(256), 0, st, r);
+            }
+        }
     unsigned* lk[2]; unsigned char* la[2]; float* lp[2];
     for (int i = 0; i < 2; i++) {
         lk[i] = (unsigned*)w; la[i] = (unsigned char*)(w + p.key_l[i]); lp[i] = (float*)(w + p.key_l[i] + p.any_l[i]);
@@ -378,16 +537,17 @@ int nl_embedding_backward(const void* table, long long V, int D, int dtype, cons
     }
     const int vec = emb_vec(D, dtype, g_out, g_table);
     EmbSum a = {};
-    a.keys = keys[(p.passes - 1) & 1]; a.pos = pos[(p.passes - 1) & 1]; a.g = g_out; a.weights = weights; a.g_table = g_table; a.V = V; a.L = p.L; a.D = D; a.dt = dtype;
-    a.bag = bag; a.scale = scale;
+    a.keys = keys[(p.passes - 1) & 1]; a.pos = pos[(p.passes - 1) & 1]; a.g = g_out; a.weights = weights; a.g_table = g_table; a.V = V; a.L = p.L; a.D = D;
+    a.bag = bag; a.scale = scale; a.chunk = p.first;
     for (int lev = 0; lev <= p.levels; lev++) {
         const bool last = lev == p.levels;
         a.out_keys = last ? nullptr : lk[lev & 1]; a.out_any = last ? nullptr : la[lev & 1]; a.out_piece = last ? nullptr : lp[lev & 1];
-        if (vec == 8) emb_level<8>(a, lev == 0, st);
-        else if (vec == 4) emb_level<4>(a, lev == 0, st);
-        else emb_level<1>(a, lev == 0, st);
+        if (vec == 8) emb_level<8>(a, dtype, lev == 0, st);
+        else if (vec == 4) emb_level<4>(a, dtype, lev == 0, st);
+        else emb_level<1>(a, dtype, lev == 0, st);
         a.keys = a.out_keys; a.any = a.out_any; a.piece = a.out_piece; a.pos = nullptr;
-        a.L = 2 * ((a.L + EMB_CHUNK - 1) / EMB_CHUNK);
+        a.L = 2 * ((a.L + a.chunk - 1) / a.chunk);
+        a.chunk = EMB_CHUNK_LATER;
     }
     NL_LAUNCH_CHECK();
     return NL_OK;

@@ -100,6 +100,7 @@ struct GemmSide {
 template <class T, bool PLANES, bool A_SLOW, bool B_SLOW, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
 {
+    constexpr int DT = PLANES ? NL_DT_F32 : __is_same(T, _Float16) ? NL_DT_F16 : NL_DT_BF16;
     constexpr int NT = 64 * WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
     typedef GemmSide<A_SLOW, BM, NT> SA;
     typedef GemmSide<B_SLOW, BN, NT> SB;
@@ -171,7 +172,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
             const nl_f32x4 p = *reinterpret_cast<const nl_f32x4*>(mine + r * (WC * 4) + (c ^ (r & CX)) * 16);
             const nl_f32x4 q = *reinterpret_cast<const nl_f32x4*>(mine + r * (WC * 4) + ((c + 1) ^ (r & CX)) * 16);
             float v[8] = {p[0], p[1], p[2], p[3], q[0], q[1], q[2], q[3]};
-            nl_epilogue8(g.ep, v, m0 + wm + half * RP + r, n0 + wn + 4 * c, g.M, g.N, (long long)blockIdx.y * g.M * g.N);
+            nl_epilogue8<DT>(g.ep, v, m0 + wm + half * RP + r, n0 + wn + 4 * c, g.M, g.N, (long long)blockIdx.y * g.M * g.N);
         }
         __builtin_amdgcn_wave_barrier();
     }

@@ -36,52 +36,76 @@ __device__ __forceinline__ unsigned short nl_f2bf(float v) { return __builtin_bi
 __device__ __forceinline__ float nl_h2f(unsigned short v) { return (float)__builtin_bit_cast(_Float16, v); }
 __device__ __forceinline__ unsigned short nl_f2h(float v) { return __builtin_bit_cast(unsigned short, (_Float16)v); }
 
-__device__ __forceinline__ float nl_load_elem(const void* p, long long i, int dt)
+// Elements of a type that is known at compile time (DT: NL_DT_*).  A type looked up at run time puts every load into a branch of its own, and a branch's end waits for
+// what it loaded: one access in flight.
+template <int DT> __device__ __forceinline__ float nl_load_elem(const void* p, long long i)
 {
-    if (dt == NL_DT_F32) return ((const float*)p)[i];
+    if (DT == NL_DT_F32) return ((const float*)p)[i];
     const unsigned short v = ((const unsigned short*)p)[i];
-    return dt == NL_DT_BF16 ? nl_bf2f(v) : nl_h2f(v);
+    return DT == NL_DT_BF16 ? nl_bf2f(v) : nl_h2f(v);
 }
-__device__ __forceinline__ void nl_store_elem(void* p, long long i, int dt, float v)
+template <int DT> __device__ __forceinline__ void nl_store_elem(void* p, long long i, float v)
 {
-    if (dt == NL_DT_F32) ((float*)p)[i] = v;
-    else ((unsigned short*)p)[i] = dt == NL_DT_BF16 ? nl_f2bf(v) : nl_f2h(v);
+    if (DT == NL_DT_F32) ((float*)p)[i] = v;
+    else ((unsigned short*)p)[i] = DT == NL_DT_BF16 ? nl_f2bf(v) : nl_f2h(v);
 }
 // four consecutive elements, aligned to four elements
-__device__ __forceinline__ nl_f32x4 nl_load4(const void* p, long long i, int dt)
+template <int DT> __device__ __forceinline__ nl_f32x4 nl_load4(const void* p, long long i)
 {
-    if (dt == NL_DT_F32) return *reinterpret_cast<const nl_f32x4*>((const float*)p + i);
-    const ushort4 u = *reinterpret_cast<const ushort4*>((const unsigned short*)p + i);
-    if (dt == NL_DT_BF16) return nl_f32x4{nl_bf2f(u.x), nl_bf2f(u.y), nl_bf2f(u.z), nl_bf2f(u.w)};
-    return nl_f32x4{nl_h2f(u.x), nl_h2f(u.y), nl_h2f(u.z), nl_h2f(u.w)};
+    if (DT == NL_DT_F32) return *reinterpret_cast<const nl_f32x4*>((const float*)p + i);
+    const nl_s16x4 u = *reinterpret_cast<const nl_s16x4*>((const unsigned short*)p + i);
+    nl_f32x4 o;
+#pragma unroll
+    for (int j = 0; j < 4; j++) o[j] = DT == NL_DT_BF16 ? nl_bf2f((unsigned short)u[j]) : nl_h2f((unsigned short)u[j]);
+    return o;
 }
-__device__ __forceinline__ void nl_store4(void* p, long long i, int dt, nl_f32x4 v)
+template <int DT> __device__ __forceinline__ void nl_store4(void* p, long long i, nl_f32x4 v)
 {
-    if (dt == NL_DT_F32) { *reinterpret_cast<nl_f32x4*>((float*)p + i) = v; return; }
-    ushort4 u;
-    if (dt == NL_DT_BF16) u = make_ushort4(nl_f2bf(v[0]), nl_f2bf(v[1]), nl_f2bf(v[2]), nl_f2bf(v[3]));
-    else u = make_ushort4(nl_f2h(v[0]), nl_f2h(v[1]), nl_f2h(v[2]), nl_f2h(v[3]));
-    *reinterpret_cast<ushort4*>((unsigned short*)p + i) = u;
+    if (DT == NL_DT_F32) { *reinterpret_cast<nl_f32x4*>((float*)p + i) = v; return; }
+    nl_s16x4 u;
+#pragma unroll
+    for (int j = 0; j < 4; j++) u[j] = (short)(DT == NL_DT_BF16 ? nl_f2bf(v[j]) : nl_f2h(v[j]));
+    *reinterpret_cast<nl_s16x4*>((unsigned short*)p + i) = u;
 }
-
-// eight consecutive elements, `left` of them inside the row; aligned: the address is a multiple of 16 bytes wherever n is one of eight elements
-__device__ __forceinline__ void nl_store8(void* p, long long i, int dt, const float* v, int left, bool aligned)
+// eight consecutive elements, aligned to eight (fp32: four) elements
+template <int DT> __device__ __forceinline__ void nl_load8_aligned(float* v, const void* p, long long i)
+{
+    if (DT == NL_DT_F32) {
+        const nl_f32x4 a = nl_load4<DT>(p, i), b = nl_load4<DT>(p, i + 4);
+#pragma unroll
+        for (int j = 0; j < 4; j++) { v[j] = a[j]; v[4 + j] = b[j]; }
+        return;
+    }
+    const nl_s16x8 u = *reinterpret_cast<const nl_s16x8*>((const unsigned short*)p + i);
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = DT == NL_DT_BF16 ? nl_bf2f((unsigned short)u[j]) : nl_h2f((unsigned short)u[j]);
+}
+// `left` of the eight are inside the row (zeros behind them); aligned: 16-byte accesses are
+template <int DT> __device__ __forceinline__ void nl_load8(float* v, const void* p, long long i, int left, bool aligned)
+{
+    if (aligned && left >= 8) { nl_load8_aligned<DT>(v, p, i); return; }
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = j < left ? nl_load_elem<DT>(p, i + j) : 0.0f;
+}
+template <int DT> __device__ __forceinline__ void nl_store8(void* p, long long i, const float* v, int left, bool aligned)
 {
     if (!aligned || left < 8) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) if (j < left) nl_store_elem(p, i + j, dt, v[j]);
+        for (int j = 0; j < 8; j++) if (j < left) nl_store_elem<DT>(p, i + j, v[j]);
         return;
     }
-    if (dt == NL_DT_F32) {
-        *reinterpret_cast<nl_f32x4*>((float*)p + i) = nl_f32x4{v[0], v[1], v[2], v[3]};
-        *reinterpret_cast<nl_f32x4*>((float*)p + i + 4) = nl_f32x4{v[4], v[5], v[6], v[7]};
+    if (DT == NL_DT_F32) {
+        nl_store4<DT>(p, i, nl_f32x4{v[0], v[1], v[2], v[3]});
+        nl_store4<DT>(p, i + 4, nl_f32x4{v[4], v[5], v[6], v[7]});
         return;
     }
     nl_s16x8 u;
 #pragma unroll
-    for (int j = 0; j < 8; j++) u[j] = (short)(dt == NL_DT_BF16 ? nl_f2bf(v[j]) : nl_f2h(v[j]));
+    for (int j = 0; j < 8; j++) u[j] = (short)(DT == NL_DT_BF16 ? nl_f2bf(v[j]) : nl_f2h(v[j]));
     *reinterpret_cast<nl_s16x8*>((unsigned short*)p + i) = u;
 }
+// 16-byte accesses at multiples of eight elements of rows `ld` elements apart
+template <int DT> __device__ __forceinline__ bool nl_rows_aligned(const void* p, long long ld) { return (ld & (DT == NL_DT_F32 ? 3 : 7)) == 0 && ((uintptr_t)p & 15) == 0; }
 
 // activations and their slopes.  Products whose epilogue or dz pass calls erff and expf are bound by vector arithmetic (dz of 16384 x 4096 gelu: 157 us against 78 us
 // of memory time), so both come from one hardware exponential and one hardware reciprocal.
@@ -155,40 +179,36 @@ __device__ __forceinline__ nl_f32x4 nl_mx_decode4(unsigned w, float scale, float
 // Every lane of a wave calls (rows and columns beyond the result do not store).
 __device__ __forceinline__ void nl_act8(float* v, int act)
 {
-    if (act == NL_ACT_NONE) return;
+    if (act == NL_ACT_RELU) {
 #pragma unroll
-    for (int j = 0; j < 8; j++) v[j] = nl_act(v[j], act);
+        for (int j = 0; j < 8; j++) v[j] = nl_act(v[j], NL_ACT_RELU);
+    } else if (act == NL_ACT_GELU) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = nl_act(v[j], NL_ACT_GELU);
+    } else if (act == NL_ACT_SILU) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = nl_act(v[j], NL_ACT_SILU);
+    }
 }
-__device__ __forceinline__ void nl_epilogue8(const NlEpilogue& ep, float* v, long long m, int n, long long M, int N, long long split_off)
+template <int DT> __device__ __forceinline__ void nl_epilogue8(const NlEpilogue& ep, float* v, long long m, int n, long long M, int N, long long split_off)
 {
-    const bool row = m < M, live = row && n < N, whole = n + 7 < N;
-    const int lane = threadIdx.x & 63;
+    const bool row = m < M, live = row && n < N;
+    const int lane = threadIdx.x & 63, left = N - n;
     if (ep.part) {
-        if (!live) return;
-        float* o = ep.part + split_off + m * N + n;
-        if (whole && (N & 3) == 0) {
-            *reinterpret_cast<nl_f32x4*>(o) = nl_f32x4{v[0], v[1], v[2], v[3]};
-            *reinterpret_cast<nl_f32x4*>(o + 4) = nl_f32x4{v[4], v[5], v[6], v[7]};
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++) if (n + j < N) o[j] = v[j];
-        }
+        if (live) nl_store8<NL_DT_F32>(ep.part + split_off, m * N + n, v, left, (N & 3) == 0);
         return;
     }
+    float r[8], b[8];
+    if (ep.r && live) nl_load8<DT>(r, ep.r, m * ep.ldr + n, left, nl_rows_aligned<DT>(ep.r, ep.ldr));
     if (ep.b && live) {
-        if (whole && ((uintptr_t)ep.b & (ep.dt == NL_DT_F32 ? 15 : 7)) == 0) {
-            const nl_f32x4 a = nl_load4(ep.b, n, ep.dt), c = nl_load4(ep.b, n + 4, ep.dt);
+        nl_load8<DT>(b, ep.b, n, left, nl_rows_aligned<DT>(ep.b, 0));
 #pragma unroll
-            for (int j = 0; j < 4; j++) { v[j] += a[j]; v[4 + j] += c[j]; }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++) if (n + j < N) v[j] += nl_load_elem(ep.b, n + j, ep.dt);
-        }
+        for (int j = 0; j < 8; j++) v[j] += b[j];
     }
     if (ep.bits) {                                                // one bit per element: z > 0
         unsigned w = 0;
 #pragma unroll
-        for (int j = 0; j < 8; j++) w |= (unsigned)(v[j] > 0.0f && n + j < N) << j;
+        for (int j = 0; j < 8; j++) w |= (unsigned)(v[j] > 0.0f && j < left) << j;
         w <<= 8 * (lane & 3);
         w |= __shfl_xor(w, 1);
         w |= __shfl_xor(w, 2);
@@ -197,7 +217,7 @@ __device__ __forceinline__ void nl_epilogue8(const NlEpilogue& ep, float* v, lon
     if (ep.z8) {                                                  // z in 8 bits, from the fp32 values; rows of codes are padded to whole blocks with zeros
         float amax = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; j++) { if (n + j >= N) v[j] = 0.0f; amax = fmaxf(amax, nl_finite_abs(v[j])); }
+        for (int j = 0; j < 8; j++) { if (j >= left) v[j] = 0.0f; amax = fmaxf(amax, nl_finite_abs(v[j])); }
         amax = fmaxf(amax, __shfl_xor(amax, 1));
         amax = fmaxf(amax, __shfl_xor(amax, 2));
         const int e = nl_mx_exponent(amax);
@@ -208,18 +228,19 @@ __device__ __forceinline__ void nl_epilogue8(const NlEpilogue& ep, float* v, lon
         }
     }
     if (!live) return;
-    if (ep.z) nl_store8(ep.z, m * ep.ldz + n, ep.dt, v, N - n, (ep.ldz & 7) == 0);
+    if (ep.z) nl_store8<DT>(ep.z, m * ep.ldz + n, v, left, (ep.ldz & 7) == 0);
     nl_act8(v, ep.act);
     if (ep.r) {
-        if (whole && (ep.ldr & 3) == 0 && ((uintptr_t)ep.r & (ep.dt == NL_DT_F32 ? 15 : 7)) == 0) {
-            const nl_f32x4 a = nl_load4(ep.r, m * ep.ldr + n, ep.dt), c = nl_load4(ep.r, m * ep.ldr + n + 4, ep.dt);
 #pragma unroll
-            for (int j = 0; j < 4; j++) { v[j] += a[j]; v[4 + j] += c[j]; }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++) if (n + j < N) v[j] += nl_load_elem(ep.r, m * ep.ldr + n + j, ep.dt);
-        }
+        for (int j = 0; j < 8; j++) v[j] += r[j];
     }
-    nl_store8(ep.y, m * ep.ldy + n, ep.dt, v, N - n, (ep.ldy & 7) == 0 && ((uintptr_t)ep.y & 15) == 0);
+    nl_store8<DT>(ep.y, m * ep.ldy + n, v, left, nl_rows_aligned<DT>(ep.y, ep.ldy));
 }
+// a kernel launch (or any statement) with the type as a compile-time constant DT
+#define NL_WITH_DTYPE(dt, ...)                                                            \
+    do {                                                                                  \
+        if ((dt) == NL_DT_F32) { constexpr int DT = NL_DT_F32; __VA_ARGS__; }             \
+        else if ((dt) == NL_DT_BF16) { constexpr int DT = NL_DT_BF16; __VA_ARGS__; }      \
+        else { constexpr int DT = NL_DT_F16; __VA_ARGS__; }                               \
+    } while (0)
 #endif

@@ -9,7 +9,7 @@
 // fp32: x = h + m + l, three bf16 numbers to nearest, exact (8 bits each of 24); of the nine products of two such numbers the six down to 2^-18 are summed, the
 // smallest first (l h, h l, m m, m h, h m, h h).  What is dropped (m l, l m, l l) is below 2^-26 |x||w|.
 // ---------------------------------------------------------------------------------------------
-struct NlPack { const void* src; const unsigned char* e; unsigned short* dst; long long rows, ld, pitch, plane; int cols, type, dt; };
+struct NlPack { const void* src; const unsigned char* e; unsigned short* dst; long long rows, ld, pitch, plane; int cols; };
 
 // x = h + m + l; a value whose rounding would overflow is cut instead, an infinity or NaN stays in h alone
 __device__ __forceinline__ void nl_split3(float x, unsigned short& h, unsigned short& m, unsigned short& l)
@@ -23,11 +23,11 @@ __device__ __forceinline__ void nl_split3(float x, unsigned short& h, unsigned s
     m = nl_f2bf(r);
     l = nl_f2bf(r - nl_bf2f(m));
 }
-// eight values to their place in a packed operand (dt: the tensors' type)
-__device__ __forceinline__ void nl_put_packed(unsigned short* dst, long long at, long long plane, int dt, const float* v)
+// eight values to their place in a packed operand (DT: the tensors' type)
+template <int DT> __device__ __forceinline__ void nl_put_packed(unsigned short* dst, long long at, long long plane, const float* v)
 {
     nl_s16x8 o[3];
-    if (dt == NL_DT_F32) {
+    if (DT == NL_DT_F32) {
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             unsigned short h, m, l;
@@ -38,40 +38,34 @@ __device__ __forceinline__ void nl_put_packed(unsigned short* dst, long long at,
         *reinterpret_cast<nl_s16x8*>(dst + 2 * plane + at) = o[2];
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++) o[0][j] = (short)(dt == NL_DT_BF16 ? nl_f2bf(v[j]) : nl_f2h(v[j]));
+        for (int j = 0; j < 8; j++) o[0][j] = (short)(DT == NL_DT_BF16 ? nl_f2bf(v[j]) : nl_f2h(v[j]));
     }
     *reinterpret_cast<nl_s16x8*>(dst + at) = o[0];
 }
+template <int DT, bool MX8>
 __global__ __launch_bounds__(256) void k_linear_pack(NlPack a)
 {
     const long long per_row = a.pitch / 8, total = a.rows * per_row;
-    const bool vec = a.type != NL_DT_MX8 && (a.ld & 3) == 0 && ((uintptr_t)a.src & (a.type == NL_DT_F32 ? 15 : 7)) == 0;
-    const float most = nl_dtype_max(a.dt);
+    const bool vec = nl_rows_aligned<DT>(a.src, a.ld);
     for (long long t = (long long)blockIdx.x * 256 + threadIdx.x; t < total; t += (long long)gridDim.x * 256) {
         const long long r = t / per_row;
         const int c = (int)(t - r * per_row) * 8;
         float v[8];
-        if (a.type == NL_DT_MX8) {
+        if (MX8) {
             const nl_i32x2 w = *reinterpret_cast<const nl_i32x2*>((const unsigned char*)a.src + r * a.ld + c);       // (rows of codes are whole blocks of 32, zeros behind the last)
             const float s = nl_mx_scale(a.e[r * (a.ld / 32) + (c >> 5)]);
-            const nl_f32x4 p = nl_mx_decode4((unsigned)w[0], s, most), q = nl_mx_decode4((unsigned)w[1], s, most);
+            const nl_f32x4 p = nl_mx_decode4((unsigned)w[0], s, nl_dtype_max(DT)), q = nl_mx_decode4((unsigned)w[1], s, nl_dtype_max(DT));
 #pragma unroll
             for (int j = 0; j < 4; j++) { v[j] = p[j]; v[4 + j] = q[j]; }
-        } else if (vec && c + 7 < a.cols) {
-            const nl_f32x4 p = nl_load4(a.src, r * a.ld + c, a.type), q = nl_load4(a.src, r * a.ld + c + 4, a.type);
-#pragma unroll
-            for (int j = 0; j < 4; j++) { v[j] = p[j]; v[4 + j] = q[j]; }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = c + j < a.cols ? nl_load_elem(a.src, r * a.ld + c + j, a.type) : 0.0f;
-        }
-        nl_put_packed(a.dst, r * a.pitch + c, a.plane, a.dt, v);
+        } else nl_load8<DT>(v, a.src, r * a.ld + c, a.cols - c, vec);
+        nl_put_packed<DT>(a.dst, r * a.pitch + c, a.plane, v);
     }
 }
 
 // ---------------------------------------------------------------------------------------------
 // k_linear_join: sums the pieces of a split contraction in their order and runs the epilogue.
 // ---------------------------------------------------------------------------------------------
+template <int DT>
 __global__ __launch_bounds__(256) void k_linear_join(const float* __restrict__ part, int splits, long long M, int N, NlEpilogue ep)
 {
     const long long per_row = (N + 31) / 32 * 4, total = M * per_row;          // eight columns a thread, whole blocks of 32 columns
@@ -92,7 +86,7 @@ __global__ __launch_bounds__(256) void k_linear_join(const float* __restrict__ p
 #pragma unroll
                     for (int j = 0; j < 8; j++) if (n + j < N) v[j] += p[j];
         }
-        nl_epilogue8(ep, v, m, n, M, N, 0);
+        nl_epilogue8<DT>(ep, v, m, n, M, N, 0);
     }
 }
 
@@ -104,49 +98,39 @@ struct NlDz {
     const void* gy; const void* z; const unsigned* bits; const unsigned char* z8; const unsigned char* z8e;
     unsigned short* dz; float* part;
     long long M, ldgy, ldz, ldbits, ldz8, ldz8e, pitch, plane, rows_per_chunk;
-    int N, dt, act;
+    int N;
 };
-__device__ __forceinline__ void nl_load8(float* v, const void* p, long long i, int dt, int left, bool vec)
-{
-    if (vec && left >= 8) {
-        const nl_f32x4 a = nl_load4(p, i, dt), b = nl_load4(p, i + 4, dt);
-#pragma unroll
-        for (int j = 0; j < 4; j++) { v[j] = a[j]; v[4 + j] = b[j]; }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = j < left ? nl_load_elem(p, i + j, dt) : 0.0f;
-    }
-}
+template <int DT, int ACT>
 __global__ __launch_bounds__(256) void k_linear_dz(NlDz a)
 {
     __shared__ float s_sum[8][257];
     const int c8 = threadIdx.x & 31, n = blockIdx.x * 256 + 8 * c8, grp = threadIdx.x >> 5;
     const long long m1 = (blockIdx.y + 1) * a.rows_per_chunk < a.M ? (blockIdx.y + 1) * a.rows_per_chunk : a.M;
-    const bool vg = (a.ldgy & 3) == 0 && ((uintptr_t)a.gy & (a.dt == NL_DT_F32 ? 15 : 7)) == 0, vz = (a.ldz & 3) == 0;
-    const float most = nl_dtype_max(a.dt);
+    const bool vg = nl_rows_aligned<DT>(a.gy, a.ldgy), vz = nl_rows_aligned<DT>(a.z, a.ldz);
+    constexpr float most = DT == NL_DT_F16 ? NL_F16_MAX : DT == NL_DT_BF16 ? 3.38953139e38f : 3.40282347e38f;
     float sum[8] = {};
     if (n < a.N)
         for (long long m = blockIdx.y * a.rows_per_chunk + grp; m < m1; m += 8) {
             float g[8], z[8];
-            nl_load8(g, a.gy, m * a.ldgy + n, a.dt, a.N - n, vg);
-            if (a.bits) {
+            nl_load8<DT>(g, a.gy, m * a.ldgy + n, a.N - n, vg);
+            if (ACT == NL_ACT_RELU) {
                 const unsigned w = a.bits[m * a.ldbits + (n >> 5)] >> (n & 31);
 #pragma unroll
                 for (int j = 0; j < 8; j++) g[j] = (w >> j & 1) ? g[j] : 0.0f;
-            } else if (a.act != NL_ACT_NONE) {
+            } else if (ACT != NL_ACT_NONE) {
                 if (a.z8) {
                     const nl_i32x2 w = *reinterpret_cast<const nl_i32x2*>(a.z8 + m * a.ldz8 + n);
                     const float s = nl_mx_scale(a.z8e[m * a.ldz8e + (n >> 5)]);
                     const nl_f32x4 p = nl_mx_decode4((unsigned)w[0], s, most), q = nl_mx_decode4((unsigned)w[1], s, most);
 #pragma unroll
                     for (int j = 0; j < 4; j++) { z[j] = p[j]; z[4 + j] = q[j]; }
-                } else nl_load8(z, a.z, m * a.ldz + n, a.dt, a.N - n, vz);
+                } else nl_load8<DT>(z, a.z, m * a.ldz + n, a.N - n, vz);
 #pragma unroll
-                for (int j = 0; j < 8; j++) g[j] = n + j < a.N ? g[j] * nl_act_slope(z[j], a.act) : 0.0f;
+                for (int j = 0; j < 8; j++) g[j] = n + j < a.N ? g[j] * nl_act_slope(z[j], ACT) : 0.0f;
             }
 #pragma unroll
             for (int j = 0; j < 8; j++) sum[j] += g[j];
-            if (a.dz) nl_put_packed(a.dz, m * a.pitch + n, a.plane, a.dt, g);
+            if (a.dz) nl_put_packed<DT>(a.dz, m * a.pitch + n, a.plane, g);
         }
     if (!a.part) return;
 #pragma unroll
@@ -161,7 +145,8 @@ __global__ __launch_bounds__(256) void k_linear_dz(NlDz a)
 }
 
 // gb[n] = sum over the chunks: 16 columns (four to a thread) x 64 runs of neighbouring chunks per workgroup, the runs joined pairwise
-__global__ __launch_bounds__(256) void k_linear_gb(const float* __restrict__ part, int chunks, int N, void* gb, int dt)
+template <int DT>
+__global__ __launch_bounds__(256) void k_linear_gb(const float* __restrict__ part, int chunks, int N, void* gb)
 {
     __shared__ nl_f32x4 s_sum[256];
     const int n = blockIdx.x * 16 + 4 * (threadIdx.x & 3), run = threadIdx.x >> 2;
@@ -180,7 +165,7 @@ __global__ __launch_bounds__(256) void k_linear_gb(const float* __restrict__ par
     }
     if (run != 0) return;
 #pragma unroll
-    for (int j = 0; j < 4; j++) if (n + j < N) nl_store_elem(gb, n + j, dt, s_sum[threadIdx.x][j]);
+    for (int j = 0; j < 4; j++) if (n + j < N) nl_store_elem<DT>(gb, n + j, s_sum[threadIdx.x][j]);
 }
 
 __global__ __launch_bounds__(256) void k_linear_zero(unsigned char* p, long long bytes)
@@ -208,10 +193,12 @@ static NlPacked nl_packed(NlWork& w, const void* p, const unsigned char* e, long
 {
     if (type == dt && dt != NL_DT_F32 && (ld & 7) == 0 && ld <= NL_LINEAR_MAX_WIDTH && (cols & 7) == 0 && ((uintptr_t)p & 15) == 0) return NlPacked{(const unsigned short*)p, ld, 0, rows, cols};
     NlPack a = {};
-    a.src = p; a.e = e; a.rows = rows; a.cols = cols; a.ld = ld; a.type = type; a.dt = dt;
+    a.src = p; a.e = e; a.rows = rows; a.cols = cols; a.ld = ld;
     a.pitch = nl_up(cols, 8); a.plane = nl_up(rows * a.pitch, 128);
     a.dst = (unsigned short*)w.take(2 * a.plane * (dt == NL_DT_F32 ? 3 : 1));
-    if (!w.dry) hipLaunchKernelGGL(k_linear_pack, dim3(nl_grid(rows * (a.pitch / 8))), dim3(256), 0, w.st, a);
+    const dim3 grid(nl_grid(rows * (a.pitch / 8)));
+    if (!w.dry) NL_WITH_DTYPE(dt, if (type == NL_DT_MX8) hipLaunchKernelGGL((k_linear_pack<DT, true>), grid, dim3(256), 0, w.st, a);
+                                  else hipLaunchKernelGGL((k_linear_pack<DT, false>), grid, dim3(256), 0, w.st, a));
     return NlPacked{a.dst, a.pitch, a.plane, rows, cols};
 }
 
@@ -259,7 +246,7 @@ static void nl_product(NlWork& w, const NlPacked& A, const NlPacked& B, int layo
     if (ep.dt == NL_DT_F32) nl_gemm_f32(g, layout, c.tile, grid, w.st);
     else if (ep.dt == NL_DT_BF16) nl_gemm_bf16(g, layout, c.tile, grid, w.st);
     else nl_gemm_f16(g, layout, c.tile, grid, w.st);
-    if (c.splits > 1) hipLaunchKernelGGL(k_linear_join, dim3(nl_grid(M * ((N + 31) / 32 * 4))), dim3(256), 0, w.st, g.ep.part, c.splits, M, N, ep);
+    if (c.splits > 1) NL_WITH_DTYPE(ep.dt, hipLaunchKernelGGL(k_linear_join<DT>, dim3(nl_grid(M * ((N + 31) / 32 * 4))), dim3(256), 0, w.st, g.ep.part, c.splits, M, N, ep));
     if (hipGetLastError() != hipSuccess) w.rc = NL_ERR_LAUNCH;
 }
 
@@ -281,7 +268,7 @@ static void nl_backward_run(const NlLinear* d, NlWork& w)
     NlPacked dz = {(const unsigned short*)d->gy, d->ldgy, 0, d->M, d->N};
     if (d->gb || (products && !in_place)) {
         NlDz a = {};
-        a.gy = d->gy; a.ldgy = d->ldgy; a.M = d->M; a.N = d->N; a.dt = d->dtype; a.act = d->act;
+        a.gy = d->gy; a.ldgy = d->ldgy; a.M = d->M; a.N = d->N;
         if (d->act == NL_ACT_RELU) { a.bits = d->bits; a.ldbits = nl_up(d->N, 32) / 32; }
         else if (d->act != NL_ACT_NONE && d->z8) { a.z8 = d->z8; a.z8e = d->z8e; a.ldz8 = nl_up(d->N, 32); a.ldz8e = a.ldz8 / 32; }
         else if (d->act != NL_ACT_NONE) { a.z = d->z; a.ldz = d->N; }
@@ -298,8 +285,12 @@ static void nl_backward_run(const NlLinear* d, NlWork& w)
             dz = NlPacked{a.dz, a.pitch, a.plane, d->M, d->N};
         }
         if (!w.dry) {
-            hipLaunchKernelGGL(k_linear_dz, dim3(colblocks, (unsigned)chunks), dim3(256), 0, w.st, a);
-            if (d->gb) hipLaunchKernelGGL(k_linear_gb, dim3((d->N + 15) / 16), dim3(256), 0, w.st, a.part, (int)chunks, d->N, d->gb, d->dtype);
+            const dim3 grid(colblocks, (unsigned)chunks);
+            NL_WITH_DTYPE(d->dtype, if (d->act == NL_ACT_NONE) hipLaunchKernelGGL((k_linear_dz<DT, NL_ACT_NONE>), grid, dim3(256), 0, w.st, a);
+                                    else if (d->act == NL_ACT_RELU) hipLaunchKernelGGL((k_linear_dz<DT, NL_ACT_RELU>), grid, dim3(256), 0, w.st, a);
+                                    else if (d->act == NL_ACT_GELU) hipLaunchKernelGGL((k_linear_dz<DT, NL_ACT_GELU>), grid, dim3(256), 0, w.st, a);
+                                    else hipLaunchKernelGGL((k_linear_dz<DT, NL_ACT_SILU>), grid, dim3(256), 0, w.st, a));
+            if (d->gb) NL_WITH_DTYPE(d->dtype, hipLaunchKernelGGL(k_linear_gb<DT>, dim3((d->N + 15) / 16), dim3(256), 0, w.st, a.part, (int)chunks, d->N, d->gb));
         }
     }
     NlEpilogue ep = {};
