@@ -5,14 +5,13 @@
 // neighbouring entries in ascending position: pieces of a fixed number of entries, the pieces of a row that spans several joined in order, level by level.
 #include "nl_layers.h"
 
-// Entries per run-summing group: at the first level 16 while there are at most EMB_FEW lookups, so that there are enough groups (32768 lookups x 1024 bf16: 31 us,
-// 91 us with 64 entries and one row in flight), else 64; at the later levels, which mostly hold entries without a piece, 128: one level less.
-#define EMB_CHUNK_FIRST 16
+// Sorted entries per run-summing group: 16 while there are at most EMB_FEW lookups, so that there are enough groups (32768 lookups x 1024 bf16: 22 us, 91 us with
+// 64 entries and one row in flight), else 64.  Pieces of a row that crosses such chunks are joined in blocks of EMB_BLOCK neighbours, level by level.
+#define EMB_CHUNK_FEW 16
 #define EMB_CHUNK_MANY 64
-#define EMB_CHUNK_LATER 128
 #define EMB_FEW 65536
-#define EMB_BATCH 8             // entries whose rows are in flight together, first level
-#define EMB_BATCH_LATER 16      // later levels
+#define EMB_BLOCK 64
+#define EMB_BATCH 8             // rows in flight together
 #define RS_TILE 1024            // keys per workgroup of a sorting pass: 4 waves x 4 rounds x 64 lanes
 #define RS_ROUNDS (RS_TILE / 256)
 #define RS_SMALL 4096           // up to here one workgroup sorts everything in LDS: one launch instead of three per pass
@@ -303,19 +302,18 @@ __global__ __launch_bounds__(1024) void k_rs_small(RsArgs a, int passes)
 }
 
 // ---- sums of neighbouring entries with one key ----
-// A group of `lanes` threads walks one chunk of the sorted list.  A run of equal keys that begins and ends inside the chunk is a finished row of the gradient;
-// a run that touches a chunk border which the row crosses becomes a piece.  Every chunk leaves two entries for the next level, its first and its last run's key
-// (a chunk of one run: the same key twice), each with a flag that says whether a piece stands behind it: the keys of the next level are sorted again.
-// What bounds it is the way position -> row: EMB_BATCH entries' keys and positions are read together, then their rows.
+// k_emb_sum: a group of `lanes` threads walks one chunk of the sorted list.  A run of equal keys that begins and ends inside the chunk is a finished row of the
+// gradient; a run that a chunk border cuts becomes a piece.  A chunk leaves its first and last key and at most two pieces: slot 0 of its first run, slot 1 of its last.
+// k_emb_join: the pieces of a row stand in neighbouring chunks, slot 1 (or the slot 0 of a chunk that is one run) of the first, then slots 0.  A group per chunk sums
+// the row that begins there, within a block of EMB_BLOCK chunks; a row that leaves the block becomes a piece of the block, and blocks are the next level's chunks.
+// What bounds both is the way position -> row: EMB_BATCH rows are fetched together.
+struct EmbPieces { unsigned* keys; unsigned char* any; float* piece; };        // [n][2] keys (first, last), [n][2] flags, [n][2][D] fp32
 struct EmbSum {
-    const unsigned* keys; const unsigned char* any;    // any: null at level 0 (every entry counts)
-    const unsigned* pos; const void* g; const float* weights;      // level 0: rows of the output gradient
-    const float* piece;                                // later levels
-    unsigned* out_keys; unsigned char* out_any; float* out_piece;  // null: this level is the last one
-    void* g_table; long long V;
+    const unsigned* keys; const unsigned* pos; const void* g; const float* weights;
+    EmbPieces out; void* g_table; long long V;
     int L, D, bag, chunk; float scale;
 };
-template <int DT, int VEC, bool LEVEL0>
+template <int DT, int VEC>
 __global__ __launch_bounds__(256) void k_emb_sum(EmbSum a, int lanes)
 {
     const int per = 256 / lanes, chunk = (int)(blockIdx.x * per + threadIdx.x / lanes);
@@ -327,66 +325,102 @@ __global__ __launch_bounds__(256) void k_emb_sum(EmbSum a, int lanes)
     const unsigned k_first = a.keys[s], k_last = a.keys[e - 1];
     const bool open_l = s > 0 && a.keys[s - 1] == k_first, open_r = e < a.L && a.keys[e] == k_last;
     EmbVec<VEC> acc = {};
-    bool some = false, any0 = false, any1 = false, in_first = true;
+    bool any0 = false, any1 = false, in_first = true;
     unsigned cur = k_first;
     // the run of `cur` ends, at the chunk's end or before it
     auto flush = [&](bool at_end) {
-        if (!some || cur >= a.V) return;
+        if (cur >= a.V) return;
         if (!((in_first && open_l) || (at_end && open_r))) { if (col) emb_store<VEC, DT>(a.g_table, (long long)cur * a.D + d, acc); return; }
-        const int slot = in_first ? 0 : 1;
         if (in_first) any0 = true; else any1 = true;
-        if (!col) return;
-        float* o = a.out_piece + (2LL * chunk + slot) * a.D + d;
-#pragma unroll
-        for (int q = 0; q < VEC; q++) o[q] = acc.v[q];
+        if (col) emb_store<VEC, NL_DT_F32>(a.out.piece, (2LL * chunk + (in_first ? 0 : 1)) * a.D + d, acc);
     };
-    constexpr int B = LEVEL0 ? EMB_BATCH : EMB_BATCH_LATER;
-    unsigned nkey[B], np[B];
-    bool nlive[B];
-    auto look = [&](int j0) {                                         // keys and positions of the next batch
+    unsigned nkey[EMB_BATCH], npos[EMB_BATCH];
+    auto look = [&](int j0) {                                         // keys and positions of the next batch; behind the chunk's end its last entry again
 #pragma unroll
-        for (int b = 0; b < B; b++) {
+        for (int b = 0; b < EMB_BATCH; b++) {
             const int j = j0 + b < e ? j0 + b : e - 1;
             nkey[b] = a.keys[j];
-            np[b] = LEVEL0 ? a.pos[j] : (unsigned)j;
-            nlive[b] = j0 + b < e && (LEVEL0 || a.any[j]);
+            npos[b] = a.pos[j];
         }
     };
     look(s);
-    for (int j0 = s; j0 < e; j0 += B) {
-        unsigned key[B], p[B];
-        bool live[B];
-        float w[B];
-        EmbVec<VEC> r[B];
+    for (int j0 = s; j0 < e; j0 += EMB_BATCH) {
+        unsigned key[EMB_BATCH];
+        float w[EMB_BATCH];
+        EmbVec<VEC> r[EMB_BATCH];
 #pragma unroll
-        for (int b = 0; b < B; b++) { key[b] = nkey[b]; p[b] = np[b]; live[b] = nlive[b]; }
-#pragma unroll
-        for (int b = 0; b < B; b++) {
-            w[b] = LEVEL0 && a.weights ? a.scale * a.weights[p[b]] : a.scale;
-            // always loaded, used where the entry counts (a load under a condition is waited for where the branch ends: one row in flight)
-            if (LEVEL0) r[b] = emb_load<VEC, DT>(a.g, (long long)(p[b] / (unsigned)a.bag) * a.D + (col ? d : 0));
-            else r[b] = emb_load<VEC, NL_DT_F32>(a.piece, (long long)p[b] * a.D + (col ? d : 0));
+        for (int b = 0; b < EMB_BATCH; b++) {
+            // every row is fetched, also where it does not count (a load under a condition is waited for where the branch ends)
+            key[b] = nkey[b];
+            w[b] = a.weights ? a.scale * a.weights[npos[b]] : a.scale;
+            r[b] = emb_load<VEC, DT>(a.g, (long long)(npos[b] / (unsigned)a.bag) * a.D + (col ? d : 0));
         }
-        if (j0 + B < e) look(j0 + B);
+        if (j0 + EMB_BATCH < e) look(j0 + EMB_BATCH);
 #pragma unroll
-        for (int b = 0; b < B; b++) {
-            if (j0 + b >= e) break;
+        for (int b = 0; b < EMB_BATCH; b++) {
             if (key[b] != cur) {
                 flush(false);
                 acc = EmbVec<VEC>{};
-                some = false; in_first = false; cur = key[b];
+                in_first = false; cur = key[b];
             }
-            if (!live[b]) continue;
-            some = true;
-            if (col && cur < a.V)
+            if (j0 + b < e)
 #pragma unroll
-                for (int q = 0; q < VEC; q++) acc.v[q] += LEVEL0 ? w[b] * r[b].v[q] : r[b].v[q];
+                for (int q = 0; q < VEC; q++) acc.v[q] += w[b] * r[b].v[q];
         }
     }
     flush(true);
-    if (lead && a.out_keys) {
-        a.out_keys[2 * chunk] = k_first; a.out_keys[2 * chunk + 1] = k_last;
-        a.out_any[2 * chunk] = any0; a.out_any[2 * chunk + 1] = any1;
+    if (lead && a.out.keys) {
+        a.out.keys[2 * chunk] = k_first; a.out.keys[2 * chunk + 1] = k_last;
+        a.out.any[2 * chunk] = any0; a.out.any[2 * chunk + 1] = any1;
+    }
+}
+
+// n chunks of one level; out.keys null: they are one block, nothing leaves it
+template <int DT, int VEC>
+__global__ __launch_bounds__(256) void k_emb_join(EmbPieces in, EmbPieces out, int n, int D, void* g_table, int lanes)
+{
+    const int per = 256 / lanes, c = (int)(blockIdx.x * per + threadIdx.x / lanes);
+    if (c >= n) return;
+    const int d = (int)(blockIdx.y * lanes + (threadIdx.x & (lanes - 1))) * VEC;
+    const bool lead = d == 0, col = d < D;
+    const int block = c / EMB_BLOCK, b0 = block * EMB_BLOCK, b1 = b0 + EMB_BLOCK < n ? b0 + EMB_BLOCK : n;
+    const unsigned block_first = in.keys[2 * b0], block_last = in.keys[2 * b1 - 1];
+    const unsigned first = in.keys[2 * c], last = in.keys[2 * c + 1];
+    const bool open_l = c > 0 && in.keys[2 * c - 1] == first;
+    const bool any0 = in.any[2 * c], any1 = in.any[2 * c + 1];
+    if (out.keys && lead && c == b0) {
+        const bool from_l = b0 > 0 && in.keys[2 * b0 - 1] == block_first, to_r = b1 < n && in.keys[2 * b1] == block_last, one = block_first == block_last;
+        out.keys[2 * block] = block_first; out.keys[2 * block + 1] = block_last;
+        out.any[2 * block] = any0 && (from_l || (one && to_r));
+        out.any[2 * block + 1] = !one && to_r && in.any[in.keys[2 * b1 - 2] == block_last ? 2 * b1 - 2 : 2 * b1 - 1];
+    }
+    // at most two sums begin here: of the first run (it comes from the left and the block begins, or the chunk is one run and the row begins with it), of the last one
+#pragma unroll 1
+    for (int which = 0; which < 2; which++) {
+        const bool mine = which == 0 ? any0 && (open_l ? c == b0 : first == last) : any1;
+        if (!mine) continue;
+        const unsigned key = which == 0 ? first : last;
+        // how far the row goes: chunks c + 1 .. c + more, their slots 0; the row goes on behind a chunk that is one run
+        int more = 0;
+        bool goes_on = which == 1 || first == last;
+        while (goes_on && c + more + 1 < b1 && in.keys[2 * (c + more + 1)] == key) {
+            more++;
+            goes_on = in.keys[2 * (c + more) + 1] == key;
+        }
+        EmbVec<VEC> acc = emb_load<VEC, NL_DT_F32>(in.piece, (2LL * c + which) * D + (col ? d : 0));
+        for (int j0 = 0; j0 < more; j0 += EMB_BATCH) {
+            EmbVec<VEC> r[EMB_BATCH];
+#pragma unroll
+            for (int b = 0; b < EMB_BATCH; b++) r[b] = emb_load<VEC, NL_DT_F32>(in.piece, 2LL * (c + 1 + (j0 + b < more ? j0 + b : more - 1)) * D + (col ? d : 0));
+#pragma unroll
+            for (int b = 0; b < EMB_BATCH; b++)
+                if (j0 + b < more)
+#pragma unroll
+                    for (int q = 0; q < VEC; q++) acc.v[q] += r[b].v[q];
+        }
+        const bool from_left = which == 0 && open_l, to_right = goes_on && c + more + 1 == b1 && b1 < n && in.keys[2 * b1] == key;
+        if (!from_left && !to_right) { if (col) emb_store<VEC, DT>(g_table, (long long)key * D + d, acc); }
+        else if (col) emb_store<VEC, NL_DT_F32>(out.piece, (2LL * block + (key == block_first ? 0 : 1)) * D + d, acc);
     }
 }
 
@@ -398,7 +432,7 @@ __global__ void k_emb_zero_tail(unsigned short* p) { *p = 0; }
 
 // ---- host ----
 #define EMB_MAX_LOOKUPS 0x7FFF0000LL
-struct EmbPlan { int L, nblk, passes, levels, first; long long keys, hist, key_l[2], any_l[2], piece_l[2], total; };
+struct EmbPlan { int L, nblk, passes, chunk, levels; long long keys, hist, key_l[2], any_l[2], piece_l[2], total; };      // levels: launches of k_emb_join
 static EmbPlan emb_plan(long long V, int D, long long L)
 {
     EmbPlan p = {};
@@ -409,12 +443,11 @@ static EmbPlan emb_plan(long long V, int D, long long L)
     p.keys = nl_up(4 * L, 256);
     p.hist = nl_up(4LL * 256 * p.nblk + 1024, 256);
     p.total = 4 * p.keys + p.hist;
-    p.first = L <= EMB_FEW ? EMB_CHUNK_FIRST : EMB_CHUNK_MANY;
-    for (long long n = L, c = p.first; n > c; c = EMB_CHUNK_LATER) {                 // two entries per chunk for the next level; levels take two buffers in turn
-        n = 2 * ((n + c - 1) / c);
+    p.chunk = L <= EMB_FEW ? EMB_CHUNK_FEW : EMB_CHUNK_MANY;
+    for (long long n = (L + p.chunk - 1) / p.chunk; n > 1; n = (n + EMB_BLOCK - 1) / EMB_BLOCK) {        // levels take two buffers in turn
         if (p.levels < 2) {
             const int i = p.levels;
-            p.key_l[i] = nl_up(4 * n, 256); p.any_l[i] = nl_up(n, 256); p.piece_l[i] = nl_up(4 * n * D, 256);
+            p.key_l[i] = nl_up(8 * n, 256); p.any_l[i] = nl_up(2 * n, 256); p.piece_l[i] = nl_up(8 * n * D, 256);
             p.total += p.key_l[i] + p.any_l[i] + p.piece_l[i];
         }
         p.levels++;
@@ -446,12 +479,18 @@ static unsigned emb_zero_blocks(long long words, int threads)
     const long long b = (words + 8LL * threads - 1) / (8LL * threads);
     return (unsigned)(b < 2048 ? b : 2048);
 }
-template <int VEC> static void emb_level(const EmbSum& a, int dt, bool level0, hipStream_t st)
+template <int VEC> static void emb_sums(const EmbPlan& p, EmbSum a, const EmbPieces* buf, int dt, hipStream_t st)
 {
-    const int lanes = emb_lanes(a.D, VEC, 256), per = 256 / lanes, chunks = (a.L + a.chunk - 1) / a.chunk;
-    const dim3 grid((chunks + per - 1) / per, (a.D + lanes * VEC - 1) / (lanes * VEC));
-    NL_WITH_DTYPE(dt, if (level0) hipLaunchKernelGGL((k_emb_sum<DT, VEC, true>), grid, dim3(256), 0, st, a, lanes);
-                      else hipLaunchKernelGGL((k_emb_sum<DT, VEC, false>), grid, dim3(256), 0, st, a, lanes));
+    const int lanes = emb_lanes(a.D, VEC, 256), per = 256 / lanes;
+    const unsigned cols = (unsigned)((a.D + lanes * VEC - 1) / (lanes * VEC));
+    int n = (a.L + p.chunk - 1) / p.chunk;
+    if (p.levels > 0) a.out = buf[0];
+    NL_WITH_DTYPE(dt, hipLaunchKernelGGL((k_emb_sum<DT, VEC>), dim3((n + per - 1) / per, cols), dim3(256), 0, st, a, lanes));
+    for (int l = 0; l < p.levels; l++) {
+        const EmbPieces out = l + 1 < p.levels ? buf[(l + 1) & 1] : EmbPieces{};
+        NL_WITH_DTYPE(dt, hipLaunchKernelGGL((k_emb_join<DT, VEC>), dim3((n + per - 1) / per, cols), dim3(256), 0, st, buf[l & 1], out, n, a.D, a.g_table, lanes));
+        n = (n + EMB_BLOCK - 1) / EMB_BLOCK;
+    }
 }
 
 extern "C" {
@@ -530,25 +569,18 @@ int nl_embedding_backward(const void* table, long long V, int D, int dtype, cons
                 else hipLaunchKernelGGL(k_rs_scatter, grid, dim3(256), 0, st, r);
             }
         }
-    unsigned* lk[2]; unsigned char* la[2]; float* lp[2];
+    EmbPieces buf[2] = {};
     for (int i = 0; i < 2; i++) {
-        lk[i] = (unsigned*)w; la[i] = (unsigned char*)(w + p.key_l[i]); lp[i] = (float*)(w + p.key_l[i] + p.any_l[i]);
+        buf[i] = EmbPieces{(unsigned*)w, (unsigned char*)(w + p.key_l[i]), (float*)(w + p.key_l[i] + p.any_l[i])};
         w += p.key_l[i] + p.any_l[i] + p.piece_l[i];
     }
-    const int vec = emb_vec(D, dtype, g_out, g_table);
     EmbSum a = {};
     a.keys = keys[(p.passes - 1) & 1]; a.pos = pos[(p.passes - 1) & 1]; a.g = g_out; a.weights = weights; a.g_table = g_table; a.V = V; a.L = p.L; a.D = D;
-    a.bag = bag; a.scale = scale; a.chunk = p.first;
-    for (int lev = 0; lev <= p.levels; lev++) {
-        const bool last = lev == p.levels;
-        a.out_keys = last ? nullptr : lk[lev & 1]; a.out_any = last ? nullptr : la[lev & 1]; a.out_piece = last ? nullptr : lp[lev & 1];
-        if (vec == 8) emb_level<8>(a, dtype, lev == 0, st);
-        else if (vec == 4) emb_level<4>(a, dtype, lev == 0, st);
-        else emb_level<1>(a, dtype, lev == 0, st);
-        a.keys = a.out_keys; a.any = a.out_any; a.piece = a.out_piece; a.pos = nullptr;
-        a.L = 2 * ((a.L + a.chunk - 1) / a.chunk);
-        a.chunk = EMB_CHUNK_LATER;
-    }
+    a.bag = bag; a.scale = scale; a.chunk = p.chunk;
+    const int vec = emb_vec(D, dtype, g_out, g_table);
+    if (vec == 8) emb_sums<8>(p, a, buf, dtype, st);
+    else if (vec == 4) emb_sums<4>(p, a, buf, dtype, st);
+    else emb_sums<1>(p, a, buf, dtype, st);
     NL_LAUNCH_CHECK();
     return NL_OK;
 }
