@@ -12,14 +12,13 @@
 struct NlGemm {
     const char* A; const char* B;      // 16-byte aligned, rows 16-byte aligned
     long long lda, ldb;                // bytes between rows
-    long long a_plane, b_plane;        // bytes between the planes of a split fp32 operand
     long long M, K;
-    int N, tiles_m, tiles_n, split;    // fp32: split = 1, the six plane products follow each other along one contraction
+    int N, tiles_m, tiles_n;
     long long kchunk;                  // contraction indices per split, a multiple of GEMM_BK
     NlEpilogue ep;
 };
 
-// layout 0: both operands' rows run along k; 1: B's rows are k; 2: both operands' rows are k.  tile 0: 256 x 256, 1: 128 x 128, 2: 64 x 64.
+// layout 0: both operands' rows run along k; 1: B's rows are k; 2: both operands' rows are k.  tile 0: 256 x 256 (16 bits only), 1: 128 x 128, 2: 64 x 64.
 void nl_gemm_bf16(const NlGemm& g, int layout, int tile, dim3 grid, hipStream_t st);
 void nl_gemm_f16(const NlGemm& g, int layout, int tile, dim3 grid, hipStream_t st);
 void nl_gemm_f32(const NlGemm& g, int layout, int tile, dim3 grid, hipStream_t st);
@@ -36,18 +35,19 @@ template <> struct NlMma<_Float16> {
 #define GEMM_OUT_OF_RANGE 0x80000000u   // a buffer load from here returns zeros: beyond every tile's range (at most GEMM_RANGE bytes)
 #define GEMM_RANGE 0x7FFFFFF0LL
 
-// One operand of a workgroup: R rows or columns (of C) x GEMM_BK contraction indices per step, NT threads.
-//   fast (k fastest):  LDS [R][64], 16-byte chunks of a row XORed with row & 7: the 16 rows of a fragment start in different banks
-//   slow (k slowest):  LDS [64][R], pairs of chunks XORed with k & 3 and, where a row has 16 chunks, k >> 3 & 1: the rows that one transposing read touches lie
+// One operand of a workgroup: R rows or columns (of C) x BK contraction indices per step, NT threads.
+//   fast (k fastest):  LDS [R][BK], 16-byte chunks of a row XORed with row & 7 (BK 32: row >> 1 & 3): eight rows of a fragment cover all banks
+//   slow (k slowest):  LDS [BK][R], pairs of chunks XORed with k & 3 and, where a row has 16 chunks, k >> 3 & 1: the rows that one transposing read touches lie
 //                      in different banks
-template <bool SLOW, int R, int NT>
+template <bool SLOW, int R, int NT, int BK = GEMM_BK>
 struct GemmSide {
-    static constexpr int BYTES = R * GEMM_BK * 2, LOADS = BYTES / (16 * NT), CH = R / 8;
+    static constexpr int BYTES = R * BK * 2, LOADS = BYTES / (16 * NT), CH = R / 8;
     unsigned off[LOADS];               // byte offset of the thread's chunks from the tile's first byte; GEMM_OUT_OF_RANGE: outside the operand
     int kk[LOADS];                     // contraction index of the chunk inside a step
     const char* base; long long step, room;
 
     static __device__ __forceinline__ int swz(int k) { return CH >= 16 ? ((k & 3) | ((k >> 1) & 4)) : (k & 3); }
+    static __device__ __forceinline__ int swz_row(int r) { return BK == 64 ? r & 7 : (r >> 1) & 3; }
 
     // p: the operand, ld: bytes per row, i0: first row / column of the tile, I: how many there are, k0: first contraction index
     __device__ __forceinline__ void init(const char* p, long long ld, long long i0, long long I, long long k0, long long K)
@@ -61,13 +61,13 @@ struct GemmSide {
                 kk[l] = k;
                 off[l] = i0 + 8 * c < I ? (unsigned)(k * ld + 16 * c) : GEMM_OUT_OF_RANGE;
             } else {
-                const int r = s >> 3, c = (s & 7) ^ (r & 7);
+                const int r = s / (BK / 8), c = (s % (BK / 8)) ^ swz_row(r);
                 kk[l] = 8 * c;
                 off[l] = i0 + r < I ? (unsigned)(r * ld + 16 * c) : GEMM_OUT_OF_RANGE;
             }
         }
         base = SLOW ? p + k0 * ld + 2 * i0 : p + i0 * ld + 2 * k0;
-        step = SLOW ? GEMM_BK * ld : GEMM_BK * 2;
+        step = SLOW ? BK * ld : BK * 2;
     }
     // one step into LDS: kleft contraction indices are left (chunks behind them read zeros); adv: bytes from the first step's place
     __device__ __forceinline__ void load(char* lds, long long adv, long long kleft) const
@@ -76,7 +76,7 @@ struct GemmSide {
         const int wave = threadIdx.x >> 6;
 #pragma unroll
         for (int l = 0; l < LOADS; l++) {
-            const unsigned o = kleft >= GEMM_BK || kk[l] < kleft ? off[l] : GEMM_OUT_OF_RANGE;
+            const unsigned o = kleft >= BK || kk[l] < kleft ? off[l] : GEMM_OUT_OF_RANGE;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(lds + (l * NT + wave * 64) * 16), 16, (int)o, 0, 0, 0);
         }
     }
@@ -92,76 +92,37 @@ struct GemmSide {
             const nl_s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(nl_s16x4*)(lds + at + 4 * R * 2));
             return nl_s16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
         }
-        const int row = i + (l & 15), c = (4 * ks + (l >> 4)) ^ (l & 7);
-        return *reinterpret_cast<const nl_s16x8*>(lds + row * (GEMM_BK * 2) + c * 16);
+        const int row = i + (l & 15), c = (4 * ks + (l >> 4)) ^ swz_row(l & 15);
+        return *reinterpret_cast<const nl_s16x8*>(lds + row * (BK * 2) + c * 16);
     }
 };
 
-template <class T, bool PLANES, bool A_SLOW, bool B_SLOW, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
+// workgroups go to the eight dies in turn: give each die neighbouring tiles, four tile rows at a time, so that its L2 holds what it shares
+template <int BM, int BN> __device__ __forceinline__ void gemm_tile_of(const NlGemm& g, long long& m0, int& n0)
 {
-    constexpr int DT = PLANES ? NL_DT_F32 : __is_same(T, _Float16) ? NL_DT_F16 : NL_DT_BF16;
-    constexpr int NT = 64 * WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
-    typedef GemmSide<A_SLOW, BM, NT> SA;
-    typedef GemmSide<B_SLOW, BN, NT> SB;
-    __shared__ __align__(256) char s_mem[2 * (SA::BYTES + SB::BYTES)];
-    char* const s_a = s_mem;
-    char* const s_b = s_mem + 2 * SA::BYTES;
-    // workgroups go to the eight dies in turn: give each die neighbouring tiles, four tile rows at a time, so that its L2 holds what it shares
     const unsigned tiles = (unsigned)g.tiles_m * g.tiles_n, q = tiles >> 3, rem = tiles & 7, die = blockIdx.x & 7;
     unsigned pid = die * q + (die < rem ? die : rem) + (blockIdx.x >> 3);
     const unsigned per_group = 4u * g.tiles_n, grp = pid / per_group, first = 4 * grp, rows = min(4u, (unsigned)g.tiles_m - first);
     pid -= grp * per_group;
-    const long long m0 = (long long)(first + pid % rows) * BM;
-    const int n0 = (int)(pid / rows) * BN;
-    const long long k0 = (long long)blockIdx.y * g.kchunk, k1 = min(k0 + g.kchunk, g.K);
-    const int ksteps = (int)((k1 - k0 + GEMM_BK - 1) / GEMM_BK), steps = PLANES ? 6 * ksteps : ksteps;
-    SA a; SB b;
-    a.init(g.A, g.lda, m0, g.M, k0, g.K);
-    b.init(g.B, g.ldb, n0, g.N, k0, g.K);
-    const int wave = threadIdx.x >> 6, wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
-    nl_f32x4 acc[FM][FN] = {};
-    auto fetch = [&](int s) {
-        const int pair = PLANES ? s / ksteps : 0, k = PLANES ? s - pair * ksteps : s;
-        // planes h, m, l = 0, 1, 2; the products by rising size: (l,h) (h,l) (m,m) (m,h) (h,m) (h,h)
-        const int qa = PLANES ? (pair == 0 ? 2 : pair == 2 || pair == 3 ? 1 : 0) : 0, qb = PLANES ? (pair == 1 ? 2 : pair == 2 || pair == 4 ? 1 : 0) : 0;
-        const long long left = k1 - k0 - (long long)k * GEMM_BK;
-        a.load(s_a + (s & 1) * SA::BYTES, k * a.step + qa * g.a_plane, left);
-        b.load(s_b + (s & 1) * SB::BYTES, k * b.step + qb * g.b_plane, left);
-    };
-    fetch(0);
-    __builtin_amdgcn_s_waitcnt(0);
-    __builtin_amdgcn_s_barrier();
-    for (int s = 0; s < steps; s++) {
-        if (s + 1 < steps) fetch(s + 1);
-        const char* la = s_a + (s & 1) * SA::BYTES;
-        const char* lb = s_b + (s & 1) * SB::BYTES;
-#pragma unroll
-        for (int ks = 0; ks < 2; ks++) {
-            nl_s16x8 fa[FM], fb[FN];
-#pragma unroll
-            for (int i = 0; i < FM; i++) fa[i] = SA::frag(la, wm + 16 * i, ks);
-#pragma unroll
-            for (int j = 0; j < FN; j++) fb[j] = SB::frag(lb, wn + 16 * j, ks);
-#pragma unroll
-            for (int i = 0; i < FM; i++)
-#pragma unroll
-                for (int j = 0; j < FN; j++) acc[i][j] = NlMma<T>::mma(fb[j], fa[i], acc[i][j]);
-        }
-        __syncthreads();
-    }
-    // results: a wave passes its rows through its own part of LDS, RP at a time, and leaves with eight neighbouring columns in a lane (16-byte stores, and the
-    // neighbours that bits and 8-bit blocks need).  16-byte chunks XORed with the row: neither side of the exchange has bank conflicts.
-    constexpr int WC = BN / WN, RP = BM / WM < 64 ? BM / WM : 64, CX = WC / 4 - 1;
-    static_assert((CX & (CX + 1)) == 0 && RP * WC * 4 * WM * WN <= 2 * (SA::BYTES + SB::BYTES), "the exchange fits into the operand buffers");
-    char* const mine = s_mem + wave * (RP * WC * 4);
+    m0 = (long long)(first + pid % rows) * BM;
+    n0 = (int)(pid / rows) * BN;
+}
+
+// Results of a wave, WR rows x WC columns from (m, n) on: it passes them through its own part of LDS, RP rows at a time, and leaves with eight neighbouring columns
+// in a lane (16-byte stores, and the neighbours that bits and 8-bit blocks need).  16-byte chunks XORed with the row: neither side of the exchange has bank conflicts.
+template <int DT, int WR, int WC, int WAVES, int LDS>
+__device__ __forceinline__ void gemm_results(const NlGemm& g, nl_f32x4 (&acc)[WR / 16][WC / 16], char* s_mem, long long m, int n)
+{
+    constexpr int RP = WR < 64 ? WR : 64, CX = WC / 4 - 1;
+    static_assert((CX & (CX + 1)) == 0 && RP * WC * 4 * WAVES <= LDS, "the exchange fits into the operand buffers");
     const int lane = threadIdx.x & 63;
+    char* const mine = s_mem + (threadIdx.x >> 6) * (RP * WC * 4);
 #pragma unroll
-    for (int half = 0; half < BM / WM / RP; half++) {
+    for (int half = 0; half < WR / RP; half++) {
 #pragma unroll
         for (int i = 0; i < RP / 16; i++)
 #pragma unroll
-            for (int j = 0; j < FN; j++) {
+            for (int j = 0; j < WC / 16; j++) {
                 const int r = 16 * i + (lane & 15), c = (4 * j + (lane >> 4)) ^ (r & CX);
                 *reinterpret_cast<nl_f32x4*>(mine + r * (WC * 4) + c * 16) = acc[half * (RP / 16) + i][j];
             }
@@ -172,24 +133,222 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
             const nl_f32x4 p = *reinterpret_cast<const nl_f32x4*>(mine + r * (WC * 4) + (c ^ (r & CX)) * 16);
             const nl_f32x4 q = *reinterpret_cast<const nl_f32x4*>(mine + r * (WC * 4) + ((c + 1) ^ (r & CX)) * 16);
             float v[8] = {p[0], p[1], p[2], p[3], q[0], q[1], q[2], q[3]};
-            nl_epilogue8<DT>(g.ep, v, m0 + wm + half * RP + r, n0 + wn + 4 * c, g.M, g.N, (long long)blockIdx.y * g.M * g.N);
+            nl_epilogue8<DT>(g.ep, v, m + half * RP + r, n + 4 * c, g.M, g.N, (long long)blockIdx.y * g.M * g.N);
         }
         __builtin_amdgcn_wave_barrier();
     }
 }
 
-template <class T, bool PLANES, bool A_SLOW, bool B_SLOW>
+template <class T, bool A_SLOW, bool B_SLOW, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
+{
+    constexpr int DT = __is_same(T, _Float16) ? NL_DT_F16 : NL_DT_BF16;
+    constexpr int NT = 64 * WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
+    typedef GemmSide<A_SLOW, BM, NT> SA;
+    typedef GemmSide<B_SLOW, BN, NT> SB;
+    __shared__ __align__(256) char s_mem[2 * (SA::BYTES + SB::BYTES)];
+    char* const s_a = s_mem;
+    char* const s_b = s_mem + 2 * SA::BYTES;
+    long long m0; int n0;
+    gemm_tile_of<BM, BN>(g, m0, n0);
+    const long long k0 = (long long)blockIdx.y * g.kchunk, k1 = min(k0 + g.kchunk, g.K);
+    const int steps = (int)((k1 - k0 + GEMM_BK - 1) / GEMM_BK);
+    SA a; SB b;
+    a.init(g.A, g.lda, m0, g.M, k0, g.K);
+    b.init(g.B, g.ldb, n0, g.N, k0, g.K);
+    const int wave = threadIdx.x >> 6, wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
+    nl_f32x4 acc[FM][FN] = {};
+    auto fetch = [&](int s) {
+        const long long left = k1 - k0 - (long long)s * GEMM_BK;
+        a.load(s_a + (s & 1) * SA::BYTES, s * a.step, left);
+        b.load(s_b + (s & 1) * SB::BYTES, s * b.step, left);
+    };
+    fetch(0);
+    __builtin_amdgcn_s_waitcnt(0);
+    __builtin_amdgcn_s_barrier();
+    for (int s = 0; s < steps; s++) {
+        const char* la = s_a + (s & 1) * SA::BYTES;
+        const char* lb = s_b + (s & 1) * SB::BYTES;
+        // fragments of both halves of the step, the loads of the next step between them: behind all fragment reads they come late (8192^3 / 16384 x 4096 x 4096,
+        // layout 1 and 2: -10 %), in front of them they hold up the reads that the first matrix instructions wait for
+        nl_s16x8 fa[2][FM], fb[2][FN];
+#pragma unroll
+        for (int j = 0; j < FN; j++) fb[0][j] = SB::frag(lb, wn + 16 * j, 0);
+#pragma unroll
+        for (int i = 0; i < FM; i++) fa[0][i] = SA::frag(la, wm + 16 * i, 0);
+        if (s + 1 < steps) fetch(s + 1);
+#pragma unroll
+        for (int j = 0; j < FN; j++) fb[1][j] = SB::frag(lb, wn + 16 * j, 1);
+#pragma unroll
+        for (int i = 0; i < FM; i++) fa[1][i] = SA::frag(la, wm + 16 * i, 1);
+#pragma unroll
+        for (int i = 0; i < FM; i++)
+#pragma unroll
+            for (int j = 0; j < FN; j++) acc[i][j] = NlMma<T>::mma(fb[0][j], fa[0][i], acc[i][j]);
+#pragma unroll
+        for (int i = 0; i < FM; i++)
+#pragma unroll
+            for (int j = 0; j < FN; j++) acc[i][j] = NlMma<T>::mma(fb[1][j], fa[1][i], acc[i][j]);
+        __syncthreads();
+    }
+    gemm_results<DT, BM / WM, BN / WN, WM * WN, 2 * (SA::BYTES + SB::BYTES)>(g, acc, s_mem, m0 + wm, n0 + wn);
+}
+
+// ---------------------------------------------------------------------------------------------
+// k_gemm_f32: fp32 operands.  x = h + m + l, three bf16 numbers to nearest, exact (8 bits each of 24); of the nine products of two such numbers the six down to
+// 2^-18 are summed, per step of 32 contraction indices the smallest first (l h, h l, m m, m h, h m, h h).  What is dropped (m l, l m, l l) is below 2^-26 |x||w|.
+// The split happens on the way into LDS: no operand is written to memory a second time (split planes in memory: 262144 x 256 x 256 spends 118 us on writing and
+// 50 us more on reading them).  A thread fetches a step's elements into registers while the step before it multiplies, splits them and writes three planes; two
+// workgroups share a compute unit, so that one splits (vector unit) while the other multiplies.  Six products: at most a sixth of the bf16 rate.
+// ---------------------------------------------------------------------------------------------
+__device__ __forceinline__ void gemm_split8(const float* x, nl_s16x8& h, nl_s16x8& m, nl_s16x8& l)
+{
+    unsigned top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) top = max(top, __float_as_uint(x[j]) & 0x7FFFFFFFu);
+    const bool plain = top < 0x7F7F8000u;                             // nothing whose rounding overflows, no infinity, no NaN
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        unsigned short a = nl_f2bf(x[j]), b, c;
+        const float r = x[j] - nl_bf2f(a);
+        b = nl_f2bf(r);
+        c = nl_f2bf(r - nl_bf2f(b));
+        h[j] = (short)a; m[j] = (short)b; l[j] = (short)c;
+    }
+    if (!plain)
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            unsigned short a = nl_f2bf(x[j]), b = 0, c = 0;
+            if (fabsf(x[j]) < INFINITY) {                             // cut instead of rounded where rounding leaves the range
+                if ((a & 0x7F80) == 0x7F80) a = (unsigned short)(__float_as_uint(x[j]) >> 16);
+                const float r = x[j] - nl_bf2f(a);
+                b = nl_f2bf(r);
+                c = nl_f2bf(r - nl_bf2f(b));
+            }
+            h[j] = (short)a; m[j] = (short)b; l[j] = (short)c;
+        }
+}
+
+// One fp32 operand: R rows or columns x 32 contraction indices per step, 256 threads; the planes' layout in LDS is GemmSide's
+template <bool SLOW, int R>
+struct GemmSide32 {
+    typedef GemmSide<SLOW, R, 256, 32> Plane;
+    static constexpr int UNITS = R * 32 / (8 * 256), BYTES = 3 * Plane::BYTES;         // a unit: eight neighbouring elements in memory
+    unsigned off[UNITS]; int kk[UNITS], lds[UNITS]; bool half[UNITS];                   // half: only the first four elements are inside (slow: columns)
+    float v[UNITS][8];
+    const char* base; long long step;
+
+    __device__ __forceinline__ void init(const char* p, long long ld, long long i0, long long I, long long k0)
+    {
+#pragma unroll
+        for (int u = 0; u < UNITS; u++) {
+            const int s = u * 256 + threadIdx.x;
+            if (SLOW) {
+                const int k = s / (R / 8), c = s % (R / 8);
+                kk[u] = k; half[u] = i0 + 8 * c + 4 >= I;
+                off[u] = i0 + 8 * c < I ? (unsigned)(k * ld + 32 * c) : GEMM_OUT_OF_RANGE;
+                lds[u] = k * (R * 2) + (c ^ (Plane::swz(k) << 1)) * 16;
+            } else {
+                const int r = s >> 2, c = s & 3;
+                kk[u] = 8 * c; half[u] = false;
+                off[u] = i0 + r < I ? (unsigned)(r * ld + 32 * c) : GEMM_OUT_OF_RANGE;
+                lds[u] = r * 64 + (c ^ Plane::swz_row(r)) * 16;
+            }
+        }
+        base = SLOW ? p + k0 * ld + 4 * i0 : p + i0 * ld + 4 * k0;
+        step = SLOW ? 32 * ld : 128;
+    }
+    __device__ __forceinline__ void fetch(long long adv, long long kleft)
+    {
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(base + adv), 0, (int)GEMM_RANGE, 0x00020000);
+#pragma unroll
+        for (int u = 0; u < UNITS; u++) {
+            const bool in = kk[u] < kleft, in2 = SLOW ? in && !half[u] : kk[u] + 4 < kleft;
+            const nl_i32x4 a = __builtin_bit_cast(nl_i32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)(in ? off[u] : GEMM_OUT_OF_RANGE), 0, 0));
+            const nl_i32x4 b = __builtin_bit_cast(nl_i32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)(in2 && off[u] != GEMM_OUT_OF_RANGE ? off[u] + 16 : GEMM_OUT_OF_RANGE), 0, 0));
+#pragma unroll
+            for (int j = 0; j < 4; j++) { v[u][j] = __int_as_float(a[j]); v[u][4 + j] = __int_as_float(b[j]); }
+        }
+    }
+    __device__ __forceinline__ void put(char* mem) const
+    {
+#pragma unroll
+        for (int u = 0; u < UNITS; u++) {
+            nl_s16x8 p[3];
+            gemm_split8(v[u], p[0], p[1], p[2]);
+#pragma unroll
+            for (int q = 0; q < 3; q++) *reinterpret_cast<nl_s16x8*>(mem + q * Plane::BYTES + lds[u]) = p[q];
+        }
+    }
+};
+
+template <bool A_SLOW, bool B_SLOW, int BT>
+__global__ __launch_bounds__(256, 2) void k_gemm_f32(NlGemm g)
+{
+    typedef GemmSide32<A_SLOW, BT> SA;
+    typedef GemmSide32<B_SLOW, BT> SB;
+    constexpr int F = BT / 32, LDS = SA::BYTES + SB::BYTES;
+    __shared__ __align__(256) char s_mem[LDS > BT * BT * 4 ? LDS : BT * BT * 4];
+    char* const s_b = s_mem + SA::BYTES;
+    long long m0; int n0;
+    gemm_tile_of<BT, BT>(g, m0, n0);
+    const long long k0 = (long long)blockIdx.y * g.kchunk, k1 = min(k0 + g.kchunk, g.K), span = k1 - k0;
+    const int steps = (int)((span + 31) / 32);
+    SA a; SB b;
+    a.init(g.A, g.lda, m0, g.M, k0);
+    b.init(g.B, g.ldb, n0, g.N, k0);
+    const int wave = threadIdx.x >> 6, wm = (wave >> 1) * (BT / 2), wn = (wave & 1) * (BT / 2);
+    nl_f32x4 acc[F][F] = {};
+    a.fetch(0, span);
+    b.fetch(0, span);
+    for (int s = 0; s < steps; s++) {
+        a.put(s_mem);
+        b.put(s_b);
+        nl_lds_barrier();
+        if (s + 1 < steps) {
+            a.fetch((s + 1) * a.step, span - (s + 1) * 32LL);
+            b.fetch((s + 1) * b.step, span - (s + 1) * 32LL);
+        }
+        nl_s16x8 fa[3][F], fb[3][F];
+#pragma unroll
+        for (int p = 2; p >= 0; p--) {
+#pragma unroll
+            for (int i = 0; i < F; i++) fa[p][i] = SA::Plane::frag(s_mem + p * SA::Plane::BYTES, wm + 16 * i, 0);
+#pragma unroll
+            for (int i = 0; i < F; i++) fb[2 - p][i] = SB::Plane::frag(s_b + (2 - p) * SB::Plane::BYTES, wn + 16 * i, 0);
+        }
+#pragma unroll
+        for (int sum = 2; sum >= 0; sum--)
+#pragma unroll
+            for (int p = sum; p >= 0; p--)
+#pragma unroll
+                for (int i = 0; i < F; i++)
+#pragma unroll
+                    for (int j = 0; j < F; j++) acc[i][j] = NlMma<__bf16>::mma(fb[sum - p][j], fa[p][i], acc[i][j]);
+        nl_lds_barrier();
+    }
+    gemm_results<NL_DT_F32, BT / 2, BT / 2, 4, sizeof(s_mem)>(g, acc, s_mem, m0 + wm, n0 + wn);
+}
+
+template <bool A_SLOW, bool B_SLOW>
+static void nl_gemm_tile_f32(const NlGemm& g, int tile, dim3 grid, hipStream_t st)
+{
+    if (tile == 1) hipLaunchKernelGGL((k_gemm_f32<A_SLOW, B_SLOW, 128>), grid, dim3(256), 0, st, g);
+    else hipLaunchKernelGGL((k_gemm_f32<A_SLOW, B_SLOW, 64>), grid, dim3(256), 0, st, g);
+}
+
+template <class T, bool A_SLOW, bool B_SLOW>
 static void nl_gemm_tile(const NlGemm& g, int tile, dim3 grid, hipStream_t st)
 {
-    if (tile == 0) hipLaunchKernelGGL((k_gemm<T, PLANES, A_SLOW, B_SLOW, 256, 256, 2, 4>), grid, dim3(512), 0, st, g);
-    else if (tile == 1) hipLaunchKernelGGL((k_gemm<T, PLANES, A_SLOW, B_SLOW, 128, 128, 2, 2>), grid, dim3(256), 0, st, g);
-    else hipLaunchKernelGGL((k_gemm<T, PLANES, A_SLOW, B_SLOW, 64, 64, 2, 2>), grid, dim3(256), 0, st, g);
+    if (tile == 0) hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, 256, 256, 2, 4>), grid, dim3(512), 0, st, g);
+    else if (tile == 1) hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, 128, 128, 2, 2>), grid, dim3(256), 0, st, g);
+    else hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, 64, 64, 2, 2>), grid, dim3(256), 0, st, g);
 }
-template <class T, bool PLANES>
+template <class T>
 static void nl_gemm_layout(const NlGemm& g, int layout, int tile, dim3 grid, hipStream_t st)
 {
-    if (layout == 0) nl_gemm_tile<T, PLANES, false, false>(g, tile, grid, st);
-    else if (layout == 1) nl_gemm_tile<T, PLANES, false, true>(g, tile, grid, st);
-    else nl_gemm_tile<T, PLANES, true, true>(g, tile, grid, st);
+    if (layout == 0) nl_gemm_tile<T, false, false>(g, tile, grid, st);
+    else if (layout == 1) nl_gemm_tile<T, false, true>(g, tile, grid, st);
+    else nl_gemm_tile<T, true, true>(g, tile, grid, st);
 }
 #endif

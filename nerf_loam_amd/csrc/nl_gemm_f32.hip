@@ -1,4 +1,9 @@
 // nl_gemm_f32.hip -- the tiled product of nl_gemm.h for float32 (six bf16 products of exact splits)
 #include "nl_gemm.h"
 
-void nl_gemm_f32(const NlGemm& g, int layout, int tile, dim3 grid, hipStream_t st) { nl_gemm_layout<__bf16, true>(g, layout, tile, grid, st); }
+void nl_gemm_f32(const NlGemm& g, int layout, int tile, dim3 grid, hipStream_t st)
+{
+    if (layout == 0) nl_gemm_tile_f32<false, false>(g, tile, grid, st);
+    else if (layout == 1) nl_gemm_tile_f32<false, true>(g, tile, grid, st);
+    else nl_gemm_tile_f32<true, true>(g, tile, grid, st);
+}

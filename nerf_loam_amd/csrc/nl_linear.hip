@@ -4,44 +4,11 @@
 #include "nl_gemm.h"
 
 // ---------------------------------------------------------------------------------------------
-// k_linear_pack: an operand as the tiled products want it - 16-bit elements, rows of up(cols, 8) elements with zeros behind the last column - from rows of any
-// stride and alignment, from fp32 (three planes) or from 8-bit codes.  Runs only where the operand does not lie that way already.
-// fp32: x = h + m + l, three bf16 numbers to nearest, exact (8 bits each of 24); of the nine products of two such numbers the six down to 2^-18 are summed, the
-// smallest first (l h, h l, m m, m h, h m, h h).  What is dropped (m l, l m, l l) is below 2^-26 |x||w|.
+// k_linear_pack: an operand as the tiled products want it - rows of up(cols, 8) elements with zeros behind the last column - from rows of any stride and
+// alignment, or from 8-bit codes.  Runs only where the operand does not lie that way already.
 // ---------------------------------------------------------------------------------------------
-struct NlPack { const void* src; const unsigned char* e; unsigned short* dst; long long rows, ld, pitch, plane; int cols; };
+struct NlPack { const void* src; const unsigned char* e; void* dst; long long rows, ld, pitch; int cols; };
 
-// x = h + m + l; a value whose rounding would overflow is cut instead, an infinity or NaN stays in h alone
-__device__ __forceinline__ void nl_split3(float x, unsigned short& h, unsigned short& m, unsigned short& l)
-{
-    h = nl_f2bf(x);
-    if ((h & 0x7F80) == 0x7F80) {
-        if (!(fabsf(x) < INFINITY)) { m = l = 0; return; }
-        h = (unsigned short)(__float_as_uint(x) >> 16);
-    }
-    const float r = x - nl_bf2f(h);
-    m = nl_f2bf(r);
-    l = nl_f2bf(r - nl_bf2f(m));
-}
-// eight values to their place in a packed operand (DT: the tensors' type)
-template <int DT> __device__ __forceinline__ void nl_put_packed(unsigned short* dst, long long at, long long plane, const float* v)
-{
-    nl_s16x8 o[3];
-    if (DT == NL_DT_F32) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            unsigned short h, m, l;
-            nl_split3(v[j], h, m, l);
-            o[0][j] = (short)h; o[1][j] = (short)m; o[2][j] = (short)l;
-        }
-        *reinterpret_cast<nl_s16x8*>(dst + plane + at) = o[1];
-        *reinterpret_cast<nl_s16x8*>(dst + 2 * plane + at) = o[2];
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; j++) o[0][j] = (short)(DT == NL_DT_BF16 ? nl_f2bf(v[j]) : nl_f2h(v[j]));
-    }
-    *reinterpret_cast<nl_s16x8*>(dst + at) = o[0];
-}
 template <int DT, bool MX8>
 __global__ __launch_bounds__(256) void k_linear_pack(NlPack a)
 {
@@ -58,7 +25,7 @@ __global__ __launch_bounds__(256) void k_linear_pack(NlPack a)
 #pragma unroll
             for (int j = 0; j < 4; j++) { v[j] = p[j]; v[4 + j] = q[j]; }
         } else nl_load8<DT>(v, a.src, r * a.ld + c, a.cols - c, vec);
-        nl_put_packed<DT>(a.dst, r * a.pitch + c, a.plane, v);
+        nl_store8<DT>(a.dst, r * a.pitch + c, v, 8, true);
     }
 }
 
@@ -96,8 +63,8 @@ __global__ __launch_bounds__(256) void k_linear_join(const float* __restrict__ p
 // ---------------------------------------------------------------------------------------------
 struct NlDz {
     const void* gy; const void* z; const unsigned* bits; const unsigned char* z8; const unsigned char* z8e;
-    unsigned short* dz; float* part;
-    long long M, ldgy, ldz, ldbits, ldz8, ldz8e, pitch, plane, rows_per_chunk;
+    void* dz; float* part;
+    long long M, ldgy, ldz, ldbits, ldz8, ldz8e, pitch, rows_per_chunk;
     int N;
 };
 template <int DT, int ACT>
@@ -130,7 +97,7 @@ __global__ __launch_bounds__(256) void k_linear_dz(NlDz a)
             }
 #pragma unroll
             for (int j = 0; j < 8; j++) sum[j] += g[j];
-            if (a.dz) nl_put_packed<DT>(a.dz, m * a.pitch + n, a.plane, g);
+            if (a.dz) nl_store8<DT>(a.dz, m * a.pitch + n, g, 8, true);
         }
     if (!a.part) return;
 #pragma unroll
@@ -184,22 +151,27 @@ struct NlWork {
     char* take(long long bytes) { char* p = base + used; used += nl_up(bytes, 256); return p; }
 };
 
-// a packed operand: rows x cols, 16-bit elements
-struct NlPacked { const unsigned short* p; long long pitch, plane, rows; int cols; };
+// a packed operand: rows `pitch` elements apart, zeros behind the last column up to a multiple of 8 (4 where an fp32 operand is used in place)
+struct NlPacked { const void* p; long long pitch; };
 
 static unsigned nl_grid(long long threads) { const long long b = (threads + 255) / 256; return (unsigned)(b < 1 ? 1 : b < 16384 ? b : 16384); }
 
+static bool nl_in_place(const void* p, int cols, long long ld, int dt)
+{
+    const int v = dt == NL_DT_F32 ? 4 : 8;
+    return ld % v == 0 && cols % v == 0 && ld <= NL_LINEAR_MAX_WIDTH && ((uintptr_t)p & 15) == 0;
+}
 static NlPacked nl_packed(NlWork& w, const void* p, const unsigned char* e, long long rows, int cols, long long ld, int type, int dt)
 {
-    if (type == dt && dt != NL_DT_F32 && (ld & 7) == 0 && ld <= NL_LINEAR_MAX_WIDTH && (cols & 7) == 0 && ((uintptr_t)p & 15) == 0) return NlPacked{(const unsigned short*)p, ld, 0, rows, cols};
+    if (type == dt && nl_in_place(p, cols, ld, dt)) return NlPacked{p, ld};
     NlPack a = {};
     a.src = p; a.e = e; a.rows = rows; a.cols = cols; a.ld = ld;
-    a.pitch = nl_up(cols, 8); a.plane = nl_up(rows * a.pitch, 128);
-    a.dst = (unsigned short*)w.take(2 * a.plane * (dt == NL_DT_F32 ? 3 : 1));
+    a.pitch = nl_up(cols, 8);
+    a.dst = w.take(rows * a.pitch * nl_dtype_size(dt));
     const dim3 grid(nl_grid(rows * (a.pitch / 8)));
     if (!w.dry) NL_WITH_DTYPE(dt, if (type == NL_DT_MX8) hipLaunchKernelGGL((k_linear_pack<DT, true>), grid, dim3(256), 0, w.st, a);
                                   else hipLaunchKernelGGL((k_linear_pack<DT, false>), grid, dim3(256), 0, w.st, a));
-    return NlPacked{a.dst, a.pitch, a.plane, rows, cols};
+    return NlPacked{a.dst, a.pitch};
 }
 
 // How a product [M,N] over K is cut: the tile, and into how many pieces the contraction goes.  The estimate behind it: workgroups that run at a time, the time of
@@ -207,11 +179,12 @@ static NlPacked nl_packed(NlWork& w, const void* p, const unsigned char* e, long
 struct NlCut { int tile, splits; long long kchunk; };
 static NlCut nl_cut(long long M, long long N, long long K, int dt)
 {
-    static const struct { int size, at_a_time; double step, rest; } T[3] = {{256, 256, 1.25, 4.0}, {128, 512, 0.85, 3.0}, {64, 1024, 0.50, 2.5}};      // microseconds
+    static const struct { int size, at_a_time; double step, rest; } T16[3] = {{256, 256, 1.25, 4.0}, {128, 512, 0.85, 3.0}, {64, 1024, 0.50, 2.5}},       // microseconds
+                                                                     T32[3] = {{256, 1, 1e9, 1e9}, {128, 512, 4.0, 4.0}, {64, 512, 1.6, 3.0}}, *T = dt == NL_DT_F32 ? T32 : T16;
     const long long ksteps = (K + GEMM_BK - 1) / GEMM_BK;
     NlCut best = {0, 1, 0};
     double least = 1e30;
-    for (int t = 0; t < 3; t++) {
+    for (int t = dt == NL_DT_F32 ? 1 : 0; t < 3; t++) {
         const long long tiles = nl_up(M, T[t].size) / T[t].size * (nl_up(N, T[t].size) / T[t].size);
         for (int s = 1; s <= 256; s *= 2) {
             if (s > 1 && (ksteps / s < 2 || 4.0 * s * M * N > 1.5e9)) break;
@@ -219,7 +192,7 @@ static NlCut nl_cut(long long M, long long N, long long K, int dt)
             const double rounds = (double)((tiles * s + T[t].at_a_time - 1) / T[t].at_a_time), full = tiles * s < T[t].at_a_time ? (double)(tiles * s) / T[t].at_a_time : 1.0;
             // fewer workgroups than fit share a compute unit with fewer others: their steps take less long
             const double step = T[t].step * (0.5 + 0.5 * full);
-            double us = rounds * (per * (dt == NL_DT_F32 ? 6 : 1) * step + T[t].rest);
+            double us = rounds * (per * step + T[t].rest);
             if (s > 1) us += 4.0 + 8.0 * s * M * N / 3.5e6;
             if (us < least) { least = us; best = NlCut{t, s, per * GEMM_BK}; }
         }
@@ -234,7 +207,7 @@ static void nl_product(NlWork& w, const NlPacked& A, const NlPacked& B, int layo
     const NlCut c = nl_cut(M, N, K, ep.dt);
     static const int size[3] = {256, 128, 64};
     NlGemm g = {};
-    g.A = (const char*)A.p; g.B = (const char*)B.p; g.lda = 2 * A.pitch; g.ldb = 2 * B.pitch; g.a_plane = 2 * A.plane; g.b_plane = 2 * B.plane;
+    g.A = (const char*)A.p; g.B = (const char*)B.p; g.lda = nl_dtype_size(ep.dt) * A.pitch; g.ldb = nl_dtype_size(ep.dt) * B.pitch;
     g.M = M; g.N = N; g.K = K; g.kchunk = c.kchunk;
     const long long tm = nl_up(M, size[c.tile]) / size[c.tile], tn = nl_up(N, size[c.tile]) / size[c.tile];
     if (tm * tn > 0x7FFFFFFF) { w.rc = NL_ERR_INVALID_ARG; return; }
@@ -263,9 +236,9 @@ static void nl_forward_run(const NlLinear* d, NlWork& w)
 
 static void nl_backward_run(const NlLinear* d, NlWork& w)
 {
-    const bool in_place = d->act == NL_ACT_NONE && d->dtype != NL_DT_F32 && (d->N & 7) == 0 && (d->ldgy & 7) == 0 && d->ldgy <= NL_LINEAR_MAX_WIDTH && ((uintptr_t)d->gy & 15) == 0;
+    const bool in_place = d->act == NL_ACT_NONE && nl_in_place(d->gy, d->N, d->ldgy, d->dtype);
     const bool products = d->gx || d->gw;
-    NlPacked dz = {(const unsigned short*)d->gy, d->ldgy, 0, d->M, d->N};
+    NlPacked dz = {d->gy, d->ldgy};
     if (d->gb || (products && !in_place)) {
         NlDz a = {};
         a.gy = d->gy; a.ldgy = d->ldgy; a.M = d->M; a.N = d->N;
@@ -280,9 +253,9 @@ static void nl_backward_run(const NlLinear* d, NlWork& w)
         chunks = (d->M + a.rows_per_chunk - 1) / a.rows_per_chunk;
         if (d->gb) a.part = (float*)w.take(4LL * chunks * d->N);
         if (products && !in_place) {
-            a.pitch = nl_up(d->N, 8); a.plane = nl_up(d->M * a.pitch, 128);
-            a.dz = (unsigned short*)w.take(2 * a.plane * (d->dtype == NL_DT_F32 ? 3 : 1));
-            dz = NlPacked{a.dz, a.pitch, a.plane, d->M, d->N};
+            a.pitch = nl_up(d->N, 8);
+            a.dz = w.take(d->M * a.pitch * nl_dtype_size(d->dtype));
+            dz = NlPacked{a.dz, a.pitch};
         }
         if (!w.dry) {
             const dim3 grid(colblocks, (unsigned)chunks);
