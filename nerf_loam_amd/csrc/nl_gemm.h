@@ -201,32 +201,44 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
 // 50 us more on reading them).  A thread fetches a step's elements into registers while the step before it multiplies, splits them and writes three planes; two
 // workgroups share a compute unit, so that one splits (vector unit) while the other multiplies.  Six products: at most a sixth of the bf16 rate.
 // ---------------------------------------------------------------------------------------------
-__device__ __forceinline__ void gemm_split8(const float* x, nl_s16x8& h, nl_s16x8& m, nl_s16x8& l)
+// two values to bf16, to nearest, in the halves of a word
+__device__ __forceinline__ unsigned gemm_pack2(float a, float b)
+{
+    typedef __attribute__((__vector_size__(2 * sizeof(float)))) float F2;
+    typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 B2;
+    return __builtin_bit_cast(unsigned, __builtin_convertvector((F2{a, b}), B2));
+}
+__device__ __forceinline__ void gemm_split8(const float* x, nl_i32x4& h, nl_i32x4& m, nl_i32x4& l)
 {
     unsigned top = 0;
 #pragma unroll
     for (int j = 0; j < 8; j++) top = max(top, __float_as_uint(x[j]) & 0x7FFFFFFFu);
-    const bool plain = top < 0x7F7F8000u;                             // nothing whose rounding overflows, no infinity, no NaN
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        unsigned short a = nl_f2bf(x[j]), b, c;
-        const float r = x[j] - nl_bf2f(a);
-        b = nl_f2bf(r);
-        c = nl_f2bf(r - nl_bf2f(b));
-        h[j] = (short)a; m[j] = (short)b; l[j] = (short)c;
+    for (int j = 0; j < 4; j++) {                                     // 11 instructions a pair
+        const unsigned a = gemm_pack2(x[2 * j], x[2 * j + 1]);
+        const float r0 = x[2 * j] - __uint_as_float(a << 16), r1 = x[2 * j + 1] - __uint_as_float(a & 0xFFFF0000u);
+        const unsigned b = gemm_pack2(r0, r1);
+        h[j] = (int)a; m[j] = (int)b;
+        l[j] = (int)gemm_pack2(r0 - __uint_as_float(b << 16), r1 - __uint_as_float(b & 0xFFFF0000u));
     }
-    if (!plain)
+    if (top < 0x7F7F8000u) return;
+    // rounding overflows, an infinity or a NaN somewhere: the first part cut instead of rounded (as exact); what is not finite stays in it alone
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            unsigned short a = nl_f2bf(x[j]), b = 0, c = 0;
-            if (fabsf(x[j]) < INFINITY) {                             // cut instead of rounded where rounding leaves the range
-                if ((a & 0x7F80) == 0x7F80) a = (unsigned short)(__float_as_uint(x[j]) >> 16);
-                const float r = x[j] - nl_bf2f(a);
-                b = nl_f2bf(r);
-                c = nl_f2bf(r - nl_bf2f(b));
-            }
-            h[j] = (short)a; m[j] = (short)b; l[j] = (short)c;
+    for (int j = 0; j < 4; j++) {
+        unsigned a[2];
+        float r[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const float v = x[2 * j + i];
+            const unsigned u = __float_as_uint(v);
+            const bool finite = (u & 0x7F800000u) != 0x7F800000u;
+            a[i] = finite ? u >> 16 : (unsigned)nl_f2bf(v);
+            r[i] = finite ? v - __uint_as_float(u & 0xFFFF0000u) : 0.0f;
         }
+        const unsigned b = gemm_pack2(r[0], r[1]);
+        h[j] = (int)(a[0] | a[1] << 16); m[j] = (int)b;
+        l[j] = (int)gemm_pack2(r[0] - __uint_as_float(b << 16), r[1] - __uint_as_float(b & 0xFFFF0000u));
+    }
 }
 
 // One fp32 operand: R rows or columns x 32 contraction indices per step, 256 threads; the planes' layout in LDS is GemmSide's
@@ -274,10 +286,10 @@ struct GemmSide32 {
     {
 #pragma unroll
         for (int u = 0; u < UNITS; u++) {
-            nl_s16x8 p[3];
+            nl_i32x4 p[3];
             gemm_split8(v[u], p[0], p[1], p[2]);
 #pragma unroll
-            for (int q = 0; q < 3; q++) *reinterpret_cast<nl_s16x8*>(mem + q * Plane::BYTES + lds[u]) = p[q];
+            for (int q = 0; q < 3; q++) *reinterpret_cast<nl_i32x4*>(mem + q * Plane::BYTES + lds[u]) = p[q];
         }
     }
 };
@@ -309,6 +321,7 @@ __global__ __launch_bounds__(256, 2) void k_gemm_f32(NlGemm g)
             a.fetch((s + 1) * a.step, span - (s + 1) * 32LL);
             b.fetch((s + 1) * b.step, span - (s + 1) * 32LL);
         }
+        __builtin_amdgcn_sched_barrier(0);
         nl_s16x8 fa[3][F], fb[3][F];
 #pragma unroll
         for (int p = 2; p >= 0; p--) {

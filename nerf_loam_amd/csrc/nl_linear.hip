@@ -3,6 +3,8 @@
 // Reference behaviour: torch.nn.Linear + ReLU of the decoder (/root/reference/src/variations/lidar.py:105-123), any width, any depth.
 #include "nl_gemm.h"
 
+#include <math.h>
+
 // ---------------------------------------------------------------------------------------------
 // k_linear_pack: an operand as the tiled products want it - rows of up(cols, 8) elements with zeros behind the last column - from rows of any stride and
 // alignment, or from 8-bit codes.  Runs only where the operand does not lie that way already.
@@ -30,30 +32,49 @@ __global__ __launch_bounds__(256) void k_linear_pack(NlPack a)
 }
 
 // ---------------------------------------------------------------------------------------------
-// k_linear_join: sums the pieces of a split contraction in their order and runs the epilogue.
+// k_linear_join: sums the pieces of a split contraction and runs the epilogue.  Eight columns a thread, whole blocks of 32 columns.  With few results and many pieces
+// one thread per result group would walk all pieces one memory latency after the other (256 x 256 results in 64 pieces: 30 us): then RUNS threads sum a run of
+// neighbouring pieces each and the runs are added in order.
 // ---------------------------------------------------------------------------------------------
-template <int DT>
+template <int DT, int RUNS>
 __global__ __launch_bounds__(256) void k_linear_join(const float* __restrict__ part, int splits, long long M, int N, NlEpilogue ep)
 {
-    const long long per_row = (N + 31) / 32 * 4, total = M * per_row;          // eight columns a thread, whole blocks of 32 columns
-    for (long long t0 = (long long)blockIdx.x * 256; t0 < total; t0 += (long long)gridDim.x * 256) {
-        const long long t = t0 + threadIdx.x, m = t / per_row;
+    constexpr int POS = 256 / RUNS;
+    __shared__ float s_sum[RUNS > 1 ? RUNS : 1][RUNS > 1 ? POS : 1][9];
+    const int at = threadIdx.x % POS, run = threadIdx.x / POS, per = (splits + RUNS - 1) / RUNS;
+    const int s0 = run * per, s1 = s0 + per < splits ? s0 + per : splits;
+    const long long per_row = (N + 31) / 32 * 4, total = M * per_row;
+    for (long long t0 = (long long)blockIdx.x * POS; t0 < total; t0 += (long long)gridDim.x * POS) {
+        const long long t = t0 + at, m = t / per_row;
         const int n = (int)(t - m * per_row) * 8;
         float v[8] = {};
         if (m < M) {
-            const float* p = part + m * N + n;
-            if (n + 7 < N && (N & 3) == 0)
-                for (int s = 0; s < splits; s++, p += M * N) {
+            const float* p = part + (long long)s0 * M * N + m * N + n;
+            if (n + 7 < N && (N & 3) == 0) {
+#pragma unroll 4
+                for (int s = s0; s < s1; s++, p += M * N) {
                     const nl_f32x4 a = *reinterpret_cast<const nl_f32x4*>(p), b = *reinterpret_cast<const nl_f32x4*>(p + 4);
 #pragma unroll
                     for (int j = 0; j < 4; j++) { v[j] += a[j]; v[4 + j] += b[j]; }
                 }
-            else
-                for (int s = 0; s < splits; s++, p += M * N)
+            } else
+                for (int s = s0; s < s1; s++, p += M * N)
 #pragma unroll
                     for (int j = 0; j < 8; j++) if (n + j < N) v[j] += p[j];
         }
-        nl_epilogue8<DT>(ep, v, m, n, M, N, 0);
+        if (RUNS > 1) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) s_sum[run][at][j] = v[j];
+            __syncthreads();
+            if (run == 0) {
+#pragma unroll
+                for (int r = 1; r < RUNS; r++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) v[j] += s_sum[r][at][j];
+                nl_epilogue8<DT>(ep, v, m, n, M, N, 0);
+            }
+            __syncthreads();
+        } else nl_epilogue8<DT>(ep, v, m, n, M, N, 0);
     }
 }
 
@@ -174,26 +195,31 @@ static NlPacked nl_packed(NlWork& w, const void* p, const unsigned char* e, long
     return NlPacked{a.dst, a.pitch};
 }
 
-// How a product [M,N] over K is cut: the tile, and into how many pieces the contraction goes.  The estimate behind it: workgroups that run at a time, the time of
-// a contraction step of 64 and of what surrounds the steps, and for a cut contraction the pieces' way through memory and the launch that joins them.
+// How a product [M,N] over K is cut: the tile, and into how many pieces the contraction goes.  The estimate: rounds of as many workgroups as run at a time, each with
+// its contraction steps of 64 (alone on a compute unit / with as many neighbours as fit) and what surrounds them; for a cut contraction the pieces' way through memory
+// and the launch that joins them.  Measured, in microseconds (bf16, 4096^3: 94 in squares of 256, 112 of 128, 172 of 64; 2048 x 256 x 256: 15, 7.7, 4.4; 256 x 256 x
+// 200000: 58 in 256 pieces of the first, 68 in 64 of the second, 87 in 32 of the third, 4200 uncut; fp32 4096^3: 576 in squares of 128, 665 of 64, 2048 x 256 x 256:
+// 21, 9.8).  The estimate's choice is within 15 % of the best of all tiles and powers of two at the 23 shapes of either kind that these come from.
 struct NlCut { int tile, splits; long long kchunk; };
-static NlCut nl_cut(long long M, long long N, long long K, int dt)
+static NlCut nl_cut(long long M, long long N, long long K, int dt, int layout)
 {
-    static const struct { int size, at_a_time; double step, rest; } T16[3] = {{256, 256, 1.25, 4.0}, {128, 512, 0.85, 3.0}, {64, 1024, 0.50, 2.5}},       // microseconds
-                                                                     T32[3] = {{256, 1, 1e9, 1e9}, {128, 512, 4.0, 4.0}, {64, 512, 1.6, 3.0}}, *T = dt == NL_DT_F32 ? T32 : T16;
+    struct Tile { int size, at_a_time; double alone, full, rest, slow; };       // slow: on the steps where both operands' rows are the contraction (narrow rows of a tile)
+    static const Tile T16[3] = {{256, 256, 1.33, 1.40, 9.0, 1.0}, {128, 512, 0.70, 0.87, 4.0, 1.25}, {64, 1024, 0.50, 0.67, 2.0, 1.4}};
+    static const Tile T32[3] = {{256, 0, 0, 0, 0, 0}, {128, 512, 3.95, 4.50, 4.0, 1.0}, {64, 1024, 1.67, 2.60, 2.5, 1.1}};
+    const Tile* T = dt == NL_DT_F32 ? T32 : T16;
     const long long ksteps = (K + GEMM_BK - 1) / GEMM_BK;
-    NlCut best = {0, 1, 0};
-    double least = 1e30;
+    const double memory = (double)nl_dtype_size(dt) * (M * K + N * K + M * N) / 4.5e6;
+    NlCut best = {1, 1, ksteps * GEMM_BK};
+    double least = 1e300;
     for (int t = dt == NL_DT_F32 ? 1 : 0; t < 3; t++) {
-        const long long tiles = nl_up(M, T[t].size) / T[t].size * (nl_up(N, T[t].size) / T[t].size);
-        for (int s = 1; s <= 256; s *= 2) {
-            if (s > 1 && (ksteps / s < 2 || 4.0 * s * M * N > 1.5e9)) break;
+        const double tiles = (double)(nl_up(M, T[t].size) / T[t].size) * (double)(nl_up(N, T[t].size) / T[t].size);
+        for (int s = 1; s <= 256 && s <= ksteps; s *= 2) {
+            if (s > 1 && 4.0 * s * M * N > 1.5e9) break;
             const long long per = (ksteps + s - 1) / s;
-            const double rounds = (double)((tiles * s + T[t].at_a_time - 1) / T[t].at_a_time), full = tiles * s < T[t].at_a_time ? (double)(tiles * s) / T[t].at_a_time : 1.0;
-            // fewer workgroups than fit share a compute unit with fewer others: their steps take less long
-            const double step = T[t].step * (0.5 + 0.5 * full);
-            double us = rounds * (per * step + T[t].rest);
-            if (s > 1) us += 4.0 + 8.0 * s * M * N / 3.5e6;
+            const double at = tiles * s / T[t].at_a_time, full = at < 1.0 ? at : 1.0, rounds = at < 1.0 ? 1.0 : at < 4.0 ? ceil(at) : at + 0.5;
+            double us = rounds * (per * (T[t].alone + (T[t].full - T[t].alone) * full) * (layout == 2 ? T[t].slow : 1.0) + T[t].rest * (0.5 + 0.5 * full));
+            if (us < memory) us = memory;
+            if (s > 1) us += 3.0 + 8.0 * s * M * N / 4.0e6;
             if (us < least) { least = us; best = NlCut{t, s, per * GEMM_BK}; }
         }
     }
@@ -204,7 +230,7 @@ static NlCut nl_cut(long long M, long long N, long long K, int dt)
 // C[M,N] = sum_k A(m,k) B(n,k).  layout 0: both operands' rows run along k; 1: B's rows are k; 2: both operands' rows are k
 static void nl_product(NlWork& w, const NlPacked& A, const NlPacked& B, int layout, long long M, int N, long long K, const NlEpilogue& ep)
 {
-    const NlCut c = nl_cut(M, N, K, ep.dt);
+    const NlCut c = nl_cut(M, N, K, ep.dt, layout);
     static const int size[3] = {256, 128, 64};
     NlGemm g = {};
     g.A = (const char*)A.p; g.B = (const char*)B.p; g.lda = nl_dtype_size(ep.dt) * A.pitch; g.ldb = nl_dtype_size(ep.dt) * B.pitch;
@@ -219,7 +245,11 @@ static void nl_product(NlWork& w, const NlPacked& A, const NlPacked& B, int layo
     if (ep.dt == NL_DT_F32) nl_gemm_f32(g, layout, c.tile, grid, w.st);
     else if (ep.dt == NL_DT_BF16) nl_gemm_bf16(g, layout, c.tile, grid, w.st);
     else nl_gemm_f16(g, layout, c.tile, grid, w.st);
-    if (c.splits > 1) NL_WITH_DTYPE(ep.dt, hipLaunchKernelGGL(k_linear_join<DT>, dim3(nl_grid(M * ((N + 31) / 32 * 4))), dim3(256), 0, w.st, g.ep.part, c.splits, M, N, ep));
+    if (c.splits > 1) {
+        const long long groups = M * ((N + 31) / 32 * 4);
+        if (c.splits >= 8 && groups < 131072) NL_WITH_DTYPE(ep.dt, hipLaunchKernelGGL((k_linear_join<DT, 8>), dim3(nl_grid(8 * groups)), dim3(256), 0, w.st, g.ep.part, c.splits, M, N, ep));
+        else NL_WITH_DTYPE(ep.dt, hipLaunchKernelGGL((k_linear_join<DT, 1>), dim3(nl_grid(groups)), dim3(256), 0, w.st, g.ep.part, c.splits, M, N, ep));
+    }
     if (hipGetLastError() != hipSuccess) w.rc = NL_ERR_LAUNCH;
 }
 
