@@ -97,26 +97,37 @@ struct GemmSide {
     }
 };
 
-// workgroups go to the eight dies in turn: give each die neighbouring tiles, four tile rows at a time, so that its L2 holds what it shares
-template <int BM, int BN> __device__ __forceinline__ void gemm_tile_of(const NlGemm& g, long long& m0, int& n0)
+// Workgroups go to the eight dies in turn: give each die neighbouring work - the tiles of one piece of the contraction, four tile rows at a time - so that its L2 holds
+// what it shares (256 x 256 over 200000 in 64 pieces, squares of 64, pieces dealt out across dies: 114 us).  -> the piece
+template <int BM, int BN> __device__ __forceinline__ unsigned gemm_tile_of(const NlGemm& g, long long& m0, int& n0)
 {
-    const unsigned tiles = (unsigned)g.tiles_m * g.tiles_n, q = tiles >> 3, rem = tiles & 7, die = blockIdx.x & 7;
-    unsigned pid = die * q + (die < rem ? die : rem) + (blockIdx.x >> 3);
+    const unsigned tiles = (unsigned)g.tiles_m * g.tiles_n, total = tiles * gridDim.y, id = blockIdx.y * tiles + blockIdx.x;
+    const unsigned q = total >> 3, rem = total & 7, die = id & 7, at = die * q + (die < rem ? die : rem) + (id >> 3);
+    const unsigned piece = at / tiles;
+    unsigned pid = at - piece * tiles;
     const unsigned per_group = 4u * g.tiles_n, grp = pid / per_group, first = 4 * grp, rows = min(4u, (unsigned)g.tiles_m - first);
     pid -= grp * per_group;
     m0 = (long long)(first + pid % rows) * BM;
     n0 = (int)(pid / rows) * BN;
+    return piece;
 }
 
 // Results of a wave, WR rows x WC columns from (m, n) on: it passes them through its own part of LDS, RP rows at a time, and leaves with eight neighbouring columns
 // in a lane (16-byte stores, and the neighbours that bits and 8-bit blocks need).  16-byte chunks XORed with the row: neither side of the exchange has bank conflicts.
 template <int DT, int WR, int WC, int WAVES, int LDS>
-__device__ __forceinline__ void gemm_results(const NlGemm& g, nl_f32x4 (&acc)[WR / 16][WC / 16], char* s_mem, long long m, int n)
+__device__ __forceinline__ void gemm_results(const NlGemm& g, nl_f32x4 (&acc)[WR / 16][WC / 16], char* s_mem, long long m, int n, unsigned piece)
 {
     constexpr int RP = WR < 64 ? WR : 64, CX = WC / 4 - 1;
     static_assert((CX & (CX + 1)) == 0 && RP * WC * 4 * WAVES <= LDS, "the exchange fits into the operand buffers");
-    const int lane = threadIdx.x & 63;
+    constexpr int TURNS = RP * WC / 512, BATCH = TURNS < 4 ? TURNS : 4;
+    static_assert(64 % (WC / 8) == 0 && TURNS % BATCH == 0, "a lane keeps its columns");
+    const NlEpilogue& ep = g.ep;
+    const int lane = threadIdx.x & 63, col = n + 8 * (lane % (WC / 8));
     char* const mine = s_mem + (threadIdx.x >> 6) * (RP * WC * 4);
+    const bool inside = m + WR <= g.M && n + WC <= g.N && (ep.part ? (g.N & 3) == 0 : nl_rows_aligned<DT>(ep.y, ep.ldy) && (!ep.r || nl_rows_aligned<DT>(ep.r, ep.ldr)) &&
+                                                           (!ep.b || nl_rows_aligned<DT>(ep.b, 0)) && (!ep.z || (ep.ldz & 7) == 0));
+    float bias[8] = {};
+    if (inside && !ep.part && ep.b) nl_unraw8<DT>(bias, nl_raw8<DT>(ep.b, col));
 #pragma unroll
     for (int half = 0; half < WR / RP; half++) {
 #pragma unroll
@@ -127,13 +138,38 @@ __device__ __forceinline__ void gemm_results(const NlGemm& g, nl_f32x4 (&acc)[WR
                 *reinterpret_cast<nl_f32x4*>(mine + r * (WC * 4) + c * 16) = acc[half * (RP / 16) + i][j];
             }
         __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-        for (int t = lane; t < RP * WC / 8; t += 64) {
+        auto value = [&](int t, float* v) {
             const int r = t / (WC / 8), c = 2 * (t % (WC / 8));
             const nl_f32x4 p = *reinterpret_cast<const nl_f32x4*>(mine + r * (WC * 4) + (c ^ (r & CX)) * 16);
             const nl_f32x4 q = *reinterpret_cast<const nl_f32x4*>(mine + r * (WC * 4) + ((c + 1) ^ (r & CX)) * 16);
-            float v[8] = {p[0], p[1], p[2], p[3], q[0], q[1], q[2], q[3]};
-            nl_epilogue8<DT>(g.ep, v, m + half * RP + r, n + 4 * c, g.M, g.N, (long long)blockIdx.y * g.M * g.N);
+#pragma unroll
+            for (int j = 0; j < 4; j++) { v[j] = p[j]; v[4 + j] = q[j]; }
+        };
+        const long long off = (long long)piece * g.M * g.N;
+        if (inside) {
+            // four rows of residuals in flight: one load and its use at a time leaves a memory latency per row (200000 x 256 x 256 with residual: 137 us)
+#pragma unroll 1
+            for (int t0 = lane; t0 < RP * WC / 8; t0 += 64 * BATCH) {
+                NlRaw8<DT> raw[BATCH];
+                if (ep.r) {
+#pragma unroll
+                    for (int u = 0; u < BATCH; u++) raw[u] = nl_raw8<DT>(ep.r, (m + half * RP + (t0 + 64 * u) / (WC / 8)) * ep.ldr + col);
+                }
+#pragma unroll
+                for (int u = 0; u < BATCH; u++) {
+                    float v[8], r[8];
+                    value(t0 + 64 * u, v);
+                    if (ep.r) nl_unraw8<DT>(r, raw[u]);
+                    nl_epilogue8<DT, true>(ep, v, bias, r, m + half * RP + (t0 + 64 * u) / (WC / 8), col, g.M, g.N, off);
+                }
+            }
+        } else {
+#pragma unroll 1
+            for (int t = lane; t < RP * WC / 8; t += 64) {
+                float v[8];
+                value(t, v);
+                nl_epilogue8_fetch<DT>(ep, v, m + half * RP + t / (WC / 8), col, g.M, g.N, off);
+            }
         }
         __builtin_amdgcn_wave_barrier();
     }
@@ -150,8 +186,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
     char* const s_a = s_mem;
     char* const s_b = s_mem + 2 * SA::BYTES;
     long long m0; int n0;
-    gemm_tile_of<BM, BN>(g, m0, n0);
-    const long long k0 = (long long)blockIdx.y * g.kchunk, k1 = min(k0 + g.kchunk, g.K);
+    const unsigned piece = gemm_tile_of<BM, BN>(g, m0, n0);
+    const long long k0 = (long long)piece * g.kchunk, k1 = min(k0 + g.kchunk, g.K);
     const int steps = (int)((k1 - k0 + GEMM_BK - 1) / GEMM_BK);
     SA a; SB b;
     a.init(g.A, g.lda, m0, g.M, k0, g.K);
@@ -191,7 +227,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
             for (int j = 0; j < FN; j++) acc[i][j] = NlMma<T>::mma(fb[1][j], fa[1][i], acc[i][j]);
         __syncthreads();
     }
-    gemm_results<DT, BM / WM, BN / WN, WM * WN, 2 * (SA::BYTES + SB::BYTES)>(g, acc, s_mem, m0 + wm, n0 + wn);
+    gemm_results<DT, BM / WM, BN / WN, WM * WN, 2 * (SA::BYTES + SB::BYTES)>(g, acc, s_mem, m0 + wm, n0 + wn, piece);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -303,8 +339,8 @@ __global__ __launch_bounds__(256, 2) void k_gemm_f32(NlGemm g)
     __shared__ __align__(256) char s_mem[LDS > BT * BT * 4 ? LDS : BT * BT * 4];
     char* const s_b = s_mem + SA::BYTES;
     long long m0; int n0;
-    gemm_tile_of<BT, BT>(g, m0, n0);
-    const long long k0 = (long long)blockIdx.y * g.kchunk, k1 = min(k0 + g.kchunk, g.K), span = k1 - k0;
+    const unsigned piece = gemm_tile_of<BT, BT>(g, m0, n0);
+    const long long k0 = (long long)piece * g.kchunk, k1 = min(k0 + g.kchunk, g.K), span = k1 - k0;
     const int steps = (int)((span + 31) / 32);
     SA a; SB b;
     a.init(g.A, g.lda, m0, g.M, k0);
@@ -340,7 +376,7 @@ __global__ __launch_bounds__(256, 2) void k_gemm_f32(NlGemm g)
                     for (int j = 0; j < F; j++) acc[i][j] = NlMma<__bf16>::mma(fb[sum - p][j], fa[p][i], acc[i][j]);
         nl_lds_barrier();
     }
-    gemm_results<NL_DT_F32, BT / 2, BT / 2, 4, sizeof(s_mem)>(g, acc, s_mem, m0 + wm, n0 + wn);
+    gemm_results<NL_DT_F32, BT / 2, BT / 2, 4, sizeof(s_mem)>(g, acc, s_mem, m0 + wm, n0 + wn, piece);
 }
 
 template <bool A_SLOW, bool B_SLOW>

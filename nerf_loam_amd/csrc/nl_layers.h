@@ -190,21 +190,39 @@ __device__ __forceinline__ void nl_act8(float* v, int act)
         for (int j = 0; j < 8; j++) v[j] = nl_act(v[j], NL_ACT_SILU);
     }
 }
-template <int DT> __device__ __forceinline__ void nl_epilogue8(const NlEpilogue& ep, float* v, long long m, int n, long long M, int N, long long split_off)
+// eight elements of a row as they lie in memory, aligned (nl_rows_aligned): fetched early, converted where they are used
+template <int DT> struct NlRaw8 { nl_i32x4 w[DT == NL_DT_F32 ? 2 : 1]; };
+template <int DT> __device__ __forceinline__ NlRaw8<DT> nl_raw8(const void* p, long long i)
 {
-    const bool row = m < M, live = row && n < N;
-    const int lane = threadIdx.x & 63, left = N - n;
+    NlRaw8<DT> o;
+    const nl_i32x4* q = reinterpret_cast<const nl_i32x4*>((const char*)p + i * (DT == NL_DT_F32 ? 4 : 2));
+    o.w[0] = q[0];
+    if constexpr (DT == NL_DT_F32) o.w[1] = q[1];
+    return o;
+}
+template <int DT> __device__ __forceinline__ void nl_unraw8(float* v, const NlRaw8<DT>& r)
+{
+    if constexpr (DT == NL_DT_F32) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = __int_as_float(r.w[j >> 2][j & 3]);
+    } else {
+        const nl_s16x8 u = __builtin_bit_cast(nl_s16x8, r.w[0]);
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = DT == NL_DT_BF16 ? nl_bf2f((unsigned short)u[j]) : nl_h2f((unsigned short)u[j]);
+    }
+}
+// b, r: the bias and the residual of the eight columns, zeros where there is none.  INSIDE: the wave's rows and columns all are inside the result and its tensors' rows are
+// aligned, no lane asks
+template <int DT, bool INSIDE> __device__ __forceinline__ void nl_epilogue8(const NlEpilogue& ep, float* v, const float* b, const float* r, long long m, int n, long long M, int N, long long split_off)
+{
+    const bool row = INSIDE || m < M, live = INSIDE || (row && n < N);
+    const int lane = threadIdx.x & 63, left = INSIDE ? 8 : N - n;
     if (ep.part) {
-        if (live) nl_store8<NL_DT_F32>(ep.part + split_off, m * N + n, v, left, (N & 3) == 0);
+        if (live) nl_store8<NL_DT_F32>(ep.part + split_off, m * N + n, v, left, INSIDE || (N & 3) == 0);
         return;
     }
-    float r[8], b[8];
-    if (ep.r && live) nl_load8<DT>(r, ep.r, m * ep.ldr + n, left, nl_rows_aligned<DT>(ep.r, ep.ldr));
-    if (ep.b && live) {
-        nl_load8<DT>(b, ep.b, n, left, nl_rows_aligned<DT>(ep.b, 0));
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] += b[j];
-    }
+    for (int j = 0; j < 8; j++) v[j] += b[j];
     if (ep.bits) {                                                // one bit per element: z > 0
         unsigned w = 0;
 #pragma unroll
@@ -228,13 +246,23 @@ template <int DT> __device__ __forceinline__ void nl_epilogue8(const NlEpilogue&
         }
     }
     if (!live) return;
-    if (ep.z) nl_store8<DT>(ep.z, m * ep.ldz + n, v, left, (ep.ldz & 7) == 0);
+    if (ep.z) nl_store8<DT>(ep.z, m * ep.ldz + n, v, left, INSIDE || (ep.ldz & 7) == 0);
     nl_act8(v, ep.act);
     if (ep.r) {
 #pragma unroll
         for (int j = 0; j < 8; j++) v[j] += r[j];
     }
-    nl_store8<DT>(ep.y, m * ep.ldy + n, v, left, nl_rows_aligned<DT>(ep.y, ep.ldy));
+    nl_store8<DT>(ep.y, m * ep.ldy + n, v, left, INSIDE || nl_rows_aligned<DT>(ep.y, ep.ldy));
+}
+// the same with bias and residual fetched on the spot
+template <int DT> __device__ __forceinline__ void nl_epilogue8_fetch(const NlEpilogue& ep, float* v, long long m, int n, long long M, int N, long long split_off)
+{
+    float b[8] = {}, r[8] = {};
+    if (!ep.part && m < M && n < N) {
+        if (ep.r) nl_load8<DT>(r, ep.r, m * ep.ldr + n, N - n, nl_rows_aligned<DT>(ep.r, ep.ldr));
+        if (ep.b) nl_load8<DT>(b, ep.b, n, N - n, nl_rows_aligned<DT>(ep.b, 0));
+    }
+    nl_epilogue8<DT, false>(ep, v, b, r, m, n, M, N, split_off);
 }
 // a kernel launch (or any statement) with the type as a compile-time constant DT
 #define NL_WITH_DTYPE(dt, ...)                                                            \

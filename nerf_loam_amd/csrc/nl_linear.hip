@@ -71,10 +71,10 @@ __global__ __launch_bounds__(256) void k_linear_join(const float* __restrict__ p
                 for (int r = 1; r < RUNS; r++)
 #pragma unroll
                     for (int j = 0; j < 8; j++) v[j] += s_sum[r][at][j];
-                nl_epilogue8<DT>(ep, v, m, n, M, N, 0);
+                nl_epilogue8_fetch<DT>(ep, v, m, n, M, N, 0);
             }
             __syncthreads();
-        } else nl_epilogue8<DT>(ep, v, m, n, M, N, 0);
+        } else nl_epilogue8_fetch<DT>(ep, v, m, n, M, N, 0);
     }
 }
 
@@ -204,7 +204,7 @@ struct NlCut { int tile, splits; long long kchunk; };
 static NlCut nl_cut(long long M, long long N, long long K, int dt, int layout)
 {
     struct Tile { int size, at_a_time; double alone, full, rest, slow; };       // slow: on the steps where both operands' rows are the contraction (narrow rows of a tile)
-    static const Tile T16[3] = {{256, 256, 1.33, 1.40, 9.0, 1.0}, {128, 512, 0.70, 0.87, 4.0, 1.25}, {64, 1024, 0.50, 0.67, 2.0, 1.4}};
+    static const Tile T16[3] = {{256, 256, 1.33, 1.40, 9.0, 1.0}, {128, 512, 0.70, 0.87, 4.0, 1.1}, {64, 1024, 0.50, 0.67, 2.0, 1.2}};
     static const Tile T32[3] = {{256, 0, 0, 0, 0, 0}, {128, 512, 3.95, 4.50, 4.0, 1.0}, {64, 1024, 1.67, 2.60, 2.5, 1.1}};
     const Tile* T = dt == NL_DT_F32 ? T32 : T16;
     const long long ksteps = (K + GEMM_BK - 1) / GEMM_BK;
@@ -236,7 +236,7 @@ static void nl_product(NlWork& w, const NlPacked& A, const NlPacked& B, int layo
     g.A = (const char*)A.p; g.B = (const char*)B.p; g.lda = nl_dtype_size(ep.dt) * A.pitch; g.ldb = nl_dtype_size(ep.dt) * B.pitch;
     g.M = M; g.N = N; g.K = K; g.kchunk = c.kchunk;
     const long long tm = nl_up(M, size[c.tile]) / size[c.tile], tn = nl_up(N, size[c.tile]) / size[c.tile];
-    if (tm * tn > 0x7FFFFFFF) { w.rc = NL_ERR_INVALID_ARG; return; }
+    if (tm * tn > 0x7FFFFFF) { w.rc = NL_ERR_INVALID_ARG; return; }
     g.tiles_m = (int)tm; g.tiles_n = (int)tn;
     g.ep = ep;
     if (c.splits > 1) { g.ep = NlEpilogue{}; g.ep.part = (float*)w.take(4LL * c.splits * M * N); }
