@@ -11,6 +11,7 @@
 
 struct NlGemm {
     const char* A; const char* B;      // 16-byte aligned, rows 16-byte aligned
+    const unsigned char* Be;           // B in 8-bit codes: its powers of two, ldb / 32 bytes between rows
     long long lda, ldb;                // bytes between rows
     long long M, K;
     int N, tiles_m, tiles_n;
@@ -18,7 +19,7 @@ struct NlGemm {
     NlEpilogue ep;
 };
 
-// layout 0: both operands' rows run along k; 1: B's rows are k; 2: both operands' rows are k.  tile 0: 256 x 256 (16 bits only), 1: 128 x 128, 2: 64 x 64.
+// layout 0: both operands' rows run along k; 1: B's rows are k; 2: both operands' rows are k; 3: the same with B in 8-bit codes (16-bit types only).  tile 0: 256 x 256 (16 bits only), 1: 128 x 128, 2: 64 x 64.
 void nl_gemm_bf16(const NlGemm& g, int layout, int tile, dim3 grid, hipStream_t st);
 void nl_gemm_f16(const NlGemm& g, int layout, int tile, dim3 grid, hipStream_t st);
 void nl_gemm_f32(const NlGemm& g, int layout, int tile, dim3 grid, hipStream_t st);
@@ -175,7 +176,68 @@ __device__ __forceinline__ void gemm_results(const NlGemm& g, nl_f32x4 (&acc)[WR
     }
 }
 
-template <class T, bool A_SLOW, bool B_SLOW, int BM, int BN, int WM, int WN>
+// An operand in 8-bit codes whose rows are the contraction: R columns x 64 indices per step.  A thread fetches 16 neighbouring codes and their power of two while the
+// step before multiplies, decodes them (exactly: four significant bits) and writes them where GemmSide would have put the 16-bit elements.
+template <class T, int R, int NT>
+struct GemmSideMx8 {
+    typedef GemmSide<true, R, NT> Plane;
+    static constexpr int BYTES = Plane::BYTES, UNITS = R * GEMM_BK / (16 * NT), CH = R / 16;
+    unsigned off[UNITS], eoff[UNITS]; int kk[UNITS], lds[UNITS];
+    nl_i32x4 v[UNITS]; unsigned char e[UNITS];
+    const char* base; const unsigned char* ebase; long long step;
+
+    __device__ __forceinline__ void init(const char* p, const unsigned char* pe, long long ld, long long i0, long long I, long long k0)
+    {
+#pragma unroll
+        for (int u = 0; u < UNITS; u++) {
+            const int s = u * NT + threadIdx.x, k = s / CH, c = s % CH;
+            const bool in = i0 + 16 * c < I;                          // (rows of codes are whole blocks of 32)
+            kk[u] = k;
+            off[u] = in ? (unsigned)(k * ld + 16 * c) : GEMM_OUT_OF_RANGE;
+            eoff[u] = in ? (unsigned)(k * (ld / 32) + c / 2) : GEMM_OUT_OF_RANGE;
+            lds[u] = k * (R * 2) + ((2 * c) ^ (Plane::swz(k) << 1)) * 16;
+        }
+        base = p + k0 * ld + i0; ebase = pe + k0 * (ld / 32) + i0 / 32;
+        step = GEMM_BK * ld;
+    }
+    __device__ __forceinline__ void fetch(int s, long long kleft)
+    {
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(base + s * step), 0, (int)GEMM_RANGE, 0x00020000);
+        const __amdgpu_buffer_rsrc_t re = __builtin_amdgcn_make_buffer_rsrc((void*)(ebase + s * (step / 32)), 0, (int)GEMM_RANGE, 0x00020000);
+#pragma unroll
+        for (int u = 0; u < UNITS; u++) {
+            const bool in = kleft >= GEMM_BK || kk[u] < kleft;
+            v[u] = __builtin_bit_cast(nl_i32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)(in ? off[u] : GEMM_OUT_OF_RANGE), 0, 0));
+            e[u] = __builtin_amdgcn_raw_buffer_load_b8(re, (int)(in ? eoff[u] : GEMM_OUT_OF_RANGE), 0, 0);
+        }
+    }
+    __device__ __forceinline__ void put(char* mem) const
+    {
+        constexpr bool F16 = __is_same(T, _Float16);
+#pragma unroll
+        for (int u = 0; u < UNITS; u++) {
+            const float s = nl_mx_scale(e[u]);
+            nl_i32x4 o[2];
+            if (e[u] < (F16 ? 127 + 8 : 127 + 120)) {                 // 448 2^e is inside the type
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) o[j >> 1][2 * (j & 1) + h] = F16 ? __builtin_bit_cast(int, h ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v[u][j], s, true) : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v[u][j], s, false))
+                                                                                 : __builtin_bit_cast(int, h ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[u][j], s, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[u][j], s, false));
+            } else
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const nl_f32x4 f = nl_mx_decode4((unsigned)v[u][j], s, nl_dtype_max(F16 ? NL_DT_F16 : NL_DT_BF16));
+#pragma unroll
+                    for (int h = 0; h < 2; h++) o[j >> 1][2 * (j & 1) + h] = (int)(F16 ? (unsigned)nl_f2h(f[2 * h]) | (unsigned)nl_f2h(f[2 * h + 1]) << 16 : (unsigned)nl_f2bf(f[2 * h]) | (unsigned)nl_f2bf(f[2 * h + 1]) << 16);
+                }
+            *reinterpret_cast<nl_i32x4*>(mem + lds[u]) = o[0];
+            *reinterpret_cast<nl_i32x4*>(mem + lds[u] + 16) = o[1];
+        }
+    }
+};
+
+template <class T, bool A_SLOW, bool B_SLOW, bool B_MX8, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
 {
     constexpr int DT = __is_same(T, _Float16) ? NL_DT_F16 : NL_DT_BF16;
@@ -190,16 +252,20 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
     const long long k0 = (long long)piece * g.kchunk, k1 = min(k0 + g.kchunk, g.K);
     const int steps = (int)((k1 - k0 + GEMM_BK - 1) / GEMM_BK);
     SA a; SB b;
+    GemmSideMx8<T, BN, NT> b8;
     a.init(g.A, g.lda, m0, g.M, k0, g.K);
-    b.init(g.B, g.ldb, n0, g.N, k0, g.K);
+    if (B_MX8) b8.init(g.B, g.Be, g.ldb, n0, g.N, k0);
+    else b.init(g.B, g.ldb, n0, g.N, k0, g.K);
     const int wave = threadIdx.x >> 6, wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
     nl_f32x4 acc[FM][FN] = {};
     auto fetch = [&](int s) {
         const long long left = k1 - k0 - (long long)s * GEMM_BK;
         a.load(s_a + (s & 1) * SA::BYTES, s * a.step, left);
-        b.load(s_b + (s & 1) * SB::BYTES, s * b.step, left);
+        if (B_MX8) b8.fetch(s, left);
+        else b.load(s_b + (s & 1) * SB::BYTES, s * b.step, left);
     };
     fetch(0);
+    if (B_MX8) b8.put(s_b);
     __builtin_amdgcn_s_waitcnt(0);
     __builtin_amdgcn_s_barrier();
     for (int s = 0; s < steps; s++) {
@@ -225,6 +291,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
         for (int i = 0; i < FM; i++)
 #pragma unroll
             for (int j = 0; j < FN; j++) acc[i][j] = NlMma<T>::mma(fb[1][j], fa[1][i], acc[i][j]);
+        if (B_MX8 && s + 1 < steps) b8.put(s_b + ((s + 1) & 1) * SB::BYTES);
         __syncthreads();
     }
     gemm_results<DT, BM / WM, BN / WN, WM * WN, 2 * (SA::BYTES + SB::BYTES)>(g, acc, s_mem, m0 + wm, n0 + wn, piece);
@@ -386,18 +453,19 @@ static void nl_gemm_tile_f32(const NlGemm& g, int tile, dim3 grid, hipStream_t s
     else hipLaunchKernelGGL((k_gemm_f32<A_SLOW, B_SLOW, 64>), grid, dim3(256), 0, st, g);
 }
 
-template <class T, bool A_SLOW, bool B_SLOW>
+template <class T, bool A_SLOW, bool B_SLOW, bool B_MX8>
 static void nl_gemm_tile(const NlGemm& g, int tile, dim3 grid, hipStream_t st)
 {
-    if (tile == 0) hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, 256, 256, 2, 4>), grid, dim3(512), 0, st, g);
-    else if (tile == 1) hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, 128, 128, 2, 2>), grid, dim3(256), 0, st, g);
-    else hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, 64, 64, 2, 2>), grid, dim3(256), 0, st, g);
+    if (tile == 0) hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, B_MX8, 256, 256, 2, 4>), grid, dim3(512), 0, st, g);
+    else if (tile == 1) hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, B_MX8, 128, 128, 2, 2>), grid, dim3(256), 0, st, g);
+    else hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, B_MX8, 64, 64, 2, 2>), grid, dim3(256), 0, st, g);
 }
 template <class T>
 static void nl_gemm_layout(const NlGemm& g, int layout, int tile, dim3 grid, hipStream_t st)
 {
-    if (layout == 0) nl_gemm_tile<T, false, false>(g, tile, grid, st);
-    else if (layout == 1) nl_gemm_tile<T, false, true>(g, tile, grid, st);
-    else nl_gemm_tile<T, true, true>(g, tile, grid, st);
+    if (layout == 0) nl_gemm_tile<T, false, false, false>(g, tile, grid, st);
+    else if (layout == 1) nl_gemm_tile<T, false, true, false>(g, tile, grid, st);
+    else if (layout == 2) nl_gemm_tile<T, true, true, false>(g, tile, grid, st);
+    else nl_gemm_tile<T, true, true, true>(g, tile, grid, st);
 }
 #endif

@@ -7,7 +7,7 @@
 
 // ---------------------------------------------------------------------------------------------
 // k_linear_pack: an operand as the tiled products want it - rows of up(cols, 8) elements with zeros behind the last column - from rows of any stride and
-// alignment, or from 8-bit codes.  Runs only where the operand does not lie that way already.
+// alignment, or (fp32) from 8-bit codes.  Runs only where the operand does not lie that way already.
 // ---------------------------------------------------------------------------------------------
 struct NlPack { const void* src; const unsigned char* e; void* dst; long long rows, ld, pitch; int cols; };
 
@@ -173,7 +173,7 @@ struct NlWork {
 };
 
 // a packed operand: rows `pitch` elements apart, zeros behind the last column up to a multiple of 8 (4 where an fp32 operand is used in place)
-struct NlPacked { const void* p; long long pitch; };
+struct NlPacked { const void* p; long long pitch; const unsigned char* e; };      // e: 8-bit codes and their powers of two instead
 
 static unsigned nl_grid(long long threads) { const long long b = (threads + 255) / 256; return (unsigned)(b < 1 ? 1 : b < 16384 ? b : 16384); }
 
@@ -184,15 +184,16 @@ static bool nl_in_place(const void* p, int cols, long long ld, int dt)
 }
 static NlPacked nl_packed(NlWork& w, const void* p, const unsigned char* e, long long rows, int cols, long long ld, int type, int dt)
 {
-    if (type == dt && nl_in_place(p, cols, ld, dt)) return NlPacked{p, ld};
+    if (type == dt && nl_in_place(p, cols, ld, dt)) return NlPacked{p, ld, nullptr};
     NlPack a = {};
     a.src = p; a.e = e; a.rows = rows; a.cols = cols; a.ld = ld;
     a.pitch = nl_up(cols, 8);
     a.dst = w.take(rows * a.pitch * nl_dtype_size(dt));
     const dim3 grid(nl_grid(rows * (a.pitch / 8)));
-    if (!w.dry) NL_WITH_DTYPE(dt, if (type == NL_DT_MX8) hipLaunchKernelGGL((k_linear_pack<DT, true>), grid, dim3(256), 0, w.st, a);
-                                  else hipLaunchKernelGGL((k_linear_pack<DT, false>), grid, dim3(256), 0, w.st, a));
-    return NlPacked{a.dst, a.pitch};
+    if (w.dry) ;
+    else if (type == NL_DT_MX8) hipLaunchKernelGGL((k_linear_pack<NL_DT_F32, true>), grid, dim3(256), 0, w.st, a);
+    else NL_WITH_DTYPE(dt, hipLaunchKernelGGL((k_linear_pack<DT, false>), grid, dim3(256), 0, w.st, a));
+    return NlPacked{a.dst, a.pitch, nullptr};
 }
 
 // How a product [M,N] over K is cut: the tile, and into how many pieces the contraction goes.  The estimate: rounds of as many workgroups as run at a time, each with
@@ -217,7 +218,7 @@ static NlCut nl_cut(long long M, long long N, long long K, int dt, int layout)
             if (s > 1 && 4.0 * s * M * N > 1.5e9) break;
             const long long per = (ksteps + s - 1) / s;
             const double at = tiles * s / T[t].at_a_time, full = at < 1.0 ? at : 1.0, rounds = at < 1.0 ? 1.0 : at < 4.0 ? ceil(at) : at + 0.5;
-            double us = rounds * (per * (T[t].alone + (T[t].full - T[t].alone) * full) * (layout == 2 ? T[t].slow : 1.0) + T[t].rest * (0.5 + 0.5 * full));
+            double us = rounds * (per * (T[t].alone + (T[t].full - T[t].alone) * full) * (layout >= 2 ? T[t].slow : 1.0) + T[t].rest * (0.5 + 0.5 * full));
             if (us < memory) us = memory;
             if (s > 1) us += 3.0 + 8.0 * s * M * N / 4.0e6;
             if (us < least) { least = us; best = NlCut{t, s, per * GEMM_BK}; }
@@ -227,13 +228,13 @@ static NlCut nl_cut(long long M, long long N, long long K, int dt, int layout)
     return best;
 }
 
-// C[M,N] = sum_k A(m,k) B(n,k).  layout 0: both operands' rows run along k; 1: B's rows are k; 2: both operands' rows are k
+// C[M,N] = sum_k A(m,k) B(n,k).  layout 0: both operands' rows run along k; 1: B's rows are k; 2: both operands' rows are k; 3: the same with B in 8-bit codes
 static void nl_product(NlWork& w, const NlPacked& A, const NlPacked& B, int layout, long long M, int N, long long K, const NlEpilogue& ep)
 {
     const NlCut c = nl_cut(M, N, K, ep.dt, layout);
     static const int size[3] = {256, 128, 64};
     NlGemm g = {};
-    g.A = (const char*)A.p; g.B = (const char*)B.p; g.lda = nl_dtype_size(ep.dt) * A.pitch; g.ldb = nl_dtype_size(ep.dt) * B.pitch;
+    g.A = (const char*)A.p; g.B = (const char*)B.p; g.Be = B.e; g.lda = nl_dtype_size(ep.dt) * A.pitch; g.ldb = layout == 3 ? B.pitch : nl_dtype_size(ep.dt) * B.pitch;
     g.M = M; g.N = N; g.K = K; g.kchunk = c.kchunk;
     const long long tm = nl_up(M, size[c.tile]) / size[c.tile], tn = nl_up(N, size[c.tile]) / size[c.tile];
     if (tm * tn > 0x7FFFFFF) { w.rc = NL_ERR_INVALID_ARG; return; }
@@ -268,7 +269,7 @@ static void nl_backward_run(const NlLinear* d, NlWork& w)
 {
     const bool in_place = d->act == NL_ACT_NONE && nl_in_place(d->gy, d->N, d->ldgy, d->dtype);
     const bool products = d->gx || d->gw;
-    NlPacked dz = {d->gy, d->ldgy};
+    NlPacked dz = {d->gy, d->ldgy, nullptr};
     if (d->gb || (products && !in_place)) {
         NlDz a = {};
         a.gy = d->gy; a.ldgy = d->ldgy; a.M = d->M; a.N = d->N;
@@ -285,7 +286,7 @@ static void nl_backward_run(const NlLinear* d, NlWork& w)
         if (products && !in_place) {
             a.pitch = nl_up(d->N, 8);
             a.dz = w.take(d->M * a.pitch * nl_dtype_size(d->dtype));
-            dz = NlPacked{a.dz, a.pitch};
+            dz = NlPacked{a.dz, a.pitch, nullptr};
         }
         if (!w.dry) {
             const dim3 grid(colblocks, (unsigned)chunks);
@@ -308,8 +309,10 @@ static void nl_backward_run(const NlLinear* d, NlWork& w)
     }
     if (d->gw) {
         ep.y = d->gw;
-        const NlPacked x = d->x8 ? nl_packed(w, d->x8, d->x8e, d->M, d->K, nl_up(d->K, 32), NL_DT_MX8, d->dtype) : nl_packed(w, d->x, nullptr, d->M, d->K, d->ldx, d->dtype, d->dtype);
-        nl_product(w, dz, x, 2, d->N, d->K, d->M, ep);
+        const bool codes = d->x8 && d->dtype != NL_DT_F32;               // (fp32 splits its operands: codes are decoded to fp32 first)
+        const NlPacked x = codes ? NlPacked{d->x8, nl_up(d->K, 32), d->x8e}
+                         : d->x8 ? nl_packed(w, d->x8, d->x8e, d->M, d->K, nl_up(d->K, 32), NL_DT_MX8, d->dtype) : nl_packed(w, d->x, nullptr, d->M, d->K, d->ldx, d->dtype, d->dtype);
+        nl_product(w, dz, x, codes ? 3 : 2, d->N, d->K, d->M, ep);
     }
     if (w.used < most) w.used = most;
 }
