@@ -10,17 +10,20 @@
 // alignment, or (fp32) from 8-bit codes.  Runs only where the operand does not lie that way already.
 // ---------------------------------------------------------------------------------------------
 struct NlPack { const void* src; const unsigned char* e; void* dst; long long rows, ld, pitch; int cols; };
+struct NlPack2 { NlPack p[2]; };                                     // one launch for both operands of a product, or both of a backward pass
 
-template <int DT, bool MX8>
-__global__ __launch_bounds__(256) void k_linear_pack(NlPack a)
+template <int DT>
+__global__ __launch_bounds__(256) void k_linear_pack(NlPack2 both)
 {
+    const NlPack a = both.p[blockIdx.y];
+    const bool mx8 = DT == NL_DT_F32 && a.e;
     const long long per_row = a.pitch / 8, total = a.rows * per_row;
     const bool vec = nl_rows_aligned<DT>(a.src, a.ld);
     for (long long t = (long long)blockIdx.x * 256 + threadIdx.x; t < total; t += (long long)gridDim.x * 256) {
         const long long r = t / per_row;
         const int c = (int)(t - r * per_row) * 8;
         float v[8];
-        if (MX8) {
+        if (mx8) {
             const nl_i32x2 w = *reinterpret_cast<const nl_i32x2*>((const unsigned char*)a.src + r * a.ld + c);       // (rows of codes are whole blocks of 32, zeros behind the last)
             const float s = nl_mx_scale(a.e[r * (a.ld / 32) + (c >> 5)]);
             const nl_f32x4 p = nl_mx_decode4((unsigned)w[0], s, nl_dtype_max(DT)), q = nl_mx_decode4((unsigned)w[1], s, nl_dtype_max(DT));
@@ -29,6 +32,88 @@ __global__ __launch_bounds__(256) void k_linear_pack(NlPack a)
         } else nl_load8<DT>(v, a.src, r * a.ld + c, a.cols - c, vec);
         nl_store8<DT>(a.dst, r * a.pitch + c, v, 8, true);
     }
+}
+
+// ---------------------------------------------------------------------------------------------
+// k_linear_rows: a few rows of x (at most ROWS_MOST) that keep nothing for a backward pass: the call that answers single queries.  It reads the weight once and computes
+// little, so no tile: a group of `lanes` threads takes two rows of the weight, eight neighbouring elements a thread at a time, several loads in flight, and sums
+// across its threads at the end.  One launch (1 x 4096 x 4096 bf16: 8 us, as tiles of 64 cut 16 times and joined 10).
+// ---------------------------------------------------------------------------------------------
+#define ROWS_MOST 8
+template <int DT, int MR>
+__global__ __launch_bounds__(256) void k_linear_rows(const void* __restrict__ x, long long ldx, const void* __restrict__ w, long long ldw, int M, int N, int K, int lanes, NlEpilogue ep)
+{
+    constexpr int R = 2, U = MR == 1 ? 4 : MR <= 4 ? 2 : 1;
+    const int lane = threadIdx.x & (lanes - 1), n0 = (int)(blockIdx.x * (256 / lanes) + threadIdx.x / lanes) * R;
+    if (n0 >= N) return;                                              // (a whole group)
+    const int n1 = n0 + 1 < N ? n0 + 1 : n0;
+    const bool vec = nl_rows_aligned<DT>(w, ldw) && nl_rows_aligned<DT>(x, ldx) && (K & 7) == 0;
+    float acc[MR][R] = {};
+    int k = lane * 8;
+    if (vec)
+        for (; k + (U - 1) * lanes * 8 < K; k += U * lanes * 8) {
+            NlRaw8<DT> a[U][R], b[U][MR];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                a[u][0] = nl_raw8<DT>(w, (long long)n0 * ldw + k + u * lanes * 8);
+                a[u][1] = nl_raw8<DT>(w, (long long)n1 * ldw + k + u * lanes * 8);
+#pragma unroll
+                for (int m = 0; m < MR; m++) b[u][m] = nl_raw8<DT>(x, (m < M ? m : 0) * ldx + k + u * lanes * 8);
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                float p[R][8];
+                nl_unraw8<DT>(p[0], a[u][0]);
+                nl_unraw8<DT>(p[1], a[u][1]);
+#pragma unroll
+                for (int m = 0; m < MR; m++) {
+                    float q[8];
+                    nl_unraw8<DT>(q, b[u][m]);
+#pragma unroll
+                    for (int r = 0; r < R; r++)
+#pragma unroll
+                        for (int j = 0; j < 8; j++) acc[m][r] = __builtin_fmaf(p[r][j], q[j], acc[m][r]);
+                }
+            }
+        }
+    for (; k < K; k += lanes * 8) {
+        float p[R][8];
+        nl_load8<DT>(p[0], w, (long long)n0 * ldw + k, K - k, vec);
+        nl_load8<DT>(p[1], w, (long long)n1 * ldw + k, K - k, vec);
+#pragma unroll
+        for (int m = 0; m < MR; m++) {
+            float q[8];
+            nl_load8<DT>(q, x, (m < M ? m : 0) * ldx + k, K - k, vec);
+#pragma unroll
+            for (int r = 0; r < R; r++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) acc[m][r] = __builtin_fmaf(p[r][j], q[j], acc[m][r]);
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < MR; m++)
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            float v = acc[m][r];
+            for (int off = lanes >> 1; off > 0; off >>= 1) v += __shfl_xor(v, off);
+            const int n = n0 + r;
+            if (lane != 0 || m >= M || n >= N) continue;
+            if (ep.b) v += nl_load_elem<DT>(ep.b, n);
+            v = nl_act(v, ep.act);
+            if (ep.r) v += nl_load_elem<DT>(ep.r, m * ep.ldr + n);
+            nl_store_elem<DT>(ep.y, m * ep.ldy + n, v);
+        }
+}
+template <int DT> static void nl_launch_rows(const NlLinear* d, const NlEpilogue& ep, hipStream_t st)
+{
+    int lanes = 8;
+    while (lanes < 64 && lanes * 8 < d->K) lanes *= 2;
+    const dim3 grid((unsigned)((d->N + 2 * (256 / lanes) - 1) / (2 * (256 / lanes))));
+    const int M = (int)d->M;
+    if (M == 1) hipLaunchKernelGGL((k_linear_rows<DT, 1>), grid, dim3(256), 0, st, d->x, d->ldx, d->w, d->ldw, M, d->N, d->K, lanes, ep);
+    else if (M == 2) hipLaunchKernelGGL((k_linear_rows<DT, 2>), grid, dim3(256), 0, st, d->x, d->ldx, d->w, d->ldw, M, d->N, d->K, lanes, ep);
+    else if (M <= 4) hipLaunchKernelGGL((k_linear_rows<DT, 4>), grid, dim3(256), 0, st, d->x, d->ldx, d->w, d->ldw, M, d->N, d->K, lanes, ep);
+    else hipLaunchKernelGGL((k_linear_rows<DT, 8>), grid, dim3(256), 0, st, d->x, d->ldx, d->w, d->ldw, M, d->N, d->K, lanes, ep);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -132,28 +217,29 @@ __global__ __launch_bounds__(256) void k_linear_dz(NlDz a)
     a.part[(long long)blockIdx.y * a.N + col] = s;
 }
 
-// gb[n] = sum over the chunks: 16 columns (four to a thread) x 64 runs of neighbouring chunks per workgroup, the runs joined pairwise
+// gb[n] = sum over the chunks: four columns a workgroup, 256 runs of neighbouring chunks, the runs joined pairwise
 template <int DT>
 __global__ __launch_bounds__(256) void k_linear_gb(const float* __restrict__ part, int chunks, int N, void* gb)
 {
     __shared__ nl_f32x4 s_sum[256];
-    const int n = blockIdx.x * 16 + 4 * (threadIdx.x & 3), run = threadIdx.x >> 2;
-    const int per = (chunks + 63) / 64, c1 = (run + 1) * per < chunks ? (run + 1) * per : chunks;
+    const int n = blockIdx.x * 4, run = threadIdx.x;
+    const int per = (chunks + 255) / 256, c1 = (run + 1) * per < chunks ? (run + 1) * per : chunks;
     nl_f32x4 s = {};
-    if (n + 3 < N && (N & 3) == 0)
+    if ((N & 3) == 0) {
+#pragma unroll 4
         for (int c = run * per; c < c1; c++) s += *reinterpret_cast<const nl_f32x4*>(part + (long long)c * N + n);
-    else
+    } else
         for (int c = run * per; c < c1; c++)
 #pragma unroll
             for (int j = 0; j < 4; j++) if (n + j < N) s[j] += part[(long long)c * N + n + j];
-    s_sum[threadIdx.x] = s;
-    for (int off = 128; off >= 4; off >>= 1) {
+    s_sum[run] = s;
+    for (int off = 128; off >= 1; off >>= 1) {
         __syncthreads();
-        if (threadIdx.x < off) s_sum[threadIdx.x] += s_sum[threadIdx.x + off];
+        if (run < off) s_sum[run] += s_sum[run + off];
     }
     if (run != 0) return;
 #pragma unroll
-    for (int j = 0; j < 4; j++) if (n + j < N) nl_store_elem<DT>(gb, n + j, s_sum[threadIdx.x][j]);
+    for (int j = 0; j < 4; j++) if (n + j < N) nl_store_elem<DT>(gb, n + j, s_sum[0][j]);
 }
 
 __global__ __launch_bounds__(256) void k_linear_zero(unsigned char* p, long long bytes)
@@ -169,6 +255,7 @@ __global__ __launch_bounds__(256) void k_linear_zero(unsigned char* p, long long
 
 struct NlWork {
     char* base; long long used; hipStream_t st; bool dry; int rc;
+    NlPack2 pack; int packs;                                      // noted by nl_packed, launched by nl_pack
     char* take(long long bytes) { char* p = base + used; used += nl_up(bytes, 256); return p; }
 };
 
@@ -182,6 +269,14 @@ static bool nl_in_place(const void* p, int cols, long long ld, int dt)
     const int v = dt == NL_DT_F32 ? 4 : 8;
     return ld % v == 0 && cols % v == 0 && ld <= NL_LINEAR_MAX_WIDTH && ((uintptr_t)p & 15) == 0;
 }
+static void nl_pack(NlWork& w, int dt)
+{
+    if (!w.packs) return;
+    long long most = 0;
+    for (int i = 0; i < w.packs; i++) { const long long t = w.pack.p[i].rows * (w.pack.p[i].pitch / 8); if (t > most) most = t; }
+    if (!w.dry) NL_WITH_DTYPE(dt, hipLaunchKernelGGL(k_linear_pack<DT>, dim3(nl_grid(most), w.packs), dim3(256), 0, w.st, w.pack));
+    w.packs = 0;
+}
 static NlPacked nl_packed(NlWork& w, const void* p, const unsigned char* e, long long rows, int cols, long long ld, int type, int dt)
 {
     if (type == dt && nl_in_place(p, cols, ld, dt)) return NlPacked{p, ld, nullptr};
@@ -189,10 +284,7 @@ static NlPacked nl_packed(NlWork& w, const void* p, const unsigned char* e, long
     a.src = p; a.e = e; a.rows = rows; a.cols = cols; a.ld = ld;
     a.pitch = nl_up(cols, 8);
     a.dst = w.take(rows * a.pitch * nl_dtype_size(dt));
-    const dim3 grid(nl_grid(rows * (a.pitch / 8)));
-    if (w.dry) ;
-    else if (type == NL_DT_MX8) hipLaunchKernelGGL((k_linear_pack<NL_DT_F32, true>), grid, dim3(256), 0, w.st, a);
-    else NL_WITH_DTYPE(dt, hipLaunchKernelGGL((k_linear_pack<DT, false>), grid, dim3(256), 0, w.st, a));
+    w.pack.p[w.packs++] = a;
     return NlPacked{a.dst, a.pitch, nullptr};
 }
 
@@ -261,7 +353,12 @@ static void nl_forward_run(const NlLinear* d, NlWork& w)
     ep.z = d->z; ep.ldz = d->N;
     ep.bits = d->bits; ep.ldbits = nl_up(d->N, 32) / 32;
     ep.z8 = d->z8; ep.z8e = d->z8e; ep.ldz8 = nl_up(d->N, 32); ep.ldz8e = ep.ldz8 / 32;
+    if (d->M <= ROWS_MOST && !d->z && !d->bits && !d->z8) {
+        if (!w.dry) NL_WITH_DTYPE(d->dtype, nl_launch_rows<DT>(d, ep, w.st));
+        return;
+    }
     const NlPacked x = nl_packed(w, d->x, nullptr, d->M, d->K, d->ldx, d->dtype, d->dtype), wt = nl_packed(w, d->w, nullptr, d->N, d->K, d->ldw, d->dtype, d->dtype);
+    nl_pack(w, d->dtype);
     nl_product(w, x, wt, 0, d->M, d->N, d->K, ep);
 }
 
@@ -294,24 +391,27 @@ static void nl_backward_run(const NlLinear* d, NlWork& w)
                                     else if (d->act == NL_ACT_RELU) hipLaunchKernelGGL((k_linear_dz<DT, NL_ACT_RELU>), grid, dim3(256), 0, w.st, a);
                                     else if (d->act == NL_ACT_GELU) hipLaunchKernelGGL((k_linear_dz<DT, NL_ACT_GELU>), grid, dim3(256), 0, w.st, a);
                                     else hipLaunchKernelGGL((k_linear_dz<DT, NL_ACT_SILU>), grid, dim3(256), 0, w.st, a));
-            if (d->gb) NL_WITH_DTYPE(d->dtype, hipLaunchKernelGGL(k_linear_gb<DT>, dim3((d->N + 15) / 16), dim3(256), 0, w.st, a.part, (int)chunks, d->N, d->gb));
+            if (d->gb) NL_WITH_DTYPE(d->dtype, hipLaunchKernelGGL(k_linear_gb<DT>, dim3((d->N + 3) / 4), dim3(256), 0, w.st, a.part, (int)chunks, d->N, d->gb));
         }
     }
     NlEpilogue ep = {};
     ep.dt = d->dtype; ep.act = NL_ACT_NONE; ep.ldy = d->K;
+    NlPacked wt = {}, x = {};
+    const bool codes = d->gw && d->x8 && d->dtype != NL_DT_F32;           // (fp32 splits its operands: codes are decoded to fp32 first)
+    if (d->gx) wt = nl_packed(w, d->w, nullptr, d->N, d->K, d->ldw, d->dtype, d->dtype);
+    if (codes) x = NlPacked{d->x8, nl_up(d->K, 32), d->x8e};
+    else if (d->gw) x = d->x8 ? nl_packed(w, d->x8, d->x8e, d->M, d->K, nl_up(d->K, 32), NL_DT_MX8, d->dtype) : nl_packed(w, d->x, nullptr, d->M, d->K, d->ldx, d->dtype, d->dtype);
+    nl_pack(w, d->dtype);
     const long long keep = w.used;
     long long most = keep;
     if (d->gx) {
         ep.y = d->gx;
-        nl_product(w, dz, nl_packed(w, d->w, nullptr, d->N, d->K, d->ldw, d->dtype, d->dtype), 1, d->M, d->K, d->N, ep);
+        nl_product(w, dz, wt, 1, d->M, d->K, d->N, ep);
         most = w.used;
         w.used = keep;                                               // (the second product follows on the stream: it takes the same place)
     }
     if (d->gw) {
         ep.y = d->gw;
-        const bool codes = d->x8 && d->dtype != NL_DT_F32;               // (fp32 splits its operands: codes are decoded to fp32 first)
-        const NlPacked x = codes ? NlPacked{d->x8, nl_up(d->K, 32), d->x8e}
-                         : d->x8 ? nl_packed(w, d->x8, d->x8e, d->M, d->K, nl_up(d->K, 32), NL_DT_MX8, d->dtype) : nl_packed(w, d->x, nullptr, d->M, d->K, d->ldx, d->dtype, d->dtype);
         nl_product(w, dz, x, codes ? 3 : 2, d->N, d->K, d->M, ep);
     }
     if (w.used < most) w.used = most;
@@ -344,7 +444,8 @@ long long nl_linear_workspace(const NlLinear* d, int backward)
 {
     if (nl_linear_check(d, backward) != NL_OK) return -1;
     if (d->M == 0) return 0;
-    NlWork w = {nullptr, 0, nullptr, true, NL_OK};
+    NlWork w = {};
+    w.dry = true;
     if (backward) nl_backward_run(d, w); else nl_forward_run(d, w);
     return w.rc == NL_OK ? w.used : -1;
 }
@@ -353,7 +454,8 @@ static int nl_linear_run(const NlLinear* d, int backward, void* stream)
 {
     const long long need = nl_linear_workspace(d, backward);
     if (need < 0 || (need > 0 && (!d->ws || d->ws_bytes < need || ((uintptr_t)d->ws & 255)))) return NL_ERR_INVALID_ARG;
-    NlWork w = {(char*)d->ws, 0, (hipStream_t)stream, false, NL_OK};
+    NlWork w = {};
+    w.base = (char*)d->ws; w.st = (hipStream_t)stream;
     if (backward) nl_backward_run(d, w); else nl_forward_run(d, w);
     if (w.rc != NL_OK) return w.rc;
     NL_LAUNCH_CHECK();
