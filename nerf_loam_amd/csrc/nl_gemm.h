@@ -8,6 +8,7 @@
 #include "nl_layers.h"
 
 #define GEMM_BK 64                     // contraction step: two matrix instructions of 32
+#define NL_GEMM_FEW_SQUARES 512        // workgroups of 64 x 64 with four buffers that run at a time (two to a compute unit)
 
 struct NlGemm {
     const char* A; const char* B;      // 16-byte aligned, rows 16-byte aligned
@@ -237,16 +238,19 @@ struct GemmSideMx8 {
     }
 };
 
-template <class T, bool A_SLOW, bool B_SLOW, bool B_MX8, int BM, int BN, int WM, int WN>
+// RING: LDS buffers per operand.  2: the next step arrives while one multiplies.  4 (squares of 64 while they leave compute units idle anyway): three steps are on their way;
+// a step of such a tile multiplies for 130 cycles and waits for memory the rest of the time.  The barrier then waits for the oldest step's loads only.
+template <class T, bool A_SLOW, bool B_SLOW, bool B_MX8, int BM, int BN, int WM, int WN, int RING>
 __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
 {
     constexpr int DT = __is_same(T, _Float16) ? NL_DT_F16 : NL_DT_BF16;
     constexpr int NT = 64 * WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
     typedef GemmSide<A_SLOW, BM, NT> SA;
     typedef GemmSide<B_SLOW, BN, NT> SB;
-    __shared__ __align__(256) char s_mem[2 * (SA::BYTES + SB::BYTES)];
+    static_assert(RING == 2 || (RING == 4 && !B_MX8), "buffers are taken in turn by the low bits of the step");
+    __shared__ __align__(256) char s_mem[RING * (SA::BYTES + SB::BYTES)];
     char* const s_a = s_mem;
-    char* const s_b = s_mem + 2 * SA::BYTES;
+    char* const s_b = s_mem + RING * SA::BYTES;
     long long m0; int n0;
     const unsigned piece = gemm_tile_of<BM, BN>(g, m0, n0);
     const long long k0 = (long long)piece * g.kchunk, k1 = min(k0 + g.kchunk, g.K);
@@ -260,17 +264,18 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
     nl_f32x4 acc[FM][FN] = {};
     auto fetch = [&](int s) {
         const long long left = k1 - k0 - (long long)s * GEMM_BK;
-        a.load(s_a + (s & 1) * SA::BYTES, s * a.step, left);
+        a.load(s_a + (s & (RING - 1)) * SA::BYTES, s * a.step, left);
         if (B_MX8) b8.fetch(s, left);
-        else b.load(s_b + (s & 1) * SB::BYTES, s * b.step, left);
+        else b.load(s_b + (s & (RING - 1)) * SB::BYTES, s * b.step, left);
     };
-    fetch(0);
+    for (int s = 0; s < RING - 1; s++) fetch(s);                      // (behind the last step nothing is inside: zeros)
     if (B_MX8) b8.put(s_b);
-    __builtin_amdgcn_s_waitcnt(0);
-    __builtin_amdgcn_s_barrier();
+    if (RING == 2) __syncthreads();
     for (int s = 0; s < steps; s++) {
-        const char* la = s_a + (s & 1) * SA::BYTES;
-        const char* lb = s_b + (s & 1) * SB::BYTES;
+        // RING 4: this step's loads have landed, two later steps' stay in flight; behind the barrier nobody reads the buffer of step s - 1 any more
+        if (RING > 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((RING - 2) * (SA::LOADS + SB::LOADS)) : "memory");
+        const char* la = s_a + (s & (RING - 1)) * SA::BYTES;
+        const char* lb = s_b + (s & (RING - 1)) * SB::BYTES;
         // fragments of both halves of the step, the loads of the next step between them: behind all fragment reads they come late (8192^3 / 16384 x 4096 x 4096,
         // layout 1 and 2: -10 %), in front of them they hold up the reads that the first matrix instructions wait for
         nl_s16x8 fa[2][FM], fb[2][FN];
@@ -278,7 +283,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
         for (int j = 0; j < FN; j++) fb[0][j] = SB::frag(lb, wn + 16 * j, 0);
 #pragma unroll
         for (int i = 0; i < FM; i++) fa[0][i] = SA::frag(la, wm + 16 * i, 0);
-        if (s + 1 < steps) fetch(s + 1);
+        if (RING > 2 || s + 1 < steps) fetch(s + RING - 1);
 #pragma unroll
         for (int j = 0; j < FN; j++) fb[1][j] = SB::frag(lb, wn + 16 * j, 1);
 #pragma unroll
@@ -292,9 +297,10 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
 #pragma unroll
             for (int j = 0; j < FN; j++) acc[i][j] = NlMma<T>::mma(fb[1][j], fa[1][i], acc[i][j]);
         if (B_MX8 && s + 1 < steps) b8.put(s_b + ((s + 1) & 1) * SB::BYTES);
-        __syncthreads();
+        if (RING == 2) __syncthreads();
     }
-    gemm_results<DT, BM / WM, BN / WN, WM * WN, 2 * (SA::BYTES + SB::BYTES)>(g, acc, s_mem, m0 + wm, n0 + wn, piece);
+    if (RING > 2) __syncthreads();                                    // (waits for all loads, the ones of zeros too)
+    gemm_results<DT, BM / WM, BN / WN, WM * WN, RING * (SA::BYTES + SB::BYTES)>(g, acc, s_mem, m0 + wm, n0 + wn, piece);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -456,9 +462,10 @@ static void nl_gemm_tile_f32(const NlGemm& g, int tile, dim3 grid, hipStream_t s
 template <class T, bool A_SLOW, bool B_SLOW, bool B_MX8>
 static void nl_gemm_tile(const NlGemm& g, int tile, dim3 grid, hipStream_t st)
 {
-    if (tile == 0) hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, B_MX8, 256, 256, 2, 4>), grid, dim3(512), 0, st, g);
-    else if (tile == 1) hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, B_MX8, 128, 128, 2, 2>), grid, dim3(256), 0, st, g);
-    else hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, B_MX8, 64, 64, 2, 2>), grid, dim3(256), 0, st, g);
+    if (tile == 0) hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, B_MX8, 256, 256, 2, 4, 2>), grid, dim3(512), 0, st, g);
+    else if (tile == 1) hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, B_MX8, 128, 128, 2, 2, 2>), grid, dim3(256), 0, st, g);
+    else if (B_MX8 || (long long)grid.x * grid.y > NL_GEMM_FEW_SQUARES) hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, B_MX8, 64, 64, 2, 2, 2>), grid, dim3(256), 0, st, g);
+    else hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, false, 64, 64, 2, 2, B_MX8 ? 2 : 4>), grid, dim3(256), 0, st, g);
 }
 template <class T>
 static void nl_gemm_layout(const NlGemm& g, int layout, int tile, dim3 grid, hipStream_t st)

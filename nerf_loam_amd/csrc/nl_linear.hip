@@ -310,7 +310,8 @@ static NlCut nl_cut(long long M, long long N, long long K, int dt, int layout)
             if (s > 1 && 4.0 * s * M * N > 1.5e9) break;
             const long long per = (ksteps + s - 1) / s;
             const double at = tiles * s / T[t].at_a_time, full = at < 1.0 ? at : 1.0, rounds = at < 1.0 ? 1.0 : at < 4.0 ? ceil(at) : at + 0.5;
-            double us = rounds * (per * (T[t].alone + (T[t].full - T[t].alone) * full) * (layout >= 2 ? T[t].slow : 1.0) + T[t].rest * (0.5 + 0.5 * full));
+            const double alone = t == 2 && dt != NL_DT_F32 && layout < 3 && tiles * s <= NL_GEMM_FEW_SQUARES ? 0.33 : T[t].alone;      // (four buffers)
+            double us = rounds * (per * (alone + (T[t].full - alone) * full) * (layout >= 2 ? T[t].slow : 1.0) + T[t].rest * (0.5 + 0.5 * full));
             if (us < memory) us = memory;
             if (s > 1) us += 3.0 + 8.0 * s * M * N / 4.0e6;
             if (us < least) { least = us; best = NlCut{t, s, per * GEMM_BK}; }
