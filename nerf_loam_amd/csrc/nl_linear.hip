@@ -35,19 +35,22 @@ __global__ __launch_bounds__(256) void k_linear_pack(NlPack2 both)
 }
 
 // ---------------------------------------------------------------------------------------------
-// k_linear_rows: a few rows of x (at most ROWS_MOST) that keep nothing for a backward pass: the call that answers single queries.  It reads the weight once and computes
-// little, so no tile: a group of `lanes` threads takes two rows of the weight, eight neighbouring elements a thread at a time, several loads in flight, and sums
-// across its threads at the end.  One launch (1 x 4096 x 4096 bf16: 8 us, as tiles of 64 cut 16 times and joined 10).
+// k_linear_rows: at most ROWS_MOST rows of x (the call that answers single queries) or of the weight (a last layer with one output), nothing kept for a backward pass.
+// It reads the other operand once and computes little, so no tile: a group of `lanes` threads takes two rows of the many, eight neighbouring elements a thread at a
+// time, several loads in flight, and sums across its threads at the end.  One launch (1 x 4096 x 4096 bf16: 6.4 us, as tiles of 64 cut 16 times and joined 9.7).
+// SWAP: the few rows are the weight's, the many are x's.
 // ---------------------------------------------------------------------------------------------
 #define ROWS_MOST 8
-template <int DT, int MR>
-__global__ __launch_bounds__(256) void k_linear_rows(const void* __restrict__ x, long long ldx, const void* __restrict__ w, long long ldw, int M, int N, int K, int lanes, NlEpilogue ep)
+struct NlRows { const void* few; const void* many; long long ldf, ldm, nmany; int nfew, K, lanes; };
+template <int DT, int MR, bool SWAP>
+__global__ __launch_bounds__(256) void k_linear_rows(NlRows g, NlEpilogue ep)
 {
     constexpr int R = 2, U = MR == 1 ? 4 : MR <= 4 ? 2 : 1;
-    const int lane = threadIdx.x & (lanes - 1), n0 = (int)(blockIdx.x * (256 / lanes) + threadIdx.x / lanes) * R;
-    if (n0 >= N) return;                                              // (a whole group)
-    const int n1 = n0 + 1 < N ? n0 + 1 : n0;
-    const bool vec = nl_rows_aligned<DT>(w, ldw) && nl_rows_aligned<DT>(x, ldx) && (K & 7) == 0;
+    const int lanes = g.lanes, lane = threadIdx.x & (lanes - 1), K = g.K;
+    const long long n0 = ((long long)blockIdx.x * (256 / lanes) + threadIdx.x / lanes) * R;
+    if (n0 >= g.nmany) return;                                        // (a whole group)
+    const long long n1 = n0 + 1 < g.nmany ? n0 + 1 : n0;
+    const bool vec = nl_rows_aligned<DT>(g.many, g.ldm) && nl_rows_aligned<DT>(g.few, g.ldf) && (K & 7) == 0;
     float acc[MR][R] = {};
     int k = lane * 8;
     if (vec)
@@ -55,10 +58,10 @@ __global__ __launch_bounds__(256) void k_linear_rows(const void* __restrict__ x,
             NlRaw8<DT> a[U][R], b[U][MR];
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                a[u][0] = nl_raw8<DT>(w, (long long)n0 * ldw + k + u * lanes * 8);
-                a[u][1] = nl_raw8<DT>(w, (long long)n1 * ldw + k + u * lanes * 8);
+                a[u][0] = nl_raw8<DT>(g.many, n0 * g.ldm + k + u * lanes * 8);
+                a[u][1] = nl_raw8<DT>(g.many, n1 * g.ldm + k + u * lanes * 8);
 #pragma unroll
-                for (int m = 0; m < MR; m++) b[u][m] = nl_raw8<DT>(x, (m < M ? m : 0) * ldx + k + u * lanes * 8);
+                for (int m = 0; m < MR; m++) b[u][m] = nl_raw8<DT>(g.few, (m < g.nfew ? m : 0) * g.ldf + k + u * lanes * 8);
             }
 #pragma unroll
             for (int u = 0; u < U; u++) {
@@ -78,12 +81,12 @@ __global__ __launch_bounds__(256) void k_linear_rows(const void* __restrict__ x,
         }
     for (; k < K; k += lanes * 8) {
         float p[R][8];
-        nl_load8<DT>(p[0], w, (long long)n0 * ldw + k, K - k, vec);
-        nl_load8<DT>(p[1], w, (long long)n1 * ldw + k, K - k, vec);
+        nl_load8<DT>(p[0], g.many, n0 * g.ldm + k, K - k, vec);
+        nl_load8<DT>(p[1], g.many, n1 * g.ldm + k, K - k, vec);
 #pragma unroll
         for (int m = 0; m < MR; m++) {
             float q[8];
-            nl_load8<DT>(q, x, (m < M ? m : 0) * ldx + k, K - k, vec);
+            nl_load8<DT>(q, g.few, (m < g.nfew ? m : 0) * g.ldf + k, K - k, vec);
 #pragma unroll
             for (int r = 0; r < R; r++)
 #pragma unroll
@@ -91,29 +94,31 @@ __global__ __launch_bounds__(256) void k_linear_rows(const void* __restrict__ x,
         }
     }
 #pragma unroll
-    for (int m = 0; m < MR; m++)
+    for (int f = 0; f < MR; f++)
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            float v = acc[m][r];
+            float v = acc[f][r];
             for (int off = lanes >> 1; off > 0; off >>= 1) v += __shfl_xor(v, off);
-            const int n = n0 + r;
-            if (lane != 0 || m >= M || n >= N) continue;
+            if (lane != 0 || f >= g.nfew || n0 + r >= g.nmany) continue;
+            const long long m = SWAP ? n0 + r : f, n = SWAP ? f : n0 + r;
             if (ep.b) v += nl_load_elem<DT>(ep.b, n);
             v = nl_act(v, ep.act);
             if (ep.r) v += nl_load_elem<DT>(ep.r, m * ep.ldr + n);
             nl_store_elem<DT>(ep.y, m * ep.ldy + n, v);
         }
 }
-template <int DT> static void nl_launch_rows(const NlLinear* d, const NlEpilogue& ep, hipStream_t st)
+template <int DT, bool SWAP> static int nl_launch_rows(const NlLinear* d, const NlEpilogue& ep, hipStream_t st)
 {
-    int lanes = 8;
-    while (lanes < 64 && lanes * 8 < d->K) lanes *= 2;
-    const dim3 grid((unsigned)((d->N + 2 * (256 / lanes) - 1) / (2 * (256 / lanes))));
-    const int M = (int)d->M;
-    if (M == 1) hipLaunchKernelGGL((k_linear_rows<DT, 1>), grid, dim3(256), 0, st, d->x, d->ldx, d->w, d->ldw, M, d->N, d->K, lanes, ep);
-    else if (M == 2) hipLaunchKernelGGL((k_linear_rows<DT, 2>), grid, dim3(256), 0, st, d->x, d->ldx, d->w, d->ldw, M, d->N, d->K, lanes, ep);
-    else if (M <= 4) hipLaunchKernelGGL((k_linear_rows<DT, 4>), grid, dim3(256), 0, st, d->x, d->ldx, d->w, d->ldw, M, d->N, d->K, lanes, ep);
-    else hipLaunchKernelGGL((k_linear_rows<DT, 8>), grid, dim3(256), 0, st, d->x, d->ldx, d->w, d->ldw, M, d->N, d->K, lanes, ep);
+    NlRows g = SWAP ? NlRows{d->w, d->x, d->ldw, d->ldx, d->M, d->N, d->K, 8} : NlRows{d->x, d->w, d->ldx, d->ldw, d->N, (int)d->M, d->K, 8};
+    while (g.lanes < 64 && g.lanes * 8 < d->K) g.lanes *= 2;
+    const long long blocks = (g.nmany + 2 * (256 / g.lanes) - 1) / (2 * (256 / g.lanes));
+    if (blocks > 0x7FFFFFFF) return NL_ERR_INVALID_ARG;
+    const dim3 grid((unsigned)blocks);
+    if (g.nfew == 1) hipLaunchKernelGGL((k_linear_rows<DT, 1, SWAP>), grid, dim3(256), 0, st, g, ep);
+    else if (g.nfew == 2) hipLaunchKernelGGL((k_linear_rows<DT, 2, SWAP>), grid, dim3(256), 0, st, g, ep);
+    else if (g.nfew <= 4) hipLaunchKernelGGL((k_linear_rows<DT, 4, SWAP>), grid, dim3(256), 0, st, g, ep);
+    else hipLaunchKernelGGL((k_linear_rows<DT, 8, SWAP>), grid, dim3(256), 0, st, g, ep);
+    return NL_OK;
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -354,8 +359,8 @@ static void nl_forward_run(const NlLinear* d, NlWork& w)
     ep.z = d->z; ep.ldz = d->N;
     ep.bits = d->bits; ep.ldbits = nl_up(d->N, 32) / 32;
     ep.z8 = d->z8; ep.z8e = d->z8e; ep.ldz8 = nl_up(d->N, 32); ep.ldz8e = ep.ldz8 / 32;
-    if (d->M <= ROWS_MOST && !d->z && !d->bits && !d->z8) {
-        if (!w.dry) NL_WITH_DTYPE(d->dtype, nl_launch_rows<DT>(d, ep, w.st));
+    if ((d->M <= ROWS_MOST || d->N <= ROWS_MOST) && !d->z && !d->bits && !d->z8) {
+        if (!w.dry) NL_WITH_DTYPE(d->dtype, w.rc = d->M <= ROWS_MOST ? nl_launch_rows<DT, false>(d, ep, w.st) : nl_launch_rows<DT, true>(d, ep, w.st));
         return;
     }
     const NlPacked x = nl_packed(w, d->x, nullptr, d->M, d->K, d->ldx, d->dtype, d->dtype), wt = nl_packed(w, d->w, nullptr, d->N, d->K, d->ldw, d->dtype, d->dtype);

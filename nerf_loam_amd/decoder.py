@@ -1,31 +1,39 @@
 """Decoder: the SDF MLP container.
 
-Mirror of /root/reference/src/variations/lidar.py:80-131 for the configuration every shipped config
-uses (depth 2, width 256, in_dim 16, skips [], embedder none => Linear(16,256)-ReLU-Linear(256,256)-
-ReLU-Linear(256,1)); parameter names match (`pts_linears.{0,1}`, `sdf_out`), so reference
-checkpoints / state_dicts load.  forward()/get_values() run the hand-written MFMA forward kernel
-(nl_decoder.hip k_decoder_fwd) - no PyTorch GEMM path; other configurations raise."""
+Mirror of /root/reference/src/variations/lidar.py:80-131; parameter names match (`pts_linears.{i}`, `sdf_out`), so reference checkpoints / state_dicts load.
+
+* The configuration every shipped config uses (depth 2, width 256, in_dim 16, skips [], embedder none => Linear(16,256)-ReLU-Linear(256,256)-ReLU-Linear(256,1)) runs
+  the fused matrix-core forward kernel (nl_decoder.hip k_decoder_fwd); the optimisation loops train it inside the engine.
+* Every other depth / width / in_dim / skips runs one layers.linear_act call per layer (csrc/nl_linear.hip) and is differentiable with respect to its input and its
+  parameters; checkpoint="mx8" keeps the activations of a training step in 8 bits (layers.linear_act).  bundle_adjust_frames / track_frame / render_rays do not take
+  such a decoder; get_scores and create_mesh do.
+
+There is no PyTorch GEMM path.  The positional embedders (lidar.py:6-77, used by no config) are not provided and raise."""
 import torch
 import torch.nn as nn
 
 from . import _lib as L
-from . import ops
+from . import layers, ops
 
 
 class Decoder(nn.Module):
     def __init__(self, depth=2, width=256, in_dim=16, sdf_dim=128, skips=(), multires=0, embedder="none", point_dim=3,
-                 local_coord=False, **kwargs):
+                 local_coord=False, checkpoint=None, **kwargs):
         super().__init__()
-        if depth != 2 or width != 256 or in_dim != 16 or len(skips) != 0 or embedder != "none":
-            raise NotImplementedError("the MI355X decoder kernels implement the reference's shipped configuration only: "
-                                      "depth 2, width 256, in_dim 16, skips [], embedder none")
-        self.D, self.W, self.skips, self.point_dim = depth, width, list(skips), point_dim
-        self.pts_linears = nn.ModuleList([nn.Linear(in_dim, width), nn.Linear(width, width)])
+        if embedder != "none":
+            raise NotImplementedError("the MI355X decoder takes its input as it is: embedder none (the reference's positional embedders are used by no shipped configuration)")
+        if depth < 1 or width < 1 or in_dim < 1 or any(s not in range(depth - 1) for s in skips):
+            raise ValueError(f"Decoder: depth {depth}, width {width} and in_dim {in_dim} must be positive, skips {list(skips)} name layers below the last one")
+        if checkpoint not in layers.CHECKPOINTS:
+            raise ValueError(f"Decoder: checkpoint {checkpoint!r} must be one of {layers.CHECKPOINTS}")
+        self.D, self.W, self.skips, self.point_dim, self.checkpoint = depth, width, list(skips), point_dim, checkpoint
+        self.fused = (depth, width, in_dim, len(skips)) == (2, L.NL_W, L.NL_C, 0)           # the engine's kernels are built for this one
+        # lidar.py:96-106: the layer behind a skip takes the input again, in front of the hidden values
+        self.pts_linears = nn.ModuleList([nn.Linear(in_dim, width)] + [nn.Linear(width + in_dim if i in self.skips else width, width) for i in range(depth - 1)])
         self.sdf_out = nn.Linear(width, 1)
 
     def param_list(self):
-        return [self.pts_linears[0].weight, self.pts_linears[0].bias, self.pts_linears[1].weight, self.pts_linears[1].bias,
-                self.sdf_out.weight, self.sdf_out.bias]
+        return [p for l in (*self.pts_linears, self.sdf_out) for p in (l.weight, l.bias)]
 
     def flat_params(self, device):
         """decoder parameter block of include/nerfloam_hip.h (W1 b1 W2 b2 W3 b3)"""
@@ -39,10 +47,13 @@ class Decoder(nn.Module):
             p.copy_(flat[off:off + n].view_as(p))
             off += n
 
-    @torch.no_grad()
     def get_values(self, x):
         if not x.is_cuda:
             raise L.NerfLoamHipError("Decoder.get_values needs a CUDA (HIP) tensor - no CPU path")
+        return self._values_fused(x) if self.fused else self._values_layers(x)
+
+    @torch.no_grad()
+    def _values_fused(self, x):
         x = x.detach().float().contiguous()
         # the device parameter block + W2 operand planes, kept until somebody writes the parameters (tensor version counters): the same
         # cache bundle_adjust_frames / track_frame use (render_helpers._decoder_device) - no re-flattening, no plane rebuild per call
@@ -51,6 +62,16 @@ class Decoder(nn.Module):
         out = torch.empty(x.shape[0], dtype=torch.float32, device=x.device)
         ops.decoder_forward(x, dec.params, dec.W2T, x.shape[0], out, L.lib().nl_decoder_grid_hint())
         return out.unsqueeze(-1)
+
+    def _values_layers(self, x):
+        """lidar.py:109-123, a call per layer; in the parameters' type"""
+        x = x.to(self.sdf_out.weight.dtype)
+        h = x
+        for i, l in enumerate(self.pts_linears):
+            h = layers.linear_act(h, l.weight, l.bias, act="relu", checkpoint=self.checkpoint)
+            if i in self.skips:
+                h = torch.cat([x, h], -1)
+        return layers.linear_act(h, self.sdf_out.weight, self.sdf_out.bias, checkpoint=self.checkpoint)
 
     def forward(self, inputs):
         return {"sdf": self.get_values(inputs)}

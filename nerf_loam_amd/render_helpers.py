@@ -21,7 +21,7 @@ import numpy as np
 import torch
 
 from . import _lib as L
-from . import ops
+from . import layers, ops
 from .lidar_frame import scan_of
 from .pipeline import BYTES_PER_SAMPLE, DecoderDevice, IterConfig, MapDevice, SdfEngine, samples_per_ray_bound
 
@@ -118,7 +118,7 @@ def _map_device(map_states, voxel_size, device):
 def _param_list(sdf_network):
     """the six parameter tensors of the shipped decoder configuration (W1 b1 W2 b2 W3 b3) of ANY module laid out like the reference's
     variations/lidar.py:105-107 (`pts_linears[0..1]`, `sdf_out`): nerf_loam_amd.decoder.Decoder and the reference's own Decoder alike"""
-    if hasattr(sdf_network, "param_list"):
+    if hasattr(sdf_network, "param_list") and getattr(sdf_network, "fused", True):
         return sdf_network.param_list()
     lin = list(getattr(sdf_network, "pts_linears", []))
     out = getattr(sdf_network, "sdf_out", None)
@@ -369,6 +369,29 @@ def render_rays(rays_o, rays_d, map_states, sdf_network, step_size, voxel_size, 
             "sampled_xyz": m.centres[eng.s_vox[:P].long()], "_engine": eng, "_cfg": cfg}
 
 
+def get_features(samples, map_states, voxel_size):
+    """render_helpers.py:74-93: features of samples inside voxels, trilinear between the eight corner rows -> {"dists", "emb" [P, 16] float32}, differentiable with
+    respect to map_states["voxel_vertex_emb"] (through layers.embedding_lookup: the gradient is summed over sorted rows, the same bits every run) and to
+    samples["sampled_point_xyz"].  A voxel index outside the map gives zeros and no gradient.  The optimisation loops do not come here (the engine interpolates inside its kernels): this is for callers that train a decoder of
+    their own on samples of their own."""
+    emb = map_states["voxel_vertex_emb"]
+    m = _map_device(map_states, voxel_size, emb.device)
+    vox = samples["sampled_point_voxel_idx"].reshape(-1).to(emb.device).long()
+    xyz = samples["sampled_point_xyz"].reshape(-1, 3).to(emb.device, torch.float32)
+    if vox.numel() != xyz.shape[0]:
+        raise ValueError(f"get_features: {vox.numel()} voxel indices for {xyz.shape[0]} points")
+    inside = (vox >= 0) & (vox < m.n_nodes)
+    vox = torch.where(inside, vox, torch.zeros_like(vox))
+    rows = torch.where(inside.unsqueeze(1), m.vertex_rows[vox], torch.full_like(m.vertex_rows[:1], -1))
+    # :40-56: p = position inside the voxel in [0, 1]^3, corner k = 4 qx + 2 qy + qz, weight = product over the axes of p or 1 - p
+    p = (xyz - m.centres[vox]) / float(voxel_size) + 0.5
+    q = torch.stack([1.0 - p, p], -1)                                                     # [P, axis, q]
+    w = (q[:, 0, :, None, None] * q[:, 1, None, :, None] * q[:, 2, None, None, :]).reshape(-1, 8)
+    # float32 rows: sums and features stay in 32 bits, the table's own type is rounded to once, in its gradient
+    feats = layers.embedding_lookup(emb.float(), rows, weights=w)
+    return {"dists": samples.get("sampled_point_distance"), "emb": feats}
+
+
 SCORES_CHUNK_POINTS = 1 << 24          # points per gather + decoder launch pair of get_scores (16.8 M points = 1 GB of X rows; the reference's chunk is 10 000 voxels)
 
 
@@ -384,7 +407,8 @@ def get_scores(sdf_network, map_states, voxel_size, bits=8, device_out=False):
     device = emb.device
     m = MapDevice.from_tensors(map_states["voxel_center_xyz"], map_states["voxel_structure"], map_states["voxel_vertex_idx"],
                                map_states["voxel_id2embedding_id"], emb, voxel_size, device, traversal=False)
-    dec = _decoder_device(sdf_network, device)
+    fused = getattr(sdf_network, "fused", True)
+    dec = _decoder_device(sdf_network, device) if fused else None
     res = int(bits)
     lin = torch.linspace(-0.5, 0.5, res).to(device)
     n = m.centres.shape[0]
@@ -393,12 +417,16 @@ def get_scores(sdf_network, map_states, voxel_size, bits=8, device_out=False):
     chunk = max(1, SCORES_CHUNK_POINTS // r3)
     X = torch.empty(min(n, chunk) * r3, L.NL_C, dtype=torch.float32, device=device)
     hint = L.lib().nl_decoder_grid_hint()
-    dec.W2T[L.NL_DEC_WS_RANGE_STATUS:L.NL_DEC_WS_RANGE_STATUS + 1].zero_()            # (the range status of THIS call)
+    if fused:
+        dec.W2T[L.NL_DEC_WS_RANGE_STATUS:L.NL_DEC_WS_RANGE_STATUS + 1].zero_()        # (the range status of THIS call)
     for i in range(0, n, chunk):
         k = min(chunk, n - i)
         ops.gather_grid(k, i, res, lin, m.centres, m.vertex_rows, m.emb, voxel_size, X)
-        ops.decoder_forward(X, dec.params, dec.W2T, k * r3, sdf[i * r3:], hint)
-    if dec.range_status() and os.environ.get("NL_ON_SATURATION", "raise") != "ignore":
+        if fused:
+            ops.decoder_forward(X, dec.params, dec.W2T, k * r3, sdf[i * r3:], hint)
+        else:                                                                          # a decoder of another size: one layer call each
+            sdf[i * r3:(i + k) * r3] = sdf_network.get_values(X[:k * r3]).reshape(-1)
+    if fused and dec.range_status() and os.environ.get("NL_ON_SATURATION", "raise") != "ignore":
         raise L.NerfLoamHipError("get_scores: an operand of the decoder left the range of the fp16-pair arithmetic and was clipped (DecoderDevice.range_status()); "
                                  "use NL_GEMM_MODE=3")
     out = sdf.view(-1, res, res, res, 1)

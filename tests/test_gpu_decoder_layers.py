@@ -1,0 +1,231 @@
+"""GPU (-m gpu): decoders of any size on the layer operators, differentiable features of samples, and a training step of the whole chain - features, decoder, the loss
+of caller tensors - against the same chain written in torch in 64 bits.
+
+Tolerances.  A layer of K terms in float32 is right to (6 K + 8) 2^-23 of the magnitudes it sums (test_gpu_layers.py); through the layers a value's error is carried
+by the next layer's weights.  Both are bounded here by running the chain on the absolute values: with A_l = |W_l| A_(l-1) + |b_l| (A_0 = |x|) the error of layer l is at most
+(6 K_l + 8) 2^-23 A_l times the number of layers so far.  Gradients: the same bound on the chain of absolute values backwards."""
+import types
+
+import numpy as np
+import pytest
+import torch
+
+from nerf_loam_amd.decoder import Decoder
+from oracle import oracle as O
+
+pytestmark = pytest.mark.gpu
+
+
+def _decoder(seed, **kw):
+    torch.manual_seed(seed)
+    return Decoder(**kw).cuda()
+
+
+def _chain64(dec, x):
+    """the decoder's formula in 64 bits with autograd -> (sdf, leaves): lidar.py:109-123"""
+    leaves = [p.detach().double().requires_grad_(True) for p in dec.param_list()]
+    x = x.detach().double().requires_grad_(True)
+    h = x
+    n = len(dec.pts_linears)
+    for i in range(n):
+        h = torch.relu(h @ leaves[2 * i].t() + leaves[2 * i + 1])
+        if i in dec.skips:
+            h = torch.cat([x, h], -1)
+    return h @ leaves[2 * n].t() + leaves[2 * n + 1], [x] + leaves
+
+
+def _chain_abs(dec, x):
+    with torch.no_grad():
+        x = x.double().abs()
+        h = x
+        p = [q.detach().double().abs() for q in dec.param_list()]
+        n = len(dec.pts_linears)
+        for i in range(n):
+            h = h @ p[2 * i].t() + p[2 * i + 1]
+            if i in dec.skips:
+                h = torch.cat([x, h], -1)
+        return h @ p[2 * n].t() + p[2 * n + 1]
+
+
+CONFIGS = [dict(depth=1, width=64), dict(depth=2, width=128), dict(depth=3, width=256, skips=[0]), dict(depth=4, width=96, skips=[1, 2]), dict(depth=2, width=33, in_dim=7), dict(depth=8, width=64, skips=[4])]
+
+
+@pytest.mark.parametrize("cfg", CONFIGS)
+@pytest.mark.parametrize("P", [1, 6, 3000])
+def test_values_of_any_decoder(cfg, P):
+    dec = _decoder(3, **cfg)
+    x = torch.randn(P, cfg.get("in_dim", 16), device="cuda")
+    want, _ = _chain64(dec, x)
+    width = cfg["width"] + cfg.get("in_dim", 16)
+    tol = (6 * width + 8) * 2.0 ** -23 * (cfg["depth"] + 1) * _chain_abs(dec, x)
+    got = dec(x)["sdf"]
+    assert got.shape == (P, 1) and got.requires_grad
+    assert bool(((got.double() - want).abs() <= tol).all())
+    with torch.no_grad():
+        quiet = dec.get_values(x)
+    assert not quiet.requires_grad and bool(((quiet.double() - want).abs() <= tol).all())
+
+
+def test_names_are_the_references_and_a_state_dict_loads():
+    dec = _decoder(5, depth=3, width=48, skips=[1])
+    assert sorted(dec.state_dict()) == sorted([f"pts_linears.{i}.{n}" for i in range(3) for n in ("weight", "bias")] + ["sdf_out.weight", "sdf_out.bias"])
+    assert [tuple(l.weight.shape) for l in dec.pts_linears] == [(48, 16), (48, 48), (48, 64)]
+    other = Decoder(depth=3, width=48, skips=[1]).cuda()
+    other.load_state_dict(dec.state_dict())
+    x = torch.randn(50, 16, device="cuda")
+    assert torch.equal(dec.get_values(x), other.get_values(x))
+    flat = dec.flat_params("cuda")
+    other.load_flat(flat * 0 + 1)
+    assert all(bool((p == 1).all()) for p in other.param_list())
+
+
+def test_the_fused_configuration_keeps_its_kernel_and_the_loops_refuse_others():
+    from nerf_loam_amd.render_helpers import _param_list
+    fused, other = _decoder(7), _decoder(7, depth=2, width=128)
+    assert fused.fused and not other.fused
+    x = torch.randn(100, 16, device="cuda")
+    want, _ = _chain64(fused, x)
+    assert not fused.get_values(x).requires_grad and float((fused.get_values(x).double() - want).abs().max()) < 1e-4
+    assert len(_param_list(fused)) == 6
+    with pytest.raises(NotImplementedError):
+        _param_list(other)
+    for bad in (dict(depth=0), dict(width=0), dict(skips=[1]), dict(depth=3, skips=[2]), dict(checkpoint="int4")):
+        with pytest.raises(ValueError):
+            Decoder(**bad)
+    with pytest.raises(NotImplementedError):
+        Decoder(embedder="nerf")
+
+
+def _scene():
+    import helpers as H
+    sc = H.build_oracle_scene(64, 16, 21)
+    ms = sc["ms"]
+    emb = torch.from_numpy(H.init_embeddings(len(ms.emb), 21)).to(torch.bfloat16).cuda()
+    states = {"voxel_vertex_idx": torch.from_numpy(ms.vertex_idx), "voxel_center_xyz": torch.from_numpy(ms.centres), "voxel_structure": torch.from_numpy(ms.structure),
+              "voxel_vertex_emb": emb, "voxel_id2embedding_id": torch.from_numpy(ms.id2row)}
+    surf = np.nonzero(ms.vertex_idx[:, 0] >= 0)[0]
+    return ms, states, surf
+
+
+def _samples(ms, surf, P, seed):
+    rng = np.random.default_rng(seed)
+    vox = surf[rng.integers(0, len(surf), P)]
+    xyz = ms.centres[vox] + rng.uniform(-0.1, 0.1, (P, 3)).astype(np.float32)
+    return vox, xyz.astype(np.float32)
+
+
+def test_features_of_samples_match_the_oracle_and_their_gradients_the_formula():
+    from nerf_loam_amd.render_helpers import get_features
+    ms, states, surf = _scene()
+    P = 5000
+    vox, xyz = _samples(ms, surf, P, 5)
+    emb = states["voxel_vertex_emb"].requires_grad_(True)
+    x = torch.from_numpy(xyz).cuda().requires_grad_(True)
+    out = get_features({"sampled_point_voxel_idx": torch.from_numpy(vox).cuda(), "sampled_point_xyz": x, "sampled_point_distance": None}, states, 0.2)
+    rows = np.where(ms.vertex_idx >= 0, ms.id2row[np.maximum(ms.vertex_idx, 0)], -1)
+    bits = emb.detach().view(torch.int16).cpu().numpy().view(np.uint16)
+    want, cache = O.trilinear_forward(xyz, vox, ms.centres, rows, bits, 0.2)
+    # eight products and their sum in another order: 16 roundings of 2^-24 of the magnitudes
+    mag = (cache["w"][:, :, None] * np.abs(cache["e"])).sum(1)
+    assert out["emb"].dtype == torch.float32 and np.all(np.abs(out["emb"].detach().cpu().numpy() - want) <= 16 * 2.0 ** -24 * mag)
+    df = torch.randn(P, 16, device="cuda")
+    gE, gx = torch.autograd.grad(out["emb"], [emb, x], df)
+    w, e, d = cache["w"].astype(np.float64), cache["e"].astype(np.float64), df.double().cpu().numpy()
+    wantE, magE, n = np.zeros((len(bits), 16)), np.zeros((len(bits), 16)), np.zeros(len(bits))
+    for k in range(8):
+        np.add.at(wantE, cache["rows"][:, k], w[:, k:k + 1] * d)
+        np.add.at(magE, cache["rows"][:, k], np.abs(w[:, k:k + 1] * d))
+        np.add.at(n, cache["rows"][:, k], 1)
+    got = gE.double().cpu().numpy()
+    assert gE.dtype == torch.bfloat16
+    assert np.all(np.abs(got - wantE) <= (n[:, None] + 8) * 2.0 ** -24 * magE + 2.0 ** -8 * np.abs(wantE) + 1e-38)      # fp32 sums, one rounding to the table's type
+    p = cache["p"].astype(np.float64)
+    s = np.einsum("pkc,pc->pk", e, d)
+    sa = np.einsum("pkc,pc->pk", np.abs(e), np.abs(d))
+    dp, mx = np.zeros((P, 3)), np.zeros((P, 3))
+    for k in range(8):
+        q = [(k >> 2) & 1, (k >> 1) & 1, k & 1]
+        for a in range(3):
+            others = np.prod([p[:, b] if q[b] else 1 - p[:, b] for b in range(3) if b != a], 0)
+            dp[:, a] += (1 if q[a] else -1) * others * s[:, k]
+            mx[:, a] += np.abs(others) * sa[:, k]
+    assert np.all(np.abs(gx.double().cpu().numpy() - dp / 0.2) <= 64 * 2.0 ** -24 * mx / 0.2 + 1e-12)
+    # a voxel outside the map: no features, no gradient
+    v2 = torch.from_numpy(vox).cuda().clone()
+    v2[3], v2[4] = -1, 10 ** 9
+    f2 = get_features({"sampled_point_voxel_idx": v2, "sampled_point_xyz": x}, states, 0.2)["emb"]
+    assert not bool(f2[3:5].any()) and torch.equal(f2[5:], out["emb"][5:]) and torch.equal(f2[:3], out["emb"][:3])
+    with pytest.raises(ValueError):
+        get_features({"sampled_point_voxel_idx": v2[:-1], "sampled_point_xyz": x}, states, 0.2)
+
+
+@pytest.mark.parametrize("checkpoint", [None, "mx8"])
+@pytest.mark.parametrize("cfg", [dict(depth=3, width=128, skips=[0]), dict(depth=2, width=64)])
+def test_a_training_step_of_the_whole_chain(cfg, checkpoint):
+    """features -> decoder -> Criterion -> gradients of the table, the decoder and the sample positions, against the chain in 64 bits.  The relu masks of the 64-bit
+    chain may differ where a pre-activation is within its own rounding of zero: gradients are compared in the 2-norm, where one flipped unit in a million is 1e-3.
+    In 8 bits the weight gradients use inputs that are off by up to 2^-4 of their value, independently: about 2^-5.8 / sqrt(samples) of a layer's gradient is left of it
+    where samples agree, at most 2^-4 where they do not"""
+    from nerf_loam_amd.criterion import Criterion
+    from nerf_loam_amd.render_helpers import get_features
+    ms, states, surf = _scene()
+    R, S = 64, 24
+    vox, xyz = _samples(ms, surf, R * S, 9)
+    emb = (states["voxel_vertex_emb"].float() * 30).bfloat16().requires_grad_(True)
+    states["voxel_vertex_emb"] = emb
+    dec = _decoder(11, checkpoint=checkpoint, **cfg)
+    rng = np.random.default_rng(3)
+    pts = torch.from_numpy(rng.normal(0, 8, (R, 3)).astype(np.float32)).cuda()
+    cos = torch.from_numpy(rng.uniform(0.3, 1.0, R).astype(np.float32)).cuda()
+    z = (pts.norm(dim=1, keepdim=True) + torch.from_numpy(rng.normal(0, 0.4, (R, S)).astype(np.float32)).cuda())
+    valid = torch.from_numpy(rng.random((R, S)) < 0.9).cuda()
+    crit = Criterion(types.SimpleNamespace(criteria=dict(eiko_weight=0.0, sdf_weight=100.0, fs_weight=1.0, sdf_truncation=0.3), data_specs=dict(max_depth=50.0)))
+    x = torch.from_numpy(xyz).cuda().requires_grad_(True)
+    feats = get_features({"sampled_point_voxel_idx": torch.from_numpy(vox).cuda(), "sampled_point_xyz": x}, states, 0.2)["emb"]
+    sdf = dec(feats)["sdf"].reshape(R, S)
+    sdf.retain_grad()
+    feats.retain_grad()
+    loss, _ = crit(dict(sdf=sdf, z_vals=z, ray_mask=torch.ones(R, dtype=torch.bool, device="cuda"), valid_mask=valid), pts, cos)
+    loss.backward()
+    # from the loss's gradient at the decoder's output down, the 64-bit chain
+    want, leaves = _chain64(dec, feats)
+    grads = torch.autograd.grad(want, leaves, sdf.grad.double().reshape(-1, 1))
+
+    def off(a, b):
+        return float((a.double() - b).norm() / b.norm())
+    assert off(sdf.detach().reshape(-1, 1), want) < 1e-5
+    assert off(feats.grad, grads[0]) < 2e-3
+    for i, (p, g) in enumerate(zip(dec.param_list(), grads[1:])):
+        assert p.grad is not None and off(p.grad, g) < (2e-3 if checkpoint is None or i % 2 else 2.0 ** -4), i
+    # the table and the positions: what the features' gradient gives (the test above holds that), finite and of the right rows
+    rows = states["_device"].vertex_rows[torch.from_numpy(vox).cuda()].reshape(-1).long()
+    touched = torch.zeros(emb.shape[0], dtype=torch.bool, device="cuda")
+    touched[rows] = True
+    assert bool(torch.isfinite(emb.grad.float()).all()) and not bool(emb.grad[~touched].any()) and bool(emb.grad.any()) and bool(torch.isfinite(x.grad).all())
+
+
+def test_scores_and_mesh_of_a_decoder_of_another_size():
+    from nerf_loam_amd.mesh_util import MeshExtractor
+    from nerf_loam_amd.render_helpers import get_features, get_scores
+    ms, states, surf = _scene()
+    keep = torch.from_numpy(surf[:300])
+    sub = {k: (v[keep] if k in ("voxel_vertex_idx", "voxel_center_xyz", "voxel_structure") else v) for k, v in states.items()}
+    sub["voxel_vertex_emb"] = (states["voxel_vertex_emb"].float() * 50).bfloat16()
+    dec = _decoder(13, depth=3, width=80, skips=[1])
+    res = 6
+    grid = get_scores(dec, sub, 0.2, bits=res, device_out=True)
+    assert grid.shape == (300, res, res, res, 1) and not grid.requires_grad
+    lin = torch.linspace(-0.5, 0.5, res, device="cuda")
+    off = torch.stack(torch.meshgrid(lin, lin, lin, indexing="ij"), -1).reshape(-1, 3) * 0.2
+    xyz = (sub["voxel_center_xyz"].cuda()[:, None, :3] + off).reshape(-1, 3)
+    full = dict(states, voxel_vertex_emb=sub["voxel_vertex_emb"])
+    full.pop("_device", None)
+    feats = get_features({"sampled_point_voxel_idx": keep.cuda().repeat_interleave(res ** 3), "sampled_point_xyz": xyz}, full, 0.2)["emb"]
+    want, _ = _chain64(dec, feats)
+    d = (grid.reshape(-1, 1).double() - want).abs()
+    # the two ways to the features differ by the rounding of xyz - centre (2^-24 of 2000 m over a voxel of 0.2 m: 6e-4 of the features' spread)
+    assert float(d.max()) <= 5e-3 * float(want.std()) + (6 * 96 + 8) * 2.0 ** -23 * 4 * float(_chain_abs(dec, feats).max())
+    with torch.no_grad():
+        dec.sdf_out.bias.sub_(float(grid.median()))
+    mesh = MeshExtractor(types.SimpleNamespace(mapper_specs={"voxel_size": 0.2})).create_mesh(dec, sub, 0.2, sub["voxel_center_xyz"], offset=-2000, res=res)
+    assert len(np.asarray(mesh.vertices)) > 100 and len(np.asarray(mesh.triangles)) > 100

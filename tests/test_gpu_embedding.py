@@ -199,3 +199,22 @@ def test_refusals():
                 lambda: ops.embedding_backward(table, ids, g, w, g_table=torch.empty_like(table), workspace=torch.empty(8, dtype=torch.uint8, device="cuda"))):
         with pytest.raises(RuntimeError):
             bad()
+
+
+@pytest.mark.parametrize("run", [1, 15, 16, 17, 32, 64, 1000, 1024, 1025, 4096])
+def test_runs_that_meet_the_borders_of_chunks_and_blocks(run):
+    """equal ids in runs of one length: rows that begin and end exactly where chunks (16 entries, 64 for many lookups) and blocks of 64 chunks do, and rows that do not"""
+    for L in (9000, 70000):
+        ids = (torch.arange(L, device="cuda") // run).to(torch.int32).view(-1, 1)
+        V = int(ids.max()) + 1
+        g = _rand(_gen(run), L, 4, dtype=torch.float32)
+        table = _rand(_gen(1), V, 4, dtype=torch.float32)
+        _check(table, ids, None, g, 1.0, *_grads(table, ids, None, g, 1.0), f"run {run} L {L}")
+
+
+def test_three_levels_of_joins():
+    """300000 lookups of two rows: 4688 chunks, 74 blocks, 2 blocks of blocks"""
+    g = _rand(_gen(3), 300000, 4, dtype=torch.float32)
+    ids = (torch.arange(300000, device="cuda") >= 131072 + 5).to(torch.int64).view(-1, 1)
+    table = _rand(_gen(4), 2, 4, dtype=torch.float32)
+    _check(table, ids, None, g, 1.0, *_grads(table, ids, None, g, 1.0), "two rows")

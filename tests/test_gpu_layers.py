@@ -212,6 +212,21 @@ def test_long_and_wide_layers(dtype, M, N, K):
     _backward_check(gy, x, w, "silu", dict(z=z, z_values=z.double()), dtype, "long")
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ["none", "silu"])
+def test_few_rows_of_either_operand(dtype, act):
+    """at most eight rows of x, or a weight with at most eight: the kernel without tiles, odd sizes and strides among them"""
+    for i, (M, N, K) in enumerate([(m, n, k) for m, n in ((1, 1000), (2, 33), (3, 500), (4, 64), (5, 129), (8, 300), (1000, 1), (999, 2), (77, 3), (513, 8), (9, 7), (8, 8)) for k in (1, 16, 40, 256, 513, 2048)]):
+        x, w, b, r = _forward_case(M, N, K, dtype, act, 900 + i, bias=i % 2 == 0, residual=i % 3 == 0)
+        _check_forward(x, w, b, r, act, layers.linear_act(x, w, b, act=act, residual=r), f"{M}x{N}x{K}")
+        wide = torch.full((M, K + 3), float("nan"), dtype=dtype, device="cuda")
+        wide[:, 1:K + 1] = x
+        out = torch.full((M, N + 2), 5.0, dtype=dtype, device="cuda")
+        ops.linear_forward(wide[:, 1:K + 1], w, b, act, r, out=out[:, 1:N + 1])
+        assert bool((out[:, 0] == 5).all()) and bool((out[:, -1] == 5).all())
+        _check_forward(x, w, b, r, act, out[:, 1:N + 1], f"strided {M}x{N}x{K}")
+
+
 @pytest.mark.parametrize("M,N,K", [(300, 256, 512), (4096, 512, 1024), (1, 512, 512)])
 def test_fp32_is_fp32(M, N, K):
     """the split products against 64 bits in the 2-norm: independent roundings of 2^-25 on average of a partial sum, not 2^-9"""

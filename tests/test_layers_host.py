@@ -115,3 +115,15 @@ def test_no_cpu_path_and_no_unknown_choice():
     with pytest.raises(ValueError, match="checkpoint"):
         layers.linear_act(x, w, checkpoint="int4")
     assert ops.linear_forward is not None
+
+
+def test_decoders_of_any_size_refuse_the_cpu_and_unknown_shapes():
+    from nerf_loam_amd.decoder import Decoder
+    dec = Decoder(depth=3, width=40, in_dim=16, skips=[0])
+    assert [tuple(l.weight.shape) for l in dec.pts_linears] == [(40, 16), (40, 56), (40, 40)] and not dec.fused and Decoder().fused
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        dec(torch.zeros(4, 16))
+    with pytest.raises(ValueError):
+        Decoder(depth=2, skips=[1])
+    with pytest.raises(NotImplementedError):
+        Decoder(embedder="gaussian")
