@@ -14,6 +14,7 @@
 #define EMB_BATCH 8             // rows in flight together
 #define RS_TILE 1024            // keys per workgroup of a sorting pass: 4 waves x 4 rounds x 64 lanes
 #define RS_ROUNDS (RS_TILE / 256)
+#define RS_FEW_BLOCKS 64        // up to here (65536 keys) the scatter sums the histograms itself: a launch less per pass
 #define RS_SMALL 4096           // up to here one workgroup sorts everything in LDS: one launch instead of three per pass
 
 __device__ __forceinline__ long long emb_id(const void* ids, int id64, long long i) { return id64 ? ((const long long*)ids)[i] : (long long)((const int*)ids)[i]; }
@@ -123,8 +124,8 @@ struct RsArgs {
     const void* ids; int id64; long long V;            // first pass
     const unsigned* keys; const unsigned* pos;         // later passes
     unsigned* out_keys; unsigned* out_pos;
-    int* hist;                                         // [256][nblk], then its exclusive sums along a row
-    int* totals;                                       // [256]
+    int* hist;                                         // [nblk][256], then (k_rs_scan) its exclusive sums over the blocks
+    int* totals;                                       // [256]; null: every workgroup of the scatter sums what is in front of it
     int L, nblk, shift;
     unsigned* zero; long long zero_words;              // first pass: the launch's workgroups behind the sorting ones clear these (the gradient's rows)
 };
@@ -154,19 +155,19 @@ __global__ __launch_bounds__(256) void k_rs_hist(RsArgs a)
         if (i < a.L) atomicAdd(&s_h[rs_key(a, i) >> a.shift & 255], 1);       // (whole numbers: the order does not matter)
     }
     __syncthreads();
-    a.hist[threadIdx.x * a.nblk + blockIdx.x] = s_h[threadIdx.x];
+    a.hist[blockIdx.x * 256 + threadIdx.x] = s_h[threadIdx.x];
 }
-// one workgroup per digit: exclusive sums along the digit's row of the histogram, and its total
+// one workgroup per digit: exclusive sums of the digit's column of the histogram, and its total
 __global__ __launch_bounds__(256) void k_rs_scan(RsArgs a)
 {
     __shared__ int s_w[4];
     if (rs_zero(a, 256)) return;
-    int* row = a.hist + (long long)blockIdx.x * a.nblk;
+    int* col = a.hist + blockIdx.x;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int run = 0;
     for (int b = 0; b < a.nblk; b += 256) {
         const int i = b + threadIdx.x;
-        const int v = i < a.nblk ? row[i] : 0;
+        const int v = i < a.nblk ? col[(long long)i * 256] : 0;
         int s = v;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) { const int t = __shfl_up(s, off); if (lane >= off) s += t; }
@@ -174,7 +175,7 @@ __global__ __launch_bounds__(256) void k_rs_scan(RsArgs a)
         __syncthreads();
         int before = run;
         for (int w = 0; w < wave; w++) before += s_w[w];
-        if (i < a.nblk) row[i] = before + s - v;
+        if (i < a.nblk) col[(long long)i * 256] = before + s - v;
         run += s_w[0] + s_w[1] + s_w[2] + s_w[3];
         __syncthreads();
     }
@@ -187,14 +188,18 @@ __global__ __launch_bounds__(256) void k_rs_scatter(RsArgs a)
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d0 = threadIdx.x;
     // where the digit begins: sums of the totals in front of it
     {
-        const int v = a.totals[d0];
+        int v = 0, front = 0;
+        if (a.totals) { v = a.totals[d0]; front = a.hist[(long long)blockIdx.x * 256 + d0]; }
+        else
+#pragma unroll 8
+            for (int b = 0; b < a.nblk; b++) { const int c = a.hist[(long long)b * 256 + d0]; front += b < (int)blockIdx.x ? c : 0; v += c; }
         int s = v;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) { const int t = __shfl_up(s, off); if (lane >= off) s += t; }
         if (lane == 63) s_w[wave] = s;
         __syncthreads();
         for (int w = 0; w < wave; w++) s += s_w[w];
-        s_base[d0] = s - v + a.hist[(long long)d0 * a.nblk + blockIdx.x];
+        s_base[d0] = s - v + front;
     }
 #pragma unroll
     for (int w = 0; w < 4; w++) s_cnt[w][d0] = 0;
@@ -400,13 +405,16 @@ __global__ __launch_bounds__(256) void k_emb_join(EmbPieces in, EmbPieces out, i
         const bool mine = which == 0 ? any0 && (open_l ? c == b0 : first == last) : any1;
         if (!mine) continue;
         const unsigned key = which == 0 ? first : last;
-        // how far the row goes: chunks c + 1 .. c + more, their slots 0; the row goes on behind a chunk that is one run
+        // how far the row goes: the chunks behind c whose first key is its key (keys are sorted: they follow each other), eight looked at together
         int more = 0;
-        bool goes_on = which == 1 || first == last;
-        while (goes_on && c + more + 1 < b1 && in.keys[2 * (c + more + 1)] == key) {
-            more++;
-            goes_on = in.keys[2 * (c + more) + 1] == key;
+        for (bool full = true; full;) {
+            bool same[EMB_BATCH];
+#pragma unroll
+            for (int i = 0; i < EMB_BATCH; i++) { const int j = c + 1 + more + i; same[i] = in.keys[2 * (j < b1 ? j : c)] == key && j < b1; }
+#pragma unroll
+            for (int i = 0; i < EMB_BATCH; i++) { full = full && same[i]; more += full; }
         }
+        const bool goes_on = more > 0 ? in.keys[2 * (c + more) + 1] == key : which == 1 || first == last;
         EmbVec<VEC> acc = emb_load<VEC, NL_DT_F32>(in.piece, (2LL * c + which) * D + (col ? d : 0));
         for (int j0 = 0; j0 < more; j0 += EMB_BATCH) {
             EmbVec<VEC> r[EMB_BATCH];
@@ -548,10 +556,10 @@ int nl_embedding_backward(const void* table, long long V, int D, int dtype, cons
     unsigned* pos[2] = {(unsigned*)(w + 2 * p.keys), (unsigned*)(w + 3 * p.keys)};
     w += 4 * p.keys;
     RsArgs r = {};
-    r.totals = (int*)w; r.hist = (int*)(w + 1024); r.L = p.L; r.nblk = p.nblk; r.V = V;
+    r.totals = p.nblk <= RS_FEW_BLOCKS ? nullptr : (int*)w; r.hist = (int*)(w + 1024); r.L = p.L; r.nblk = p.nblk; r.V = V;
     w += p.hist;
-    // the gradient's rows are cleared beside the first sorting pass, a third of them by each of its launches
-    const long long words = bytes / 4, third = p.L <= RS_SMALL ? words : (words / 3 + 63) / 64 * 64;
+    // the gradient's rows are cleared beside the first sorting pass, an equal part by each of its launches
+    const long long words = bytes / 4, launches = p.nblk <= RS_FEW_BLOCKS ? 2 : 3, part = (words / launches + 63) / 64 * 64;
     if (p.L <= RS_SMALL) {
         r.ids = ids; r.id64 = id64; r.out_keys = keys[(p.passes - 1) & 1]; r.out_pos = pos[(p.passes - 1) & 1];
         r.zero = (unsigned*)g_table; r.zero_words = words;
@@ -561,7 +569,8 @@ int nl_embedding_backward(const void* table, long long V, int D, int dtype, cons
             r.ids = i == 0 ? ids : nullptr; r.id64 = id64; r.shift = 8 * i;
             r.keys = keys[(i + 1) & 1]; r.pos = pos[(i + 1) & 1]; r.out_keys = keys[i & 1]; r.out_pos = pos[i & 1];
             for (int k = 0; k < 3; k++) {
-                const long long z0 = k * third < words ? k * third : words, z1 = k == 2 ? words : (k + 1) * third < words ? (k + 1) * third : words;
+                if (k == 1 && p.nblk <= RS_FEW_BLOCKS) continue;
+                const long long nth = k == 2 ? launches - 1 : k, z0 = nth * part < words ? nth * part : words, z1 = k == 2 ? words : z0 + part < words ? z0 + part : words;
                 r.zero = (unsigned*)g_table + z0; r.zero_words = i == 0 ? z1 - z0 : 0;
                 const dim3 grid((k == 1 ? 256 : p.nblk) + emb_zero_blocks(r.zero_words, 256));
                 if (k == 0) hipLaunchKernelGGL(k_rs_hist, grid, dim3(256), 0, st, r);

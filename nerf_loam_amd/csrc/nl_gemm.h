@@ -119,7 +119,7 @@ template <int BM, int BN> __device__ __forceinline__ unsigned gemm_tile_of(const
 template <int DT, int WR, int WC, int WAVES, int LDS>
 __device__ __forceinline__ void gemm_results(const NlGemm& g, nl_f32x4 (&acc)[WR / 16][WC / 16], char* s_mem, long long m, int n, unsigned piece)
 {
-    constexpr int RP = WR < 64 ? WR : 64, CX = WC / 4 - 1;
+    constexpr int RP = WR < 64 ? WR : (DT == NL_DT_F32 && WR == 64 ? 32 : 64), CX = WC / 4 - 1;
     static_assert((CX & (CX + 1)) == 0 && RP * WC * 4 * WAVES <= LDS, "the exchange fits into the operand buffers");
     constexpr int TURNS = RP * WC / 512, BATCH = TURNS < 4 ? TURNS : 4;
     static_assert(64 % (WC / 8) == 0 && TURNS % BATCH == 0, "a lane keeps its columns");
@@ -239,7 +239,8 @@ struct GemmSideMx8 {
 };
 
 // RING: LDS buffers per operand.  2: the next step arrives while one multiplies.  4 (squares of 64 while they leave compute units idle anyway): three steps are on their way;
-// a step of such a tile multiplies for 130 cycles and waits for memory the rest of the time.  The barrier then waits for the oldest step's loads only.
+// a step of such a tile multiplies for 130 cycles and waits for memory the rest of the time.  One barrier per step, in front of it every wave waits for its own loads of
+// the step (the RING - 2 later ones stay in flight) and for its fragment reads of the step before, whose buffer the loads behind the barrier overwrite.
 template <class T, bool A_SLOW, bool B_SLOW, bool B_MX8, int BM, int BN, int WM, int WN, int RING>
 __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
 {
@@ -268,12 +269,11 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
         if (B_MX8) b8.fetch(s, left);
         else b.load(s_b + (s & (RING - 1)) * SB::BYTES, s * b.step, left);
     };
+#pragma unroll
     for (int s = 0; s < RING - 1; s++) fetch(s);                      // (behind the last step nothing is inside: zeros)
     if (B_MX8) b8.put(s_b);
-    if (RING == 2) __syncthreads();
     for (int s = 0; s < steps; s++) {
-        // RING 4: this step's loads have landed, two later steps' stay in flight; behind the barrier nobody reads the buffer of step s - 1 any more
-        if (RING > 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((RING - 2) * (SA::LOADS + SB::LOADS)) : "memory");
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((RING - 2) * (SA::LOADS + SB::LOADS)) : "memory");
         const char* la = s_a + (s & (RING - 1)) * SA::BYTES;
         const char* lb = s_b + (s & (RING - 1)) * SB::BYTES;
         // fragments of both halves of the step, the loads of the next step between them: behind all fragment reads they come late (8192^3 / 16384 x 4096 x 4096,
@@ -297,9 +297,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
 #pragma unroll
             for (int j = 0; j < FN; j++) acc[i][j] = NlMma<T>::mma(fb[1][j], fa[1][i], acc[i][j]);
         if (B_MX8 && s + 1 < steps) b8.put(s_b + ((s + 1) & 1) * SB::BYTES);
-        if (RING == 2) __syncthreads();
     }
-    if (RING > 2) __syncthreads();                                    // (waits for all loads, the ones of zeros too)
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");        // (all loads, the ones of zeros too: the results pass through the same memory)
     gemm_results<DT, BM / WM, BN / WN, WM * WN, RING * (SA::BYTES + SB::BYTES)>(g, acc, s_mem, m0 + wm, n0 + wn, piece);
 }
 
@@ -409,7 +408,7 @@ __global__ __launch_bounds__(256, 2) void k_gemm_f32(NlGemm g)
     typedef GemmSide32<A_SLOW, BT> SA;
     typedef GemmSide32<B_SLOW, BT> SB;
     constexpr int F = BT / 32, LDS = SA::BYTES + SB::BYTES;
-    __shared__ __align__(256) char s_mem[LDS > BT * BT * 4 ? LDS : BT * BT * 4];
+    __shared__ __align__(256) char s_mem[LDS > BT * BT * 2 ? LDS : BT * BT * 2];
     char* const s_b = s_mem + SA::BYTES;
     long long m0; int n0;
     const unsigned piece = gemm_tile_of<BT, BT>(g, m0, n0);
@@ -431,22 +430,23 @@ __global__ __launch_bounds__(256, 2) void k_gemm_f32(NlGemm g)
             b.fetch((s + 1) * b.step, span - (s + 1) * 32LL);
         }
         __builtin_amdgcn_sched_barrier(0);
-        nl_s16x8 fa[3][F], fb[3][F];
+        nl_s16x8 fb[3][F];
 #pragma unroll
-        for (int p = 2; p >= 0; p--) {
+        for (int p = 0; p < 3; p++)
 #pragma unroll
-            for (int i = 0; i < F; i++) fa[p][i] = SA::Plane::frag(s_mem + p * SA::Plane::BYTES, wm + 16 * i, 0);
+            for (int j = 0; j < F; j++) fb[p][j] = SB::Plane::frag(s_b + p * SB::Plane::BYTES, wn + 16 * j, 0);
 #pragma unroll
-            for (int i = 0; i < F; i++) fb[2 - p][i] = SB::Plane::frag(s_b + (2 - p) * SB::Plane::BYTES, wn + 16 * i, 0);
+        for (int i = 0; i < F; i++) {
+            nl_s16x8 fa[3];
+#pragma unroll
+            for (int p = 0; p < 3; p++) fa[p] = SA::Plane::frag(s_mem + p * SA::Plane::BYTES, wm + 16 * i, 0);
+#pragma unroll
+            for (int sum = 2; sum >= 0; sum--)
+#pragma unroll
+                for (int p = sum; p >= 0; p--)
+#pragma unroll
+                    for (int j = 0; j < F; j++) acc[i][j] = NlMma<__bf16>::mma(fb[sum - p][j], fa[p], acc[i][j]);
         }
-#pragma unroll
-        for (int sum = 2; sum >= 0; sum--)
-#pragma unroll
-            for (int p = sum; p >= 0; p--)
-#pragma unroll
-                for (int i = 0; i < F; i++)
-#pragma unroll
-                    for (int j = 0; j < F; j++) acc[i][j] = NlMma<__bf16>::mma(fb[sum - p][j], fa[p][i], acc[i][j]);
         nl_lds_barrier();
     }
     gemm_results<NL_DT_F32, BT / 2, BT / 2, 4, sizeof(s_mem)>(g, acc, s_mem, m0 + wm, n0 + wn, piece);

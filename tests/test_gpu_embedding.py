@@ -218,3 +218,21 @@ def test_three_levels_of_joins():
     ids = (torch.arange(300000, device="cuda") >= 131072 + 5).to(torch.int64).view(-1, 1)
     table = _rand(_gen(4), 2, 4, dtype=torch.float32)
     _check(table, ids, None, g, 1.0, *_grads(table, ids, None, g, 1.0), "two rows")
+
+
+def test_tables_beyond_32_bits():
+    """a table of more than 2^31 elements: rows at the far end, forward and backward"""
+    V, D, M = 700000, 3200, 600
+    table = torch.zeros(V, D, dtype=torch.bfloat16, device="cuda")
+    ids = (torch.arange(M, device="cuda") * 7 % 13 + V - 13).to(torch.int64).view(-1, 1)
+    ids[5] = 671089
+    g = _rand(_gen(9), M, D, dtype=torch.bfloat16)
+    rows = torch.unique(ids)
+    table[rows] = _rand(_gen(8), len(rows), D, dtype=torch.bfloat16)
+    y = ops.embedding_forward(table, ids)
+    assert torch.equal(y, table[ids.view(-1)])
+    gt = torch.full_like(table, 3.0)
+    ops.embedding_backward(table, ids, g, g_table=gt)
+    want = torch.zeros(V - 671089, D, dtype=torch.float64, device="cuda").index_add_(0, ids.view(-1) - 671089, g.double())
+    assert bool(((gt[671089:].double() - want).abs() <= 64 * 2.0 ** -24 * 50 * 5 + 2.0 ** -8 * want.abs()).all())       # at most 50 lookups a row, |g| < 5
+    assert not bool(gt[:671089].any())

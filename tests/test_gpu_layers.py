@@ -479,3 +479,84 @@ def test_mixed_types_and_shapes_are_refused():
                       (lambda: layers.embedding_lookup(x, torch.zeros(2, 3, dtype=torch.int64, device="cuda"), weights=torch.zeros(2, 2, device="cuda")), "weights")):
         with pytest.raises(ValueError, match=word):
             bad()
+
+
+def test_offsets_beyond_32_bits():
+    """operands and results of more than 2^31 elements: rows at the far end come out as they do in a small call"""
+    M, K, N = 270000, 8192, 64
+    g = _gen(201)
+    w = _rand(g, N, K, dtype=torch.bfloat16, std=K ** -0.5)
+    x = torch.zeros(M, K, dtype=torch.bfloat16, device="cuda")
+    far = torch.tensor([0, 1, 262143, 262144, 262145, M - 65, M - 2, M - 1], device="cuda")
+    x[far] = _rand(g, len(far), K, dtype=torch.bfloat16)
+    y = layers.linear_act(x, w, act="none")
+    _check_forward(x[far], w, None, None, "none", y[far], "far rows")
+    assert int((y != 0).any(1).sum()) == len(far)
+    one = layers.linear_act(x, w[:1], act="none")
+    _check_forward(x[far], w[:1], None, None, "none", one[far], "far rows, one output")
+    gy = torch.zeros(M, N, dtype=torch.bfloat16, device="cuda")
+    gy[far] = _rand(g, len(far), N, dtype=torch.bfloat16)
+    c8, e8 = ops.mx8_encode(x)
+    assert torch.equal(ops.mx8_decode(c8, e8, K, torch.bfloat16)[far], ops.mx8_decode(*ops.mx8_encode(x[far]), K, torch.bfloat16))
+    gw, gw8, gx = torch.empty_like(w), torch.empty_like(w), torch.empty_like(x)
+    ops.linear_backward(gy, x, w, gw=gw, gx=gx)
+    ops.linear_backward(gy, None, w, x8=c8, x8e=e8, gw=gw8)
+    want = gy[far].double().t() @ x[far].double()
+    S = gy[far].double().abs().t() @ x[far].double().abs()
+    _close(gw, want, _e(M, torch.bfloat16) * S + _half(want, torch.bfloat16), "gw")
+    x8 = ops.mx8_decode(*ops.mx8_encode(x[far]), K, torch.bfloat16).double()
+    want = gy[far].double().t() @ x8
+    _close(gw8, want, _e(M, torch.bfloat16) * (gy[far].double().abs().t() @ x8.abs()) + _half(want, torch.bfloat16), "gw from codes")
+    want, S = gy[far].double() @ w.double(), gy[far].double().abs() @ w.double().abs()
+    _close(gx[far], want, _e(N, torch.bfloat16) * S + _half(want, torch.bfloat16), "gx")
+
+
+def test_one_tensor_in_several_places():
+    """x as its own residual, the weight of one layer in another: the gradients add up"""
+    g = _gen(211)
+    x = _rand(g, 90, 64, dtype=torch.float32).requires_grad_(True)
+    w = _rand(g, 64, 64, dtype=torch.float32, std=0.1).requires_grad_(True)
+    gy = _rand(g, 90, 64, dtype=torch.float32)
+
+    def chain(f, x, w):
+        return f(f(x, w, x), w, x)
+    got = torch.autograd.grad(chain(lambda a, b, r: layers.linear_act(a, b, act="silu", residual=r), x, w), [x, w], gy)
+    xd, wd = x.detach().double().requires_grad_(True), w.detach().double().requires_grad_(True)
+    want = torch.autograd.grad(chain(lambda a, b, r: torch.nn.functional.silu(a @ b.t()) + r, xd, wd), [xd, wd], gy.double())
+    for a, b in zip(got, want):
+        assert float((a.double() - b).norm() / b.norm()) < 1e-5                # two layers of float32, 64 and 90 terms
+
+
+def test_a_tensor_changed_after_the_forward_pass_is_noticed():
+    x, w, b, _ = _forward_case(40, 32, 48, torch.float32, "none", 221)
+    for t in (x, w):
+        t.requires_grad_(True)
+    y = layers.linear_act(x, w, b, act="relu")
+    with torch.no_grad():
+        w.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(torch.ones_like(y))
+
+
+def test_under_no_grad_nothing_is_kept():
+    x, w, b, _ = _forward_case(4000, 512, 512, torch.bfloat16, "gelu", 231)
+    w.requires_grad_(True)
+    layers.linear_act(x, w, b, act="gelu")
+    torch.cuda.synchronize()
+    base = torch.cuda.memory_allocated()
+    with torch.no_grad():
+        y = layers.linear_act(x, w, b, act="gelu")
+    assert not y.requires_grad and torch.cuda.memory_allocated() - base == y.numel() * 2
+
+
+def test_eight_bit_checkpoints_take_a_quarter_of_float32():
+    x, w, b, _ = _forward_case(8192, 1024, 1024, torch.float32, "silu", 241)
+    w.requires_grad_(True)
+    kept = {}
+    for ck in (None, "mx8"):
+        x1 = x.clone().requires_grad_(True)
+        base = torch.cuda.memory_allocated()
+        y = layers.linear_act(x1, w, b, act="silu", checkpoint=ck)
+        kept[ck] = torch.cuda.memory_allocated() - base - y.numel() * 4 + (0 if ck else x1.numel() * 4)
+        del y, x1
+    assert kept["mx8"] * 3.8 < kept[None]                                      # 8.25 bits instead of 32 for the input and for z
