@@ -562,11 +562,12 @@ int nl_dist_rows_union_prefix(const int* gathered, int stride_ints, int offset_i
  * nl_linear_forward reads x w b(or NULL) r(or NULL), writes y and, where the pointer is set, what the backward pass needs of z:
  *   z     gelu / silu: z [M,N] in dtype, rows N apart                     z8, z8e   instead of z: codes [M][up(N,32)] and exponents [M][ceil(N/32)]
  *   bits  relu: one bit per element, z > 0: words [M][ceil(N/32)], column n in bit n % 32 of word n / 32
+ *   x8, x8e   x in 8 bits for gw, [M][up(K,32)] and [M][ceil(K/32)], what nl_mx8_encode writes
  * nl_linear_backward reads gy, w (for gx), x or x8 / x8e (for gw), what the forward pass kept of z, and writes gx [M,K], gw [N,K], gb [N], each where its
  * pointer is set, in dtype.  dz = gy act'(z) is rounded to dtype once for the two products (fp32: not at all); gb sums the unrounded values.
  * fp32 products run as six bf16 products of the exact three-term splits of both operands (dropped terms below 2^-26 of |x||w|); an infinity among the
  * operands gives NaN there.  Sums are fp32 and their order depends on the sizes only.  M = 0 is a legal call (gw, gb = 0).
- * x8 / x8e: [M][up(K,32)] and [M][ceil(K/32)] as nl_mx8_encode writes them; a decoded value beyond dtype's largest number counts as that.
+ * A decoded value of x8 / x8e beyond dtype's largest number counts as that.
  * ws: nl_linear_workspace(desc, backward) bytes, 256-byte aligned; contents are free between calls. */
 typedef struct NlLinear {
     int struct_size, dtype, act, K, N, reserved;
@@ -577,7 +578,7 @@ typedef struct NlLinear {
     const void* r; long long ldr;
     void* y; long long ldy;
     void* z; unsigned* bits; unsigned char* z8; unsigned char* z8e;
-    const unsigned char* x8; const unsigned char* x8e;
+    unsigned char* x8; unsigned char* x8e;
     const void* gy; long long ldgy;
     void* gx; void* gw; void* gb;
     void* ws; long long ws_bytes;

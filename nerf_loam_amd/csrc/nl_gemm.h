@@ -13,6 +13,8 @@
 struct NlGemm {
     const char* A; const char* B;      // 16-byte aligned, rows 16-byte aligned
     const unsigned char* Be;           // B in 8-bit codes: its powers of two, ldb / 32 bytes between rows
+    unsigned char* A8; unsigned char* A8e;      // layout 4: where A's codes go, ld8 and ld8 / 32 bytes between rows
+    long long ld8;
     long long lda, ldb;                // bytes between rows
     long long M, K;
     int N, tiles_m, tiles_n;
@@ -20,7 +22,8 @@ struct NlGemm {
     NlEpilogue ep;
 };
 
-// layout 0: both operands' rows run along k; 1: B's rows are k; 2: both operands' rows are k; 3: the same with B in 8-bit codes (16-bit types only).  tile 0: 256 x 256 (16 bits only), 1: 128 x 128, 2: 64 x 64.
+// layout 0: both operands' rows run along k; 1: B's rows are k; 2: both operands' rows are k; 3: the same with B in 8-bit codes;
+// 4: layout 0, and A is written out in 8-bit codes (both for 16-bit types only).  tile 0: 256 x 256 (16 bits only), 1: 128 x 128, 2: 64 x 64.
 void nl_gemm_bf16(const NlGemm& g, int layout, int tile, dim3 grid, hipStream_t st);
 void nl_gemm_f16(const NlGemm& g, int layout, int tile, dim3 grid, hipStream_t st);
 void nl_gemm_f32(const NlGemm& g, int layout, int tile, dim3 grid, hipStream_t st);
@@ -238,17 +241,66 @@ struct GemmSideMx8 {
     }
 };
 
+// A step's rows of A in 8-bit codes, from LDS (GemmSide's fast layout): a thread takes a block of 32.  With a value that is not finite in the block every element is asked
+// (nl_mx_encode4 as in k_mx8_encode: the same codes); otherwise the largest magnitude is found among the 16-bit patterns, whose order is that of the magnitudes.
+template <class T, int BM, int NT>
+__device__ __forceinline__ void gemm_encode(const NlGemm& g, const char* lds, long long m0, long long k)
+{
+    constexpr int DT = __is_same(T, _Float16) ? NL_DT_F16 : NL_DT_BF16;
+    typedef __attribute__((__vector_size__(4))) unsigned short U2;
+    typedef GemmSide<false, BM, NT> Side;
+#pragma unroll
+    for (int u = 0; u < (2 * BM + NT - 1) / NT; u++) {
+        const int at = u * NT + threadIdx.x, row = at >> 1;
+        if (row >= BM || m0 + row >= g.M || k + 32 * (at & 1) >= g.ld8) continue;
+        nl_i32x4 raw[4];
+        U2 top = {};
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            raw[q] = *reinterpret_cast<const nl_i32x4*>(lds + row * (GEMM_BK * 2) + ((4 * (at & 1) + q) ^ Side::swz_row(row)) * 16);
+#pragma unroll
+            for (int j = 0; j < 4; j++) top = __builtin_elementwise_max(top, __builtin_bit_cast(U2, raw[q][j] & 0x7FFF7FFF));
+        }
+        const unsigned short most = top[0] > top[1] ? top[0] : top[1];
+        float amax = DT == NL_DT_BF16 ? nl_bf2f(most) : nl_h2f(most);
+        if (!(amax < INFINITY)) {
+            amax = 0.0f;
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                float v[8];
+                nl_unraw8<DT>(v, NlRaw8<DT>{{raw[q]}});
+#pragma unroll
+                for (int j = 0; j < 8; j++) amax = fmaxf(amax, nl_finite_abs(v[j]));
+            }
+        }
+        const int e = nl_mx_exponent(amax);
+        const float s = nl_pow2(-e);
+        unsigned char* const to = g.A8 + (m0 + row) * g.ld8 + k + 32 * (at & 1);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            float v[16];
+            nl_unraw8<DT>(v, NlRaw8<DT>{{raw[2 * h]}});
+            nl_unraw8<DT>(v + 8, NlRaw8<DT>{{raw[2 * h + 1]}});
+            nl_i32x4 w;
+#pragma unroll
+            for (int j = 0; j < 4; j++) w[j] = (int)nl_mx_encode4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3], s);
+            *reinterpret_cast<nl_i32x4*>(to + 16 * h) = w;
+        }
+        g.A8e[(m0 + row) * (g.ld8 / 32) + ((k >> 5) + (at & 1))] = (unsigned char)(e + 127);
+    }
+}
+
 // RING: LDS buffers per operand.  2: the next step arrives while one multiplies.  4 (squares of 64 while they leave compute units idle anyway): three steps are on their way;
 // a step of such a tile multiplies for 130 cycles and waits for memory the rest of the time.  One barrier per step, in front of it every wave waits for its own loads of
 // the step (the RING - 2 later ones stay in flight) and for its fragment reads of the step before, whose buffer the loads behind the barrier overwrite.
-template <class T, bool A_SLOW, bool B_SLOW, bool B_MX8, int BM, int BN, int WM, int WN, int RING>
+template <class T, bool A_SLOW, bool B_SLOW, bool B_MX8, int BM, int BN, int WM, int WN, int RING, bool ENC = false>
 __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
 {
     constexpr int DT = __is_same(T, _Float16) ? NL_DT_F16 : NL_DT_BF16;
     constexpr int NT = 64 * WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
     typedef GemmSide<A_SLOW, BM, NT> SA;
     typedef GemmSide<B_SLOW, BN, NT> SB;
-    static_assert(RING == 2 || (RING == 4 && !B_MX8), "buffers are taken in turn by the low bits of the step");
+    static_assert(RING == 2 || (RING == 4 && !B_MX8 && !ENC), "buffers are taken in turn by the low bits of the step");
     __shared__ __align__(256) char s_mem[RING * (SA::BYTES + SB::BYTES)];
     char* const s_a = s_mem;
     char* const s_b = s_mem + RING * SA::BYTES;
@@ -263,6 +315,9 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
     else b.init(g.B, g.ldb, n0, g.N, k0, g.K);
     const int wave = threadIdx.x >> 6, wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
     nl_f32x4 acc[FM][FN] = {};
+    // the tiles of a row of tiles take turns at writing A's codes: tile column c the steps c, c + tiles_n, .. of the contraction
+    int mine = 0;
+    if (ENC) { const int past = (int)((k0 / GEMM_BK) % g.tiles_n); mine = n0 / BN - past; if (mine < 0) mine += g.tiles_n; }
     auto fetch = [&](int s) {
         const long long left = k1 - k0 - (long long)s * GEMM_BK;
         a.load(s_a + (s & (RING - 1)) * SA::BYTES, s * a.step, left);
@@ -296,6 +351,10 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
         for (int i = 0; i < FM; i++)
 #pragma unroll
             for (int j = 0; j < FN; j++) acc[i][j] = NlMma<T>::mma(fb[1][j], fa[1][i], acc[i][j]);
+        if (ENC && s == mine) {
+            gemm_encode<T, BM, NT>(g, la, m0, k0 + (long long)s * GEMM_BK);
+            mine += g.tiles_n;
+        }
         if (B_MX8 && s + 1 < steps) b8.put(s_b + ((s + 1) & 1) * SB::BYTES);
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");        // (all loads, the ones of zeros too: the results pass through the same memory)
@@ -459,13 +518,13 @@ static void nl_gemm_tile_f32(const NlGemm& g, int tile, dim3 grid, hipStream_t s
     else hipLaunchKernelGGL((k_gemm_f32<A_SLOW, B_SLOW, 64>), grid, dim3(256), 0, st, g);
 }
 
-template <class T, bool A_SLOW, bool B_SLOW, bool B_MX8>
+template <class T, bool A_SLOW, bool B_SLOW, bool B_MX8, bool ENC = false>
 static void nl_gemm_tile(const NlGemm& g, int tile, dim3 grid, hipStream_t st)
 {
-    if (tile == 0) hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, B_MX8, 256, 256, 2, 4, 2>), grid, dim3(512), 0, st, g);
-    else if (tile == 1) hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, B_MX8, 128, 128, 2, 2, 2>), grid, dim3(256), 0, st, g);
-    else if (B_MX8 || (long long)grid.x * grid.y > NL_GEMM_FEW_SQUARES) hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, B_MX8, 64, 64, 2, 2, 2>), grid, dim3(256), 0, st, g);
-    else hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, false, 64, 64, 2, 2, B_MX8 ? 2 : 4>), grid, dim3(256), 0, st, g);
+    if (tile == 0) hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, B_MX8, 256, 256, 2, 4, 2, ENC>), grid, dim3(512), 0, st, g);
+    else if (tile == 1) hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, B_MX8, 128, 128, 2, 2, 2, ENC>), grid, dim3(256), 0, st, g);
+    else if (B_MX8 || ENC || (long long)grid.x * grid.y > NL_GEMM_FEW_SQUARES) hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, B_MX8, 64, 64, 2, 2, 2, ENC>), grid, dim3(256), 0, st, g);
+    else hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, false, 64, 64, 2, 2, B_MX8 || ENC ? 2 : 4>), grid, dim3(256), 0, st, g);
 }
 template <class T>
 static void nl_gemm_layout(const NlGemm& g, int layout, int tile, dim3 grid, hipStream_t st)
@@ -473,6 +532,7 @@ static void nl_gemm_layout(const NlGemm& g, int layout, int tile, dim3 grid, hip
     if (layout == 0) nl_gemm_tile<T, false, false, false>(g, tile, grid, st);
     else if (layout == 1) nl_gemm_tile<T, false, true, false>(g, tile, grid, st);
     else if (layout == 2) nl_gemm_tile<T, true, true, false>(g, tile, grid, st);
-    else nl_gemm_tile<T, true, true, true>(g, tile, grid, st);
+    else if (layout == 3) nl_gemm_tile<T, true, true, true>(g, tile, grid, st);
+    else nl_gemm_tile<T, false, false, false, true>(g, tile, grid, st);
 }
 #endif

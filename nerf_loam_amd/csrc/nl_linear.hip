@@ -121,20 +121,54 @@ template <int DT, bool SWAP> static int nl_launch_rows(const NlLinear* d, const 
     return NL_OK;
 }
 
+// gb[n] = sum over the chunks of k_linear_dz: four columns a workgroup, 256 runs of neighbouring chunks, the runs joined pairwise
+struct NlGb { const float* part; void* gb; int chunks, N, blocks; };      // blocks: workgroups that it takes
+template <int DT>
+__device__ __forceinline__ void nl_gb_block(const NlGb& a, int block, nl_f32x4* s_sum)
+{
+    const int n = block * 4, run = threadIdx.x, N = a.N;
+    const int per = (a.chunks + 255) / 256, c1 = (run + 1) * per < a.chunks ? (run + 1) * per : a.chunks;
+    nl_f32x4 s = {};
+    if ((N & 3) == 0) {
+#pragma unroll 4
+        for (int c = run * per; c < c1; c++) s += *reinterpret_cast<const nl_f32x4*>(a.part + (long long)c * N + n);
+    } else
+        for (int c = run * per; c < c1; c++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) if (n + j < N) s[j] += a.part[(long long)c * N + n + j];
+    s_sum[run] = s;
+    for (int off = 128; off >= 1; off >>= 1) {
+        __syncthreads();
+        if (run < off) s_sum[run] += s_sum[run + off];
+    }
+    if (run != 0) return;
+#pragma unroll
+    for (int j = 0; j < 4; j++) if (n + j < N) nl_store_elem<DT>(a.gb, n + j, s_sum[0][j]);
+}
+template <int DT>
+__global__ __launch_bounds__(256) void k_linear_gb(NlGb a)
+{
+    __shared__ nl_f32x4 s_sum[256];
+    nl_gb_block<DT>(a, blockIdx.x, s_sum);
+}
+
 // ---------------------------------------------------------------------------------------------
 // k_linear_join: sums the pieces of a split contraction and runs the epilogue.  Eight columns a thread, whole blocks of 32 columns.  With few results and many pieces
 // one thread per result group would walk all pieces one memory latency after the other (256 x 256 results in 64 pieces: 30 us): then RUNS threads sum a run of
-// neighbouring pieces each and the runs are added in order.
+// neighbouring pieces each and the runs are added in order.  The first gb.blocks workgroups sum a bias gradient: one launch less where a weight gradient is joined.
 // ---------------------------------------------------------------------------------------------
 template <int DT, int RUNS>
-__global__ __launch_bounds__(256) void k_linear_join(const float* __restrict__ part, int splits, long long M, int N, NlEpilogue ep)
+__global__ __launch_bounds__(256) void k_linear_join(const float* __restrict__ part, int splits, long long M, int N, NlEpilogue ep, NlGb gb)
 {
     constexpr int POS = 256 / RUNS;
-    __shared__ float s_sum[RUNS > 1 ? RUNS : 1][RUNS > 1 ? POS : 1][9];
+    __shared__ __align__(16) char s_mem[RUNS > 1 ? RUNS * POS * 9 * 4 : 256 * 16];
+    if ((int)blockIdx.x < gb.blocks) { nl_gb_block<DT>(gb, blockIdx.x, (nl_f32x4*)s_mem); return; }
+    float (*const s_sum)[POS][9] = (float (*)[POS][9])s_mem;
+    const unsigned block = blockIdx.x - gb.blocks, blocks = gridDim.x - gb.blocks;
     const int at = threadIdx.x % POS, run = threadIdx.x / POS, per = (splits + RUNS - 1) / RUNS;
     const int s0 = run * per, s1 = s0 + per < splits ? s0 + per : splits;
     const long long per_row = (N + 31) / 32 * 4, total = M * per_row;
-    for (long long t0 = (long long)blockIdx.x * POS; t0 < total; t0 += (long long)gridDim.x * POS) {
+    for (long long t0 = (long long)block * POS; t0 < total; t0 += (long long)blocks * POS) {
         const long long t = t0 + at, m = t / per_row;
         const int n = (int)(t - m * per_row) * 8;
         float v[8] = {};
@@ -222,31 +256,6 @@ __global__ __launch_bounds__(256) void k_linear_dz(NlDz a)
     a.part[(long long)blockIdx.y * a.N + col] = s;
 }
 
-// gb[n] = sum over the chunks: four columns a workgroup, 256 runs of neighbouring chunks, the runs joined pairwise
-template <int DT>
-__global__ __launch_bounds__(256) void k_linear_gb(const float* __restrict__ part, int chunks, int N, void* gb)
-{
-    __shared__ nl_f32x4 s_sum[256];
-    const int n = blockIdx.x * 4, run = threadIdx.x;
-    const int per = (chunks + 255) / 256, c1 = (run + 1) * per < chunks ? (run + 1) * per : chunks;
-    nl_f32x4 s = {};
-    if ((N & 3) == 0) {
-#pragma unroll 4
-        for (int c = run * per; c < c1; c++) s += *reinterpret_cast<const nl_f32x4*>(part + (long long)c * N + n);
-    } else
-        for (int c = run * per; c < c1; c++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) if (n + j < N) s[j] += part[(long long)c * N + n + j];
-    s_sum[run] = s;
-    for (int off = 128; off >= 1; off >>= 1) {
-        __syncthreads();
-        if (run < off) s_sum[run] += s_sum[run + off];
-    }
-    if (run != 0) return;
-#pragma unroll
-    for (int j = 0; j < 4; j++) if (n + j < N) nl_store_elem<DT>(gb, n + j, s_sum[0][j]);
-}
-
 __global__ __launch_bounds__(256) void k_linear_zero(unsigned char* p, long long bytes)
 {
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < bytes; i += (long long)gridDim.x * 256) p[i] = 0;
@@ -316,7 +325,7 @@ static NlCut nl_cut(long long M, long long N, long long K, int dt, int layout)
             const long long per = (ksteps + s - 1) / s;
             const double at = tiles * s / T[t].at_a_time, full = at < 1.0 ? at : 1.0, rounds = at < 1.0 ? 1.0 : at < 4.0 ? ceil(at) : at + 0.5;
             const double alone = t == 2 && dt != NL_DT_F32 && layout < 3 && tiles * s <= NL_GEMM_FEW_SQUARES ? 0.33 : T[t].alone;      // (four buffers)
-            double us = rounds * (per * (alone + (T[t].full - alone) * full) * (layout >= 2 ? T[t].slow : 1.0) + T[t].rest * (0.5 + 0.5 * full));
+            double us = rounds * (per * (alone + (T[t].full - alone) * full) * (layout == 2 || layout == 3 ? T[t].slow : 1.0) + T[t].rest * (0.5 + 0.5 * full));
             if (us < memory) us = memory;
             if (s > 1) us += 3.0 + 8.0 * s * M * N / 4.0e6;
             if (us < least) { least = us; best = NlCut{t, s, per * GEMM_BK}; }
@@ -326,13 +335,14 @@ static NlCut nl_cut(long long M, long long N, long long K, int dt, int layout)
     return best;
 }
 
-// C[M,N] = sum_k A(m,k) B(n,k).  layout 0: both operands' rows run along k; 1: B's rows are k; 2: both operands' rows are k; 3: the same with B in 8-bit codes
-static void nl_product(NlWork& w, const NlPacked& A, const NlPacked& B, int layout, long long M, int N, long long K, const NlEpilogue& ep)
+// C[M,N] = sum_k A(m,k) B(n,k), layouts as in nl_gemm.h.  A8, A8e: layout 4's codes.  gb: a bias gradient to sum in the same launch if there is one; then it is cleared
+static void nl_product(NlWork& w, const NlPacked& A, const NlPacked& B, int layout, long long M, int N, long long K, const NlEpilogue& ep, unsigned char* A8, unsigned char* A8e, NlGb* gb)
 {
-    const NlCut c = nl_cut(M, N, K, ep.dt, layout);
+    const NlCut c = nl_cut(M, N, K, ep.dt, layout == 4 ? 0 : layout);      // (the codes do not change the sums)
     static const int size[3] = {256, 128, 64};
     NlGemm g = {};
     g.A = (const char*)A.p; g.B = (const char*)B.p; g.Be = B.e; g.lda = nl_dtype_size(ep.dt) * A.pitch; g.ldb = layout == 3 ? B.pitch : nl_dtype_size(ep.dt) * B.pitch;
+    g.A8 = A8; g.A8e = A8e; g.ld8 = nl_up(K, NL_MX_BLOCK);
     g.M = M; g.N = N; g.K = K; g.kchunk = c.kchunk;
     const long long tm = nl_up(M, size[c.tile]) / size[c.tile], tn = nl_up(N, size[c.tile]) / size[c.tile];
     if (tm * tn > 0x7FFFFFF) { w.rc = NL_ERR_INVALID_ARG; return; }
@@ -346,8 +356,10 @@ static void nl_product(NlWork& w, const NlPacked& A, const NlPacked& B, int layo
     else nl_gemm_f16(g, layout, c.tile, grid, w.st);
     if (c.splits > 1) {
         const long long groups = M * ((N + 31) / 32 * 4);
-        if (c.splits >= 8 && groups < 131072) NL_WITH_DTYPE(ep.dt, hipLaunchKernelGGL((k_linear_join<DT, 8>), dim3(nl_grid(8 * groups)), dim3(256), 0, w.st, g.ep.part, c.splits, M, N, ep));
-        else NL_WITH_DTYPE(ep.dt, hipLaunchKernelGGL((k_linear_join<DT, 1>), dim3(nl_grid(groups)), dim3(256), 0, w.st, g.ep.part, c.splits, M, N, ep));
+        const NlGb bias = gb ? *gb : NlGb{};
+        if (gb) *gb = NlGb{};
+        if (c.splits >= 8 && groups < 131072) NL_WITH_DTYPE(ep.dt, hipLaunchKernelGGL((k_linear_join<DT, 8>), dim3(nl_grid(8 * groups) + bias.blocks), dim3(256), 0, w.st, g.ep.part, c.splits, M, N, ep, bias));
+        else NL_WITH_DTYPE(ep.dt, hipLaunchKernelGGL((k_linear_join<DT, 1>), dim3(nl_grid(groups) + bias.blocks), dim3(256), 0, w.st, g.ep.part, c.splits, M, N, ep, bias));
     }
     if (hipGetLastError() != hipSuccess) w.rc = NL_ERR_LAUNCH;
 }
@@ -359,13 +371,20 @@ static void nl_forward_run(const NlLinear* d, NlWork& w)
     ep.z = d->z; ep.ldz = d->N;
     ep.bits = d->bits; ep.ldbits = nl_up(d->N, 32) / 32;
     ep.z8 = d->z8; ep.z8e = d->z8e; ep.ldz8 = nl_up(d->N, 32); ep.ldz8e = ep.ldz8 / 32;
-    if ((d->M <= ROWS_MOST || d->N <= ROWS_MOST) && !d->z && !d->bits && !d->z8) {
+    const bool rows = (d->M <= ROWS_MOST || d->N <= ROWS_MOST) && !d->z && !d->bits && !d->z8;
+    // the codes of x come out of the product's own tiles; fp32's are split there, and few rows have no tiles: a pass of their own
+    const bool codes = d->x8 && d->dtype != NL_DT_F32 && !rows;
+    if (d->x8 && !codes && !w.dry) {
+        w.rc = nl_mx8_encode(d->x, d->ldx, d->M, d->K, d->dtype, d->x8, d->x8e, w.st);
+        if (w.rc != NL_OK) return;
+    }
+    if (rows) {
         if (!w.dry) NL_WITH_DTYPE(d->dtype, w.rc = d->M <= ROWS_MOST ? nl_launch_rows<DT, false>(d, ep, w.st) : nl_launch_rows<DT, true>(d, ep, w.st));
         return;
     }
     const NlPacked x = nl_packed(w, d->x, nullptr, d->M, d->K, d->ldx, d->dtype, d->dtype), wt = nl_packed(w, d->w, nullptr, d->N, d->K, d->ldw, d->dtype, d->dtype);
     nl_pack(w, d->dtype);
-    nl_product(w, x, wt, 0, d->M, d->N, d->K, ep);
+    nl_product(w, x, wt, codes ? 4 : 0, d->M, d->N, d->K, ep, d->x8, d->x8e, nullptr);
 }
 
 static void nl_backward_run(const NlLinear* d, NlWork& w)
@@ -373,6 +392,7 @@ static void nl_backward_run(const NlLinear* d, NlWork& w)
     const bool in_place = d->act == NL_ACT_NONE && nl_in_place(d->gy, d->N, d->ldgy, d->dtype);
     const bool products = d->gx || d->gw;
     NlPacked dz = {d->gy, d->ldgy, nullptr};
+    NlGb gb = {};
     if (d->gb || (products && !in_place)) {
         NlDz a = {};
         a.gy = d->gy; a.ldgy = d->ldgy; a.M = d->M; a.N = d->N;
@@ -397,8 +417,8 @@ static void nl_backward_run(const NlLinear* d, NlWork& w)
                                     else if (d->act == NL_ACT_RELU) hipLaunchKernelGGL((k_linear_dz<DT, NL_ACT_RELU>), grid, dim3(256), 0, w.st, a);
                                     else if (d->act == NL_ACT_GELU) hipLaunchKernelGGL((k_linear_dz<DT, NL_ACT_GELU>), grid, dim3(256), 0, w.st, a);
                                     else hipLaunchKernelGGL((k_linear_dz<DT, NL_ACT_SILU>), grid, dim3(256), 0, w.st, a));
-            if (d->gb) NL_WITH_DTYPE(d->dtype, hipLaunchKernelGGL(k_linear_gb<DT>, dim3((d->N + 3) / 4), dim3(256), 0, w.st, a.part, (int)chunks, d->N, d->gb));
         }
+        if (d->gb) gb = NlGb{a.part, d->gb, (int)chunks, d->N, (d->N + 3) / 4};
     }
     NlEpilogue ep = {};
     ep.dt = d->dtype; ep.act = NL_ACT_NONE; ep.ldy = d->K;
@@ -412,14 +432,15 @@ static void nl_backward_run(const NlLinear* d, NlWork& w)
     long long most = keep;
     if (d->gx) {
         ep.y = d->gx;
-        nl_product(w, dz, wt, 1, d->M, d->K, d->N, ep);
+        nl_product(w, dz, wt, 1, d->M, d->K, d->N, ep, nullptr, nullptr, nullptr);
         most = w.used;
         w.used = keep;                                               // (the second product follows on the stream: it takes the same place)
     }
     if (d->gw) {
         ep.y = d->gw;
-        nl_product(w, dz, x, codes ? 3 : 2, d->N, d->K, d->M, ep);
+        nl_product(w, dz, x, codes ? 3 : 2, d->N, d->K, d->M, ep, nullptr, nullptr, &gb);
     }
+    if (gb.blocks && !w.dry) NL_WITH_DTYPE(d->dtype, hipLaunchKernelGGL(k_linear_gb<DT>, dim3(gb.blocks), dim3(256), 0, w.st, gb));
     if (w.used < most) w.used = most;
 }
 
@@ -434,7 +455,7 @@ static int nl_linear_check(const NlLinear* d, int backward)
     if (((uintptr_t)d->z & 15) || ((uintptr_t)d->bits & 3) || ((uintptr_t)d->z8 & 15) || ((uintptr_t)d->x8 & 15)) return NL_ERR_INVALID_ARG;
     if (!backward) {
         if (!d->x || !d->w || !d->y || d->ldx < d->K || d->ldw < d->K || d->ldy < d->N || (d->r && d->ldr < d->N)) return NL_ERR_INVALID_ARG;
-        if ((!d->z8) != (!d->z8e)) return NL_ERR_INVALID_ARG;
+        if ((!d->z8) != (!d->z8e) || (!d->x8) != (!d->x8e)) return NL_ERR_INVALID_ARG;
         return NL_OK;
     }
     if (!d->gy || d->ldgy < d->N) return NL_ERR_INVALID_ARG;

@@ -320,9 +320,9 @@ def _workspace(need, ws, like, name):
     return ws, need
 
 
-def linear_forward(x, weight, bias=None, act="none", residual=None, out=None, z=None, bits=None, z8=None, z8e=None, workspace=None):
+def linear_forward(x, weight, bias=None, act="none", residual=None, out=None, z=None, bits=None, z8=None, z8e=None, x8=None, x8e=None, workspace=None):
     """y = act(x weight^T + bias) + residual; x [M,K], weight [N,K], bias [N], residual / out [M,N], rows may be strided.  z, bits, z8 / z8e: what
-    linear_backward needs of z, written where given (layers.linear_act allocates them)"""
+    linear_backward needs of z; x8 / x8e: x as mx8_encode writes it; each is written where given (layers.linear_act allocates them)"""
     stream, guard = _on_device(x)
     if x.dim() != 2 or weight.dim() != 2:
         raise L.NerfLoamHipError(f"linear_forward: x {tuple(x.shape)} must be [M, K] and weight {tuple(weight.shape)} [N, K]")
@@ -344,6 +344,9 @@ def linear_forward(x, weight, bias=None, act="none", residual=None, out=None, z=
     d.bits = _flat(bits, (M, NB), I32, x, "bits")
     d.z8 = _flat(z8, (M, 32 * NB), torch.uint8, x, "z8")
     d.z8e = _flat(z8e, (M, NB), torch.uint8, x, "z8e")
+    KB = (K + 31) // 32
+    d.x8 = _flat(x8, (M, 32 * KB), torch.uint8, x, "x8")
+    d.x8e = _flat(x8e, (M, KB), torch.uint8, x, "x8e")
     with guard:
         ws, d.ws_bytes = _workspace(L.lib().nl_linear_workspace(ctypes.byref(d), 0), workspace, x, "nl_linear_forward")
         d.ws = ws.data_ptr() if ws is not None else None

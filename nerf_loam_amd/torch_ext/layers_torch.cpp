@@ -88,9 +88,9 @@ void once_differentiable(torch::autograd::variable_list& out, bool differentiabl
     out = (*err)(std::move(in));
 }
 
-struct Kept { Tensor z, bits, z8, z8e; };
+struct Kept { Tensor z, bits, z8, z8e, x8, x8e; };
 
-Tensor linear_forward(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& r, int act, bool mx8, bool keep, Kept* kept)
+Tensor linear_forward(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& r, int act, bool mx8, bool keep, bool keep_x, Kept* kept)
 {
     const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
     c10::DeviceGuard guard(x.device());
@@ -101,6 +101,7 @@ Tensor linear_forward(const Tensor& x, const Tensor& w, const Tensor& b, const T
         else if (mx8) { kept->z8 = at::empty({M, 32 * nb}, bytes); kept->z8e = at::empty({M, nb}, bytes); }
         else kept->z = at::empty({M, N}, x.options());
     }
+    if (keep_x && mx8) { kept->x8 = at::empty({M, (K + 31) / 32 * 32}, bytes); kept->x8e = at::empty({M, (K + 31) / 32}, bytes); }
     Tensor y = at::empty({M, N}, x.options());
     NlLinear d = {};
     d.struct_size = (int)sizeof d; d.dtype = dtype_of(x, "x"); d.act = act; d.M = M;
@@ -110,6 +111,7 @@ Tensor linear_forward(const Tensor& x, const Tensor& w, const Tensor& b, const T
     if (r.defined()) { d.r = ptr(r); d.ldr = row_stride(r); }
     d.y = ptr(y); d.ldy = N;
     d.z = ptr(kept->z); d.bits = (unsigned*)ptr(kept->bits); d.z8 = (unsigned char*)ptr(kept->z8); d.z8e = (unsigned char*)ptr(kept->z8e);
+    d.x8 = (unsigned char*)ptr(kept->x8); d.x8e = (unsigned char*)ptr(kept->x8e);
     const Tensor ws = workspace(f_workspace(&d, 0), x, "nl_linear_forward");
     d.ws = ptr(ws); d.ws_bytes = ws.defined() ? ws.numel() : 0;
     check(f_forward(&d, stream_of(x)), "nl_linear_forward");
@@ -131,10 +133,8 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
     {
         const bool gx = x.requires_grad(), gw = w.requires_grad(), gb = b && b->requires_grad(), gr = r && r->requires_grad();
         Kept kept;
-        Tensor y = linear_forward(x, w, b ? *b : Tensor(), r ? *r : Tensor(), (int)act, mx8, gx || gw || gb, &kept);
-        Tensor x8, x8e;
-        if (gw && mx8) encode(x, x8, x8e);
-        ctx->save_for_backward({gw && !mx8 ? x : Tensor(), w, x8, x8e, kept.z, kept.bits, kept.z8, kept.z8e});
+        Tensor y = linear_forward(x, w, b ? *b : Tensor(), r ? *r : Tensor(), (int)act, mx8, gx || gw || gb, gw, &kept);
+        ctx->save_for_backward({gw && !mx8 ? x : Tensor(), w, kept.x8, kept.x8e, kept.z, kept.bits, kept.z8, kept.z8e});
         ctx->saved_data["c"] = std::vector<int64_t>{act, gx, gw, gb, gr, b.has_value(), r.has_value()};
         return y;
     }
@@ -192,7 +192,7 @@ Tensor linear_act(const Tensor& x, const Tensor& weight, const OptTensor& bias, 
     if (at::GradMode::is_enabled() && (x2.requires_grad() || w2.requires_grad() || (b && b->requires_grad()) || (r && r->requires_grad()))) y = LinearFn::apply(x2, w2, b, r, act, mx8);
     else {
         Kept kept;
-        y = linear_forward(x2, w2, b ? *b : Tensor(), r ? *r : Tensor(), (int)act, mx8, false, &kept);
+        y = linear_forward(x2, w2, b ? *b : Tensor(), r ? *r : Tensor(), (int)act, mx8, false, false, &kept);
     }
     return shape.size() == 2 ? y : y.view(shape);
 }

@@ -560,3 +560,56 @@ def test_eight_bit_checkpoints_take_a_quarter_of_float32():
         kept[ck] = torch.cuda.memory_allocated() - base - y.numel() * 4 + (0 if ck else x1.numel() * 4)
         del y, x1
     assert kept["mx8"] * 3.8 < kept[None]                                      # 8.25 bits instead of 32 for the input and for z
+
+
+CODES_SIZES = [(1, 64, 40), (300, 40, 1), (70, 33, 70), (65, 8, 200), (1003, 1001, 777), (300, 64, 2048), (4096, 96, 512), (129, 8200, 136), (5000, 512, 1024), (4100, 2080, 4096), (20000, 256, 256)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_forward_writes_the_codes_of_its_input(dtype):
+    """x8 / x8e of linear_forward are what mx8_encode writes, bit by bit: few rows, every tile, cut contractions, padded and strided rows, values that are not
+    finite, blocks of zeros and of denormal numbers; the output does not change"""
+    for M, K, N in CODES_SIZES:
+        g = torch.Generator(device="cuda").manual_seed(M + K)
+        x = torch.randn(M, K + 8, generator=g, device="cuda")
+        x = (x * torch.exp(3 * torch.randn(M, K + 8, generator=g, device="cuda"))).to(dtype)
+        x[:: 7, : 32] = 0.0
+        x[1:: 7, : 32] *= torch.finfo(dtype).smallest_normal
+        x = x[:, :K] if M % 2 else x[:, :K].contiguous()
+        w = (torch.randn(N, K, generator=g, device="cuda") * K ** -0.5).to(dtype)
+        for bad in (False, True):
+            if bad:
+                x[M // 2, K // 2] = float("nan")
+                x[M - 1, K - 1] = -float("inf")
+                x[0, : 33] = float("inf")
+            want, want_e = ops.mx8_encode(x)
+            got, got_e = torch.full_like(want, 77), torch.full_like(want_e, 77)
+            y = ops.linear_forward(x, w, x8=got, x8e=got_e)
+            assert torch.equal(got, want) and torch.equal(got_e, want_e), (M, K, N, bad)
+            z = torch.empty(M, N, dtype=dtype, device="cuda")
+            y2 = ops.linear_forward(x, w, act="silu", z=z, x8=got.fill_(77), x8e=got_e.fill_(77))
+            assert torch.equal(got, want) and torch.equal(got_e, want_e), (M, K, N, bad)
+            if not bad:
+                # (fp16: the large values overflow, and the sums of infinities are NaN on both sides)
+                for a, b in ((y, ops.linear_forward(x, w)), (y2, ops.linear_forward(x, w, act="silu", z=z))):
+                    assert bool(((a == b) | (a.isnan() & b.isnan())).all()), (M, K, N)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_forward_writes_the_codes_of_every_number(dtype):
+    """every 16-bit pattern, next to a large, a middling and a small neighbour that sets its block's power of two"""
+    every = torch.arange(65536, dtype=torch.int32, device="cuda").to(torch.int16).view(dtype)
+    lead = torch.tensor([1.0, 300.0, 2.0 ** -12], device="cuda").to(dtype)
+    x = torch.cat([torch.cat([every.view(-1, 16), lead[i].expand(4096, 16)], 1) for i in range(3)] + [every.view(2048, 32).repeat(2, 1)], 0)
+    w = torch.ones(96, 32, dtype=dtype, device="cuda")
+    want, want_e = ops.mx8_encode(x)
+    got, got_e = torch.empty_like(want), torch.empty_like(want_e)
+    ops.linear_forward(x, w, x8=got, x8e=got_e)
+    assert torch.equal(got, want) and torch.equal(got_e, want_e)
+    # in order of magnitude, so that a block holds similar numbers
+    order = every[torch.isfinite(every)].view(-1)
+    order = order[order.float().abs().argsort()].reshape(-1, 32)
+    want, want_e = ops.mx8_encode(order)
+    got, got_e = torch.empty_like(want), torch.empty_like(want_e)
+    ops.linear_forward(order, w, x8=got, x8e=got_e)
+    assert torch.equal(got, want) and torch.equal(got_e, want_e)
