@@ -567,6 +567,7 @@ int nl_dist_rows_union_prefix(const int* gathered, int stride_ints, int offset_i
  * pointer is set, in dtype.  dz = gy act'(z) is rounded to dtype once for the two products (fp32: not at all); gb sums the unrounded values.
  * fp32 products run as six bf16 products of the exact three-term splits of both operands (dropped terms below 2^-26 of |x||w|); an infinity among the
  * operands gives NaN there.  Sums are fp32 and their order depends on the sizes only.  M = 0 is a legal call (gw, gb = 0).
+ * Taken are at most 2^30 rows, 2^22 columns, and results of fewer than 2^24 tiles (of 64 x 64 where they are small).
  * A decoded value of x8 / x8e beyond dtype's largest number counts as that.
  * ws: nl_linear_workspace(desc, backward) bytes, 256-byte aligned; contents are free between calls. */
 typedef struct NlLinear {
@@ -597,7 +598,7 @@ int nl_mx8_decode(const unsigned char* codes, const unsigned char* exps, long lo
  * int64; an id outside [0, V) selects no row.  table [V,D], out [M,D] of dtype.
  * nl_embedding_backward: g_table [V,D] of dtype (every row written: zero where no id selects it), g_weights [M,bag] fp32; each where its pointer is set.
  * The (id, position) pairs are sorted and every row's sum runs over its positions in ascending order, in pieces joined in order: no float atomics, the same
- * bits every run.  ws: nl_embedding_workspace bytes (0 without g_table). */
+ * bits every run.  M * bag up to 2^30 - 64, V below 2^31, D up to 2^20.  ws: nl_embedding_workspace bytes (0 without g_table). */
 int nl_embedding_forward(const void* table, long long V, int D, int dtype, const void* ids, int id64, const float* weights, long long M, int bag, float scale,
                          void* out, void* stream);
 int nl_embedding_backward(const void* table, long long V, int D, int dtype, const void* ids, int id64, const float* weights, long long M, int bag, float scale,

@@ -49,7 +49,7 @@ __global__ __launch_bounds__(256) void k_emb_forward(const void* __restrict__ ta
                                                      const float* __restrict__ weights, long long M, int bag, float scale, void* __restrict__ out, int lanes)
 {
     const int per = 256 / lanes, grp = threadIdx.x / lanes;
-    const long long m = (long long)blockIdx.x * per + grp;
+    const long long m = nl_block() * per + grp;
     if (m >= M) return;
     const bool ids32 = !id64 && ((uintptr_t)ids & 15) == 0 && ((uintptr_t)weights & 15) == 0;
     for (int d = (threadIdx.x & (lanes - 1)) * VEC; d < D; d += lanes * VEC) {
@@ -104,7 +104,7 @@ __global__ __launch_bounds__(256) void k_emb_gweights(const void* __restrict__ t
                                                       int bag, float scale, const void* __restrict__ g, float* __restrict__ gw, int lanes)
 {
     const int per = 256 / lanes, grp = threadIdx.x / lanes;
-    const long long i = (long long)blockIdx.x * per + grp;
+    const long long i = nl_block() * per + grp;
     if (i >= L) return;
     const long long id = emb_id(ids, id64, i);
     float s = 0.0f;
@@ -439,7 +439,7 @@ __global__ __launch_bounds__(256) void k_emb_zero(unsigned* p, long long words)
 __global__ void k_emb_zero_tail(unsigned short* p) { *p = 0; }
 
 // ---- host ----
-#define EMB_MAX_LOOKUPS 0x7FFF0000LL
+#define EMB_MAX_LOOKUPS ((1LL << 30) - EMB_CHUNK_MANY)      // below 2^24 chunks: a launch with a workgroup for each has fewer than 2^32 threads
 struct EmbPlan { int L, nblk, passes, chunk, levels; long long keys, hist, key_l[2], any_l[2], piece_l[2], total; };      // levels: launches of k_emb_join
 static EmbPlan emb_plan(long long V, int D, long long L)
 {
@@ -517,7 +517,7 @@ int nl_embedding_forward(const void* table, long long V, int D, int dtype, const
     if (!out || ((uintptr_t)out & (nl_dtype_size(dtype) - 1)) || ((uintptr_t)weights & 3)) return NL_ERR_INVALID_ARG;
     hipStream_t st = (hipStream_t)stream;
     const int vec = emb_vec(D, dtype, table, out), lanes = emb_lanes(D, vec, 256), per = 256 / lanes;
-    const dim3 grid((unsigned)((M + per - 1) / per));
+    const dim3 grid = nl_blocks((M + per - 1) / per);
     if (vec == 8) emb_forward<8>(grid, st, table, V, D, dtype, ids, id64, weights, M, bag, scale, out, lanes);
     else if (vec == 4) emb_forward<4>(grid, st, table, V, D, dtype, ids, id64, weights, M, bag, scale, out, lanes);
     else emb_forward<1>(grid, st, table, V, D, dtype, ids, id64, weights, M, bag, scale, out, lanes);
@@ -536,7 +536,7 @@ int nl_embedding_backward(const void* table, long long V, int D, int dtype, cons
     const long long L = M * bag;
     if (g_weights && M > 0) {
         const int vec = emb_vec(D, dtype, table, g_out), lanes = emb_lanes(D, vec, 64), per = 256 / lanes;
-        const dim3 grid((unsigned)((L + per - 1) / per));
+        const dim3 grid = nl_blocks((L + per - 1) / per);
         if (vec == 8) NL_WITH_DTYPE(dtype, hipLaunchKernelGGL((k_emb_gweights<DT, 8>), grid, dim3(256), 0, st, table, V, D, ids, id64, L, bag, scale, g_out, g_weights, lanes));
         else if (vec == 4) NL_WITH_DTYPE(dtype, hipLaunchKernelGGL((k_emb_gweights<DT, 4>), grid, dim3(256), 0, st, table, V, D, ids, id64, L, bag, scale, g_out, g_weights, lanes));
         else NL_WITH_DTYPE(dtype, hipLaunchKernelGGL((k_emb_gweights<DT, 1>), grid, dim3(256), 0, st, table, V, D, ids, id64, L, bag, scale, g_out, g_weights, lanes));

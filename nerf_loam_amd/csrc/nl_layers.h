@@ -264,6 +264,9 @@ template <int DT> __device__ __forceinline__ void nl_epilogue8_fetch(const NlEpi
     }
     nl_epilogue8<DT, false>(ep, v, b, r, m, n, M, N, split_off);
 }
+// Workgroups in one row as long as a launch takes it (a grid's axis has at most 2^32 - 1 threads), else in several; the number of a workgroup
+__device__ __forceinline__ long long nl_block() { return (long long)blockIdx.y * gridDim.x + blockIdx.x; }
+inline dim3 nl_blocks(long long n) { const long long row = 1 << 22; return n <= row ? dim3((unsigned)n) : dim3((unsigned)row, (unsigned)((n + row - 1) / row)); }
 // a kernel launch (or any statement) with the type as a compile-time constant DT
 #define NL_WITH_DTYPE(dt, ...)                                                            \
     do {                                                                                  \

@@ -47,7 +47,7 @@ __global__ __launch_bounds__(256) void k_linear_rows(NlRows g, NlEpilogue ep)
 {
     constexpr int R = 2, U = MR == 1 ? 4 : MR <= 4 ? 2 : 1;
     const int lanes = g.lanes, lane = threadIdx.x & (lanes - 1), K = g.K;
-    const long long n0 = ((long long)blockIdx.x * (256 / lanes) + threadIdx.x / lanes) * R;
+    const long long n0 = (nl_block() * (256 / lanes) + threadIdx.x / lanes) * R;
     if (n0 >= g.nmany) return;                                        // (a whole group)
     const long long n1 = n0 + 1 < g.nmany ? n0 + 1 : n0;
     const bool vec = nl_rows_aligned<DT>(g.many, g.ldm) && nl_rows_aligned<DT>(g.few, g.ldf) && (K & 7) == 0;
@@ -112,8 +112,7 @@ template <int DT, bool SWAP> static int nl_launch_rows(const NlLinear* d, const 
     NlRows g = SWAP ? NlRows{d->w, d->x, d->ldw, d->ldx, d->M, d->N, d->K, 8} : NlRows{d->x, d->w, d->ldx, d->ldw, d->N, (int)d->M, d->K, 8};
     while (g.lanes < 64 && g.lanes * 8 < d->K) g.lanes *= 2;
     const long long blocks = (g.nmany + 2 * (256 / g.lanes) - 1) / (2 * (256 / g.lanes));
-    if (blocks > 0x7FFFFFFF) return NL_ERR_INVALID_ARG;
-    const dim3 grid((unsigned)blocks);
+    const dim3 grid = nl_blocks(blocks);
     if (g.nfew == 1) hipLaunchKernelGGL((k_linear_rows<DT, 1, SWAP>), grid, dim3(256), 0, st, g, ep);
     else if (g.nfew == 2) hipLaunchKernelGGL((k_linear_rows<DT, 2, SWAP>), grid, dim3(256), 0, st, g, ep);
     else if (g.nfew <= 4) hipLaunchKernelGGL((k_linear_rows<DT, 4, SWAP>), grid, dim3(256), 0, st, g, ep);
@@ -265,7 +264,7 @@ __global__ __launch_bounds__(256) void k_linear_zero(unsigned char* p, long long
 // host: plans and launches.  Every function below runs twice: first without a workspace, to say how much it takes, then with it, to launch.
 // ---------------------------------------------------------------------------------------------
 #define NL_LINEAR_MAX_WIDTH (1 << 22)
-#define NL_LINEAR_MAX_ROWS (1LL << 36)
+#define NL_LINEAR_MAX_ROWS (1LL << 30)
 
 struct NlWork {
     char* base; long long used; hipStream_t st; bool dry; int rc;
@@ -345,7 +344,8 @@ static void nl_product(NlWork& w, const NlPacked& A, const NlPacked& B, int layo
     g.A8 = A8; g.A8e = A8e; g.ld8 = nl_up(K, NL_MX_BLOCK);
     g.M = M; g.N = N; g.K = K; g.kchunk = c.kchunk;
     const long long tm = nl_up(M, size[c.tile]) / size[c.tile], tn = nl_up(N, size[c.tile]) / size[c.tile];
-    if (tm * tn > 0x7FFFFFF) { w.rc = NL_ERR_INVALID_ARG; return; }
+    if (tm * tn * (c.tile == 0 ? 512 : 256) > 0xFFFFFFFFLL) {      // (a grid's axis)
+        w.rc = NL_ERR_INVALID_ARG; return; }
     g.tiles_m = (int)tm; g.tiles_n = (int)tn;
     g.ep = ep;
     if (c.splits > 1) { g.ep = NlEpilogue{}; g.ep.part = (float*)w.take(4LL * c.splits * M * N); }

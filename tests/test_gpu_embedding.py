@@ -236,3 +236,36 @@ def test_tables_beyond_32_bits():
     want = torch.zeros(V - 671089, D, dtype=torch.float64, device="cuda").index_add_(0, ids.view(-1) - 671089, g.double())
     assert bool(((gt[671089:].double() - want).abs() <= 64 * 2.0 ** -24 * 50 * 5 + 2.0 ** -8 * want.abs()).all())       # at most 50 lookups a row, |g| < 5
     assert not bool(gt[:671089].any())
+
+
+def test_more_groups_of_threads_than_a_grid_axis_has_threads():
+    """2^30 - 64 lookups, the most there may be: forward with four threads a row (2^32 in all) and backward, whose sums are exact whole numbers"""
+    V, M = 1 << 24, (1 << 30) - 64
+    if torch.cuda.mem_get_info()[0] < 80e9:
+        pytest.skip("needs 80 GB of free memory")
+    ids = (torch.arange(M, dtype=torch.int32, device="cuda") & (V - 1)).view(M, 1)
+    table = (torch.arange(3 * 4096, device="cuda") % 251).to(torch.bfloat16).view(4096, 3)
+    small = ids & 4095
+    y = ops.embedding_forward(table, small)
+    for i in (0, (1 << 22) * 64 - 1, (1 << 22) * 64, (1 << 29) + 5, M - 1):
+        assert torch.equal(y[i], table[i & 4095]), i
+    assert torch.equal(y[-4096:], table[small[-4096:, 0].long()])
+    del y, small
+    g = torch.ones(M, 1, dtype=torch.float32, device="cuda")
+    gt = torch.empty(V, 1, dtype=torch.float32, device="cuda")
+    ops.embedding_backward(torch.empty(V, 1, dtype=torch.float32, device="cuda"), ids, g, g_table=gt)
+    want = torch.full((V, 1), 64.0, device="cuda")
+    want[-64:] = 63.0
+    assert torch.equal(gt, want)
+
+
+def test_products_of_a_row_with_more_rows_than_a_grid_axis_has_threads():
+    M = 1 << 30
+    if torch.cuda.mem_get_info()[0] < 40e9:
+        pytest.skip("needs 40 GB of free memory")
+    x = torch.ones(M, 1, dtype=torch.bfloat16, device="cuda")
+    at = [0, (1 << 22) * 64 - 1, (1 << 22) * 64, (1 << 29) + 7, M - 1]
+    x[at] = 3.0
+    w = torch.full((1, 1), 0.5, dtype=torch.bfloat16, device="cuda")
+    y = ops.linear_forward(x, w)
+    assert bool((y[at] == 1.5).all()) and int((y == 0.5).sum()) == M - len(at)

@@ -127,3 +127,22 @@ def test_decoders_of_any_size_refuse_the_cpu_and_unknown_shapes():
         Decoder(depth=2, skips=[1])
     with pytest.raises(NotImplementedError):
         Decoder(embedder="gaussian")
+
+
+def test_sizes_beyond_a_launch_are_refused():
+    """what would need more than 2^32 threads along a grid's axis is refused where its workspace is asked for, not where it is launched"""
+    lib = L.lib()
+    for sizes in [dict(M=(1 << 30) + 1), dict(M=1 << 30, N=2048), dict(K=(1 << 22) + 1, ldx=1 << 23, ldw=1 << 23)]:
+        d = _desc(**sizes)
+        d.ldy = d.ldgy = d.ldr = max(d.N, d.ldy)
+        assert lib.nl_linear_workspace(ctypes.byref(d), 0) == -1 and lib.nl_linear_forward(ctypes.byref(d), None) == 1, sizes
+    assert lib.nl_embedding_workspace(10, 4, (1 << 30) - 63, 1) == -1 and lib.nl_embedding_workspace(10, 4, (1 << 30) - 64, 1) > 0
+
+
+@pytest.mark.parametrize("bad", [dict(x8=4096), dict(x8e=4096), dict(x8=4104, x8e=4096)])
+def test_linear_forward_refuses_half_a_checkpoint(bad):
+    lib = L.lib()
+    assert lib.nl_linear_workspace(ctypes.byref(_desc(x8=4096, x8e=4096)), 0) >= 0
+    d = _desc(**bad)
+    assert lib.nl_linear_workspace(ctypes.byref(d), 0) == -1
+    assert lib.nl_linear_forward(ctypes.byref(d), None) == 1
