@@ -269,3 +269,34 @@ def test_products_of_a_row_with_more_rows_than_a_grid_axis_has_threads():
     w = torch.full((1, 1), 0.5, dtype=torch.bfloat16, device="cuda")
     y = ops.linear_forward(x, w)
     assert bool((y[at] == 1.5).all()) and int((y == 0.5).sum()) == M - len(at)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [4, 8, 12, 16, 20, 24, 72, 1000, 2056])
+def test_bags_of_eight(dtype, D):
+    """32-bit ids and weights, aligned or not, few and odd numbers of rows, threads of a group without columns; weights of ids without a row may be anything"""
+    for M in (1, 3, 257):
+        table, ids, w, g = _case(97, D, M, 8, dtype, 1000 * M + D)
+        ids[0, 3], ids[0, 4], ids[-1, 7] = -1, 97, 2 ** 31 - 1
+        for shift in (0, 1):
+            flat = torch.empty(8 * M + shift, dtype=torch.int32, device="cuda")[shift:].view(M, 8).copy_(ids)
+            wflat = torch.empty(8 * M + shift, device="cuda")[shift:].view(M, 8).copy_(w)
+            _check(table, flat, wflat, g, 0.5, *_grads(table, flat, wflat, g, 0.5), f"D {D} M {M} shift {shift}")
+        y = ops.embedding_forward(table, ids, w, 0.5)
+        w[(ids < 0) | (ids >= 97)] = float("nan")
+        assert torch.equal(ops.embedding_forward(table, ids, w, 0.5), y)
+
+
+def test_bags_of_eight_over_tables_around_two_gigabytes():
+    for V in (67108863, 67108864, 70000001):                                 # 16 bf16: 2^31 - 32 bytes (as far as 32-bit offsets go), 2^31, more
+        table = torch.zeros(V, 16, dtype=torch.bfloat16, device="cuda")
+        rows = [0, 1, V // 2, V - 2, V - 1]
+        table[rows] = (torch.arange(5 * 16, device="cuda").view(5, 16) + 1.0).to(torch.bfloat16)
+        ids = torch.tensor([[0, 1, V // 2, V - 2, V - 1, -1, V, 2 ** 31 - 1]], dtype=torch.int32, device="cuda").expand(5, 8).contiguous()
+        for k in range(5):
+            w = torch.zeros(5, 8, device="cuda")
+            w[:, k] = 1.0
+            assert torch.equal(ops.embedding_forward(table, ids, w), table[rows[k]].expand(5, 16)), (V, k)
+        w = torch.zeros(5, 8, device="cuda")
+        w[:, 5:] = 1.0
+        assert not bool(ops.embedding_forward(table, ids, w).any())
