@@ -122,7 +122,7 @@ template <int BM, int BN> __device__ __forceinline__ unsigned gemm_tile_of(const
 template <int DT, int WR, int WC, int WAVES, int LDS>
 __device__ __forceinline__ void gemm_results(const NlGemm& g, nl_f32x4 (&acc)[WR / 16][WC / 16], char* s_mem, long long m, int n, unsigned piece)
 {
-    constexpr int RP = WR < 64 ? WR : (DT == NL_DT_F32 && WR == 64 ? 32 : 64), CX = WC / 4 - 1;
+    constexpr int RP = WR < 64 ? WR : (WAVES * 64 * WC * 4 > LDS ? 32 : 64), CX = WC / 4 - 1;
     static_assert((CX & (CX + 1)) == 0 && RP * WC * 4 * WAVES <= LDS, "the exchange fits into the operand buffers");
     constexpr int TURNS = RP * WC / 512, BATCH = TURNS < 4 ? TURNS : 4;
     static_assert(64 % (WC / 8) == 0 && TURNS % BATCH == 0, "a lane keeps its columns");
@@ -290,9 +290,14 @@ __device__ __forceinline__ void gemm_encode(const NlGemm& g, const char* lds, lo
     }
 }
 
-// RING: LDS buffers per operand.  2: the next step arrives while one multiplies.  4 (squares of 64 while they leave compute units idle anyway): three steps are on their way;
+// RING: LDS buffers.  2: the next step arrives while one multiplies.  4 (squares of 64 while they leave compute units idle anyway): three steps are on their way;
 // a step of such a tile multiplies for 130 cycles and waits for memory the rest of the time.  One barrier per step, in front of it every wave waits for its own loads of
 // the step (the RING - 2 later ones stay in flight) and for its fragment reads of the step before, whose buffer the loads behind the barrier overwrite.
+//
+// The compiler lets a transposing read wait for every load into LDS that may write the same array.  Where a step has such reads behind the next step's loads, the buffers
+// therefore are arrays of their own and the steps are written out one per buffer (APART); otherwise each step waits in its middle for loads that it does not need
+// (4096 x 4096 x 16384, both operands transposed: 456 us, APART 416; 8192^3: 898, 820).  With only B transposed its reads simply come first (8192^3: 878, now 805).
+// Bound: 256 x 256 x 64 steps take 1.47 us, 1460 TFLOP/s, at the clock that the power limit leaves (the library's best here: 1475); a tile's beginning and end add 11 us.
 template <class T, bool A_SLOW, bool B_SLOW, bool B_MX8, int BM, int BN, int WM, int WN, int RING, bool ENC = false>
 __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
 {
@@ -301,9 +306,12 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
     typedef GemmSide<A_SLOW, BM, NT> SA;
     typedef GemmSide<B_SLOW, BN, NT> SB;
     static_assert(RING == 2 || (RING == 4 && !B_MX8 && !ENC), "buffers are taken in turn by the low bits of the step");
-    __shared__ __align__(256) char s_mem[RING * (SA::BYTES + SB::BYTES)];
-    char* const s_a = s_mem;
-    char* const s_b = s_mem + RING * SA::BYTES;
+    constexpr bool APART = A_SLOW || (B_SLOW && RING == 4), B_FIRST = B_SLOW && !APART;
+    constexpr int BUF = SA::BYTES + SB::BYTES, LDS = APART ? BUF : RING * BUF;
+    __shared__ __align__(256) char s_mem[LDS];
+    __shared__ __align__(256) char s_1[BUF];                          // (APART; the last two with RING 4)
+    __shared__ __align__(256) char s_2[BUF];
+    __shared__ __align__(256) char s_3[BUF];
     long long m0; int n0;
     const unsigned piece = gemm_tile_of<BM, BN>(g, m0, n0);
     const long long k0 = (long long)piece * g.kchunk, k1 = min(k0 + g.kchunk, g.K);
@@ -318,29 +326,32 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
     // the tiles of a row of tiles take turns at writing A's codes: tile column c the steps c, c + tiles_n, .. of the contraction
     int mine = 0;
     if (ENC) { const int past = (int)((k0 / GEMM_BK) % g.tiles_n); mine = n0 / BN - past; if (mine < 0) mine += g.tiles_n; }
-    auto fetch = [&](int s) {
+    auto fetch = [&](int s, char* to) {
         const long long left = k1 - k0 - (long long)s * GEMM_BK;
-        a.load(s_a + (s & (RING - 1)) * SA::BYTES, s * a.step, left);
+        a.load(to, s * a.step, left);
         if (B_MX8) b8.fetch(s, left);
-        else b.load(s_b + (s & (RING - 1)) * SB::BYTES, s * b.step, left);
+        else b.load(to + SA::BYTES, s * b.step, left);
     };
-#pragma unroll
-    for (int s = 0; s < RING - 1; s++) fetch(s);                      // (behind the last step nothing is inside: zeros)
-    if (B_MX8) b8.put(s_b);
-    for (int s = 0; s < steps; s++) {
+    auto step = [&](int s, char* buf, char* next) {
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((RING - 2) * (SA::LOADS + SB::LOADS)) : "memory");
-        const char* la = s_a + (s & (RING - 1)) * SA::BYTES;
-        const char* lb = s_b + (s & (RING - 1)) * SB::BYTES;
-        // fragments of both halves of the step, the loads of the next step between them: behind all fragment reads they come late (8192^3 / 16384 x 4096 x 4096,
+        const char* la = buf;
+        const char* lb = buf + SA::BYTES;
+        // fragments of both halves of the step, the loads of a later step between them: behind all fragment reads they come late (8192^3 / 16384 x 4096 x 4096,
         // layout 1 and 2: -10 %), in front of them they hold up the reads that the first matrix instructions wait for
         nl_s16x8 fa[2][FM], fb[2][FN];
 #pragma unroll
         for (int j = 0; j < FN; j++) fb[0][j] = SB::frag(lb, wn + 16 * j, 0);
 #pragma unroll
         for (int i = 0; i < FM; i++) fa[0][i] = SA::frag(la, wm + 16 * i, 0);
-        if (RING > 2 || s + 1 < steps) fetch(s + RING - 1);
+        if (B_FIRST) {
 #pragma unroll
-        for (int j = 0; j < FN; j++) fb[1][j] = SB::frag(lb, wn + 16 * j, 1);
+            for (int j = 0; j < FN; j++) fb[1][j] = SB::frag(lb, wn + 16 * j, 1);
+        }
+        if (RING > 2 || s + 1 < steps) fetch(s + RING - 1, next);
+        if (!B_FIRST) {
+#pragma unroll
+            for (int j = 0; j < FN; j++) fb[1][j] = SB::frag(lb, wn + 16 * j, 1);
+        }
 #pragma unroll
         for (int i = 0; i < FM; i++) fa[1][i] = SA::frag(la, wm + 16 * i, 1);
 #pragma unroll
@@ -355,10 +366,29 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
             gemm_encode<T, BM, NT>(g, la, m0, k0 + (long long)s * GEMM_BK);
             mine += g.tiles_n;
         }
-        if (B_MX8 && s + 1 < steps) b8.put(s_b + ((s + 1) & 1) * SB::BYTES);
+        if (B_MX8 && s + 1 < steps) b8.put(next + SA::BYTES);
+    };
+    // (behind the last step nothing is inside: zeros)
+    fetch(0, s_mem);
+    if constexpr (RING == 4) { fetch(1, APART ? s_1 : s_mem + BUF); fetch(2, APART ? s_2 : s_mem + 2 * BUF); }
+    if (B_MX8) b8.put(s_mem + SA::BYTES);
+    if constexpr (!APART) {
+        for (int s = 0; s < steps; s++) step(s, s_mem + (s & (RING - 1)) * BUF, s_mem + ((s + RING - 1) & (RING - 1)) * BUF);
+    } else if constexpr (RING == 2) {
+        for (int s = 0; s < steps; s += 2) {
+            step(s, s_mem, s_1);
+            if (s + 1 < steps) step(s + 1, s_1, s_mem);
+        }
+    } else {
+        for (int s = 0; s < steps; s += 4) {
+            step(s, s_mem, s_3);
+            if (s + 1 < steps) step(s + 1, s_1, s_mem);
+            if (s + 2 < steps) step(s + 2, s_2, s_1);
+            if (s + 3 < steps) step(s + 3, s_3, s_2);
+        }
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");        // (all loads, the ones of zeros too: the results pass through the same memory)
-    gemm_results<DT, BM / WM, BN / WN, WM * WN, RING * (SA::BYTES + SB::BYTES)>(g, acc, s_mem, m0 + wm, n0 + wn, piece);
+    gemm_results<DT, BM / WM, BN / WN, WM * WN, LDS>(g, acc, s_mem, m0 + wm, n0 + wn, piece);
 }
 
 // ---------------------------------------------------------------------------------------------
