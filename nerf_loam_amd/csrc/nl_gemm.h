@@ -306,7 +306,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
     typedef GemmSide<A_SLOW, BM, NT> SA;
     typedef GemmSide<B_SLOW, BN, NT> SB;
     static_assert(RING == 2 || (RING == 4 && !B_MX8 && !ENC), "buffers are taken in turn by the low bits of the step");
-    constexpr bool APART = A_SLOW || (B_SLOW && RING == 4), B_FIRST = B_SLOW && !APART;
+    constexpr bool APART = A_SLOW || (B_SLOW && RING == 4), B_FIRST = B_SLOW && !APART, MIX = FM * FN == 32 && !B_FIRST;      // (MIX: 32768 x 2048 x 2048 225 -> 220 us)
     constexpr int BUF = SA::BYTES + SB::BYTES, LDS = APART ? BUF : RING * BUF;
     __shared__ __align__(256) char s_mem[LDS];
     __shared__ __align__(256) char s_1[BUF];                          // (APART; the last two with RING 4)
@@ -348,6 +348,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
             for (int j = 0; j < FN; j++) fb[1][j] = SB::frag(lb, wn + 16 * j, 1);
         }
         if (RING > 2 || s + 1 < steps) fetch(s + RING - 1, next);
+        if constexpr (MIX) __builtin_amdgcn_sched_barrier(0);
         if (!B_FIRST) {
 #pragma unroll
             for (int j = 0; j < FN; j++) fb[1][j] = SB::frag(lb, wn + 16 * j, 1);
@@ -362,6 +363,12 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
         for (int i = 0; i < FM; i++)
 #pragma unroll
             for (int j = 0; j < FN; j++) acc[i][j] = NlMma<T>::mma(fb[1][j], fa[1][i], acc[i][j]);
+        if constexpr (MIX) {                                          // the second half's reads among the first half's products, not where they are used
+#pragma unroll
+            for (int q = 0; q < FM + FN; q++) { __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); }
+            __builtin_amdgcn_sched_group_barrier(0x008, 2 * FM * FN - FM - FN, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         if (ENC && s == mine) {
             gemm_encode<T, BM, NT>(g, la, m0, k0 + (long long)s * GEMM_BK);
             mine += g.tiles_n;
