@@ -5,16 +5,17 @@
 // neighbouring entries in ascending position: pieces of a fixed number of entries, the pieces of a row that spans several joined in order, level by level.
 #include "nl_layers.h"
 
-// Sorted entries per run-summing group: 16 while there are at most EMB_FEW lookups, so that there are enough groups (32768 lookups x 1024 bf16: 22 us, 91 us with
-// 64 entries and one row in flight), else 64.  Pieces of a row that crosses such chunks are joined in blocks of EMB_BLOCK neighbours, level by level.
+// Sorted entries per run-summing group: 16 while that leaves at most EMB_THREADS threads of eight columns, so that there are enough of them (EMBNOTE), else 64.
+// Pieces of a row that crosses such chunks are joined in blocks of EMB_BLOCK neighbours, level by level.
 #define EMB_CHUNK_FEW 16
 #define EMB_CHUNK_MANY 64
-#define EMB_FEW 65536
+#define EMB_THREADS (1 << 20)
 #define EMB_BLOCK 64
 #define EMB_BATCH 8             // rows in flight together
-#define RS_TILE 1024            // keys per workgroup of a sorting pass: 4 waves x 4 rounds x 64 lanes
-#define RS_ROUNDS (RS_TILE / 256)
-#define RS_FEW_BLOCKS 64        // up to here (65536 keys) the scatter sums the histograms itself: a launch less per pass
+// A sorting pass takes 1024 keys a workgroup (4 waves x 4 rounds x 64 lanes) up to RS_FEW keys, else 4096 and puts them in order in LDS first, so that what it writes
+// lies in runs of 16 keys on average (2.1 M keys, a pass: RSNOTE).  Up to RS_FEW_BLOCKS workgroups the scatter sums the histograms itself: a launch less per pass.
+#define RS_FEW 65536
+#define RS_FEW_BLOCKS 64
 #define RS_SMALL 4096           // up to here one workgroup sorts everything in LDS: one launch instead of three per pass
 
 __device__ __forceinline__ long long emb_id(const void* ids, int id64, long long i) { return id64 ? ((const long long*)ids)[i] : (long long)((const int*)ids)[i]; }
@@ -173,7 +174,7 @@ struct RsArgs {
     unsigned* out_keys; unsigned* out_pos;
     int* hist;                                         // [nblk][256], then (k_rs_scan) its exclusive sums over the blocks
     int* totals;                                       // [256]; null: every workgroup of the scatter sums what is in front of it
-    int L, nblk, shift;
+    int L, nblk, shift;                                // nblk workgroups of 256 ROUNDS keys
     unsigned* zero; long long zero_words;              // first pass: the launch's workgroups behind the sorting ones clear these (the gradient's rows)
 };
 __device__ __forceinline__ bool rs_zero(const RsArgs& a, int sorting)
@@ -189,15 +190,16 @@ __device__ __forceinline__ unsigned rs_key(const RsArgs& a, int i)
     const long long id = emb_id(a.ids, a.id64, i);
     return id < 0 || id >= a.V ? (unsigned)a.V : (unsigned)id;
 }
+template <int ROUNDS>
 __global__ __launch_bounds__(256) void k_rs_hist(RsArgs a)
 {
     __shared__ int s_h[256];
     if (rs_zero(a, a.nblk)) return;
     s_h[threadIdx.x] = 0;
     __syncthreads();
-    const int base = blockIdx.x * RS_TILE;
+    const int base = blockIdx.x * (256 * ROUNDS);
 #pragma unroll
-    for (int r = 0; r < RS_ROUNDS; r++) {
+    for (int r = 0; r < ROUNDS; r++) {
         const int i = base + r * 256 + threadIdx.x;
         if (i < a.L) atomicAdd(&s_h[rs_key(a, i) >> a.shift & 255], 1);       // (whole numbers: the order does not matter)
     }
@@ -228,9 +230,12 @@ __global__ __launch_bounds__(256) void k_rs_scan(RsArgs a)
     }
     if (threadIdx.x == 0) a.totals[blockIdx.x] = run;
 }
+template <int ROUNDS>
 __global__ __launch_bounds__(256) void k_rs_scatter(RsArgs a)
 {
+    constexpr bool STAGE = ROUNDS > 4;
     __shared__ int s_cnt[4][256], s_base[256], s_w[4];
+    __shared__ unsigned s_key[STAGE ? 256 * ROUNDS : 1], s_pos[STAGE ? 256 * ROUNDS : 1];
     if (rs_zero(a, a.nblk)) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d0 = threadIdx.x;
     // where the digit begins: sums of the totals in front of it
@@ -251,11 +256,11 @@ __global__ __launch_bounds__(256) void k_rs_scatter(RsArgs a)
 #pragma unroll
     for (int w = 0; w < 4; w++) s_cnt[w][d0] = 0;
     __syncthreads();
-    // a wave ranks its 512 neighbouring keys, 64 at a time: lanes with the same digit find each other by eight ballots
-    unsigned key[RS_ROUNDS], rank[RS_ROUNDS];
-    const int first = blockIdx.x * RS_TILE + wave * (RS_TILE / 4);
+    // a wave ranks its neighbouring keys, 64 at a time: lanes with the same digit find each other by eight ballots
+    unsigned key[ROUNDS], rank[ROUNDS];
+    const int tile = blockIdx.x * (256 * ROUNDS), first = tile + wave * (64 * ROUNDS);
 #pragma unroll
-    for (int r = 0; r < RS_ROUNDS; r++) {
+    for (int r = 0; r < ROUNDS; r++) {
         const int i = first + r * 64 + lane;
         const bool in = i < a.L;
         key[r] = in ? rs_key(a, i) : 0;
@@ -271,17 +276,52 @@ __global__ __launch_bounds__(256) void k_rs_scatter(RsArgs a)
         __builtin_amdgcn_wave_barrier();
     }
     __syncthreads();
-    int before = s_base[d0];
+    if constexpr (STAGE) {
+        // in LDS a digit's keys begin behind those of the smaller digits of the tile; from there on they lie as they will in memory
+        int total = 0;
 #pragma unroll
-    for (int w = 0; w < 4; w++) { const int c = s_cnt[w][d0]; s_cnt[w][d0] = before; before += c; }
-    __syncthreads();
+        for (int w = 0; w < 4; w++) total += s_cnt[w][d0];
+        int s = total;
 #pragma unroll
-    for (int r = 0; r < RS_ROUNDS; r++) {
-        const int i = first + r * 64 + lane;
-        if (i >= a.L) continue;
-        const unsigned to = s_cnt[wave][key[r] >> a.shift & 255] + rank[r];
-        a.out_keys[to] = key[r];
-        a.out_pos[to] = a.ids ? (unsigned)i : a.pos[i];
+        for (int off = 1; off < 64; off <<= 1) { const int t = __shfl_up(s, off); if (lane >= off) s += t; }
+        if (lane == 63) s_w[wave] = s;
+        __syncthreads();
+        for (int w = 0; w < wave; w++) s += s_w[w];
+        int before = s - total;
+        s_base[d0] -= before;                                         // place in memory minus place in the tile
+#pragma unroll
+        for (int w = 0; w < 4; w++) { const int c = s_cnt[w][d0]; s_cnt[w][d0] = before; before += c; }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < ROUNDS; r++) {
+            const int i = first + r * 64 + lane;
+            if (i >= a.L) continue;
+            const unsigned to = s_cnt[wave][key[r] >> a.shift & 255] + rank[r];
+            s_key[to] = key[r];
+            s_pos[to] = a.ids ? (unsigned)i : a.pos[i];
+        }
+        __syncthreads();
+        const int n = a.L - tile < 256 * ROUNDS ? a.L - tile : 256 * ROUNDS;
+#pragma unroll 4
+        for (int i = threadIdx.x; i < n; i += 256) {
+            const unsigned k = s_key[i];
+            const int to = s_base[k >> a.shift & 255] + i;
+            a.out_keys[to] = k;
+            a.out_pos[to] = s_pos[i];
+        }
+    } else {
+        int before = s_base[d0];
+#pragma unroll
+        for (int w = 0; w < 4; w++) { const int c = s_cnt[w][d0]; s_cnt[w][d0] = before; before += c; }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < ROUNDS; r++) {
+            const int i = first + r * 64 + lane;
+            if (i >= a.L) continue;
+            const unsigned to = s_cnt[wave][key[r] >> a.shift & 255] + rank[r];
+            a.out_keys[to] = key[r];
+            a.out_pos[to] = a.ids ? (unsigned)i : a.pos[i];
+        }
     }
 }
 
@@ -487,18 +527,19 @@ __global__ void k_emb_zero_tail(unsigned short* p) { *p = 0; }
 
 // ---- host ----
 #define EMB_MAX_LOOKUPS ((1LL << 30) - EMB_CHUNK_MANY)      // below 2^24 chunks: a launch with a workgroup for each has fewer than 2^32 threads
-struct EmbPlan { int L, nblk, passes, chunk, levels; long long keys, hist, key_l[2], any_l[2], piece_l[2], total; };      // levels: launches of k_emb_join
+struct EmbPlan { int L, nblk, rounds, passes, chunk, levels; long long keys, hist, key_l[2], any_l[2], piece_l[2], total; };      // levels: launches of k_emb_join
 static EmbPlan emb_plan(long long V, int D, long long L)
 {
     EmbPlan p = {};
     p.L = (int)L;
-    p.nblk = (int)((L + RS_TILE - 1) / RS_TILE);
+    p.rounds = L <= RS_FEW ? 4 : 16;
+    p.nblk = (int)((L + 256 * p.rounds - 1) / (256 * p.rounds));
     p.passes = 1;
     while (p.passes < 4 && (V >> (8 * p.passes)) != 0) p.passes++;
     p.keys = nl_up(4 * L, 256);
     p.hist = nl_up(4LL * 256 * p.nblk + 1024, 256);
     p.total = 4 * p.keys + p.hist;
-    p.chunk = L <= EMB_FEW ? EMB_CHUNK_FEW : EMB_CHUNK_MANY;
+    p.chunk = L / EMB_CHUNK_FEW * ((D + 7) / 8) <= EMB_THREADS ? EMB_CHUNK_FEW : EMB_CHUNK_MANY;
     for (long long n = (L + p.chunk - 1) / p.chunk; n > 1; n = (n + EMB_BLOCK - 1) / EMB_BLOCK) {        // levels take two buffers in turn
         if (p.levels < 2) {
             const int i = p.levels;
@@ -620,9 +661,11 @@ int nl_embedding_backward(const void* table, long long V, int D, int dtype, cons
                 const long long nth = k == 2 ? launches - 1 : k, z0 = nth * part < words ? nth * part : words, z1 = k == 2 ? words : z0 + part < words ? z0 + part : words;
                 r.zero = (unsigned*)g_table + z0; r.zero_words = i == 0 ? z1 - z0 : 0;
                 const dim3 grid((k == 1 ? 256 : p.nblk) + emb_zero_blocks(r.zero_words, 256));
-                if (k == 0) hipLaunchKernelGGL(k_rs_hist, grid, dim3(256), 0, st, r);
-                else if (k == 1) hipLaunchKernelGGL(k_rs_scan, grid, dim3(256), 0, st, r);
-                else hipLaunchKernelGGL(k_rs_scatter, grid, dim3(256), 0, st, r);
+                if (k == 1) hipLaunchKernelGGL(k_rs_scan, grid, dim3(256), 0, st, r);
+                else if (k == 0 && p.rounds == 4) hipLaunchKernelGGL(k_rs_hist<4>, grid, dim3(256), 0, st, r);
+                else if (k == 0) hipLaunchKernelGGL(k_rs_hist<16>, grid, dim3(256), 0, st, r);
+                else if (p.rounds == 4) hipLaunchKernelGGL(k_rs_scatter<4>, grid, dim3(256), 0, st, r);
+                else hipLaunchKernelGGL(k_rs_scatter<16>, grid, dim3(256), 0, st, r);
             }
         }
     EmbPieces buf[2] = {};
