@@ -5,7 +5,8 @@
 // neighbouring entries in ascending position: pieces of a fixed number of entries, the pieces of a row that spans several joined in order, level by level.
 #include "nl_layers.h"
 
-// Sorted entries per run-summing group: 16 while that leaves at most EMB_THREADS threads of eight columns, so that there are enough of them (EMBNOTE), else 64.
+// Sorted entries per run-summing group: 16 while that leaves at most EMB_THREADS threads of eight columns, so that there are enough of them (32768 lookups x 1024 bf16:
+// 21 us, 91 us with 64 entries and one row in flight; 2.1 M x 16 bf16: 69, 74), else 64.
 // Pieces of a row that crosses such chunks are joined in blocks of EMB_BLOCK neighbours, level by level.
 #define EMB_CHUNK_FEW 16
 #define EMB_CHUNK_MANY 64
@@ -13,7 +14,9 @@
 #define EMB_BLOCK 64
 #define EMB_BATCH 8             // rows in flight together
 // A sorting pass takes 1024 keys a workgroup (4 waves x 4 rounds x 64 lanes) up to RS_FEW keys, else 4096 and puts them in order in LDS first, so that what it writes
-// lies in runs of 16 keys on average (2.1 M keys, a pass: RSNOTE).  Up to RS_FEW_BLOCKS workgroups the scatter sums the histograms itself: a launch less per pass.
+// lies in runs of 16 keys on average (2.1 M keys, a pass: 18 us and 5 for the scan, 40 and 14 in workgroups of 1024).  There the weights of bags move along: 7 us a
+// pass, and the sums fetch a line of 128 bytes less per lookup (2.1 M x 16 bf16: 43 us instead of 69).  Up to RS_FEW_BLOCKS workgroups the scatter sums the histograms
+// itself: a launch less per pass.
 #define RS_FEW 65536
 #define RS_FEW_BLOCKS 64
 #define RS_SMALL 4096           // up to here one workgroup sorts everything in LDS: one launch instead of three per pass
@@ -172,6 +175,7 @@ struct RsArgs {
     const void* ids; int id64; long long V;            // first pass
     const unsigned* keys; const unsigned* pos;         // later passes
     unsigned* out_keys; unsigned* out_pos;
+    const float* w; float* out_w;                      // weights that go along (staged passes; null: none)
     int* hist;                                         // [nblk][256], then (k_rs_scan) its exclusive sums over the blocks
     int* totals;                                       // [256]; null: every workgroup of the scatter sums what is in front of it
     int L, nblk, shift;                                // nblk workgroups of 256 ROUNDS keys
@@ -236,6 +240,7 @@ __global__ __launch_bounds__(256) void k_rs_scatter(RsArgs a)
     constexpr bool STAGE = ROUNDS > 4;
     __shared__ int s_cnt[4][256], s_base[256], s_w[4];
     __shared__ unsigned s_key[STAGE ? 256 * ROUNDS : 1], s_pos[STAGE ? 256 * ROUNDS : 1];
+    __shared__ float s_wt[STAGE ? 256 * ROUNDS : 1];
     if (rs_zero(a, a.nblk)) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d0 = threadIdx.x;
     // where the digit begins: sums of the totals in front of it
@@ -299,6 +304,7 @@ __global__ __launch_bounds__(256) void k_rs_scatter(RsArgs a)
             const unsigned to = s_cnt[wave][key[r] >> a.shift & 255] + rank[r];
             s_key[to] = key[r];
             s_pos[to] = a.ids ? (unsigned)i : a.pos[i];
+            if (a.w) s_wt[to] = a.w[i];
         }
         __syncthreads();
         const int n = a.L - tile < 256 * ROUNDS ? a.L - tile : 256 * ROUNDS;
@@ -308,6 +314,7 @@ __global__ __launch_bounds__(256) void k_rs_scatter(RsArgs a)
             const int to = s_base[k >> a.shift & 255] + i;
             a.out_keys[to] = k;
             a.out_pos[to] = s_pos[i];
+            if (a.w) a.out_w[to] = s_wt[i];
         }
     } else {
         int before = s_base[d0];
@@ -401,7 +408,7 @@ __global__ __launch_bounds__(1024) void k_rs_small(RsArgs a, int passes)
 // What bounds both is the way position -> row: EMB_BATCH rows are fetched together.
 struct EmbPieces { unsigned* keys; unsigned char* any; float* piece; };        // [n][2] keys (first, last), [n][2] flags, [n][2][D] fp32
 struct EmbSum {
-    const unsigned* keys; const unsigned* pos; const void* g; const float* weights;
+    const unsigned* keys; const unsigned* pos; const void* g; const float* weights; bool sorted;      // sorted: the weights lie as the keys do
     EmbPieces out; void* g_table; long long V;
     int L, D, bag, chunk; float scale;
 };
@@ -427,12 +434,14 @@ __global__ __launch_bounds__(256) void k_emb_sum(EmbSum a, int lanes)
         if (col) emb_store<VEC, NL_DT_F32>(a.out.piece, (2LL * chunk + (in_first ? 0 : 1)) * a.D + d, acc);
     };
     unsigned nkey[EMB_BATCH], npos[EMB_BATCH];
+    int at[EMB_BATCH];
     auto look = [&](int j0) {                                         // keys and positions of the next batch; behind the chunk's end its last entry again
 #pragma unroll
         for (int b = 0; b < EMB_BATCH; b++) {
             const int j = j0 + b < e ? j0 + b : e - 1;
             nkey[b] = a.keys[j];
             npos[b] = a.pos[j];
+            at[b] = j;
         }
     };
     look(s);
@@ -444,7 +453,7 @@ __global__ __launch_bounds__(256) void k_emb_sum(EmbSum a, int lanes)
         for (int b = 0; b < EMB_BATCH; b++) {
             // every row is fetched, also where it does not count (a load under a condition is waited for where the branch ends)
             key[b] = nkey[b];
-            w[b] = a.weights ? a.scale * a.weights[npos[b]] : a.scale;
+            w[b] = a.weights ? a.scale * a.weights[a.sorted ? (unsigned)at[b] : npos[b]] : a.scale;
             r[b] = emb_load<VEC, DT>(a.g, (long long)(npos[b] / (unsigned)a.bag) * a.D + (col ? d : 0));
         }
         if (j0 + EMB_BATCH < e) look(j0 + EMB_BATCH);
@@ -527,8 +536,8 @@ __global__ void k_emb_zero_tail(unsigned short* p) { *p = 0; }
 
 // ---- host ----
 #define EMB_MAX_LOOKUPS ((1LL << 30) - EMB_CHUNK_MANY)      // below 2^24 chunks: a launch with a workgroup for each has fewer than 2^32 threads
-struct EmbPlan { int L, nblk, rounds, passes, chunk, levels; long long keys, hist, key_l[2], any_l[2], piece_l[2], total; };      // levels: launches of k_emb_join
-static EmbPlan emb_plan(long long V, int D, long long L)
+struct EmbPlan { bool carry; int L, nblk, rounds, passes, chunk, levels; long long keys, hist, key_l[2], any_l[2], piece_l[2], total; };      // levels: launches of k_emb_join
+static EmbPlan emb_plan(long long V, int D, long long L, int bag)
 {
     EmbPlan p = {};
     p.L = (int)L;
@@ -538,7 +547,8 @@ static EmbPlan emb_plan(long long V, int D, long long L)
     while (p.passes < 4 && (V >> (8 * p.passes)) != 0) p.passes++;
     p.keys = nl_up(4 * L, 256);
     p.hist = nl_up(4LL * 256 * p.nblk + 1024, 256);
-    p.total = 4 * p.keys + p.hist;
+    p.carry = bag > 1 && p.rounds > 4;                                // (a weight fetched by position moves a line of 128 bytes)
+    p.total = (p.carry ? 6 : 4) * p.keys + p.hist;
     p.chunk = L / EMB_CHUNK_FEW * ((D + 7) / 8) <= EMB_THREADS ? EMB_CHUNK_FEW : EMB_CHUNK_MANY;
     for (long long n = (L + p.chunk - 1) / p.chunk; n > 1; n = (n + EMB_BLOCK - 1) / EMB_BLOCK) {        // levels take two buffers in turn
         if (p.levels < 2) {
@@ -594,7 +604,7 @@ extern "C" {
 long long nl_embedding_workspace(long long V, int D, long long M, int bag)
 {
     if (V < 1 || V > 0x7FFFFFFF || D < 1 || D > (1 << 20) || M < 0 || bag < 1 || M > EMB_MAX_LOOKUPS / bag) return -1;
-    return M == 0 ? 0 : emb_plan(V, D, M * bag).total;
+    return M == 0 ? 0 : emb_plan(V, D, M * bag, bag).total;
 }
 
 int nl_embedding_forward(const void* table, long long V, int D, int dtype, const void* ids, int id64, const float* weights, long long M, int bag, float scale,
@@ -637,12 +647,15 @@ int nl_embedding_backward(const void* table, long long V, int D, int dtype, cons
         NL_LAUNCH_CHECK();
         return NL_OK;
     }
-    const EmbPlan p = emb_plan(V, D, L);
+    const EmbPlan p = emb_plan(V, D, L, bag);
     if (!ws || ws_bytes < p.total || ((uintptr_t)ws & 255)) return NL_ERR_INVALID_ARG;
     char* w = (char*)ws;
     unsigned* keys[2] = {(unsigned*)w, (unsigned*)(w + p.keys)};
     unsigned* pos[2] = {(unsigned*)(w + 2 * p.keys), (unsigned*)(w + 3 * p.keys)};
     w += 4 * p.keys;
+    float* const moved[2] = {(float*)w, (float*)(w + p.keys)};
+    const bool carry = p.carry && weights;
+    if (p.carry) w += 2 * p.keys;
     RsArgs r = {};
     r.totals = p.nblk <= RS_FEW_BLOCKS ? nullptr : (int*)w; r.hist = (int*)(w + 1024); r.L = p.L; r.nblk = p.nblk; r.V = V;
     w += p.hist;
@@ -656,6 +669,7 @@ int nl_embedding_backward(const void* table, long long V, int D, int dtype, cons
         for (int i = 0; i < p.passes; i++) {
             r.ids = i == 0 ? ids : nullptr; r.id64 = id64; r.shift = 8 * i;
             r.keys = keys[(i + 1) & 1]; r.pos = pos[(i + 1) & 1]; r.out_keys = keys[i & 1]; r.out_pos = pos[i & 1];
+            if (carry) { r.w = i == 0 ? weights : moved[(i + 1) & 1]; r.out_w = moved[i & 1]; }
             for (int k = 0; k < 3; k++) {
                 if (k == 1 && p.nblk <= RS_FEW_BLOCKS) continue;
                 const long long nth = k == 2 ? launches - 1 : k, z0 = nth * part < words ? nth * part : words, z1 = k == 2 ? words : z0 + part < words ? z0 + part : words;
@@ -674,7 +688,7 @@ int nl_embedding_backward(const void* table, long long V, int D, int dtype, cons
         w += p.key_l[i] + p.any_l[i] + p.piece_l[i];
     }
     EmbSum a = {};
-    a.keys = keys[(p.passes - 1) & 1]; a.pos = pos[(p.passes - 1) & 1]; a.g = g_out; a.weights = weights; a.g_table = g_table; a.V = V; a.L = p.L; a.D = D;
+    a.keys = keys[(p.passes - 1) & 1]; a.pos = pos[(p.passes - 1) & 1]; a.g = g_out; a.weights = carry ? moved[(p.passes - 1) & 1] : weights; a.sorted = carry; a.g_table = g_table; a.V = V; a.L = p.L; a.D = D;
     a.bag = bag; a.scale = scale; a.chunk = p.chunk;
     const int vec = emb_vec(D, dtype, g_out, g_table);
     if (vec == 8) emb_sums<8>(p, a, buf, dtype, st);

@@ -300,3 +300,15 @@ def test_bags_of_eight_over_tables_around_two_gigabytes():
         w = torch.zeros(5, 8, device="cuda")
         w[:, 5:] = 1.0
         assert not bool(ops.embedding_forward(table, ids, w).any())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_weights_move_with_their_lookups(dtype):
+    """sorts of more than 65536 weighted lookups, one to four passes, whole and partial workgroups; and bags without weights"""
+    for V, D, M, bag in ((200, 8, 40000, 2), (40000, 4, 8193, 9), (100000, 3, 22000, 3), (20000003, 2, 33000, 3), (3000, 16, 65537, 8)):
+        table, ids, w, g = _case(V, D, M, bag, dtype, V + M)
+        _check(table, ids, w, g, 0.75, *_grads(table, ids, w, g, 0.75), f"V {V} D {D} M {M} bag {bag}")
+        gt, gt1 = torch.empty_like(table), torch.empty_like(table)
+        ops.embedding_backward(table, ids, g, None, 0.75, gt)
+        ops.embedding_backward(table, ids, g, torch.ones_like(w), 0.75, gt1)
+        assert torch.equal(gt, gt1), (V, M)
