@@ -5,12 +5,12 @@
 // neighbouring entries in ascending position: pieces of a fixed number of entries, the pieces of a row that spans several joined in order, level by level.
 #include "nl_layers.h"
 
-// Sorted entries per run-summing group: 16 while that leaves at most EMB_THREADS threads of eight columns, so that there are enough of them (32768 lookups x 1024 bf16:
-// 21 us, 91 us with 64 entries and one row in flight; 2.1 M x 16 bf16: 69, 74), else 64.
+// Sorted entries per run-summing group: 16 while that leaves at most EMB_THREADS threads of eight columns, so that there are enough of them, else 64, so that there
+// are fewer pieces (whole backward pass, bf16: 16384 lookups x 1024 50 us with 16, 58 with 64; 2.1 M x 16 145, 154; 262144 x 256 99, 87; 131072 x 1024 162, 144).
 // Pieces of a row that crosses such chunks are joined in blocks of EMB_BLOCK neighbours, level by level.
 #define EMB_CHUNK_FEW 16
 #define EMB_CHUNK_MANY 64
-#define EMB_THREADS (1 << 20)
+#define EMB_THREADS (1 << 18)
 #define EMB_BLOCK 64
 #define EMB_BATCH 8             // rows in flight together
 // A sorting pass takes 1024 keys a workgroup (4 waves x 4 rounds x 64 lanes) up to RS_FEW keys, else 4096 and puts them in order in LDS first, so that what it writes
