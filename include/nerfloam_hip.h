@@ -564,7 +564,8 @@ int nl_dist_rows_union_prefix(const int* gathered, int stride_ints, int offset_i
  *   bits  relu: one bit per element, z > 0: words [M][ceil(N/32)], column n in bit n % 32 of word n / 32
  *   x8, x8e   x in 8 bits for gw, [M][up(K,32)] and [M][ceil(K/32)], what nl_mx8_encode writes
  * nl_linear_backward reads gy, w (for gx), x or x8 / x8e (for gw), what the forward pass kept of z, and writes gx [M,K], gw [N,K], gb [N], each where its
- * pointer is set, in dtype.  dz = gy act'(z) is rounded to dtype once for the two products (fp32: not at all); gb sums the unrounded values.
+ * pointer is set, in dtype.  dz = gy act'(z) is rounded to dtype once for the two products (not at all in fp32, and for gelu and silu while
+ * M N K <= 2^23, which run as fp32 products); gb sums the unrounded values.
  * fp32 products run as six bf16 products of the exact three-term splits of both operands (dropped terms below 2^-26 of |x||w|); an infinity among the
  * operands gives NaN there.  Sums are fp32 and their order depends on the sizes only.  M = 0 is a legal call (gw, gb = 0).
  * Taken are at most 2^30 rows, 2^22 columns, and results of fewer than 2^24 tiles (of 64 x 64 where they are small).

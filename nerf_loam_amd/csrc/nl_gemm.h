@@ -27,6 +27,7 @@ struct NlGemm {
 void nl_gemm_bf16(const NlGemm& g, int layout, int tile, dim3 grid, hipStream_t st);
 void nl_gemm_f16(const NlGemm& g, int layout, int tile, dim3 grid, hipStream_t st);
 void nl_gemm_f32(const NlGemm& g, int layout, int tile, dim3 grid, hipStream_t st);
+void nl_gemm_f32_to16(const NlGemm& g, int dt, int layout, dim3 grid, hipStream_t st);      // A fp32, B and the result of dt; layouts 1 and 2, squares of 64
 
 #ifdef __HIPCC__
 template <class T> struct NlMma;
@@ -445,13 +446,13 @@ __device__ __forceinline__ void gemm_split8(const float* x, nl_i32x4& h, nl_i32x
     }
 }
 
-// One fp32 operand: R rows or columns x 32 contraction indices per step, 256 threads; the planes' layout in LDS is GemmSide's
-template <bool SLOW, int R>
+// One operand: R rows or columns x 32 contraction indices per step, 256 threads; the planes' layout in LDS is GemmSide's.  SRC: its elements' type in memory
+template <bool SLOW, int R, int SRC>
 struct GemmSide32 {
     typedef GemmSide<SLOW, R, 256, 32> Plane;
-    static constexpr int UNITS = R * 32 / (8 * 256), BYTES = 3 * Plane::BYTES;         // a unit: eight neighbouring elements in memory
-    unsigned off[UNITS]; int kk[UNITS], lds[UNITS]; bool half[UNITS];                   // half: only the first four elements are inside (slow: columns)
-    float v[UNITS][8];
+    static constexpr int UNITS = R * 32 / (8 * 256), BYTES = 3 * Plane::BYTES, ES = SRC == NL_DT_F32 ? 4 : 2;       // a unit: eight neighbouring elements in memory
+    unsigned off[UNITS]; int kk[UNITS], lds[UNITS]; bool half[UNITS];                   // half: only the first four elements are inside (fp32, slow: columns)
+    NlRaw8<SRC> v[UNITS];
     const char* base; long long step;
 
     __device__ __forceinline__ void init(const char* p, long long ld, long long i0, long long I, long long k0)
@@ -462,17 +463,17 @@ struct GemmSide32 {
             if (SLOW) {
                 const int k = s / (R / 8), c = s % (R / 8);
                 kk[u] = k; half[u] = i0 + 8 * c + 4 >= I;
-                off[u] = i0 + 8 * c < I ? (unsigned)(k * ld + 32 * c) : GEMM_OUT_OF_RANGE;
+                off[u] = i0 + 8 * c < I ? (unsigned)(k * ld + 8 * ES * c) : GEMM_OUT_OF_RANGE;
                 lds[u] = k * (R * 2) + (c ^ (Plane::swz(k) << 1)) * 16;
             } else {
                 const int r = s >> 2, c = s & 3;
                 kk[u] = 8 * c; half[u] = false;
-                off[u] = i0 + r < I ? (unsigned)(r * ld + 32 * c) : GEMM_OUT_OF_RANGE;
+                off[u] = i0 + r < I ? (unsigned)(r * ld + 8 * ES * c) : GEMM_OUT_OF_RANGE;
                 lds[u] = r * 64 + (c ^ Plane::swz_row(r)) * 16;
             }
         }
-        base = SLOW ? p + k0 * ld + 4 * i0 : p + i0 * ld + 4 * k0;
-        step = SLOW ? 32 * ld : 128;
+        base = SLOW ? p + k0 * ld + ES * i0 : p + i0 * ld + ES * k0;
+        step = SLOW ? 32 * ld : 32 * ES;
     }
     __device__ __forceinline__ void fetch(long long adv, long long kleft)
     {
@@ -480,29 +481,31 @@ struct GemmSide32 {
 #pragma unroll
         for (int u = 0; u < UNITS; u++) {
             const bool in = kk[u] < kleft, in2 = SLOW ? in && !half[u] : kk[u] + 4 < kleft;
-            const nl_i32x4 a = __builtin_bit_cast(nl_i32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)(in ? off[u] : GEMM_OUT_OF_RANGE), 0, 0));
-            const nl_i32x4 b = __builtin_bit_cast(nl_i32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)(in2 && off[u] != GEMM_OUT_OF_RANGE ? off[u] + 16 : GEMM_OUT_OF_RANGE), 0, 0));
-#pragma unroll
-            for (int j = 0; j < 4; j++) { v[u][j] = __int_as_float(a[j]); v[u][4 + j] = __int_as_float(b[j]); }
+            v[u].w[0] = __builtin_bit_cast(nl_i32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)(in ? off[u] : GEMM_OUT_OF_RANGE), 0, 0));
+            if constexpr (SRC == NL_DT_F32)
+                v[u].w[1] = __builtin_bit_cast(nl_i32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)(in2 && off[u] != GEMM_OUT_OF_RANGE ? off[u] + 16 : GEMM_OUT_OF_RANGE), 0, 0));
         }
     }
     __device__ __forceinline__ void put(char* mem) const
     {
 #pragma unroll
         for (int u = 0; u < UNITS; u++) {
+            float x[8];
             nl_i32x4 p[3];
-            gemm_split8(v[u], p[0], p[1], p[2]);
+            nl_unraw8<SRC>(x, v[u]);
+            gemm_split8(x, p[0], p[1], p[2]);
 #pragma unroll
             for (int q = 0; q < 3; q++) *reinterpret_cast<nl_i32x4*>(mem + q * Plane::BYTES + lds[u]) = p[q];
         }
     }
 };
 
-template <bool A_SLOW, bool B_SLOW, int BT>
+// DT: the type of B's elements and of the results; A's are fp32 (a 16-bit DT: small backward products whose dz is not rounded)
+template <bool A_SLOW, bool B_SLOW, int BT, int DT>
 __global__ __launch_bounds__(256, 2) void k_gemm_f32(NlGemm g)
 {
-    typedef GemmSide32<A_SLOW, BT> SA;
-    typedef GemmSide32<B_SLOW, BT> SB;
+    typedef GemmSide32<A_SLOW, BT, NL_DT_F32> SA;
+    typedef GemmSide32<B_SLOW, BT, DT> SB;
     constexpr int F = BT / 32, LDS = SA::BYTES + SB::BYTES;
     __shared__ __align__(256) char s_mem[LDS > BT * BT * 2 ? LDS : BT * BT * 2];
     char* const s_b = s_mem + SA::BYTES;
@@ -545,14 +548,14 @@ __global__ __launch_bounds__(256, 2) void k_gemm_f32(NlGemm g)
         }
         nl_lds_barrier();
     }
-    gemm_results<NL_DT_F32, BT / 2, BT / 2, 4, sizeof(s_mem)>(g, acc, s_mem, m0 + wm, n0 + wn, piece);
+    gemm_results<DT, BT / 2, BT / 2, 4, sizeof(s_mem)>(g, acc, s_mem, m0 + wm, n0 + wn, piece);
 }
 
 template <bool A_SLOW, bool B_SLOW>
 static void nl_gemm_tile_f32(const NlGemm& g, int tile, dim3 grid, hipStream_t st)
 {
-    if (tile == 1) hipLaunchKernelGGL((k_gemm_f32<A_SLOW, B_SLOW, 128>), grid, dim3(256), 0, st, g);
-    else hipLaunchKernelGGL((k_gemm_f32<A_SLOW, B_SLOW, 64>), grid, dim3(256), 0, st, g);
+    if (tile == 1) hipLaunchKernelGGL((k_gemm_f32<A_SLOW, B_SLOW, 128, NL_DT_F32>), grid, dim3(256), 0, st, g);
+    else hipLaunchKernelGGL((k_gemm_f32<A_SLOW, B_SLOW, 64, NL_DT_F32>), grid, dim3(256), 0, st, g);
 }
 
 template <class T, bool A_SLOW, bool B_SLOW, bool B_MX8, bool ENC = false>

@@ -7,7 +7,7 @@
 
 // ---------------------------------------------------------------------------------------------
 // k_linear_pack: an operand as the tiled products want it - rows of up(cols, 8) elements with zeros behind the last column - from rows of any stride and
-// alignment, or (fp32) from 8-bit codes.  Runs only where the operand does not lie that way already.
+// alignment, or from 8-bit codes (for fp32 arithmetic).  Runs only where the operand does not lie that way already.
 // ---------------------------------------------------------------------------------------------
 struct NlPack { const void* src; const unsigned char* e; void* dst; long long rows, ld, pitch; int cols; };
 struct NlPack2 { NlPack p[2]; };                                     // one launch for both operands of a product, or both of a backward pass
@@ -16,14 +16,13 @@ template <int DT>
 __global__ __launch_bounds__(256) void k_linear_pack(NlPack2 both)
 {
     const NlPack a = both.p[blockIdx.y];
-    const bool mx8 = DT == NL_DT_F32 && a.e;
     const long long per_row = a.pitch / 8, total = a.rows * per_row;
     const bool vec = nl_rows_aligned<DT>(a.src, a.ld);
     for (long long t = (long long)blockIdx.x * 256 + threadIdx.x; t < total; t += (long long)gridDim.x * 256) {
         const long long r = t / per_row;
         const int c = (int)(t - r * per_row) * 8;
         float v[8];
-        if (mx8) {
+        if (a.e) {
             const nl_i32x2 w = *reinterpret_cast<const nl_i32x2*>((const unsigned char*)a.src + r * a.ld + c);       // (rows of codes are whole blocks of 32, zeros behind the last)
             const float s = nl_mx_scale(a.e[r * (a.ld / 32) + (c >> 5)]);
             const nl_f32x4 p = nl_mx_decode4((unsigned)w[0], s, nl_dtype_max(DT)), q = nl_mx_decode4((unsigned)w[1], s, nl_dtype_max(DT));
@@ -211,7 +210,7 @@ struct NlDz {
     long long M, ldgy, ldz, ldbits, ldz8, ldz8e, pitch, rows_per_chunk;
     int N;
 };
-template <int DT, int ACT>
+template <int DT, int ACT, int OUT>
 __global__ __launch_bounds__(256) void k_linear_dz(NlDz a)
 {
     __shared__ float s_sum[8][257];
@@ -241,7 +240,7 @@ __global__ __launch_bounds__(256) void k_linear_dz(NlDz a)
             }
 #pragma unroll
             for (int j = 0; j < 8; j++) sum[j] += g[j];
-            if (a.dz) nl_store8<DT>(a.dz, m * a.pitch + n, g, 8, true);
+            if (a.dz) nl_store8<OUT>(a.dz, m * a.pitch + n, g, 8, true);
         }
     if (!a.part) return;
 #pragma unroll
@@ -307,7 +306,7 @@ static NlPacked nl_packed(NlWork& w, const void* p, const unsigned char* e, long
 // 200000: 56 in 256 pieces of the first, 46 in 128 of the second, 48 in 32 of the third, 4200 uncut; fp32 4096^3: 576 in squares of 128, 665 of 64, 2048 x 256 x 256:
 // 21, 9.8).  The estimate's choice is within 15 % of the best of all tiles and powers of two at the 23 shapes of either kind that these come from.
 struct NlCut { int tile, splits; long long kchunk; };
-static NlCut nl_cut(long long M, long long N, long long K, int dt, int layout)
+static NlCut nl_cut(long long M, long long N, long long K, int dt, int layout, int largest)
 {
     struct Tile { int size, at_a_time; double alone, full, rest, slow; };       // slow: on the steps where both operands' rows are the contraction (narrow rows of a tile)
     static const Tile T16[3] = {{256, 256, 1.33, 1.40, 9.0, 1.0}, {128, 512, 0.70, 0.87, 4.0, 1.0}, {64, 1024, 0.50, 0.67, 2.0, 1.0}};
@@ -315,9 +314,9 @@ static NlCut nl_cut(long long M, long long N, long long K, int dt, int layout)
     const Tile* T = dt == NL_DT_F32 ? T32 : T16;
     const long long ksteps = (K + GEMM_BK - 1) / GEMM_BK;
     const double memory = (double)nl_dtype_size(dt) * (M * K + N * K + M * N) / 4.5e6;
-    NlCut best = {1, 1, ksteps * GEMM_BK};
+    NlCut best = {2, 1, ksteps * GEMM_BK};
     double least = 1e300;
-    for (int t = dt == NL_DT_F32 ? 1 : 0; t < 3; t++) {
+    for (int t = largest; t < 3; t++) {
         const double tiles = (double)(nl_up(M, T[t].size) / T[t].size) * (double)(nl_up(N, T[t].size) / T[t].size);
         for (int s = 1; s <= 256 && s <= ksteps; s *= 2) {
             if (s > 1 && 4.0 * s * M * N > 1.5e9) break;
@@ -334,13 +333,14 @@ static NlCut nl_cut(long long M, long long N, long long K, int dt, int layout)
     return best;
 }
 
-// C[M,N] = sum_k A(m,k) B(n,k), layouts as in nl_gemm.h.  A8, A8e: layout 4's codes.  gb: a bias gradient to sum in the same launch if there is one; then it is cleared
-static void nl_product(NlWork& w, const NlPacked& A, const NlPacked& B, int layout, long long M, int N, long long K, const NlEpilogue& ep, unsigned char* A8, unsigned char* A8e, NlGb* gb)
+// C[M,N] = sum_k A(m,k) B(n,k), layouts as in nl_gemm.h.  A8, A8e: layout 4's codes.  gb: a bias gradient to sum in the same launch if there is one; then it is cleared.
+// wide: A is fp32 whatever the type
+static void nl_product(NlWork& w, const NlPacked& A, const NlPacked& B, int layout, long long M, int N, long long K, const NlEpilogue& ep, unsigned char* A8, unsigned char* A8e, NlGb* gb, bool wide)
 {
-    const NlCut c = nl_cut(M, N, K, ep.dt, layout == 4 ? 0 : layout);      // (the codes do not change the sums)
+    const NlCut c = nl_cut(M, N, K, wide ? NL_DT_F32 : ep.dt, layout == 4 ? 0 : layout, wide ? 2 : ep.dt == NL_DT_F32 ? 1 : 0);      // (the codes do not change the sums)
     static const int size[3] = {256, 128, 64};
     NlGemm g = {};
-    g.A = (const char*)A.p; g.B = (const char*)B.p; g.Be = B.e; g.lda = nl_dtype_size(ep.dt) * A.pitch; g.ldb = layout == 3 ? B.pitch : nl_dtype_size(ep.dt) * B.pitch;
+    g.A = (const char*)A.p; g.B = (const char*)B.p; g.Be = B.e; g.lda = (wide ? 4 : nl_dtype_size(ep.dt)) * A.pitch; g.ldb = layout == 3 ? B.pitch : nl_dtype_size(ep.dt) * B.pitch;
     g.A8 = A8; g.A8e = A8e; g.ld8 = nl_up(K, NL_MX_BLOCK);
     g.M = M; g.N = N; g.K = K; g.kchunk = c.kchunk;
     const long long tm = nl_up(M, size[c.tile]) / size[c.tile], tn = nl_up(N, size[c.tile]) / size[c.tile];
@@ -351,7 +351,8 @@ static void nl_product(NlWork& w, const NlPacked& A, const NlPacked& B, int layo
     if (c.splits > 1) { g.ep = NlEpilogue{}; g.ep.part = (float*)w.take(4LL * c.splits * M * N); }
     if (w.dry) return;
     const dim3 grid((unsigned)(tm * tn), (unsigned)c.splits);
-    if (ep.dt == NL_DT_F32) nl_gemm_f32(g, layout, c.tile, grid, w.st);
+    if (wide) nl_gemm_f32_to16(g, ep.dt, layout, grid, w.st);
+    else if (ep.dt == NL_DT_F32) nl_gemm_f32(g, layout, c.tile, grid, w.st);
     else if (ep.dt == NL_DT_BF16) nl_gemm_bf16(g, layout, c.tile, grid, w.st);
     else nl_gemm_f16(g, layout, c.tile, grid, w.st);
     if (c.splits > 1) {
@@ -384,13 +385,22 @@ static void nl_forward_run(const NlLinear* d, NlWork& w)
     }
     const NlPacked x = nl_packed(w, d->x, nullptr, d->M, d->K, d->ldx, d->dtype, d->dtype), wt = nl_packed(w, d->w, nullptr, d->N, d->K, d->ldw, d->dtype, d->dtype);
     nl_pack(w, d->dtype);
-    nl_product(w, x, wt, codes ? 4 : 0, d->M, d->N, d->K, ep, d->x8, d->x8e, nullptr);
+    nl_product(w, x, wt, codes ? 4 : 0, d->M, d->N, d->K, ep, d->x8, d->x8e, nullptr, false);
+}
+
+// dz = gy act'(z) in 16 bits is a second rounding of half a step besides the gradients' own (1.41 times the error of one; with few results up to 1.9 times).  Where the
+// products are short, and launches are what the pass takes, dz stays in fp32 and the products run as fp32's do (2^22 multiplications in either, both products, bf16: 18.5
+// instead of 13.7 us of a pass that takes 70 from autograd; 2^25 in either: 21 instead of 15.5).
+#define NL_WIDE_MOST (1LL << 23)
+static bool nl_wide(const NlLinear* d)
+{
+    return d->dtype != NL_DT_F32 && (d->act == NL_ACT_GELU || d->act == NL_ACT_SILU) && (double)d->M * d->N * d->K <= (double)NL_WIDE_MOST;
 }
 
 static void nl_backward_run(const NlLinear* d, NlWork& w)
 {
     const bool in_place = d->act == NL_ACT_NONE && nl_in_place(d->gy, d->N, d->ldgy, d->dtype);
-    const bool products = d->gx || d->gw;
+    const bool products = d->gx || d->gw, wide = nl_wide(d);
     NlPacked dz = {d->gy, d->ldgy, nullptr};
     NlGb gb = {};
     if (d->gb || (products && !in_place)) {
@@ -408,22 +418,24 @@ static void nl_backward_run(const NlLinear* d, NlWork& w)
         if (d->gb) a.part = (float*)w.take(4LL * chunks * d->N);
         if (products && !in_place) {
             a.pitch = nl_up(d->N, 8);
-            a.dz = w.take(d->M * a.pitch * nl_dtype_size(d->dtype));
+            a.dz = w.take(d->M * a.pitch * (wide ? 4 : nl_dtype_size(d->dtype)));
             dz = NlPacked{a.dz, a.pitch, nullptr};
         }
         if (!w.dry) {
             const dim3 grid(colblocks, (unsigned)chunks);
-            NL_WITH_DTYPE(d->dtype, if (d->act == NL_ACT_NONE) hipLaunchKernelGGL((k_linear_dz<DT, NL_ACT_NONE>), grid, dim3(256), 0, w.st, a);
-                                    else if (d->act == NL_ACT_RELU) hipLaunchKernelGGL((k_linear_dz<DT, NL_ACT_RELU>), grid, dim3(256), 0, w.st, a);
-                                    else if (d->act == NL_ACT_GELU) hipLaunchKernelGGL((k_linear_dz<DT, NL_ACT_GELU>), grid, dim3(256), 0, w.st, a);
-                                    else hipLaunchKernelGGL((k_linear_dz<DT, NL_ACT_SILU>), grid, dim3(256), 0, w.st, a));
+            NL_WITH_DTYPE(d->dtype, if (d->act == NL_ACT_NONE) hipLaunchKernelGGL((k_linear_dz<DT, NL_ACT_NONE, DT>), grid, dim3(256), 0, w.st, a);
+                                    else if (d->act == NL_ACT_RELU) hipLaunchKernelGGL((k_linear_dz<DT, NL_ACT_RELU, DT>), grid, dim3(256), 0, w.st, a);
+                                    else if (d->act == NL_ACT_GELU && wide) hipLaunchKernelGGL((k_linear_dz<DT, NL_ACT_GELU, NL_DT_F32>), grid, dim3(256), 0, w.st, a);
+                                    else if (d->act == NL_ACT_GELU) hipLaunchKernelGGL((k_linear_dz<DT, NL_ACT_GELU, DT>), grid, dim3(256), 0, w.st, a);
+                                    else if (wide) hipLaunchKernelGGL((k_linear_dz<DT, NL_ACT_SILU, NL_DT_F32>), grid, dim3(256), 0, w.st, a);
+                                    else hipLaunchKernelGGL((k_linear_dz<DT, NL_ACT_SILU, DT>), grid, dim3(256), 0, w.st, a));
         }
         if (d->gb) gb = NlGb{a.part, d->gb, (int)chunks, d->N, (d->N + 3) / 4};
     }
     NlEpilogue ep = {};
     ep.dt = d->dtype; ep.act = NL_ACT_NONE; ep.ldy = d->K;
     NlPacked wt = {}, x = {};
-    const bool codes = d->gw && d->x8 && d->dtype != NL_DT_F32;           // (fp32 splits its operands: codes are decoded to fp32 first)
+    const bool codes = d->gw && d->x8 && d->dtype != NL_DT_F32 && !wide;  // (fp32 arithmetic splits its operands: codes are decoded first)
     if (d->gx) wt = nl_packed(w, d->w, nullptr, d->N, d->K, d->ldw, d->dtype, d->dtype);
     if (codes) x = NlPacked{d->x8, nl_up(d->K, 32), d->x8e};
     else if (d->gw) x = d->x8 ? nl_packed(w, d->x8, d->x8e, d->M, d->K, nl_up(d->K, 32), NL_DT_MX8, d->dtype) : nl_packed(w, d->x, nullptr, d->M, d->K, d->ldx, d->dtype, d->dtype);
@@ -432,13 +444,13 @@ static void nl_backward_run(const NlLinear* d, NlWork& w)
     long long most = keep;
     if (d->gx) {
         ep.y = d->gx;
-        nl_product(w, dz, wt, 1, d->M, d->K, d->N, ep, nullptr, nullptr, nullptr);
+        nl_product(w, dz, wt, 1, d->M, d->K, d->N, ep, nullptr, nullptr, nullptr, wide);
         most = w.used;
         w.used = keep;                                               // (the second product follows on the stream: it takes the same place)
     }
     if (d->gw) {
         ep.y = d->gw;
-        nl_product(w, dz, x, codes ? 3 : 2, d->N, d->K, d->M, ep, nullptr, nullptr, &gb);
+        nl_product(w, dz, x, codes ? 3 : 2, d->N, d->K, d->M, ep, nullptr, nullptr, &gb, wide);
     }
     if (gb.blocks && !w.dry) NL_WITH_DTYPE(d->dtype, hipLaunchKernelGGL(k_linear_gb<DT>, dim3(gb.blocks), dim3(256), 0, w.st, gb));
     if (w.used < most) w.used = most;

@@ -613,3 +613,26 @@ def test_forward_writes_the_codes_of_every_number(dtype):
     got, got_e = torch.empty_like(want), torch.empty_like(want_e)
     ops.linear_forward(order, w, x8=got, x8e=got_e)
     assert torch.equal(got, want) and torch.equal(got_e, want_e)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("checkpoint", [None, "mx8"])
+def test_small_backward_passes_do_not_round_dz(dtype, act, checkpoint):
+    """the tolerances of _backward_check without the rounding of dz, with those of an fp32 product"""
+    for M, N, K in ((1, 1, 1), (2, 8, 16), (4, 8, 16), (26, 8, 64), (34, 18, 56), (3, 3968, 16), (22, 106, 3119), (1505, 8, 64), (65, 129, 257), (128, 256, 256), (20000, 20, 20)):
+        x, w, b, _ = _forward_case(M, N, K, dtype, act, 900 + M)
+        gy = _rand(_gen(901 + M), M, N, dtype=dtype)
+        z = _rand(_gen(902 + M), M, N, dtype=dtype)
+        kw, xd, zd = dict(z=z), x.double(), z.double()
+        if checkpoint:
+            kw = dict(zip(("z8", "z8e", "x8", "x8e"), (*ops.mx8_encode(z), *ops.mx8_encode(x))))
+            xd, zd = (torch.from_numpy(mx8_values(t.double().cpu().numpy())[0]).cuda() for t in (x, z))
+        gx, gw = torch.empty(M, K, dtype=dtype, device="cuda"), torch.empty(N, K, dtype=dtype, device="cuda")
+        ops.linear_backward(gy, None if checkpoint else x, w, act, gx=gx, gw=gw, **kw)
+        dz = gy.double() * _slope64(zd, act)
+        e_dz = gy.double().abs() * 16 * 2.0 ** -24 * (1 + zd.abs()) + 2.0 ** -24 * dz.abs()
+        S, Sw = dz.abs() + e_dz, w.double().abs()
+        for got, want, e, name in ((gx, dz @ w.double(), e_dz @ Sw + _e(N, torch.float32) * (S @ Sw), "gx"),
+                                   (gw, dz.t() @ xd, e_dz.t() @ xd.abs() + _e(M, torch.float32) * (S.t() @ xd.abs()), "gw")):
+            _close(got, want, e + _half(want.abs() + e, dtype), f"{name} {M}x{N}x{K}")
