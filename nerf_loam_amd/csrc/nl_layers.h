@@ -107,8 +107,8 @@ template <int DT> __device__ __forceinline__ void nl_store8(void* p, long long i
 // 16-byte accesses at multiples of eight elements of rows `ld` elements apart
 template <int DT> __device__ __forceinline__ bool nl_rows_aligned(const void* p, long long ld) { return (ld & (DT == NL_DT_F32 ? 3 : 7)) == 0 && ((uintptr_t)p & 15) == 0; }
 
-// activations and their slopes.  Products whose epilogue or dz pass calls erff and expf are bound by vector arithmetic (dz of 16384 x 4096 gelu: 157 us against 78 us
-// of memory time), so both come from one hardware exponential and one hardware reciprocal.
+// activations and their slopes.  Products whose epilogue or dz pass calls erff and expf are bound by vector arithmetic (dz of 16384 x 4096 gelu: 157 us, where
+// memory takes 78), so both come from one hardware exponential and one hardware reciprocal.
 // Phi(z) = (1 + erf(z / sqrt 2)) / 2 after Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26: with x = |z| / sqrt 2 and t = 1 / (1 + 0.3275911 x),
 // erfc(x) = (a1 t + .. + a5 t^5) exp(-x^2) to 1.5e-7; the same exponential is the density of gelu's slope.
 __device__ __forceinline__ float nl_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
@@ -246,7 +246,7 @@ template <int DT, bool INSIDE> __device__ __forceinline__ void nl_epilogue8(cons
         }
     }
     if (!live) return;
-    if (ep.z) nl_store8<DT>(ep.z, m * ep.ldz + n, v, left, INSIDE || (ep.ldz & 7) == 0);
+    if (ep.z) nl_store8<DT>(ep.z, m * ep.ldz + n, v, left, INSIDE || (ep.ldz & 7) == 0);      // (rounded to the type: half the bytes; only slopes are taken of it)
     nl_act8(v, ep.act);
     if (ep.r) {
 #pragma unroll
