@@ -372,8 +372,8 @@ def render_rays(rays_o, rays_d, map_states, sdf_network, step_size, voxel_size, 
 def get_features(samples, map_states, voxel_size):
     """render_helpers.py:74-93: features of samples inside voxels, trilinear between the eight corner rows -> {"dists", "emb" [P, 16] float32}, differentiable with
     respect to map_states["voxel_vertex_emb"] (through layers.embedding_lookup: the gradient is summed over sorted rows, the same bits every run) and to
-    samples["sampled_point_xyz"].  A voxel index outside the map gives zeros and no gradient.  The optimisation loops do not come here (the engine interpolates inside its kernels): this is for callers that train a decoder of
-    their own on samples of their own."""
+    samples["sampled_point_xyz"].  A voxel index outside the map gives zeros and no gradient.  The optimisation loops do not come here (the engine interpolates
+    inside its kernels): this is for callers that train a decoder of their own on samples of their own."""
     emb = map_states["voxel_vertex_emb"]
     m = _map_device(map_states, voxel_size, emb.device)
     vox = samples["sampled_point_voxel_idx"].reshape(-1).to(emb.device).long()

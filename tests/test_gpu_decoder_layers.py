@@ -10,6 +10,7 @@ import numpy as np
 import pytest
 import torch
 
+from nerf_loam_amd import layers, ops
 from nerf_loam_amd.decoder import Decoder
 from oracle import oracle as O
 
@@ -229,3 +230,86 @@ def test_scores_and_mesh_of_a_decoder_of_another_size():
         dec.sdf_out.bias.sub_(float(grid.median()))
     mesh = MeshExtractor(types.SimpleNamespace(mapper_specs={"voxel_size": 0.2})).create_mesh(dec, sub, 0.2, sub["voxel_center_xyz"], offset=-2000, res=res)
     assert len(np.asarray(mesh.vertices)) > 100 and len(np.asarray(mesh.triangles)) > 100
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_the_operators_together_in_a_graph(dtype):
+    """lookup of eight corners, two layers whose inputs are kept in 8 bits, and all gradients, on tensors of the caller: captured once, replayed over new inputs with eager
+    work between, every replay like the eager result; more than 65536 lookups (weights move with their sort), layers on either side of the short ones"""
+    V, D, M = 5000, 16, 9000
+    for H in (24, 160):
+        g = torch.Generator(device="cuda").manual_seed(H)
+        r = lambda *s: torch.randn(*s, generator=g, device="cuda").to(dtype)  # noqa: E731
+        table, w1, b1, w2, gy = r(V, D), r(H, D), r(H), r(H, H) * H ** -0.5, r(M, H)
+        ids = torch.randint(-1, V, (M, 8), generator=g, device="cuda", dtype=torch.int32)
+        wt = torch.rand(M, 8, generator=g, device="cuda")
+        kb = (H + 31) // 32
+        new = lambda *s, t=dtype: torch.empty(*s, dtype=t, device="cuda")  # noqa: E731
+        u8 = torch.uint8
+
+        def buffers():
+            return dict(x=new(M, D), x8=new(M, 32, t=u8), x8e=new(M, 1, t=u8), h=new(M, H), z8=new(M, 32 * kb, t=u8), z8e=new(M, kb, t=u8), h8=new(M, 32 * kb, t=u8), h8e=new(M, kb, t=u8),
+                        bits=new(M, kb, t=torch.int32), y=new(M, H), gh=new(M, H), gw2=new(H, H), gx=new(M, D), gw1=new(H, D), gb1=new(H), gt=new(V, D), gwt=new(M, 8, t=torch.float32))
+
+        def step(b):
+            ops.embedding_forward(table, ids, wt, out=b["x"])
+            ops.linear_forward(b["x"], w1, b1, "silu", out=b["h"], z8=b["z8"], z8e=b["z8e"], x8=b["x8"], x8e=b["x8e"])
+            ops.linear_forward(b["h"], w2, None, "relu", residual=b["h"], out=b["y"], bits=b["bits"], x8=b["h8"], x8e=b["h8e"])
+            ops.linear_backward(gy, None, w2, "relu", bits=b["bits"], x8=b["h8"], x8e=b["h8e"], gx=b["gh"], gw=b["gw2"])
+            ops.linear_backward(b["gh"], None, w1, "silu", z8=b["z8"], z8e=b["z8e"], x8=b["x8"], x8e=b["x8e"], gx=b["gx"], gw=b["gw1"], gb=b["gb1"])
+            ops.embedding_backward(table, ids, b["gx"], wt, 1.0, b["gt"], b["gwt"])
+        eager, kept = buffers(), buffers()
+        step(eager)
+        torch.cuda.synchronize()
+        gph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gph):
+            step(kept)
+        for it in range(4):
+            ids.copy_(torch.randint(-1, V, (M, 8), generator=g, device="cuda", dtype=torch.int32))
+            table.copy_(r(V, D))
+            gy.copy_(r(M, H))
+            for t in kept.values():
+                t.zero_()
+            step(eager)
+            gph.replay()
+            torch.cuda.synchronize()
+            for k in eager:
+                assert torch.equal(eager[k], kept[k]), (H, it, k)
+
+
+def test_two_threads_at_once():
+    """training steps of two threads, a stream each, give what they give one after the other"""
+    import threading
+    table = torch.randn(3000, 32, device="cuda").to(torch.bfloat16)
+
+    def inputs(seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        x = torch.randn(700, 96, generator=g, device="cuda").to(torch.bfloat16).requires_grad_(True)
+        w = (torch.randn(32, 96, generator=g, device="cuda") * 0.1).to(torch.bfloat16).requires_grad_(True)
+        return x, w, torch.randint(0, 3000, (700,), generator=g, device="cuda"), table.clone().requires_grad_(True)
+
+    def step(x, w, ids, t):
+        y = layers.linear_act(x, w, act="gelu", residual=layers.embedding_lookup(t, ids), checkpoint="mx8")
+        return torch.autograd.grad(y, (x, w, t), torch.ones_like(y))
+    data = [inputs(s) for s in (1, 2)]
+    want = [step(*d) for d in data]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(30):
+                    got = step(*data[i])
+                    s.synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                        wrong.append(i)
+        except Exception as e:  # noqa: BLE001
+            wrong.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong
