@@ -22,6 +22,13 @@ struct NlGemm {
     NlEpilogue ep;
 };
 
+struct NlDz {                          // dz = gy act'(z): where gy and z are, where dz and the bias' partial sums go
+    const void* gy; const void* z; const unsigned* bits; const unsigned char* z8; const unsigned char* z8e;
+    void* dz; float* part;
+    long long M, ldgy, ldz, ldbits, ldz8, ldz8e, pitch, rows_per_chunk;
+    int N;
+};
+
 // layout 0: both operands' rows run along k; 1: B's rows are k; 2: both operands' rows are k; 3: the same with B in 8-bit codes;
 // 4: layout 0, and A is written out in 8-bit codes (both for 16-bit types only).  tile 0: 256 x 256 (16 bits only), 1: 128 x 128, 2: 64 x 64.
 void nl_gemm_bf16(const NlGemm& g, int layout, int tile, dim3 grid, hipStream_t st);
@@ -246,50 +253,54 @@ struct GemmSideMx8 {
 // A step's rows of A in 8-bit codes, from LDS (GemmSide's fast layout): a thread takes a block of 32.  With a value that is not finite in the block every element is asked
 // (nl_mx_encode4 as in k_mx8_encode: the same codes); otherwise the largest magnitude is found among the 16-bit patterns, whose order is that of the magnitudes.
 // 200000 x 256: the product takes 14 us more, a pass of its own over x 30; 32768 x 2048: 16 and 41.
-template <class T, int BM, int NT>
-__device__ __forceinline__ void gemm_encode(const NlGemm& g, const char* lds, long long m0, long long k)
+template <class T>
+__device__ __forceinline__ void gemm_encode_block(const NlGemm& g, const char* lds, int row, int half, long long m, long long k)      // half: which 32 of the 64 from k on
 {
     constexpr int DT = __is_same(T, _Float16) ? NL_DT_F16 : NL_DT_BF16;
     typedef __attribute__((__vector_size__(4))) unsigned short U2;
-    typedef GemmSide<false, BM, NT> Side;
+    if (m >= g.M || k + 32 * half >= g.ld8) return;
+    nl_i32x4 raw[4];
+    U2 top = {};
 #pragma unroll
-    for (int u = 0; u < (2 * BM + NT - 1) / NT; u++) {
-        const int at = u * NT + threadIdx.x, row = at >> 1;
-        if (row >= BM || m0 + row >= g.M || k + 32 * (at & 1) >= g.ld8) continue;
-        nl_i32x4 raw[4];
-        U2 top = {};
+    for (int q = 0; q < 4; q++) {
+        raw[q] = *reinterpret_cast<const nl_i32x4*>(lds + row * (GEMM_BK * 2) + ((4 * half + q) ^ (row & 7)) * 16);
+#pragma unroll
+        for (int j = 0; j < 4; j++) top = __builtin_elementwise_max(top, __builtin_bit_cast(U2, raw[q][j] & 0x7FFF7FFF));
+    }
+    const unsigned short most = top[0] > top[1] ? top[0] : top[1];
+    float amax = DT == NL_DT_BF16 ? nl_bf2f(most) : nl_h2f(most);
+    if (!(amax < INFINITY)) {
+        amax = 0.0f;
 #pragma unroll
         for (int q = 0; q < 4; q++) {
-            raw[q] = *reinterpret_cast<const nl_i32x4*>(lds + row * (GEMM_BK * 2) + ((4 * (at & 1) + q) ^ Side::swz_row(row)) * 16);
+            float v[8];
+            nl_unraw8<DT>(v, NlRaw8<DT>{{raw[q]}});
 #pragma unroll
-            for (int j = 0; j < 4; j++) top = __builtin_elementwise_max(top, __builtin_bit_cast(U2, raw[q][j] & 0x7FFF7FFF));
+            for (int j = 0; j < 8; j++) amax = fmaxf(amax, nl_finite_abs(v[j]));
         }
-        const unsigned short most = top[0] > top[1] ? top[0] : top[1];
-        float amax = DT == NL_DT_BF16 ? nl_bf2f(most) : nl_h2f(most);
-        if (!(amax < INFINITY)) {
-            amax = 0.0f;
+    }
+    const int e = nl_mx_exponent(amax);
+    const float s = nl_pow2(-e);
+    unsigned char* const to = g.A8 + m * g.ld8 + k + 32 * half;
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                float v[8];
-                nl_unraw8<DT>(v, NlRaw8<DT>{{raw[q]}});
+    for (int h = 0; h < 2; h++) {
+        float v[16];
+        nl_unraw8<DT>(v, NlRaw8<DT>{{raw[2 * h]}});
+        nl_unraw8<DT>(v + 8, NlRaw8<DT>{{raw[2 * h + 1]}});
+        nl_i32x4 w;
 #pragma unroll
-                for (int j = 0; j < 8; j++) amax = fmaxf(amax, nl_finite_abs(v[j]));
-            }
-        }
-        const int e = nl_mx_exponent(amax);
-        const float s = nl_pow2(-e);
-        unsigned char* const to = g.A8 + (m0 + row) * g.ld8 + k + 32 * (at & 1);
+        for (int j = 0; j < 4; j++) w[j] = (int)nl_mx_encode4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3], s);
+        *reinterpret_cast<nl_i32x4*>(to + 16 * h) = w;
+    }
+    g.A8e[m * (g.ld8 / 32) + (k >> 5) + half] = (unsigned char)(e + 127);
+}
+template <class T, int BM, int NT>
+__device__ __forceinline__ void gemm_encode(const NlGemm& g, const char* lds, long long m0, long long k)
+{
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            float v[16];
-            nl_unraw8<DT>(v, NlRaw8<DT>{{raw[2 * h]}});
-            nl_unraw8<DT>(v + 8, NlRaw8<DT>{{raw[2 * h + 1]}});
-            nl_i32x4 w;
-#pragma unroll
-            for (int j = 0; j < 4; j++) w[j] = (int)nl_mx_encode4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3], s);
-            *reinterpret_cast<nl_i32x4*>(to + 16 * h) = w;
-        }
-        g.A8e[(m0 + row) * (g.ld8 / 32) + ((k >> 5) + (at & 1))] = (unsigned char)(e + 127);
+    for (int u = 0; u < (2 * BM + NT - 1) / NT; u++) {
+        const int at = u * NT + threadIdx.x;
+        if (at < 2 * BM) gemm_encode_block<T>(g, lds, at >> 1, at & 1, m0 + (at >> 1), k);
     }
 }
 

@@ -1,7 +1,7 @@
 // nl_linear.hip -- one linear layer: z = x w^T + b, y = act(z) + r, and its backward pass (include/nerfloam_hip.h NlLinear).
 //
 // Reference behaviour: torch.nn.Linear + ReLU of the decoder (/root/reference/src/variations/lidar.py:105-123), any width, any depth.
-#include "nl_gemm.h"
+#include "nl_narrow.h"
 
 #include <math.h>
 
@@ -207,12 +207,6 @@ __global__ __launch_bounds__(256) void k_linear_join(const float* __restrict__ p
 // multiplies (OUT fp32 where nl_wide says so).  Bound by memory: 16384 x 4096 bf16 gelu 403 MB in 78 us, 65536 x 512 fp32 silu 403 MB in 79 us, 5.1 TB/s, what a large
 // copy reaches; hence one exponential and one reciprocal per element.
 // ---------------------------------------------------------------------------------------------
-struct NlDz {
-    const void* gy; const void* z; const unsigned* bits; const unsigned char* z8; const unsigned char* z8e;
-    void* dz; float* part;
-    long long M, ldgy, ldz, ldbits, ldz8, ldz8e, pitch, rows_per_chunk;
-    int N;
-};
 template <int DT, int ACT, int OUT>
 __global__ __launch_bounds__(256) void k_linear_dz(NlDz a)
 {
@@ -368,6 +362,21 @@ static void nl_product(NlWork& w, const NlPacked& A, const NlPacked& B, int layo
     if (hipGetLastError() != hipSuccess) w.rc = NL_ERR_LAUNCH;
 }
 
+// Many rows and a weight of at most 256 x 256 in 16 bits: the streaming product (STREAMNOTE)
+#define NL_STREAM_GROUPS 256
+static bool nl_streams(long long M, int K, int N, int dt) { return dt != NL_DT_F32 && M >= 32768 && K <= 256 && N <= 256 && (K > 64 || N > 64); }
+static void nl_stream(NlWork& w, const NlPacked& A, const NlPacked& B, bool b_slow, long long M, int N, int K, const NlEpilogue& ep, unsigned char* A8, unsigned char* A8e, const NlDz& z, int act, int dz)
+{
+    if (w.dry) return;
+    NlGemm g = {};
+    g.A = (const char*)A.p; g.B = (const char*)B.p; g.lda = 2 * A.pitch; g.ldb = 2 * B.pitch;
+    g.A8 = A8; g.A8e = A8e; g.ld8 = nl_up(K, NL_MX_BLOCK);
+    g.M = M; g.N = N; g.K = K; g.ep = ep;
+    if (ep.dt == NL_DT_BF16) nl_narrow_bf16(g, z, act, b_slow, dz, NL_STREAM_GROUPS, w.st);
+    else nl_narrow_f16(g, z, act, b_slow, dz, NL_STREAM_GROUPS, w.st);
+    if (hipGetLastError() != hipSuccess) w.rc = NL_ERR_LAUNCH;
+}
+
 static void nl_forward_run(const NlLinear* d, NlWork& w)
 {
     NlEpilogue ep = {};
@@ -388,7 +397,8 @@ static void nl_forward_run(const NlLinear* d, NlWork& w)
     }
     const NlPacked x = nl_packed(w, d->x, nullptr, d->M, d->K, d->ldx, d->dtype, d->dtype), wt = nl_packed(w, d->w, nullptr, d->N, d->K, d->ldw, d->dtype, d->dtype);
     nl_pack(w, d->dtype);
-    nl_product(w, x, wt, codes ? 4 : 0, d->M, d->N, d->K, ep, d->x8, d->x8e, nullptr, false);
+    if (nl_streams(d->M, d->K, d->N, d->dtype)) nl_stream(w, x, wt, false, d->M, d->N, d->K, ep, d->x8, d->x8e, NlDz{}, 0, 0);
+    else nl_product(w, x, wt, codes ? 4 : 0, d->M, d->N, d->K, ep, d->x8, d->x8e, nullptr, false);
 }
 
 // dz = gy act'(z) in 16 bits is a second rounding of half a step besides the gradients' own (1.41 times the error of one; with few results up to 1.9 times).  Where the
@@ -406,8 +416,11 @@ static void nl_backward_run(const NlLinear* d, NlWork& w)
     const bool products = d->gx || d->gw, wide = nl_wide(d);
     NlPacked dz = {d->gy, d->ldgy, nullptr};
     NlGb gb = {};
+    // the streaming data gradient makes dz on its way
+    const bool streams = d->gx && !wide && nl_streams(d->M, d->N, d->K, d->dtype) && nl_in_place(d->gy, d->N, d->ldgy, d->dtype) && (d->K & 7) == 0;
+    const int on_its_way = !streams || d->act == NL_ACT_NONE ? 0 : d->act == NL_ACT_RELU ? 1 : d->z8 ? 3 : 2;
+    NlDz a = {};
     if (d->gb || (products && !in_place)) {
-        NlDz a = {};
         a.gy = d->gy; a.ldgy = d->ldgy; a.M = d->M; a.N = d->N;
         if (d->act == NL_ACT_RELU) { a.bits = d->bits; a.ldbits = nl_up(d->N, 32) / 32; }
         else if (d->act != NL_ACT_NONE && d->z8) { a.z8 = d->z8; a.z8e = d->z8e; a.ldz8 = nl_up(d->N, 32); a.ldz8e = a.ldz8 / 32; }
@@ -417,14 +430,14 @@ static void nl_backward_run(const NlLinear* d, NlWork& w)
         chunks = chunks < 1 ? 1 : chunks > most ? most : chunks;
         if (chunks > 32768) chunks = 32768;
         a.rows_per_chunk = nl_up((d->M + chunks - 1) / chunks, 8);
-        chunks = (d->M + a.rows_per_chunk - 1) / a.rows_per_chunk;
+        chunks = on_its_way ? NL_STREAM_GROUPS : (d->M + a.rows_per_chunk - 1) / a.rows_per_chunk;
         if (d->gb) a.part = (float*)w.take(4LL * chunks * d->N);
-        if (products && !in_place) {
+        if (on_its_way ? d->gw != nullptr : products && !in_place) {
             a.pitch = nl_up(d->N, 8);
             a.dz = w.take(d->M * a.pitch * (wide ? 4 : nl_dtype_size(d->dtype)));
             dz = NlPacked{a.dz, a.pitch, nullptr};
         }
-        if (!w.dry) {
+        if (!w.dry && !on_its_way) {
             const dim3 grid(colblocks, (unsigned)chunks);
             NL_WITH_DTYPE(d->dtype, if (d->act == NL_ACT_NONE) hipLaunchKernelGGL((k_linear_dz<DT, NL_ACT_NONE, DT>), grid, dim3(256), 0, w.st, a);
                                     else if (d->act == NL_ACT_RELU) hipLaunchKernelGGL((k_linear_dz<DT, NL_ACT_RELU, DT>), grid, dim3(256), 0, w.st, a);
@@ -447,7 +460,8 @@ static void nl_backward_run(const NlLinear* d, NlWork& w)
     long long most = keep;
     if (d->gx) {
         ep.y = d->gx;
-        nl_product(w, dz, wt, 1, d->M, d->K, d->N, ep, nullptr, nullptr, nullptr, wide);
+        if (streams) nl_stream(w, NlPacked{d->gy, d->ldgy, nullptr}, wt, true, d->M, d->K, d->N, ep, nullptr, nullptr, a, d->act, on_its_way);
+        else nl_product(w, dz, wt, 1, d->M, d->K, d->N, ep, nullptr, nullptr, nullptr, wide);
         most = w.used;
         w.used = keep;                                               // (the second product follows on the stream: it takes the same place)
     }

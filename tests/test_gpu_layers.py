@@ -636,3 +636,53 @@ def test_small_backward_passes_do_not_round_dz(dtype, act, checkpoint):
         for got, want, e, name in ((gx, dz @ w.double(), e_dz @ Sw + _e(N, torch.float32) * (S @ Sw), "gx"),
                                    (gw, dz.t() @ xd, e_dz.t() @ xd.abs() + _e(M, torch.float32) * (S.t() @ xd.abs()), "gw")):
             _close(got, want, e + _half(want.abs() + e, dtype), f"{name} {M}x{N}x{K}")
+
+
+# many rows, a weight of at most 256 x 256: whole and partial last tiles and widths, rows that are not whole vectors, one output
+STREAM_SIZES = [(32768, 256, 256), (32801, 256, 256), (40007, 136, 72), (33000, 256, 16), (33001, 40, 200), (50000, 8, 256), (32769, 250, 136), (34000, 128, 128), (70001, 72, 8), (32800, 1, 100), (40000, 65, 33)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "silu"])
+def test_many_rows_narrow_layers_forward(dtype, act, monkeypatch):
+    monkeypatch.setitem(globals(), "SIZES", STREAM_SIZES)
+    test_forward_over_sizes(dtype, act)
+    if act == "gelu":
+        test_what_the_forward_pass_keeps(dtype)
+    if act == "none":
+        monkeypatch.setitem(globals(), "CODES_SIZES", [(M, K, N) for M, N, K in STREAM_SIZES])
+        test_forward_writes_the_codes_of_its_input(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "silu"])
+@pytest.mark.parametrize("checkpoint", [None, "mx8"])
+def test_many_rows_narrow_layers_backward(dtype, act, checkpoint):
+    for i, (M, N, K) in enumerate(STREAM_SIZES):
+        x, w, b, _ = _forward_case(M, N, K, dtype, act, 600 + i)
+        gy = _rand(_gen(700 + i), M, N, dtype=dtype)
+        nb = (N + 31) // 32
+        saved, x_values = {}, None
+        if act == "relu":
+            saved["bits"] = torch.randint(-2 ** 31, 2 ** 31 - 1, (M, nb), dtype=torch.int32, device="cuda", generator=_gen(i))
+            saved["on"] = ((saved["bits"].view(M, nb, 1) >> torch.arange(32, device="cuda", dtype=torch.int32)) & 1).bool().view(M, -1)[:, :N]
+        elif act != "none":
+            z = _rand(_gen(800 + i), M, N, dtype=dtype, std=2.0)
+            if checkpoint:
+                saved["z8"], saved["z8e"] = ops.mx8_encode(z)
+                saved["z_values"] = ops.mx8_decode(saved["z8"], saved["z8e"], N, torch.float32).double()
+            else:
+                saved["z"], saved["z_values"] = z, z.double()
+        if checkpoint:
+            saved["x8"], saved["x8e"] = ops.mx8_encode(x)
+            x_values = ops.mx8_decode(saved["x8"], saved["x8e"], K, torch.float32).double()
+        gx, gw, gb = _backward_check(gy, None if checkpoint else x, w, act, saved, dtype, f"{M}x{N}x{K}", x_values)
+        # each gradient alone, gy in rows of another pitch: the same bits where the sums have the same order
+        kw = {k: v for k, v in saved.items() if k in ("z", "bits", "z8", "z8e")}
+        alone = torch.empty_like(gx)
+        ops.linear_backward(gy, None, w, act, gx=alone, **kw)
+        assert torch.equal(alone, gx), (M, N, K)
+        wide = torch.zeros(M, N + 8, dtype=dtype, device="cuda")
+        wide[:, :N] = gy
+        ops.linear_backward(wide[:, :N], None, w, act, gx=alone.zero_(), **kw)
+        assert torch.equal(alone, gx), (M, N, K)
