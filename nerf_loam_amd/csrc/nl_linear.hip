@@ -362,9 +362,16 @@ static void nl_product(NlWork& w, const NlPacked& A, const NlPacked& B, int layo
     if (hipGetLastError() != hipSuccess) w.rc = NL_ERR_LAUNCH;
 }
 
-// Many rows and a weight of at most 256 x 256 in 16 bits: the streaming product (STREAMNOTE)
-#define NL_STREAM_GROUPS 256
-static bool nl_streams(long long M, int K, int N, int dt) { return dt != NL_DT_F32 && M >= 32768 && K <= 256 && N <= 256 && (K > 64 || N > 64); }
+// A weight of at most 256 x 256 in 16 bits: when the product streams (nl_narrow.h).  K: the contraction, N: the results' columns; dz: the data gradient that makes dz on
+// its way, which saves a pass and a launch.  Without dz it pays for wide results that do not stay in the caches (bf16, us, tiles / streaming: 262144 x 256 -> 256 relu 93 / 78,
+// 262144 x 16 -> 256 56 / 46, 65536 x 256 -> 256 22.6 / 24.0; 262144 x 256 -> 64 45 / 47, 262144 x 64 -> 64 17 / 39); with it everywhere (all gradients: 64 x 256 x 256
+// 13.0 / 12.1, 4096 x 256 x 256 17.5 / 16.9, 65536 x 256 x 256 57 / 46, 262144 x 256 x 64 123 / 103; only 262144 x 64 x 64 53 / 55).
+static int nl_stream_groups(long long M) { const long long tiles = (M + NL_NARROW_ROWS - 1) / NL_NARROW_ROWS; return tiles < 256 ? (int)tiles : 256; }      // one to a compute unit
+static bool nl_streams(long long M, int K, int N, int dt, bool dz)
+{
+    if (dt == NL_DT_F32 || K > 256 || N > 256) return false;
+    return dz || (M >= 65536 && N > 128);
+}
 static void nl_stream(NlWork& w, const NlPacked& A, const NlPacked& B, bool b_slow, long long M, int N, int K, const NlEpilogue& ep, unsigned char* A8, unsigned char* A8e, const NlDz& z, int act, int dz)
 {
     if (w.dry) return;
@@ -372,8 +379,8 @@ static void nl_stream(NlWork& w, const NlPacked& A, const NlPacked& B, bool b_sl
     g.A = (const char*)A.p; g.B = (const char*)B.p; g.lda = 2 * A.pitch; g.ldb = 2 * B.pitch;
     g.A8 = A8; g.A8e = A8e; g.ld8 = nl_up(K, NL_MX_BLOCK);
     g.M = M; g.N = N; g.K = K; g.ep = ep;
-    if (ep.dt == NL_DT_BF16) nl_narrow_bf16(g, z, act, b_slow, dz, NL_STREAM_GROUPS, w.st);
-    else nl_narrow_f16(g, z, act, b_slow, dz, NL_STREAM_GROUPS, w.st);
+    if (ep.dt == NL_DT_BF16) nl_narrow_bf16(g, z, act, b_slow, dz, (unsigned)nl_stream_groups(M), w.st);
+    else nl_narrow_f16(g, z, act, b_slow, dz, (unsigned)nl_stream_groups(M), w.st);
     if (hipGetLastError() != hipSuccess) w.rc = NL_ERR_LAUNCH;
 }
 
@@ -397,7 +404,7 @@ static void nl_forward_run(const NlLinear* d, NlWork& w)
     }
     const NlPacked x = nl_packed(w, d->x, nullptr, d->M, d->K, d->ldx, d->dtype, d->dtype), wt = nl_packed(w, d->w, nullptr, d->N, d->K, d->ldw, d->dtype, d->dtype);
     nl_pack(w, d->dtype);
-    if (nl_streams(d->M, d->K, d->N, d->dtype)) nl_stream(w, x, wt, false, d->M, d->N, d->K, ep, d->x8, d->x8e, NlDz{}, 0, 0);
+    if (nl_streams(d->M, d->K, d->N, d->dtype, false)) nl_stream(w, x, wt, false, d->M, d->N, d->K, ep, d->x8, d->x8e, NlDz{}, 0, 0);
     else nl_product(w, x, wt, codes ? 4 : 0, d->M, d->N, d->K, ep, d->x8, d->x8e, nullptr, false);
 }
 
@@ -417,7 +424,7 @@ static void nl_backward_run(const NlLinear* d, NlWork& w)
     NlPacked dz = {d->gy, d->ldgy, nullptr};
     NlGb gb = {};
     // the streaming data gradient makes dz on its way
-    const bool streams = d->gx && !wide && nl_streams(d->M, d->N, d->K, d->dtype) && nl_in_place(d->gy, d->N, d->ldgy, d->dtype) && (d->K & 7) == 0;
+    const bool streams = d->gx && !wide && nl_streams(d->M, d->N, d->K, d->dtype, d->act != NL_ACT_NONE) && nl_in_place(d->gy, d->N, d->ldgy, d->dtype) && (d->K & 7) == 0;
     const int on_its_way = !streams || d->act == NL_ACT_NONE ? 0 : d->act == NL_ACT_RELU ? 1 : d->z8 ? 3 : 2;
     NlDz a = {};
     if (d->gb || (products && !in_place)) {
@@ -430,7 +437,7 @@ static void nl_backward_run(const NlLinear* d, NlWork& w)
         chunks = chunks < 1 ? 1 : chunks > most ? most : chunks;
         if (chunks > 32768) chunks = 32768;
         a.rows_per_chunk = nl_up((d->M + chunks - 1) / chunks, 8);
-        chunks = on_its_way ? NL_STREAM_GROUPS : (d->M + a.rows_per_chunk - 1) / a.rows_per_chunk;
+        chunks = on_its_way ? nl_stream_groups(d->M) : (d->M + a.rows_per_chunk - 1) / a.rows_per_chunk;
         if (d->gb) a.part = (float*)w.take(4LL * chunks * d->N);
         if (on_its_way ? d->gw != nullptr : products && !in_place) {
             a.pitch = nl_up(d->N, 8);

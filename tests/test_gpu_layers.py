@@ -638,8 +638,8 @@ def test_small_backward_passes_do_not_round_dz(dtype, act, checkpoint):
             _close(got, want, e + _half(want.abs() + e, dtype), f"{name} {M}x{N}x{K}")
 
 
-# many rows, a weight of at most 256 x 256: whole and partial last tiles and widths, rows that are not whole vectors, one output
-STREAM_SIZES = [(32768, 256, 256), (32801, 256, 256), (40007, 136, 72), (33000, 256, 16), (33001, 40, 200), (50000, 8, 256), (32769, 250, 136), (34000, 128, 128), (70001, 72, 8), (32800, 1, 100), (40000, 65, 33)]
+# many rows (and few), a weight of at most 256 x 256: whole and partial last tiles and widths, rows that are not whole vectors, one output
+STREAM_SIZES = [(1, 8, 8), (31, 64, 64), (33, 256, 256), (700, 200, 120), (2000, 256, 256), (4100, 64, 64), (131075, 160, 24), (65536, 136, 256), (32768, 256, 256), (32801, 256, 256), (40007, 136, 72), (33000, 256, 16), (33001, 40, 200), (50000, 8, 256), (32769, 250, 136), (34000, 128, 128), (70001, 72, 8), (32800, 1, 100), (40000, 65, 33)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
