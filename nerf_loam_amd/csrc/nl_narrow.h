@@ -185,7 +185,8 @@ __global__ __launch_bounds__(1024) void k_narrow(NlGemm g, NlDz z, int act)
         z_fetch(first + G);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    constexpr int ZS = DZ == 0 ? 0 : DZ == 3 ? 2 : 1;                 // loads of z_fetch
+    constexpr int ZS = DZ == 3 ? 2 : 1;                               // loads of z_fetch
+    const bool fetches = __ballot(mine) != 0;
     for (int tile = first, i = 0;; tile += G, i++) {
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (DZ && tile + G < tiles) make_dz(tile + G, (i + 1) & 3);
@@ -209,9 +210,10 @@ __global__ __launch_bounds__(1024) void k_narrow(NlGemm g, NlDz z, int act)
             const int r = wm + 16 * f + (lane & 15), c = (wn / 4 + (lane >> 4)) ^ (r & 15);
             *reinterpret_cast<nl_f32x4*>(s_ex + (i & 1) * EX + r * (NW * 4) + c * 16) = acc[f];
         }
-        // loads of tile i + 2 and all before them have landed; in flight stay at most tile i + 3's and what this iteration fetched beside it
-        if (residual) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 + ZS) : "memory");
-        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(1 + ZS) : "memory");
+        // loads of tile i + 2 and all before them have landed; in flight stay at most tile i + 3's and what this iteration fetched beside it.  (A wave whose columns lie
+        // behind the contraction fetches nothing of z; one without results no residual, and then waits for tile i + 1's at least, which is what it needs.)
+        if (residual || (DZ && fetches)) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(DZ ? 1 + ZS : 2) : "memory");
+        else asm volatile("s_waitcnt vmcnt(1)" ::: "memory");
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");       // (all loads, the ones of zeros behind the last tile too)
     if (DZ && z.part) {
