@@ -14,7 +14,7 @@ struct NlGemm {
     const char* A; const char* B;      // 16-byte aligned, rows 16-byte aligned
     const unsigned char* Be;           // B in 8-bit codes: its powers of two, ldb / 32 bytes between rows
     unsigned char* A8; unsigned char* A8e;      // layout 4: where A's codes go, ld8 and ld8 / 32 bytes between rows
-    long long ld8;
+    long long ld8, plane;              // plane: bytes between the planes of a split B (0: B is fp32)
     long long lda, ldb;                // bytes between rows
     long long M, K;
     int N, tiles_m, tiles_n;
@@ -418,7 +418,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
 // The split happens on the way into LDS: no operand is written to memory a second time (split planes in memory: 262144 x 256 x 256 spends 118 us on writing and
 // 50 us more on reading them).  A thread fetches a step's elements into registers while the step before it multiplies, splits them and writes three planes; two
 // workgroups share a compute unit, so that one splits (vector unit) while the other multiplies.  Six products: at most a sixth of the bf16 rate, 246 TFLOP/s.
-// 4096^3: 671 us, 205 TFLOP/s (the library's fp32 product: 150); 262144 x 256 x 256: 226 us, 152 TFLOP/s (library 97) - eight steps per tile, whose loads and stores
+// 4096^3: 688 us, 200 TFLOP/s, 220 with B split beforehand (the library's fp32 product: 150); 262144 x 256 x 256: 226 us, 152 TFLOP/s (library 97) - eight steps per tile, whose loads and stores
 // (537 MB, 105 us) overlap only with the other workgroup's steps.  Starting the second workgroup of a unit later changes nothing.
 // ---------------------------------------------------------------------------------------------
 // two values to bf16, to nearest, in the halves of a word
@@ -566,9 +566,68 @@ __global__ __launch_bounds__(256, 2) void k_gemm_f32(NlGemm g)
     gemm_results<DT, BT / 2, BT / 2, 4, sizeof(s_mem)>(g, acc, s_mem, m0 + wm, n0 + wn, piece);
 }
 
+// The same with B already split, in three planes g.plane bytes apart (nl_linear.hip splits a weight once where many rows of tiles would split it again each): its planes go
+// straight into LDS, into two buffers in turn (arrays of their own, as in k_gemm), and only A passes through registers.  4096^3: 624 us, 220 TFLOP/s, 688 without.
+template <bool A_SLOW, bool B_SLOW, int BT>
+__global__ __launch_bounds__(256, 2) void k_gemm_f32_planes(NlGemm g)
+{
+    typedef GemmSide32<A_SLOW, BT, NL_DT_F32> SA;
+    typedef GemmSide<B_SLOW, BT, 256, 32> PB;
+    constexpr int F = BT / 32;
+    __shared__ __align__(256) char s_mem[SA::BYTES + 3 * PB::BYTES];
+    __shared__ __align__(256) char s_1[3 * PB::BYTES];
+    long long m0; int n0;
+    const unsigned piece = gemm_tile_of<BT, BT>(g, m0, n0);
+    const long long k0 = (long long)piece * g.kchunk, k1 = min(k0 + g.kchunk, g.K), span = k1 - k0;
+    const int steps = (int)((span + 31) / 32);
+    SA a; PB b;
+    a.init(g.A, g.lda, m0, g.M, k0);
+    b.init(g.B, g.ldb, n0, g.N, k0, g.K);
+    const int wave = threadIdx.x >> 6, wm = (wave >> 1) * (BT / 2), wn = (wave & 1) * (BT / 2);
+    nl_f32x4 acc[F][F] = {};
+    auto fetch = [&](int s, char* to) {
+        a.fetch(s * a.step, span - s * 32LL);
+#pragma unroll
+        for (int q = 0; q < 3; q++) b.load(to + q * PB::BYTES, s * b.step + q * g.plane, span - s * 32LL);
+    };
+    auto step = [&](int s, const char* buf, char* next) {
+        a.put(s_mem);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        nl_s16x8 fb[3][F];
+#pragma unroll
+        for (int p = 0; p < 3; p++)
+#pragma unroll
+            for (int j = 0; j < F; j++) fb[p][j] = PB::frag(buf + p * PB::BYTES, wn + 16 * j, 0);
+        if (s + 1 < steps) fetch(s + 1, next);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < F; i++) {
+            nl_s16x8 fa[3];
+#pragma unroll
+            for (int p = 0; p < 3; p++) fa[p] = SA::Plane::frag(s_mem + p * SA::Plane::BYTES, wm + 16 * i, 0);
+#pragma unroll
+            for (int sum = 2; sum >= 0; sum--)
+#pragma unroll
+                for (int p = sum; p >= 0; p--)
+#pragma unroll
+                    for (int j = 0; j < F; j++) acc[i][j] = NlMma<__bf16>::mma(fb[sum - p][j], fa[p], acc[i][j]);
+        }
+        nl_lds_barrier();
+    };
+    fetch(0, s_mem + SA::BYTES);
+    for (int s = 0; s < steps; s += 2) {
+        step(s, s_mem + SA::BYTES, s_1);
+        if (s + 1 < steps) step(s + 1, s_1, s_mem + SA::BYTES);
+    }
+    gemm_results<NL_DT_F32, BT / 2, BT / 2, 4, sizeof(s_mem)>(g, acc, s_mem, m0 + wm, n0 + wn, piece);
+}
+
 template <bool A_SLOW, bool B_SLOW>
 static void nl_gemm_tile_f32(const NlGemm& g, int tile, dim3 grid, hipStream_t st)
 {
+    if constexpr (!A_SLOW) {
+        if (g.plane) { hipLaunchKernelGGL((k_gemm_f32_planes<A_SLOW, B_SLOW, 128>), grid, dim3(256), 0, st, g); return; }
+    }
     if (tile == 1) hipLaunchKernelGGL((k_gemm_f32<A_SLOW, B_SLOW, 128, NL_DT_F32>), grid, dim3(256), 0, st, g);
     else hipLaunchKernelGGL((k_gemm_f32<A_SLOW, B_SLOW, 64, NL_DT_F32>), grid, dim3(256), 0, st, g);
 }

@@ -34,6 +34,23 @@ __global__ __launch_bounds__(256) void k_linear_pack(NlPack2 both)
     }
 }
 
+// A weight in three bf16 planes [3][rows][pitch] for k_gemm_f32_planes, zeros behind the last column (512 x 256: 4 us)
+__global__ __launch_bounds__(256) void k_linear_split(const float* src, long long ld, long long rows, int cols, unsigned short* dst, long long pitch)
+{
+    const long long per_row = pitch / 8, total = rows * per_row;
+    const bool vec = nl_rows_aligned<NL_DT_F32>(src, ld);
+    for (long long t = (long long)blockIdx.x * 256 + threadIdx.x; t < total; t += (long long)gridDim.x * 256) {
+        const long long r = t / per_row;
+        const int c = (int)(t - r * per_row) * 8;
+        float v[8];
+        nl_i32x4 p[3];
+        nl_load8<NL_DT_F32>(v, src, r * ld + c, cols - c, vec);
+        gemm_split8(v, p[0], p[1], p[2]);
+#pragma unroll
+        for (int q = 0; q < 3; q++) *reinterpret_cast<nl_i32x4*>(dst + (q * rows + r) * pitch + c) = p[q];
+    }
+}
+
 // ---------------------------------------------------------------------------------------------
 // k_linear_rows: at most ROWS_MOST rows of x (the call that answers single queries) or of the weight (a last layer with one output), nothing kept for a backward pass.
 // It reads the other operand once and computes little, so no tile: a group of `lanes` threads takes two rows of the many, eight neighbouring elements a thread at a
@@ -269,7 +286,7 @@ struct NlWork {
 };
 
 // a packed operand: rows `pitch` elements apart, zeros behind the last column up to a multiple of 8 (4 where an fp32 operand is used in place)
-struct NlPacked { const void* p; long long pitch; const unsigned char* e; };      // e: 8-bit codes and their powers of two instead
+struct NlPacked { const void* p; long long pitch; const unsigned char* e; long long plane; };      // e: 8-bit codes and their powers of two instead; plane: bytes between bf16 planes instead
 
 static unsigned nl_grid(long long threads) { const long long b = (threads + 255) / 256; return (unsigned)(b < 1 ? 1 : b < 16384 ? b : 16384); }
 
@@ -330,6 +347,18 @@ static NlCut nl_cut(long long M, long long N, long long K, int dt, int layout, i
     return best;
 }
 
+// The weight of an fp32 product, split beforehand where that saves more than it costs: every row of tiles splits it again otherwise (4096^3 688 -> 624 us, 65536 x 512 -> 256
+// 122 -> 113, 262144 x 256 -> 256 243 -> 236); the pass over the weight takes a launch, 5 us, and 10 bytes an element.  M, N, K: the product's; squares of 128 only
+static NlPacked nl_weight(NlWork& w, const NlLinear* d, long long M, int N, int K, int layout)
+{
+    if (d->dtype != NL_DT_F32 || M < 4096 || K < 512 || (double)M * N * K < 4e9 || nl_cut(M, N, K, NL_DT_F32, layout, 1).tile != 1)
+        return nl_packed(w, d->w, nullptr, d->N, d->K, d->ldw, d->dtype, d->dtype);
+    const long long pitch = nl_up(d->K, 8);
+    unsigned short* const to = (unsigned short*)w.take(6 * d->N * pitch);
+    if (!w.dry) hipLaunchKernelGGL(k_linear_split, dim3(nl_grid(d->N * (pitch / 8))), dim3(256), 0, w.st, (const float*)d->w, d->ldw, (long long)d->N, d->K, to, pitch);
+    return NlPacked{to, pitch, nullptr, 2 * d->N * pitch};
+}
+
 // C[M,N] = sum_k A(m,k) B(n,k), layouts as in nl_gemm.h.  A8, A8e: layout 4's codes.  gb: a bias gradient to sum in the same launch if there is one; then it is cleared.
 // wide: A is fp32 whatever the type
 static void nl_product(NlWork& w, const NlPacked& A, const NlPacked& B, int layout, long long M, int N, long long K, const NlEpilogue& ep, unsigned char* A8, unsigned char* A8e, NlGb* gb, bool wide)
@@ -338,6 +367,7 @@ static void nl_product(NlWork& w, const NlPacked& A, const NlPacked& B, int layo
     static const int size[3] = {256, 128, 64};
     NlGemm g = {};
     g.A = (const char*)A.p; g.B = (const char*)B.p; g.Be = B.e; g.lda = (wide ? 4 : nl_dtype_size(ep.dt)) * A.pitch; g.ldb = layout == 3 ? B.pitch : nl_dtype_size(ep.dt) * B.pitch;
+    if (B.plane) { g.plane = B.plane; g.ldb = 2 * B.pitch; }
     g.A8 = A8; g.A8e = A8e; g.ld8 = nl_up(K, NL_MX_BLOCK);
     g.M = M; g.N = N; g.K = K; g.kchunk = c.kchunk;
     const long long tm = nl_up(M, size[c.tile]) / size[c.tile], tn = nl_up(N, size[c.tile]) / size[c.tile];
@@ -402,7 +432,7 @@ static void nl_forward_run(const NlLinear* d, NlWork& w)
         if (!w.dry) NL_WITH_DTYPE(d->dtype, w.rc = d->M <= ROWS_MOST ? nl_launch_rows<DT, false>(d, ep, w.st) : nl_launch_rows<DT, true>(d, ep, w.st));
         return;
     }
-    const NlPacked x = nl_packed(w, d->x, nullptr, d->M, d->K, d->ldx, d->dtype, d->dtype), wt = nl_packed(w, d->w, nullptr, d->N, d->K, d->ldw, d->dtype, d->dtype);
+    const NlPacked x = nl_packed(w, d->x, nullptr, d->M, d->K, d->ldx, d->dtype, d->dtype), wt = nl_weight(w, d, d->M, d->N, d->K, 0);
     nl_pack(w, d->dtype);
     if (nl_streams(d->M, d->K, d->N, d->dtype, false)) nl_stream(w, x, wt, false, d->M, d->N, d->K, ep, d->x8, d->x8e, NlDz{}, 0, 0);
     else nl_product(w, x, wt, codes ? 4 : 0, d->M, d->N, d->K, ep, d->x8, d->x8e, nullptr, false);
@@ -459,7 +489,7 @@ static void nl_backward_run(const NlLinear* d, NlWork& w)
     ep.dt = d->dtype; ep.act = NL_ACT_NONE; ep.ldy = d->K;
     NlPacked wt = {}, x = {};
     const bool codes = d->gw && d->x8 && d->dtype != NL_DT_F32 && !wide;  // (fp32 arithmetic splits its operands: codes are decoded first)
-    if (d->gx) wt = nl_packed(w, d->w, nullptr, d->N, d->K, d->ldw, d->dtype, d->dtype);
+    if (d->gx) wt = nl_weight(w, d, d->M, d->K, d->N, 1);
     if (codes) x = NlPacked{d->x8, nl_up(d->K, 32), d->x8e};
     else if (d->gw) x = d->x8 ? nl_packed(w, d->x8, d->x8e, d->M, d->K, nl_up(d->K, 32), NL_DT_MX8, d->dtype) : nl_packed(w, d->x, nullptr, d->M, d->K, d->ldx, d->dtype, d->dtype);
     nl_pack(w, d->dtype);

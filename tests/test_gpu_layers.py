@@ -686,3 +686,24 @@ def test_many_rows_narrow_layers_backward(dtype, act, checkpoint):
         wide[:, :N] = gy
         ops.linear_backward(wide[:, :N], None, w, act, gx=alone.zero_(), **kw)
         assert torch.equal(alone, gx), (M, N, K)
+
+
+@pytest.mark.parametrize("M,N,K", [(16384, 512, 512), (8200, 520, 1001), (4100, 1000, 1030), (65536, 136, 520)])
+def test_large_fp32_products_with_a_weight_split_beforehand(M, N, K):
+    """against the formula with an fp32 product's tolerances; a weight in rows of another pitch gives the same bits; numbers that are not finite stay in their rows and columns"""
+    x, w, b, _ = _forward_case(M, N, K, torch.float32, "none", 31, residual=False)
+    y = ops.linear_forward(x, w, b)
+    _check_forward(x, w, b, None, "none", y, "y")
+    gy = _rand(_gen(32), M, N, dtype=torch.float32)
+    gx, _, _ = _backward_check(gy, x, w, "none", {}, torch.float32, "gradients")
+    wide = torch.zeros(N, K + 3, device="cuda")
+    wide[:, 1:K + 1] = w
+    assert torch.equal(ops.linear_forward(x, wide[:, 1:K + 1], b), y)
+    again = torch.empty_like(gx)
+    ops.linear_backward(gy, None, wide[:, 1:K + 1], gx=again)
+    assert torch.equal(again, gx)
+    w[3, 5], w[7, K - 1], x[11, 2] = float("nan"), float("inf"), float("nan")
+    y = ops.linear_forward(x, w, b)
+    bad = torch.zeros(M, N, dtype=torch.bool, device="cuda")
+    bad[:, 3] = bad[:, 7] = bad[11] = True
+    assert bool((torch.isfinite(y) == ~bad).all())
