@@ -9,7 +9,7 @@
 #pragma once
 #include "nl_gemm.h"
 
-// dz: how the rows of A become gy act'(z).  0: they are multiplied as they are; 1: z > 0 in bits; 2: z in the type; 3: z in 8-bit codes
+// dz: how the rows of A (of gy, b_slow) become gy act'(z).  0: they are multiplied as they are; 1: z > 0 in bits; 2: z in the type; 3: z in 8-bit codes.  With 0 the results have more than 128 columns
 #define NL_NARROW_ROWS 32
 void nl_narrow_bf16(const NlGemm& g, const NlDz& z, int act, bool b_slow, int dz, unsigned grid, hipStream_t st);
 void nl_narrow_f16(const NlGemm& g, const NlDz& z, int act, bool b_slow, int dz, unsigned grid, hipStream_t st);
@@ -234,12 +234,14 @@ __global__ __launch_bounds__(1024) void k_narrow(NlGemm g, NlDz z, int act)
 template <class T, int KS, int NW>
 static void nl_narrow_sized(const NlGemm& g, const NlDz& z, int act, bool b_slow, int dz, unsigned grid, hipStream_t st)
 {
-    if (!b_slow && g.A8) hipLaunchKernelGGL((k_narrow<T, KS, NW, false, true, 0>), dim3(grid), dim3(1024), 0, st, g, z, act);
-    else if (!b_slow) hipLaunchKernelGGL((k_narrow<T, KS, NW, false, false, 0>), dim3(grid), dim3(1024), 0, st, g, z, act);
-    else if (dz == 0) hipLaunchKernelGGL((k_narrow<T, KS, NW, true, false, 0>), dim3(grid), dim3(1024), 0, st, g, z, act);
-    else if (dz == 1) hipLaunchKernelGGL((k_narrow<T, KS, NW, true, false, 1>), dim3(grid), dim3(1024), 0, st, g, z, act);
+    if (dz == 1) hipLaunchKernelGGL((k_narrow<T, KS, NW, true, false, 1>), dim3(grid), dim3(1024), 0, st, g, z, act);
     else if (dz == 2) hipLaunchKernelGGL((k_narrow<T, KS, NW, true, false, 2>), dim3(grid), dim3(1024), 0, st, g, z, act);
-    else hipLaunchKernelGGL((k_narrow<T, KS, NW, true, false, 3>), dim3(grid), dim3(1024), 0, st, g, z, act);
+    else if (dz == 3) hipLaunchKernelGGL((k_narrow<T, KS, NW, true, false, 3>), dim3(grid), dim3(1024), 0, st, g, z, act);
+    else if constexpr (NW == 256) {                                   // (without dz only wide results come here)
+        if (b_slow) hipLaunchKernelGGL((k_narrow<T, KS, NW, true, false, 0>), dim3(grid), dim3(1024), 0, st, g, z, act);
+        else if (g.A8) hipLaunchKernelGGL((k_narrow<T, KS, NW, false, true, 0>), dim3(grid), dim3(1024), 0, st, g, z, act);
+        else hipLaunchKernelGGL((k_narrow<T, KS, NW, false, false, 0>), dim3(grid), dim3(1024), 0, st, g, z, act);
+    }
 }
 template <class T>
 static void nl_narrow_launch(const NlGemm& g, const NlDz& z, int act, bool b_slow, int dz, unsigned grid, hipStream_t st)
