@@ -7,7 +7,6 @@ template <int DT>
 __global__ __launch_bounds__(256) void k_mx8_encode(const void* __restrict__ x, long long ldx, long long M, int K, unsigned char* codes, unsigned char* exps, long long pitch)
 {
     const long long per_row = pitch / 8, total = M * per_row;
-    const bool row_aligned = nl_rows_aligned<DT>(x, ldx);
     // whole blocks of threads run every round: the four threads of a 32-block stay together
     for (long long t0 = (long long)blockIdx.x * 256; t0 < total; t0 += (long long)gridDim.x * 256) {
         const long long t = t0 + threadIdx.x;
@@ -16,7 +15,7 @@ __global__ __launch_bounds__(256) void k_mx8_encode(const void* __restrict__ x, 
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) v[j] = 0.0f;
-        if (t < total) nl_load8<DT>(v, x, m * ldx + k, K - k, row_aligned);
+        if (t < total) nl_load8<DT>(v, x, m * ldx + k, K - k);
         float amax = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; j++) amax = fmaxf(amax, nl_finite_abs(v[j]));
@@ -42,7 +41,7 @@ __global__ __launch_bounds__(256) void k_mx8_decode(const unsigned char* __restr
         const float s = nl_mx_scale(exps[m * (pitch / 32) + (k >> 5)]);
         const nl_f32x4 a = nl_mx_decode4((unsigned)c[0], s, nl_dtype_max(DT)), b = nl_mx_decode4((unsigned)c[1], s, nl_dtype_max(DT));
         const float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-        nl_store8<DT>(out, m * K + k, v, K - k, nl_rows_aligned<DT>(out, K));
+        nl_store8<DT>(out, m * K + k, v, K - k);
     }
 }
 

@@ -137,8 +137,7 @@ __device__ __forceinline__ void gemm_results(const NlGemm& g, nl_f32x4 (&acc)[WR
     const NlEpilogue& ep = g.ep;
     const int lane = threadIdx.x & 63, col = n + 8 * (lane % (WC / 8));
     char* const mine = s_mem + (threadIdx.x >> 6) * (RP * WC * 4);
-    const bool inside = m + WR <= g.M && n + WC <= g.N && (ep.part ? (g.N & 3) == 0 : nl_rows_aligned<DT>(ep.y, ep.ldy) && (!ep.r || nl_rows_aligned<DT>(ep.r, ep.ldr)) &&
-                                                           (!ep.b || nl_rows_aligned<DT>(ep.b, 0)) && (!ep.z || (ep.ldz & 7) == 0));
+    const bool inside = m + WR <= g.M && n + WC <= g.N;
     float bias[8] = {};
     if (inside && !ep.part && ep.b) nl_unraw8<DT>(bias, nl_raw8<DT>(ep.b, col));
 #pragma unroll

@@ -8,7 +8,7 @@
 // ---------------------------------------------------------------------------------------------
 // k_linear_pack: an operand as the tiled products want it - rows of up(cols, 8) elements with zeros behind the last column - from rows of any stride and
 // alignment, or from 8-bit codes (for fp32 arithmetic).  Runs only where the operand does not lie that way already
-// (1003 x 1001 and 777 x 1001 bf16, odd rows: 6 us in one launch, a quarter of it the launch; the product behind it 13 us).
+// (1003 x 1001 and 777 x 1001 bf16, odd rows: 4.9 us in one launch, the product behind it 10.3).
 // ---------------------------------------------------------------------------------------------
 struct NlPack { const void* src; const unsigned char* e; void* dst; long long rows, ld, pitch; int cols; };
 struct NlPack2 { NlPack p[2]; };                                     // one launch for both operands of a product, or both of a backward pass
@@ -18,7 +18,6 @@ __global__ __launch_bounds__(256) void k_linear_pack(NlPack2 both)
 {
     const NlPack a = both.p[blockIdx.y];
     const long long per_row = a.pitch / 8, total = a.rows * per_row;
-    const bool vec = nl_rows_aligned<DT>(a.src, a.ld);
     for (long long t = (long long)blockIdx.x * 256 + threadIdx.x; t < total; t += (long long)gridDim.x * 256) {
         const long long r = t / per_row;
         const int c = (int)(t - r * per_row) * 8;
@@ -29,8 +28,8 @@ __global__ __launch_bounds__(256) void k_linear_pack(NlPack2 both)
             const nl_f32x4 p = nl_mx_decode4((unsigned)w[0], s, nl_dtype_max(DT)), q = nl_mx_decode4((unsigned)w[1], s, nl_dtype_max(DT));
 #pragma unroll
             for (int j = 0; j < 4; j++) { v[j] = p[j]; v[4 + j] = q[j]; }
-        } else nl_load8<DT>(v, a.src, r * a.ld + c, a.cols - c, vec);
-        nl_store8<DT>(a.dst, r * a.pitch + c, v, 8, true);
+        } else nl_load8<DT>(v, a.src, r * a.ld + c, a.cols - c);
+        nl_store8<DT>(a.dst, r * a.pitch + c, v, 8);
     }
 }
 
@@ -38,13 +37,12 @@ __global__ __launch_bounds__(256) void k_linear_pack(NlPack2 both)
 __global__ __launch_bounds__(256) void k_linear_split(const float* src, long long ld, long long rows, int cols, unsigned short* dst, long long pitch)
 {
     const long long per_row = pitch / 8, total = rows * per_row;
-    const bool vec = nl_rows_aligned<NL_DT_F32>(src, ld);
     for (long long t = (long long)blockIdx.x * 256 + threadIdx.x; t < total; t += (long long)gridDim.x * 256) {
         const long long r = t / per_row;
         const int c = (int)(t - r * per_row) * 8;
         float v[8];
         nl_i32x4 p[3];
-        nl_load8<NL_DT_F32>(v, src, r * ld + c, cols - c, vec);
+        nl_load8<NL_DT_F32>(v, src, r * ld + c, cols - c);
         gemm_split8(v, p[0], p[1], p[2]);
 #pragma unroll
         for (int q = 0; q < 3; q++) *reinterpret_cast<nl_i32x4*>(dst + (q * rows + r) * pitch + c) = p[q];
@@ -67,43 +65,41 @@ __global__ __launch_bounds__(256) void k_linear_rows(NlRows g, NlEpilogue ep)
     const long long n0 = (nl_block() * (256 / lanes) + threadIdx.x / lanes) * R;
     if (n0 >= g.nmany) return;                                        // (a whole group)
     const long long n1 = n0 + 1 < g.nmany ? n0 + 1 : n0;
-    const bool vec = nl_rows_aligned<DT>(g.many, g.ldm) && nl_rows_aligned<DT>(g.few, g.ldf) && (K & 7) == 0;
     float acc[MR][R] = {};
     int k = lane * 8;
-    if (vec)
-        for (; k + (U - 1) * lanes * 8 < K; k += U * lanes * 8) {
-            NlRaw8<DT> a[U][R], b[U][MR];
+    for (; k + (U - 1) * lanes * 8 + 8 <= K; k += U * lanes * 8) {
+        NlRaw8<DT> a[U][R], b[U][MR];
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                a[u][0] = nl_raw8<DT>(g.many, n0 * g.ldm + k + u * lanes * 8);
-                a[u][1] = nl_raw8<DT>(g.many, n1 * g.ldm + k + u * lanes * 8);
+        for (int u = 0; u < U; u++) {
+            a[u][0] = nl_raw8<DT>(g.many, n0 * g.ldm + k + u * lanes * 8);
+            a[u][1] = nl_raw8<DT>(g.many, n1 * g.ldm + k + u * lanes * 8);
 #pragma unroll
-                for (int m = 0; m < MR; m++) b[u][m] = nl_raw8<DT>(g.few, (m < g.nfew ? m : 0) * g.ldf + k + u * lanes * 8);
-            }
+            for (int m = 0; m < MR; m++) b[u][m] = nl_raw8<DT>(g.few, (m < g.nfew ? m : 0) * g.ldf + k + u * lanes * 8);
+        }
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                float p[R][8];
-                nl_unraw8<DT>(p[0], a[u][0]);
-                nl_unraw8<DT>(p[1], a[u][1]);
+        for (int u = 0; u < U; u++) {
+            float p[R][8];
+            nl_unraw8<DT>(p[0], a[u][0]);
+            nl_unraw8<DT>(p[1], a[u][1]);
 #pragma unroll
-                for (int m = 0; m < MR; m++) {
-                    float q[8];
-                    nl_unraw8<DT>(q, b[u][m]);
+            for (int m = 0; m < MR; m++) {
+                float q[8];
+                nl_unraw8<DT>(q, b[u][m]);
 #pragma unroll
-                    for (int r = 0; r < R; r++)
+                for (int r = 0; r < R; r++)
 #pragma unroll
-                        for (int j = 0; j < 8; j++) acc[m][r] = __builtin_fmaf(p[r][j], q[j], acc[m][r]);
-                }
+                    for (int j = 0; j < 8; j++) acc[m][r] = __builtin_fmaf(p[r][j], q[j], acc[m][r]);
             }
         }
+    }
     for (; k < K; k += lanes * 8) {
         float p[R][8];
-        nl_load8<DT>(p[0], g.many, n0 * g.ldm + k, K - k, vec);
-        nl_load8<DT>(p[1], g.many, n1 * g.ldm + k, K - k, vec);
+        nl_load8<DT>(p[0], g.many, n0 * g.ldm + k, K - k);
+        nl_load8<DT>(p[1], g.many, n1 * g.ldm + k, K - k);
 #pragma unroll
         for (int m = 0; m < MR; m++) {
             float q[8];
-            nl_load8<DT>(q, g.few, (m < g.nfew ? m : 0) * g.ldf + k, K - k, vec);
+            nl_load8<DT>(q, g.few, (m < g.nfew ? m : 0) * g.ldf + k, K - k);
 #pragma unroll
             for (int r = 0; r < R; r++)
 #pragma unroll
@@ -230,13 +226,12 @@ __global__ __launch_bounds__(256) void k_linear_dz(NlDz a)
     __shared__ float s_sum[8][257];
     const int c8 = threadIdx.x & 31, n = blockIdx.x * 256 + 8 * c8, grp = threadIdx.x >> 5;
     const long long m1 = (blockIdx.y + 1) * a.rows_per_chunk < a.M ? (blockIdx.y + 1) * a.rows_per_chunk : a.M;
-    const bool vg = nl_rows_aligned<DT>(a.gy, a.ldgy), vz = nl_rows_aligned<DT>(a.z, a.ldz);
     constexpr float most = DT == NL_DT_F16 ? NL_F16_MAX : DT == NL_DT_BF16 ? 3.38953139e38f : 3.40282347e38f;
     float sum[8] = {};
     if (n < a.N)
         for (long long m = blockIdx.y * a.rows_per_chunk + grp; m < m1; m += 8) {
             float g[8], z[8];
-            nl_load8<DT>(g, a.gy, m * a.ldgy + n, a.N - n, vg);
+            nl_load8<DT>(g, a.gy, m * a.ldgy + n, a.N - n);
             if (ACT == NL_ACT_RELU) {
                 const unsigned w = a.bits[m * a.ldbits + (n >> 5)] >> (n & 31);
 #pragma unroll
@@ -248,13 +243,13 @@ __global__ __launch_bounds__(256) void k_linear_dz(NlDz a)
                     const nl_f32x4 p = nl_mx_decode4((unsigned)w[0], s, most), q = nl_mx_decode4((unsigned)w[1], s, most);
 #pragma unroll
                     for (int j = 0; j < 4; j++) { z[j] = p[j]; z[4 + j] = q[j]; }
-                } else nl_load8<DT>(z, a.z, m * a.ldz + n, a.N - n, vz);
+                } else nl_load8<DT>(z, a.z, m * a.ldz + n, a.N - n);
 #pragma unroll
                 for (int j = 0; j < 8; j++) g[j] = n + j < a.N ? g[j] * nl_act_slope(z[j], ACT) : 0.0f;
             }
 #pragma unroll
             for (int j = 0; j < 8; j++) sum[j] += g[j];
-            if (a.dz) nl_store8<OUT>(a.dz, m * a.pitch + n, g, 8, true);
+            if (a.dz) nl_store8<OUT>(a.dz, m * a.pitch + n, g, 8);
         }
     if (!a.part) return;
 #pragma unroll

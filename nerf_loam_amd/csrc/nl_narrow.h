@@ -154,7 +154,7 @@ __global__ __launch_bounds__(1024) void k_narrow(NlGemm g, NlDz z, int act)
     // ---- the results: a thread's eight columns of one row ----
     const NlEpilogue& ep = g.ep;
     const int orow = t / (NW / 8), col = 8 * (t % (NW / 8));
-    const bool leaves = t < EX / 32, whole = (g.N & 7) == 0 && nl_rows_aligned<DT>(ep.y, ep.ldy) && (!ep.r || nl_rows_aligned<DT>(ep.r, ep.ldr)) && (!ep.b || nl_rows_aligned<DT>(ep.b, 0));
+    const bool leaves = t < EX / 32, whole = (g.N & 7) == 0;
     const bool residual = !B_SLOW && whole && ep.r;                   // (a data gradient is stored as it is)
     NlRaw8<DT> bias = {}, res = {};
     if (!B_SLOW && whole && ep.b && col < g.N) bias = nl_raw8<DT>(ep.b, col);
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(1024) void k_narrow(NlGemm g, NlDz z, int act)
         const nl_f32x4 q = *reinterpret_cast<const nl_f32x4*>(from + ((col / 4 + 1) ^ (orow & 15)) * 16);
         float v[8] = {p[0], p[1], p[2], p[3], q[0], q[1], q[2], q[3]};
         if constexpr (B_SLOW) {
-            if (m < g.M && col < g.N) nl_store8<DT>(ep.y, m * ep.ldy + col, v, g.N - col, whole);
+            if (m < g.M && col < g.N) nl_store8<DT>(ep.y, m * ep.ldy + col, v, g.N - col);
         } else if (whole) {
             float b[8], x[8];
             nl_unraw8<DT>(b, bias);
