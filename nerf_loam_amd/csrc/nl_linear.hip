@@ -312,17 +312,18 @@ static NlPacked nl_packed(NlWork& w, const void* p, const unsigned char* e, long
 // How a product [M,N] over K is cut: the tile, and into how many pieces the contraction goes.  The estimate: rounds of as many workgroups as run at a time, each with
 // its contraction steps of 64 (alone on a compute unit / with as many neighbours as fit) and what surrounds them; for a cut contraction the pieces' way through memory
 // and the launch that joins them.  Measured, in microseconds (bf16, 4096^3: 95 in squares of 256, 105 of 128, 172 of 64; 2048 x 256 x 256: 14, 7.3, 4.4; 256 x 256 x
-// 200000: 56 in 256 pieces of the first, 46 in 128 of the second, 48 in 32 of the third, 4200 uncut; fp32 4096^3: 576 in squares of 128, 665 of 64, 2048 x 256 x 256:
-// 21, 9.8).  The estimate's choice is within 15 % of the best of all tiles and powers of two at the 23 shapes of either kind that these come from.
+// 200000: 56 in 256 pieces of the first, 46 in 128 of the second, 48 in 32 of the third, 4200 uncut; 8-bit codes, 256 x 256 x 200000 from memory: 73
+// in 64 pieces of the second, 52 in 128, 80 in squares of 64; fp32 4096^3: 576 in squares of 128, 665 of 64, 2048 x 256 x 256:
+// 21, 9.8).  The estimate's choice is within 17 % of the best of all tiles and powers of two at the 23 shapes of either kind that these come from, contractions above 4096 within 10 %.
 struct NlCut { int tile, splits; long long kchunk; };
 static NlCut nl_cut(long long M, long long N, long long K, int dt, int layout, int largest)
 {
-    struct Tile { int size, at_a_time; double alone, full, rest, slow; };       // slow: on the steps where both operands' rows are the contraction (narrow rows of a tile)
-    static const Tile T16[3] = {{256, 256, 1.33, 1.40, 9.0, 1.0}, {128, 512, 0.70, 0.87, 4.0, 1.0}, {64, 1024, 0.50, 0.67, 2.0, 1.0}};
-    static const Tile T32[3] = {{256, 0, 0, 0, 0, 0}, {128, 512, 3.95, 4.50, 4.0, 1.0}, {64, 1024, 1.67, 2.60, 2.5, 1.1}};
+    struct Tile { int size, at_a_time; double alone, full, rest, codes; };      // codes: on the steps of layout 3 (a thread decodes as much, the tile multiplies less)
+    static const Tile T16[3] = {{256, 256, 1.33, 1.40, 9.0, 1.0}, {128, 512, 0.70, 0.87, 4.0, 1.0}, {64, 1024, 0.50, 0.67, 2.0, 1.6}};
+    static const Tile T32[3] = {{256, 0, 0, 0, 0, 0}, {128, 512, 3.95, 4.50, 4.0, 1.0}, {64, 1024, 1.67, 2.60, 2.5, 1.0}};
     const Tile* T = dt == NL_DT_F32 ? T32 : T16;
     const long long ksteps = (K + GEMM_BK - 1) / GEMM_BK;
-    const double memory = (double)nl_dtype_size(dt) * (M * K + N * K + M * N) / 4.5e6;
+    const double memory = ((double)nl_dtype_size(dt) * (M * K + M * N) + (layout == 3 ? 1.0 : nl_dtype_size(dt)) * N * K) / 4.5e6;
     NlCut best = {2, 1, ksteps * GEMM_BK};
     double least = 1e300;
     for (int t = largest; t < 3; t++) {
@@ -331,10 +332,12 @@ static NlCut nl_cut(long long M, long long N, long long K, int dt, int layout, i
             if (s > 1 && 4.0 * s * M * N > 1.5e9) break;
             const long long per = (ksteps + s - 1) / s;
             const double at = tiles * s / T[t].at_a_time, full = at < 1.0 ? at : 1.0, rounds = at < 1.0 ? 1.0 : at < 4.0 ? ceil(at) : at + 0.5;
-            const double alone = t == 2 && dt != NL_DT_F32 && layout < 3 && tiles * s <= NL_GEMM_FEW_SQUARES ? 0.28 : T[t].alone;      // (four buffers)
-            double us = rounds * (per * (alone + (T[t].full - alone) * full) * (layout == 2 || layout == 3 ? T[t].slow : 1.0) + T[t].rest * (0.5 + 0.5 * full));
-            if (us < memory) us = memory;
-            if (s > 1) us += 3.0 + 8.0 * s * M * N / 4.0e6;
+            const bool ring = t == 2 && dt != NL_DT_F32 && layout < 3 && tiles * s <= NL_GEMM_FEW_SQUARES;      // (four buffers)
+            // two buffers: one workgroup to a compute unit draws half of the bandwidth (of squares of 256 all of it)
+            const double alone = ring ? 0.28 : T[t].alone, draws = tiles * s / (t == 0 ? 256 : 512), reach = ring || draws > 1.0 ? 1.0 : draws;
+            double us = rounds * (per * (alone + (T[t].full - alone) * full) * (layout == 3 ? T[t].codes : 1.0) + T[t].rest * (0.5 + 0.5 * full));
+            if (us < memory / reach) us = memory / reach;
+            if (s > 1) us += 5.0 + 4.0 * s * M * N / 4.0e6;
             if (us < least) { least = us; best = NlCut{t, s, per * GEMM_BK}; }
         }
     }
