@@ -78,14 +78,12 @@ Tensor workspace(int64_t need, const Tensor& like, const char* what)
     if (need < 0) fail(cat(what, " failed: invalid argument"));
     return need == 0 ? Tensor() : at::empty({need}, like.options().dtype(at::kByte));
 }
-// gradients that a later backward pass would need are not provided: the error comes when somebody asks for them
-void once_differentiable(torch::autograd::variable_list& out, bool differentiable)
+// Gradients of gradients are not provided: a gradient that depends on a tensor somebody differentiates by (`depends`) carries an error that comes when it is
+// differentiated itself; one that does not is a constant
+void once_differentiable(Tensor& t, bool depends)
 {
-    if (!at::GradMode::is_enabled() || !differentiable) return;
-    auto err = std::make_shared<torch::autograd::DelayedError>("gradients of gradients of the layer operators are not provided", (int64_t)out.size());
-    torch::autograd::variable_list in;
-    for (auto& t : out) in.push_back(t.defined() ? t.detach().requires_grad_(true) : t);
-    out = (*err)(std::move(in));
+    if (!at::GradMode::is_enabled() || !t.defined() || !depends) return;
+    t = (*std::make_shared<torch::autograd::DelayedError>("gradients of gradients of the layer operators are not provided", 1))({t.detach().requires_grad_(true)})[0];
 }
 
 struct Kept { Tensor z, bits, z8, z8e, x8, x8e; };
@@ -166,7 +164,11 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
             d.ws = ptr(ws); d.ws_bytes = ws.defined() ? ws.numel() : 0;
             check(f_backward(&d, stream_of(g2)), "nl_linear_backward");
         }
-        once_differentiable(out, g.requires_grad() || w.requires_grad() || (saved[0].defined() && saved[0].requires_grad()));
+        // gx = dz w, gw = dz^T x, gb = sum of dz with dz = gy act'(x w^T + b); act' of none and relu is constant almost everywhere
+        const bool dz = g.requires_grad() || ((c[0] == NL_ACT_GELU || c[0] == NL_ACT_SILU) && (c[1] || c[2] || c[3]));
+        once_differentiable(out[0], dz || c[2]);
+        once_differentiable(out[1], dz || c[1]);
+        once_differentiable(out[2], dz);
         if (gr) out[3] = g;
         return out;
     }
@@ -257,7 +259,8 @@ struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
             check(f_emb_backward(ptr(table), table.size(0), (int)table.size(1), dtype_of(table, "table"), ptr(ids), ids.scalar_type() == at::kLong, (const float*)ptr(w), ids.size(0), (int)ids.size(1),
                                  (float)ctx->saved_data["scale"].toDouble(), ptr(g), ptr(out[0]), (float*)ptr(out[2]), ptr(ws), ws.defined() ? ws.numel() : 0, stream_of(table)), "nl_embedding_backward");
         }
-        once_differentiable(out, grads[0].requires_grad() || (w.defined() && (w.requires_grad() || table.requires_grad())));
+        once_differentiable(out[0], grads[0].requires_grad() || c[1]);        // sums of w g
+        once_differentiable(out[2], grads[0].requires_grad() || c[0]);        // <g, table>
         return out;
     }
 };
