@@ -57,6 +57,13 @@ void same_kind(const Tensor& t, const Tensor& like, const char* name)
         fail(cat(name, " must be ", like.scalar_type(), " on ", like.device(), ", got ", t.scalar_type(), " on ", t.device()));
 }
 void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+// a result would come without the tangent, and nobody would notice
+void no_tangent(const char* what, std::initializer_list<const Tensor*> in)
+{
+    for (const Tensor* t : in)
+        if (t && t->defined() && t->_fw_grad(0).defined()) fail(cat(what, ": forward-mode derivatives are not provided"));
+}
+const Tensor* opt(const OptTensor& t) { return t ? &*t : nullptr; }
 void no_capture(const char* what)
 {
     if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
@@ -176,6 +183,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
 
 Tensor linear_act(const Tensor& x, const Tensor& weight, const OptTensor& bias, int64_t act, const OptTensor& residual, bool mx8)
 {
+    no_tangent("linear_act", {&x, &weight, opt(bias), opt(residual)});
     on_gpu(x, "linear_act");
     if (weight.dim() != 2 || x.dim() < 1 || x.size(-1) != weight.size(1)) throw py::value_error(cat("linear_act: x ", x.sizes(), " must be [..., K] and weight ", weight.sizes(), " [N, K]"));
     const int64_t K = weight.size(1), N = weight.size(0);
@@ -267,6 +275,7 @@ struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
 
 Tensor embedding_lookup(const Tensor& table, const Tensor& ids, double scale, const OptTensor& weights)
 {
+    no_tangent("embedding_lookup", {&table, opt(weights)});
     on_gpu(table, "embedding_lookup");
     if (table.dim() != 2) throw py::value_error(cat("embedding_lookup: table ", table.sizes(), " must be [V, D]"));
     if (weights && (weights->sizes() != ids.sizes() || ids.dim() < 1 || ids.size(-1) < 1))

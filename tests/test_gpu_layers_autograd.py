@@ -4,6 +4,7 @@ import itertools
 import pytest
 import torch
 
+from nerf_loam_amd import _lib as L
 from nerf_loam_amd import layers
 
 pytestmark = pytest.mark.gpu
@@ -79,3 +80,23 @@ def test_an_embedding_gradient_that_depends_on_a_trained_tensor_is_no_constant()
     table = torch.randn(30, 8, device="cuda", requires_grad=True)
     y = layers.embedding_lookup(table, torch.randint(0, 30, (20,), device="cuda"))
     assert not torch.autograd.grad(y.sum(), table, create_graph=True)[0].requires_grad
+
+
+def test_tangents_and_function_transforms_are_refused():
+    """on the device as on the host (tests/test_layers_autograd_host.py); a transform's tensors have no memory to read"""
+    import torch.autograd.forward_ad as fw
+    x, w, table = torch.randn(6, 8, device="cuda"), torch.randn(4, 8, device="cuda"), torch.randn(9, 8, device="cuda")
+    ids = torch.zeros(6, dtype=torch.int64, device="cuda")
+    for quiet in (False, True):
+        with fw.dual_level(), torch.set_grad_enabled(not quiet):
+            for a in ((fw.make_dual(x, x), w), (x, fw.make_dual(w, w)), (fw.make_dual(x.requires_grad_(not quiet), x.detach()), w)):
+                with pytest.raises(L.NerfLoamHipError, match="forward-mode"):
+                    layers.linear_act(*a)
+            with pytest.raises(L.NerfLoamHipError, match="forward-mode"):
+                layers.embedding_lookup(fw.make_dual(table, table), ids)
+    x = x.detach()
+    for call in (lambda: torch.func.grad(lambda t: layers.linear_act(t, w).sum())(x), lambda: torch.func.jvp(lambda t: layers.linear_act(t, w), (x,), (x,)),
+                 lambda: torch.func.vmap(lambda t: layers.linear_act(t, w))(x[None]), lambda: torch.func.grad(lambda t: layers.embedding_lookup(t, ids).sum())(table)):
+        with pytest.raises(RuntimeError):
+            call()
+    assert torch.equal(layers.linear_act(x, w), layers.linear_act(x, w))

@@ -1,0 +1,28 @@
+"""CPU: what the layer operators refuse to derive: forward-mode derivatives, before anything else is asked of the tensors"""
+import pytest
+import torch
+import torch.autograd.forward_ad as fw
+
+from nerf_loam_amd import _lib as L
+from nerf_loam_amd import layers
+
+
+@pytest.mark.parametrize("grad_mode", [True, False])
+@pytest.mark.parametrize("which", ["x", "weight", "bias", "residual"])
+def test_linear_act_refuses_a_tangent(which, grad_mode):
+    t = dict(x=torch.randn(4, 8), weight=torch.randn(3, 8), bias=torch.randn(3), residual=torch.randn(4, 3))
+    with fw.dual_level(), torch.set_grad_enabled(grad_mode):
+        t[which] = fw.make_dual(t[which], torch.ones_like(t[which]))
+        with pytest.raises(L.NerfLoamHipError, match="forward-mode"):
+            layers.linear_act(**t)
+
+
+@pytest.mark.parametrize("which", ["table", "weights"])
+def test_embedding_lookup_refuses_a_tangent(which):
+    t = dict(table=torch.randn(5, 8), ids=torch.zeros(2, 3, dtype=torch.int64), weights=torch.rand(2, 3))
+    with fw.dual_level():
+        t[which] = fw.make_dual(t[which], torch.ones_like(t[which]))
+        with pytest.raises(L.NerfLoamHipError, match="forward-mode"):
+            layers.embedding_lookup(**t)
+    with fw.dual_level(), pytest.raises(L.NerfLoamHipError, match="no CPU path"):       # a plain tensor inside a level is as ever
+        layers.embedding_lookup(torch.randn(5, 8), t["ids"])
