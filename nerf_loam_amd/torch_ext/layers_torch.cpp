@@ -139,8 +139,9 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
         const bool gx = x.requires_grad(), gw = w.requires_grad(), gb = b && b->requires_grad(), gr = r && r->requires_grad();
         Kept kept;
         Tensor y = linear_forward(x, w, b ? *b : Tensor(), r ? *r : Tensor(), (int)act, mx8, gx || gw || gb, gw, &kept);
-        ctx->save_for_backward({gw && !mx8 ? x : Tensor(), w, kept.x8, kept.x8e, kept.z, kept.bits, kept.z8, kept.z8e});
-        ctx->saved_data["c"] = std::vector<int64_t>{act, gx, gw, gb, gr, b.has_value(), r.has_value()};
+        // only what a gradient holds: what is not saved may be written before the backward pass
+        ctx->save_for_backward({gw && !mx8 ? x : Tensor(), gx ? w : Tensor(), kept.x8, kept.x8e, kept.z, kept.bits, kept.z8, kept.z8e});
+        ctx->saved_data["c"] = std::vector<int64_t>{act, gx, gw, gb, gr, b.has_value(), r.has_value(), w.size(0), w.size(1)};
         return y;
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads)
@@ -153,8 +154,9 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
         if (!g.defined()) return out;
         // edges: x, w, then bias and residual where given
         const bool gx = c[1] && ctx->needs_input_grad(0), gw = c[2] && ctx->needs_input_grad(1), gb = c[3] && ctx->needs_input_grad(2), gr = c[4] && ctx->needs_input_grad(2 + c[5]);
-        const Tensor g2 = rows2d(g, w.size(0));
-        const int64_t M = g2.size(0), N = w.size(0), K = w.size(1);
+        const int64_t N = c[7], K = c[8];
+        const Tensor g2 = rows2d(g, N);
+        const int64_t M = g2.size(0);
         if (gx || gw || gb) {
             c10::DeviceGuard guard(g.device());
             if (gx) out[0] = at::empty({M, K}, g.options());
@@ -162,7 +164,8 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
             if (gb) out[2] = at::empty({N}, g.options());
             NlLinear d = {};
             d.struct_size = (int)sizeof d; d.dtype = dtype_of(g2, "gy"); d.act = (int)c[0]; d.M = M; d.K = (int)K; d.N = (int)N;
-            d.gy = ptr(g2); d.ldgy = row_stride(g2); d.w = ptr(w); d.ldw = row_stride(w);
+            d.gy = ptr(g2); d.ldgy = row_stride(g2);
+            if (w.defined()) { d.w = ptr(w); d.ldw = row_stride(w); }
             if (saved[0].defined()) { d.x = ptr(saved[0]); d.ldx = row_stride(saved[0]); }
             d.x8 = (unsigned char*)ptr(saved[2]); d.x8e = (unsigned char*)ptr(saved[3]);
             d.z = ptr(saved[4]); d.bits = (unsigned*)ptr(saved[5]); d.z8 = (unsigned char*)ptr(saved[6]); d.z8e = (unsigned char*)ptr(saved[7]);
@@ -245,9 +248,11 @@ Tensor emb_forward(const Tensor& table, const Tensor& ids, const Tensor& w, doub
 struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& table, const Tensor& ids, const OptTensor& w, double scale)
     {
-        ctx->save_for_backward({table, ids, w ? *w : Tensor()});
+        const bool gt = table.requires_grad(), gw = w && w->requires_grad();
+        // g_table holds the weights, g_weights the table: what is not saved may be written before the backward pass
+        ctx->save_for_backward({gw ? table : Tensor(), ids, gt && w ? *w : Tensor()});
         ctx->saved_data["scale"] = scale;
-        ctx->saved_data["c"] = std::vector<int64_t>{table.requires_grad(), w && w->requires_grad()};
+        ctx->saved_data["c"] = std::vector<int64_t>{gt, gw, table.size(0), table.size(1)};
         return emb_forward(table, ids, w ? *w : Tensor(), scale);
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads)
@@ -259,13 +264,14 @@ struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
         torch::autograd::variable_list out(4);
         if (!grads[0].defined()) return out;
         const Tensor g = grads[0].contiguous();
-        c10::DeviceGuard guard(table.device());
-        if (c[0] && ctx->needs_input_grad(0)) out[0] = at::empty(table.sizes(), table.options());
-        if (c[1] && ctx->needs_input_grad(2)) out[2] = at::empty(w.sizes(), w.options());
+        c10::DeviceGuard guard(g.device());
+        const int64_t V = c[2], D = c[3];
+        if (c[0] && ctx->needs_input_grad(0)) out[0] = at::empty({V, D}, g.options());
+        if (c[1] && ctx->needs_input_grad(2)) out[2] = at::empty(ids.sizes(), g.options().dtype(at::kFloat));
         if (out[0].defined() || out[2].defined()) {
-            const Tensor ws = workspace(out[0].defined() ? f_emb_workspace(table.size(0), (int)table.size(1), ids.size(0), (int)ids.size(1)) : 0, table, "nl_embedding_backward");
-            check(f_emb_backward(ptr(table), table.size(0), (int)table.size(1), dtype_of(table, "table"), ptr(ids), ids.scalar_type() == at::kLong, (const float*)ptr(w), ids.size(0), (int)ids.size(1),
-                                 (float)ctx->saved_data["scale"].toDouble(), ptr(g), ptr(out[0]), (float*)ptr(out[2]), ptr(ws), ws.defined() ? ws.numel() : 0, stream_of(table)), "nl_embedding_backward");
+            const Tensor ws = workspace(out[0].defined() ? f_emb_workspace(V, (int)D, ids.size(0), (int)ids.size(1)) : 0, g, "nl_embedding_backward");
+            check(f_emb_backward(ptr(table), V, (int)D, dtype_of(g, "g"), ptr(ids), ids.scalar_type() == at::kLong, (const float*)ptr(w), ids.size(0), (int)ids.size(1),
+                                 (float)ctx->saved_data["scale"].toDouble(), ptr(g), ptr(out[0]), (float*)ptr(out[2]), ptr(ws), ws.defined() ? ws.numel() : 0, stream_of(g)), "nl_embedding_backward");
         }
         once_differentiable(out[0], grads[0].requires_grad() || c[1]);        // sums of w g
         once_differentiable(out[2], grads[0].requires_grad() || c[0]);        // <g, table>

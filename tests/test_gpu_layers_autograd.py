@@ -100,3 +100,51 @@ def test_tangents_and_function_transforms_are_refused():
         with pytest.raises(RuntimeError):
             call()
     assert torch.equal(layers.linear_act(x, w), layers.linear_act(x, w))
+
+
+@pytest.mark.parametrize("bag", [1, 4])
+def test_a_table_may_change_before_its_gradient_is_taken(bag):
+    """the table's gradient does not hold its values: an update in place between the passes changes nothing, unless the weights' gradient needs them"""
+    table = torch.randn(50, 12, device="cuda", requires_grad=True)
+    ids = torch.randint(-1, 50, (30, bag) if bag > 1 else (30,), device="cuda")
+    wt = torch.rand(30, bag, device="cuda") if bag > 1 else None
+    g = torch.randn(30, 12, device="cuda")
+    want, = torch.autograd.grad(layers.embedding_lookup(table, ids, weights=wt), table, g)
+    y = layers.embedding_lookup(table, ids, weights=wt)
+    with torch.no_grad():
+        table.mul_(2.0)
+    assert torch.equal(torch.autograd.grad(y, table, g)[0], want)
+    if bag > 1:
+        wt.requires_grad_(True)
+        y = layers.embedding_lookup(table, ids, weights=wt)
+        with torch.no_grad():
+            table.mul_(2.0)
+        with pytest.raises(RuntimeError, match="inplace operation"):
+            torch.autograd.grad(y, [table, wt], g)
+        # the weights' own values count in the table's gradient alone
+        y = layers.embedding_lookup(table.detach(), ids, weights=wt)
+        want, = torch.autograd.grad(y, wt, g, retain_graph=True)
+        with torch.no_grad():
+            wt.add_(1.0)
+        assert torch.equal(torch.autograd.grad(y, wt, g)[0], want)
+
+
+@pytest.mark.parametrize("checkpoint", [None, "mx8"])
+@pytest.mark.parametrize("act", ["none", "relu", "gelu"])
+def test_a_weight_may_change_where_the_gradients_do_not_hold_it(act, checkpoint):
+    """gw = dz^T x and gb = sum of dz do not hold w; gx = dz w does"""
+    x, w, b = torch.randn(33, 20, device="cuda"), torch.randn(9, 20, device="cuda", requires_grad=True), torch.randn(9, device="cuda", requires_grad=True)
+    gy = torch.randn(33, 9, device="cuda")
+    want = torch.autograd.grad(layers.linear_act(x, w, b, act=act, checkpoint=checkpoint), [w, b], gy)
+    y = layers.linear_act(x, w, b, act=act, checkpoint=checkpoint)
+    with torch.no_grad():
+        w.mul_(3.0)
+        b.add_(1.0)
+    got = torch.autograd.grad(y, [w, b], gy)
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+    x.requires_grad_(True)
+    y = layers.linear_act(x, w, b, act=act, checkpoint=checkpoint)
+    with torch.no_grad():
+        w.mul_(3.0)
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        torch.autograd.grad(y, [x, w, b], gy)
