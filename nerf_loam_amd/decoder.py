@@ -40,6 +40,8 @@ class _FusedValues(torch.autograd.Function):
 
 
 class Decoder(nn.Module):
+    fused, checkpoint = True, None              # of a module that was pickled whole when there was one configuration
+
     def __init__(self, depth=2, width=256, in_dim=16, sdf_dim=128, skips=(), multires=0, embedder="none", point_dim=3,
                  local_coord=False, checkpoint=None, **kwargs):
         super().__init__()

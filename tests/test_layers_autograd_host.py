@@ -1,4 +1,4 @@
-"""CPU: what the layer operators refuse to derive: forward-mode derivatives, before anything else is asked of the tensors"""
+"""CPU: what the layer operators refuse to derive - forward-mode derivatives, before anything else is asked of the tensors -, and modules of an earlier version"""
 import pytest
 import torch
 import torch.autograd.forward_ad as fw
@@ -26,3 +26,19 @@ def test_embedding_lookup_refuses_a_tangent(which):
             layers.embedding_lookup(**t)
     with fw.dual_level(), pytest.raises(L.NerfLoamHipError, match="no CPU path"):       # a plain tensor inside a level is as ever
         layers.embedding_lookup(torch.randn(5, 8), t["ids"])
+
+
+def test_a_module_pickled_before_it_had_a_choice_is_the_one_configuration():
+    import io
+
+    from nerf_loam_amd.decoder import Decoder
+    old = Decoder()
+    for name in ("fused", "checkpoint"):                     # the attributes of a choice that it did not have
+        del old.__dict__[name]
+    f = io.BytesIO()
+    torch.save(old, f)
+    f.seek(0)
+    new = torch.load(f, weights_only=False)                  # (a file of this test's own)
+    assert new.fused and new.checkpoint is None and len(new.param_list()) == 6
+    with pytest.raises(L.NerfLoamHipError, match="no CPU path"):
+        new(torch.zeros(2, 16))
