@@ -566,8 +566,9 @@ int nl_dist_rows_union_prefix(const int* gathered, int stride_ints, int offset_i
  * nl_linear_backward reads gy, w (for gx), x or x8 / x8e (for gw), what the forward pass kept of z, and writes gx [M,K], gw [N,K], gb [N], each where its
  * pointer is set, in dtype.  dz = gy act'(z) is rounded to dtype once for the two products (not at all in fp32, and for gelu and silu while
  * M N K <= 2^23, which run as fp32 products); gb sums the unrounded values.
- * fp32 products run as six bf16 products of the exact three-term splits of both operands (dropped terms below 2^-26 of |x||w|); an infinity among the
- * operands gives NaN there.  Sums are fp32 and their order depends on the sizes only.  M = 0 is a legal call (gw, gb = 0).
+ * fp32 products run as six bf16 products of the three-term splits of both operands: exact for magnitudes from 2^-110 on (7.7e-34), below that an operand is off by
+ * at most 2^-134; dropped terms are below 2^-26 of |x||w|.  An infinity among the operands gives NaN there.  Forward products with at most eight rows of x or of w
+ * that keep nothing of z do not split: they multiply in fp32, and an infinity stays one.  Sums are fp32 and their order depends on the sizes only.  M = 0 is a legal call (gw, gb = 0).
  * Taken are at most 2^30 rows, 2^22 columns, and results of fewer than 2^24 tiles (of 64 x 64 where they are small).
  * A decoded value of x8 / x8e beyond dtype's largest number counts as that.
  * ws: nl_linear_workspace(desc, backward) bytes, 256-byte aligned; contents are free between calls. */

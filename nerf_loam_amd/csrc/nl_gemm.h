@@ -412,7 +412,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
 }
 
 // ---------------------------------------------------------------------------------------------
-// k_gemm_f32: fp32 operands.  x = h + m + l, three bf16 numbers to nearest, exact (8 bits each of 24); of the nine products of two such numbers the six down to
+// k_gemm_f32: fp32 operands.  x = h + m + l, three bf16 numbers to nearest, exact (8 bits each of 24) from |x| = 2^-110 on: the
+// last bit of such a number is 2^-133 at least, bf16's smallest, which the matrix unit does not flush; below that x is off by at most 2^-134.  Of the nine products of two such numbers the six down to
 // 2^-18 are summed, per step of 32 contraction indices the smallest first (l h, h l, m m, m h, h m, h h).  What is dropped (m l, l m, l l) is below 2^-26 |x||w|.
 // The split happens on the way into LDS: no operand is written to memory a second time (split planes in memory: 262144 x 256 x 256 spends 118 us on writing and
 // 50 us more on reading them).  A thread fetches a step's elements into registers while the step before it multiplies, splits them and writes three planes; two

@@ -48,8 +48,8 @@ def linear_act(x, weight, bias=None, act="none", residual=None, checkpoint=None)
     x [..., K], weight [N, K], bias [N] or None, residual [..., N] or None, all of one type -> [..., N].  act: "none", "relu", "gelu" (exact, with erf), "silu".
     Differentiable with respect to the four tensors.  Kept for the backward pass: x and weight, and of z = x weight^T + bias one bit per element (relu) or z itself
     (gelu, silu); with checkpoint="mx8" x and z are kept in 8 bits with a power of two per 32 features (checkpoint_encode): a quarter of float32's memory, and
-    gradients computed from the rounded values.  float32 products are as exact as float32 sums (six bf16 products of exact splits); an infinity among float32
-    operands gives NaN.  In 16 bits the gradient of z is rounded once to the type before it is multiplied (not for short gelu and silu layers, up to 2^23
+    gradients computed from the rounded values.  float32 products are as exact as float32 sums (six bf16 products of splits, exact for magnitudes from 2^-110 on,
+    below that off by at most 2^-134); an infinity among float32 operands gives NaN, in calls with more than eight rows and outputs and in backward passes.  In 16 bits the gradient of z is rounded once to the type before it is multiplied (not for short gelu and silu layers, up to 2^23
     multiplications a product: their backward products run like float32's)."""
     code = L.NL_ACTS.get(act)
     if code is None:
