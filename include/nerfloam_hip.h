@@ -589,6 +589,7 @@ typedef struct NlLinear {
 int nl_linear_forward(const NlLinear* desc, void* stream);
 int nl_linear_backward(const NlLinear* desc, void* stream);
 long long nl_linear_workspace(const NlLinear* desc, int backward);      /* bytes; -1: the descriptor is invalid */
+int nl_linear_streams(const NlLinear* desc, int backward);              /* 1: the product (backward: the data gradient) runs as the streaming one, 0: otherwise, -1: invalid */
 
 /* 8-bit checkpoints: x [M,K] of dtype, rows ldx apart -> codes [M][up(K,32)] (padding: zeros), exponents [M][ceil(K/32)]; and back.
  * e = the smallest exponent >= -126 with max |x| <= 448 2^e over the block; codes to nearest, ties to even; infinities and NaN become NaN;

@@ -210,6 +210,7 @@ _SIGS = {
     "nl_linear_forward": ([_P, _P], _I),
     "nl_linear_backward": ([_P, _P], _I),
     "nl_linear_workspace": ([_P, _I], _LL),
+    "nl_linear_streams": ([_P, _I], _I),
     "nl_mx8_encode": ([_P, _LL, _LL, _I, _I, _P, _P, _P], _I),
     "nl_mx8_decode": ([_P, _P, _LL, _I, _I, _P, _P], _I),
     "nl_embedding_forward": ([_P, _LL, _I, _I, _P, _I, _P, _LL, _I, _F, _P, _P], _I),

@@ -412,6 +412,10 @@ static void nl_stream(NlWork& w, const NlPacked& A, const NlPacked& B, bool b_sl
     if (hipGetLastError() != hipSuccess) w.rc = NL_ERR_LAUNCH;
 }
 
+// what a pass runs as: few rows without tiles; the streaming product (backward: the data gradient as one)
+static bool nl_forward_rows(const NlLinear* d) { return (d->M <= ROWS_MOST || d->N <= ROWS_MOST) && !d->z && !d->bits && !d->z8; }
+static bool nl_forward_streams(const NlLinear* d) { return !nl_forward_rows(d) && nl_streams(d->M, d->K, d->N, d->dtype, false); }
+
 static void nl_forward_run(const NlLinear* d, NlWork& w)
 {
     NlEpilogue ep = {};
@@ -419,7 +423,7 @@ static void nl_forward_run(const NlLinear* d, NlWork& w)
     ep.z = d->z; ep.ldz = d->N;
     ep.bits = d->bits; ep.ldbits = nl_up(d->N, 32) / 32;
     ep.z8 = d->z8; ep.z8e = d->z8e; ep.ldz8 = nl_up(d->N, 32); ep.ldz8e = ep.ldz8 / 32;
-    const bool rows = (d->M <= ROWS_MOST || d->N <= ROWS_MOST) && !d->z && !d->bits && !d->z8;
+    const bool rows = nl_forward_rows(d);
     // the codes of x come out of the product's own tiles; fp32's are split there, and few rows have no tiles: a pass of their own
     const bool codes = d->x8 && d->dtype != NL_DT_F32 && !rows;
     if (d->x8 && !codes && !w.dry) {
@@ -432,7 +436,7 @@ static void nl_forward_run(const NlLinear* d, NlWork& w)
     }
     const NlPacked x = nl_packed(w, d->x, nullptr, d->M, d->K, d->ldx, d->dtype, d->dtype), wt = nl_weight(w, d, d->M, d->N, d->K, 0);
     nl_pack(w, d->dtype);
-    if (nl_streams(d->M, d->K, d->N, d->dtype, false)) nl_stream(w, x, wt, false, d->M, d->N, d->K, ep, d->x8, d->x8e, NlDz{}, 0, 0);
+    if (nl_forward_streams(d)) nl_stream(w, x, wt, false, d->M, d->N, d->K, ep, d->x8, d->x8e, NlDz{}, 0, 0);
     else nl_product(w, x, wt, codes ? 4 : 0, d->M, d->N, d->K, ep, d->x8, d->x8e, nullptr, false);
 }
 
@@ -445,6 +449,11 @@ static bool nl_wide(const NlLinear* d)
     return d->dtype != NL_DT_F32 && (d->act == NL_ACT_GELU || d->act == NL_ACT_SILU) && (double)d->M * d->N * d->K <= (double)NL_WIDE_MOST;
 }
 
+static bool nl_backward_streams(const NlLinear* d)
+{
+    return d->gx && !nl_wide(d) && nl_streams(d->M, d->N, d->K, d->dtype, d->act != NL_ACT_NONE) && nl_in_place(d->gy, d->N, d->ldgy, d->dtype) && (d->K & 7) == 0;
+}
+
 static void nl_backward_run(const NlLinear* d, NlWork& w)
 {
     const bool in_place = d->act == NL_ACT_NONE && nl_in_place(d->gy, d->N, d->ldgy, d->dtype);
@@ -452,7 +461,7 @@ static void nl_backward_run(const NlLinear* d, NlWork& w)
     NlPacked dz = {d->gy, d->ldgy, nullptr};
     NlGb gb = {};
     // the streaming data gradient makes dz on its way
-    const bool streams = d->gx && !wide && nl_streams(d->M, d->N, d->K, d->dtype, d->act != NL_ACT_NONE) && nl_in_place(d->gy, d->N, d->ldgy, d->dtype) && (d->K & 7) == 0;
+    const bool streams = nl_backward_streams(d);
     const int on_its_way = !streams || d->act == NL_ACT_NONE ? 0 : d->act == NL_ACT_RELU ? 1 : d->z8 ? 3 : 2;
     NlDz a = {};
     if (d->gb || (products && !in_place)) {
@@ -539,6 +548,12 @@ long long nl_linear_workspace(const NlLinear* d, int backward)
     w.dry = true;
     if (backward) nl_backward_run(d, w); else nl_forward_run(d, w);
     return w.rc == NL_OK ? w.used : -1;
+}
+
+int nl_linear_streams(const NlLinear* d, int backward)
+{
+    if (nl_linear_check(d, backward) != NL_OK) return -1;
+    return d->M > 0 && (backward ? nl_backward_streams(d) : nl_forward_streams(d));
 }
 
 static int nl_linear_run(const NlLinear* d, int backward, void* stream)
