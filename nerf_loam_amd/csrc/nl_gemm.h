@@ -637,8 +637,12 @@ static void nl_gemm_tile(const NlGemm& g, int tile, dim3 grid, hipStream_t st)
 {
     if (tile == 0) hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, B_MX8, 256, 256, 2, 4, 2, ENC>), grid, dim3(512), 0, st, g);
     else if (tile == 1) hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, B_MX8, 128, 128, 2, 2, 2, ENC>), grid, dim3(256), 0, st, g);
-    else if (B_MX8 || ENC || (long long)grid.x * grid.y > NL_GEMM_FEW_SQUARES) hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, B_MX8, 64, 64, 2, 2, 2, ENC>), grid, dim3(256), 0, st, g);
-    else hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, false, 64, 64, 2, 2, B_MX8 || ENC ? 2 : 4>), grid, dim3(256), 0, st, g);
+    else {
+        if constexpr (!B_MX8 && !ENC) {
+            if ((long long)grid.x * grid.y <= NL_GEMM_FEW_SQUARES) { hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, false, 64, 64, 2, 2, 4>), grid, dim3(256), 0, st, g); return; }
+        }
+        hipLaunchKernelGGL((k_gemm<T, A_SLOW, B_SLOW, B_MX8, 64, 64, 2, 2, 2, ENC>), grid, dim3(256), 0, st, g);
+    }
 }
 template <class T>
 static void nl_gemm_layout(const NlGemm& g, int layout, int tile, dim3 grid, hipStream_t st)
