@@ -631,6 +631,7 @@ int nl_embedding_backward(const void* table, long long V, int D, int dtype, cons
         return NL_ERR_INVALID_ARG;
     hipStream_t st = (hipStream_t)stream;
     const long long L = M * bag;
+    if (g_table && M > 0 && (!ws || ws_bytes < emb_plan(V, D, L, bag).total || ((uintptr_t)ws & 255))) return NL_ERR_INVALID_ARG;      // (before anything is written)
     if (g_weights && M > 0) {
         const int vec = emb_vec(D, dtype), lanes = emb_lanes(D, vec, 64), per = 256 / lanes;
         const dim3 grid = nl_blocks((L + per - 1) / per);
@@ -647,7 +648,6 @@ int nl_embedding_backward(const void* table, long long V, int D, int dtype, cons
         return NL_OK;
     }
     const EmbPlan p = emb_plan(V, D, L, bag);
-    if (!ws || ws_bytes < p.total || ((uintptr_t)ws & 255)) return NL_ERR_INVALID_ARG;
     char* w = (char*)ws;
     unsigned* keys[2] = {(unsigned*)w, (unsigned*)(w + p.keys)};
     unsigned* pos[2] = {(unsigned*)(w + 2 * p.keys), (unsigned*)(w + 3 * p.keys)};

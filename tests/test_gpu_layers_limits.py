@@ -1,4 +1,4 @@
-"""GPU (-m gpu): where fp32 products stop being exact.
+"""GPU (-m gpu): where fp32 products stop being exact, and refusals that must leave their outputs alone.
 
 x = h + m + l, three bf16 numbers.  A number of magnitude 2^e has its last bit at 2^(e - 23); bf16's smallest is 2^-133.  From e = -110 on the three parts hold every bit; below, the
 last part is rounded to a multiple of 2^-133, so x is off by at most 2^-134.  With weights of size 2^100 every product is far inside fp32's range, so that is all that is lost beside
@@ -6,6 +6,7 @@ the product's own (6 K + 8) 2^-23 of its magnitudes."""
 import pytest
 import torch
 
+from nerf_loam_amd import _lib as L
 from nerf_loam_amd import ops
 
 pytestmark = pytest.mark.gpu
@@ -61,3 +62,20 @@ def test_an_infinity_by_size(dtype):
         y = ops.linear_forward(x, w)
         assert bool(torch.isfinite(y[0]).all() and torch.isfinite(y[2:]).all())
         assert bool((y[1] == float("inf")).all()) if few or dtype != torch.float32 else bool(y[1].isnan().all()), (M, N)
+
+
+@pytest.mark.parametrize("V,D,dtype", [(7, 3, torch.bfloat16), (40, 16, torch.float32)])
+def test_a_refused_embedding_gradient_writes_nothing(V, D, dtype):
+    """a workspace that is missing, too small or misaligned: refused before the first launch"""
+    table, g = torch.randn(V, D, device="cuda").to(dtype), torch.randn(20, D, device="cuda").to(dtype)
+    ids, wt = torch.zeros(20, 2, dtype=torch.int32, device="cuda"), torch.rand(20, 2, device="cuda")
+    gt, gw = torch.full_like(table, 7.0), torch.full_like(wt, 7.0)
+    need = L.lib().nl_embedding_workspace(V, D, 20, 2)
+    ws = torch.empty(need + 256, dtype=torch.uint8, device="cuda")
+    for p, n in ((None, need), (ws.data_ptr(), need - 1), (ws.data_ptr() + 8, need)):
+        assert L.lib().nl_embedding_backward(table.data_ptr(), V, D, L.NL_DTYPES[str(dtype)], ids.data_ptr(), 0, wt.data_ptr(), 20, 2, 1.0, g.data_ptr(), gt.data_ptr(), gw.data_ptr(), p, n,
+                                             None) == 1
+    torch.cuda.synchronize()
+    assert bool((gt == 7).all() and (gw == 7).all())
+    ops.embedding_backward(table, ids, g, wt, 1.0, gt, gw, ws)
+    assert not bool((gt[0] == 7).all()) and not bool(gt[1:].any()) and not bool((gw == 7).any())
