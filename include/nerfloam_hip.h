@@ -571,7 +571,9 @@ int nl_dist_rows_union_prefix(const int* gathered, int stride_ints, int offset_i
  * that keep nothing of z do not split: they multiply in fp32, and an infinity stays one.  Sums are fp32 and their order depends on the sizes only.  M = 0 is a legal call (gw, gb = 0).
  * Taken are at most 2^30 rows, 2^22 columns, and results of fewer than 2^24 tiles (of 64 x 64 where they are small).
  * A decoded value of x8 / x8e beyond dtype's largest number counts as that.
- * ws: nl_linear_workspace(desc, backward) bytes, 256-byte aligned; contents are free between calls. */
+ * Tensors lie at their elements' size; z, z8 and x8 at 16 bytes.
+ * ws: nl_linear_workspace(desc, backward) bytes, 256-byte aligned; contents are free between calls.  It holds copies of operands whose rows are no whole 16 bytes, the split of an
+ * fp32 weight (6 bytes an element), dz [M,up(N,8)] of backward passes (in fp32 where it is not rounded) unless act is none and gy's rows are whole 16 bytes, up to 32 MB of the bias' partial sums, and at most 1.5 GB of pieces where a long contraction is cut. */
 typedef struct NlLinear {
     int struct_size, dtype, act, K, N, reserved;
     long long M;
@@ -593,7 +595,7 @@ int nl_linear_streams(const NlLinear* desc, int backward);              /* 1: th
 
 /* 8-bit checkpoints: x [M,K] of dtype, rows ldx apart -> codes [M][up(K,32)] (padding: zeros), exponents [M][ceil(K/32)]; and back.
  * e = the smallest exponent >= -126 with max |x| <= 448 2^e over the block; codes to nearest, ties to even; infinities and NaN become NaN;
- * a decoded value beyond dtype's largest number (the largest ones round up) is that number. */
+ * a decoded value beyond dtype's largest number (the largest ones round up) is that number.  codes lie at 8 bytes, out at 16. */
 int nl_mx8_encode(const void* x, long long ldx, long long M, int K, int dtype, unsigned char* codes, unsigned char* exps, void* stream);
 int nl_mx8_decode(const unsigned char* codes, const unsigned char* exps, long long M, int K, int dtype, void* out, void* stream);
 
@@ -601,7 +603,8 @@ int nl_mx8_decode(const unsigned char* codes, const unsigned char* exps, long lo
  * int64; an id outside [0, V) selects no row.  table [V,D], out [M,D] of dtype.
  * nl_embedding_backward: g_table [V,D] of dtype (every row written: zero where no id selects it), g_weights [M,bag] fp32; each where its pointer is set.
  * The (id, position) pairs are sorted and every row's sum runs over its positions in ascending order, in pieces joined in order: no float atomics, the same
- * bits every run.  M * bag up to 2^30 - 64, V below 2^31, D up to 2^20.  ws: nl_embedding_workspace bytes (0 without g_table). */
+ * bits every run.  M * bag up to 2^30 - 64, V below 2^31, D up to 2^20.  g_table lies at 4 bytes in every type.  ws: nl_embedding_workspace bytes (0 without g_table), 256-byte aligned;
+ * a call that is refused writes nothing. */
 int nl_embedding_forward(const void* table, long long V, int D, int dtype, const void* ids, int id64, const float* weights, long long M, int bag, float scale,
                          void* out, void* stream);
 int nl_embedding_backward(const void* table, long long V, int D, int dtype, const void* ids, int id64, const float* weights, long long M, int bag, float scale,
