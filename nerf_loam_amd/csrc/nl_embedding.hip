@@ -6,7 +6,7 @@
 #include "nl_layers.h"
 
 // Sorted entries per run-summing group: 16 while that leaves at most EMB_THREADS threads of eight columns, so that there are enough of them, else 64, so that there
-// are fewer pieces (whole backward pass, bf16: 16384 lookups x 1024 50 us with 16, 58 with 64; 2.1 M x 16 145, 154; 262144 x 256 99, 87; 131072 x 1024 162, 144).
+// are fewer pieces (table's gradient, bf16: 16384 lookups x 1024 50 us with 16, 58 with 64; 2.1 M x 16 135, 142; 262144 x 256 98, 86; 131072 x 1024 160, 143).
 // Pieces of a row that crosses such chunks are joined in blocks of EMB_BLOCK neighbours, level by level.
 #define EMB_CHUNK_FEW 16
 #define EMB_CHUNK_MANY 64
@@ -15,7 +15,8 @@
 #define EMB_BATCH 8             // rows in flight together
 // A sorting pass takes 1024 keys a workgroup (4 waves x 4 rounds x 64 lanes) up to RS_FEW keys, else 4096 and puts them in order in LDS first, so that what it writes
 // lies in runs of 16 keys on average (2.1 M keys, a pass: 18 us and 5 for the scan, 40 and 14 in workgroups of 1024).  There the weights of bags move along: 7 us a
-// pass, and the sums fetch a line of 128 bytes less per lookup (2.1 M x 16 bf16: 43 us instead of 69).  Up to RS_FEW_BLOCKS workgroups the scatter sums the histograms
+// pass, and the sums fetch a line of 128 bytes less per lookup (2.1 M x 16 bf16: 43 us instead of 69).  Whole gradient in workgroups of 4096 / 1024: 2.1 M weighted lookups x 16
+// 135 / 205 us, 131072 lookups x 256 77 / 57, 32768 60 / 40: RS_FEW lies below where they cross.  Up to RS_FEW_BLOCKS workgroups the scatter sums the histograms
 // itself: a launch less per pass.
 #define RS_FEW 65536
 #define RS_FEW_BLOCKS 64
@@ -69,8 +70,8 @@ __device__ __forceinline__ EmbVec<VEC> emb_fetch(__amdgpu_buffer_rsrc_t r, unsig
 // One group of `lanes` threads (a power of two, at most 256) per output row.  The ids of a bag are read BAG at a time and their rows fetched together: what bounds
 // a small row is the way id -> row, once per batch instead of once per lookup.
 // EIGHT: bags of eight 32-bit ids and weights, both 16-byte aligned (a voxel's corners).  Two neighbouring threads load half of them each and exchange them, past the
-// caches that the table's rows should stay in, as the results are stored: 262144 rows of 16 bf16 from a table of 1.7 MB 11.5 us, 13.5 with every thread loading all
-// eight through the caches (from cold ones 16.5, 21.3).  Of it 3.4 us are the streams; the rest is 2.1 M lookups of 32 bytes that move a line of 128 from L2 to L1 each.
+// caches that the table's rows should stay in, as the results are stored: 262144 rows of 16 bf16 from a table of 1.7 MB 11.5 us on the same inputs again and again, 14.4 on
+// inputs that change; with every thread loading all eight through the caches 13.5 (from cold ones 16.5, 21.3).  Of it 3.4 us are the streams; the rest is 2.1 M lookups of 32 bytes that move a line of 128 from L2 to L1 each.
 // The table is below 2 GB: 32-bit offsets, and an id without a row reads zeros from behind the buffer's range.
 template <int DT, int VEC, int BAG, bool EIGHT>
 __global__ __launch_bounds__(256) void k_emb_forward(const void* __restrict__ table, long long V, int D, const void* __restrict__ ids, int id64,

@@ -418,7 +418,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm(NlGemm g)
 // The split happens on the way into LDS: no operand is written to memory a second time (split planes in memory: 262144 x 256 x 256 spends 118 us on writing and
 // 50 us more on reading them).  A thread fetches a step's elements into registers while the step before it multiplies, splits them and writes three planes; two
 // workgroups share a compute unit, so that one splits (vector unit) while the other multiplies.  Six products: at most a sixth of the bf16 rate, 246 TFLOP/s.
-// 4096^3: 688 us, 200 TFLOP/s, 220 with B split beforehand (the library's fp32 product: 150); 262144 x 256 x 256: 226 us, 152 TFLOP/s (library 97) - eight steps per tile, whose loads and stores
+// 4096^3: 699 us, 197 TFLOP/s, 209 with B split beforehand (the library's fp32 product: 151); 262144 x 256 x 256: 226 us, 152 TFLOP/s (library 97) - eight steps per tile, whose loads and stores
 // (537 MB, 105 us) overlap only with the other workgroup's steps.  Starting the second workgroup of a unit later changes nothing.
 // ---------------------------------------------------------------------------------------------
 // two values to bf16, to nearest, in the halves of a word
@@ -567,7 +567,7 @@ __global__ __launch_bounds__(256, 2) void k_gemm_f32(NlGemm g)
 }
 
 // The same with B already split, in three planes g.plane bytes apart (nl_linear.hip splits a weight once where many rows of tiles would split it again each): its planes go
-// straight into LDS, into two buffers in turn (arrays of their own, as in k_gemm), and only A passes through registers.  4096^3: 624 us, 220 TFLOP/s, 688 without.
+// straight into LDS, into two buffers in turn (arrays of their own, as in k_gemm), and only A passes through registers.  4096^3: 658 us, 209 TFLOP/s, 699 without.
 template <bool A_SLOW, bool B_SLOW, int BT>
 __global__ __launch_bounds__(256, 2) void k_gemm_f32_planes(NlGemm g)
 {

@@ -311,10 +311,11 @@ static NlPacked nl_packed(NlWork& w, const void* p, const unsigned char* e, long
 
 // How a product [M,N] over K is cut: the tile, and into how many pieces the contraction goes.  The estimate: rounds of as many workgroups as run at a time, each with
 // its contraction steps of 64 (alone on a compute unit / with as many neighbours as fit) and what surrounds them; for a cut contraction the pieces' way through memory
-// and the launch that joins them.  Measured, in microseconds (bf16, 4096^3: 95 in squares of 256, 105 of 128, 172 of 64; 2048 x 256 x 256: 14, 7.3, 4.4; 256 x 256 x
-// 200000: 56 in 256 pieces of the first, 46 in 128 of the second, 48 in 32 of the third, 4200 uncut; 8-bit codes, 256 x 256 x 200000 from memory: 73
-// in 64 pieces of the second, 52 in 128, 80 in squares of 64; fp32 4096^3: 576 in squares of 128, 665 of 64, 2048 x 256 x 256:
-// 21, 9.8).  The estimate's choice is within 17 % of the best of all tiles and powers of two at the 23 shapes of either kind that these come from, contractions above 4096 within 10 %.
+// and the launch that joins them.  Measured, in microseconds, on operands of numbers (zeros draw less power: 4096^3 takes 95 and 576 of them) (bf16, 4096^3: 111 in squares of 256, 124 of 128, 193 of 64;
+// 2048 x 256 x 256: 14, 7.2, 4.3; 256 x 256 x 200000: 55 in 256 pieces of the first, 47 in 128 of the second, 50 in 32 of the third, 4000 uncut; 8-bit codes, 256 x 256 x 200000
+// from memory: 73 in 64 pieces of the second, 52 in 128, 80 in squares of 64; fp32 4096^3: 680 in squares of 128, 864 of 64, 2048 x 256 x 256: 20, 9.6).  At 23 shapes of either kind
+// the estimate's choice is the best of all tiles and powers of two or within 6 % of it, but for 256 x 4096 x 4096 (20 and 16 %), 256 x 256 x 200000 bf16 (11), 512^3 and 2048^3 fp32
+// (12 and 16) and 128 x 128 x 4096 bf16 (13.2 instead of 8.8).
 struct NlCut { int tile, splits; long long kchunk; };
 static NlCut nl_cut(long long M, long long N, long long K, int dt, int layout, int largest)
 {
@@ -345,8 +346,8 @@ static NlCut nl_cut(long long M, long long N, long long K, int dt, int layout, i
     return best;
 }
 
-// The weight of an fp32 product, split beforehand where that saves more than it costs: every row of tiles splits it again otherwise (4096^3 688 -> 624 us, 65536 x 512 -> 256
-// 122 -> 113, 262144 x 256 -> 256 243 -> 236); the pass over the weight takes a launch, 5 us, and 10 bytes an element.  M, N, K: the product's; squares of 128 only
+// The weight of an fp32 product, split beforehand where that saves more than it costs: every row of tiles splits it again otherwise (4096^3 699 -> 658 us, 65536 x 512 -> 256
+// 100 -> 93, 262144 x 256 -> 256 226 -> 226, 4096 x 512 -> 2048 54 -> 54); the pass over the weight takes a launch, 5 us, and 10 bytes an element.  M, N, K: the product's; squares of 128 only
 static NlPacked nl_weight(NlWork& w, const NlLinear* d, long long M, int N, int K, int layout)
 {
     if (d->dtype != NL_DT_F32 || M < 4096 || K < 512 || (double)M * N * K < 4e9 || nl_cut(M, N, K, NL_DT_F32, layout, 1).tile != 1)
@@ -391,9 +392,9 @@ static void nl_product(NlWork& w, const NlPacked& A, const NlPacked& B, int layo
 }
 
 // A weight of at most 256 x 256 in 16 bits: when the product streams (nl_narrow.h).  K: the contraction, N: the results' columns; dz: the data gradient that makes dz on
-// its way, which saves a pass and a launch.  Without dz it pays for wide results that do not stay in the caches (bf16, us, tiles / streaming: 262144 x 256 -> 256 relu 93 / 78,
-// 262144 x 16 -> 256 56 / 46, 65536 x 256 -> 256 22.6 / 24.0; 262144 x 256 -> 64 45 / 47, 262144 x 64 -> 64 17 / 39); with it everywhere (all gradients: 64 x 256 x 256
-// 13.0 / 12.1, 4096 x 256 x 256 17.5 / 16.9, 65536 x 256 x 256 57 / 46, 262144 x 256 x 64 123 / 103; only 262144 x 64 x 64 53 / 55).
+// its way, which saves a pass and a launch.  Without dz it pays for wide results that do not stay in the caches (bf16, us, tiles / streaming: 262144 x 256 -> 256 relu 90 / 74,
+// 262144 x 16 -> 256 55 / 44, 65536 x 256 -> 256 22.3 / 23.8, 262144 x 64 -> 160 39 / 44; 262144 x 256 -> 64 45 / 47, 262144 x 64 -> 64 17 / 39); with it everywhere (all gradients, relu:
+// 64 x 256 -> 256 24 / 21, 4096 x 256 -> 256 24.5 / 22.0, 65536 x 256 -> 256 58 / 46, 262144 x 256 -> 64 121 / 103; only 262144 x 64 -> 64 52 / 54).
 static int nl_stream_groups(long long M) { const long long tiles = (M + NL_NARROW_ROWS - 1) / NL_NARROW_ROWS; return tiles < 256 ? (int)tiles : 256; }      // one to a compute unit
 static bool nl_streams(long long M, int K, int N, int dt, bool dz)
 {
@@ -440,7 +441,8 @@ static void nl_forward_run(const NlLinear* d, NlWork& w)
     else nl_product(w, x, wt, codes ? 4 : 0, d->M, d->N, d->K, ep, d->x8, d->x8e, nullptr, false);
 }
 
-// dz = gy act'(z) in 16 bits is a second rounding of half a step besides the gradients' own (1.41 times the error of one; with few results up to 1.9 times).  Where the
+// dz = gy act'(z) in 16 bits is a second rounding of half a step besides the gradients' own (1.41 times the error of one, 1.45 with z kept in the type, whose rounding costs the bias'
+// gradient 5 %; with few results up to 1.9 times).  Where the
 // products are short, and launches are what the pass takes, dz stays in fp32 and the products run as fp32's do (2^22 multiplications in either, both products, bf16: 18.5
 // instead of 13.7 us of a pass that takes 70 from autograd; 2^25 in either: 21 instead of 15.5).
 #define NL_WIDE_MOST (1LL << 23)
