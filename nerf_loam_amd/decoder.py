@@ -33,7 +33,7 @@ class _FusedValues(torch.autograd.Function):
         again = torch.is_grad_enabled()                                                     # create_graph: the layers say which gradients depend on what
         with torch.enable_grad():
             t = [v.view_as(v) if again else v.detach().requires_grad_(need) for v, need in zip(ctx.saved_tensors, ctx.needs_input_grad[1:])]
-            y = ctx.dec._values_layers(t[0].float(), [v.float() for v in t[1:]])            # the kernel's type
+            y = ctx.dec._values_layers(t[0].float(), [v.to(g.device, torch.float32) for v in t[1:]])            # the kernel's type, and its device where the module is elsewhere
             wanted = [v for v, need in zip(t, ctx.needs_input_grad[1:]) if need]
             grads = iter(torch.autograd.grad(y, wanted, g, create_graph=again))
         return (None, *(next(grads) if need else None for need in ctx.needs_input_grad[1:]))

@@ -8,7 +8,7 @@ here each is one call into hand-written kernels (csrc/nl_linear.hip, nl_checkpoi
 * checkpoint_encode / checkpoint_decode  the 8-bit format itself
 
 Tensors live on the GPU (there is no CPU path), types are float32, bfloat16 and float16.  Gradients of gradients and forward-mode derivatives are not provided
-and refused.  The backward passes refuse to run through autograd while a stream is being captured: capture ops.linear_forward / linear_backward and ops.embedding_forward / embedding_backward
+and refused (a gradient that depends on no trained tensor is a constant).  The backward passes refuse to run through autograd while a stream is being captured: capture ops.linear_forward / linear_backward and ops.embedding_forward / embedding_backward
 instead, which are the same kernels on caller-owned tensors (autograd's leaf nodes belong to the stream of an earlier eager pass, and waiting for that stream
 inside a capture cannot be undone)."""
 import ctypes

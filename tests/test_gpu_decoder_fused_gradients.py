@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from nerf_loam_amd import _lib as L
+from nerf_loam_amd.decoder import Decoder
 from test_gpu_decoder_layers import _chain64, _decoder
 
 pytestmark = pytest.mark.gpu
@@ -77,3 +78,22 @@ def test_an_optimiser_step_between_calls_is_seen(dtype):
         grads = torch.autograd.grad(want, leaves, 2 * want.detach() / want.numel())
         assert x.grad.dtype == dtype and float((x.grad.double() - grads[0]).norm() / grads[0].norm()) < (2e-3 if dtype == torch.float32 else 2.0 ** -8)
         opt.step()
+
+
+def test_a_module_on_the_host_and_a_second_stream():
+    """the fused kernel takes a module's parameters from wherever they are: the gradients go back there; passes on another stream than the input's give the same bits"""
+    host = Decoder()
+    dec = Decoder().cuda()
+    dec.load_state_dict(host.state_dict())
+    x = torch.randn(700, 16, device="cuda")
+    for d in (host, dec):
+        d(x)["sdf"].square().sum().backward()
+    assert all(a.grad.device.type == "cpu" and torch.equal(a.grad, b.grad.cpu()) for a, b in zip(host.param_list(), dec.param_list()))
+    want = [p.grad.clone() for p in dec.param_list()]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        dec.zero_grad()
+        dec(x)["sdf"].square().sum().backward()
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(a, p.grad) for a, p in zip(want, dec.param_list()))
